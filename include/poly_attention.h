@@ -238,6 +238,52 @@ typedef struct {
 POLY_API int poly_head_rmsnorm(const PolyHeadNorm* norms, int n, void* stream);
 
 /*
+ * Rotary positions of up to 8 query / key tensors in ONE launch. Over the
+ * first rot features of a row, in pairs (a, b) = (2i, 2i + 1) (interleaved) or
+ * (i, i + rot / 2):
+ *   y_a = factor (x_a cos t - x_b sin t),  y_b = factor (x_b cos t + x_a sin t)
+ * and y = x past rot. t = position * inv_freq[i], the product exact and reduced
+ * in 64 bits, or angles[b][row][i]. inverse != 0 negates sin: the transpose,
+ * which is the gradient. The tensors of a call share batch, rows, positions
+ * and dtype; strides are in elements, the feature axis contiguous; dst may be
+ * src with src's strides. The position of row i is pos_start plus positions
+ * (int32, or int64 if pos_wide) if given, or the row's place in its sequence if
+ * cu_seqlens is given (batch 1), else i.
+ */
+#define POLY_MAX_ROTARY 8
+typedef struct {
+  const void* src;
+  void* dst;
+  int32_t heads;
+  int32_t reserved;
+  int64_t src_stride[3]; /* elements: batch, head, row */
+  int64_t dst_stride[3];
+} PolyRotaryTensor;
+
+typedef struct {
+  int32_t batch;
+  int32_t rows;
+  int32_t dim;         /* <= 256 */
+  int32_t rot;         /* even, 2 .. dim */
+  int32_t dtype;
+  int32_t interleaved;
+  int32_t inverse;
+  int32_t n;           /* tensors */
+  float factor;        /* amplitude (1, or the long-context attention factor) */
+  int32_t pos_wide;
+  const void* positions;      int64_t pos_stride[2];   /* [batch, rows] | NULL; elements, 0 broadcasts */
+  int64_t pos_start;
+  const float* inv_freq;                               /* [rot / 2] | NULL */
+  const float* angles;        int64_t angle_stride[2]; /* [batch, rows, rot / 2] | NULL */
+  const int32_t* cu_seqlens;                           /* device [seqs + 1] | NULL */
+  int32_t seqs;
+  int32_t reserved;
+  PolyRotaryTensor t[POLY_MAX_ROTARY];
+} PolyRotaryArgs;
+
+POLY_API int poly_rotary(const PolyRotaryArgs* args, void* stream);
+
+/*
  * poly_pass_bwd without a caller workspace. No counterpart in the reference:
  * it exists for callers that cannot allocate device memory (FFI hosts that
  * only pass existing buffers, processes whose device memory another
@@ -287,6 +333,7 @@ POLY_API int poly_abi_version(void);
 POLY_API size_t poly_sizeof_pass_args(void);
 POLY_API size_t poly_sizeof_pass_bwd_args(void);
 POLY_API size_t poly_sizeof_merge_args(void);
+POLY_API size_t poly_sizeof_rotary_args(void);
 
 #ifdef __cplusplus
 }

@@ -82,6 +82,7 @@ int poly_abi_version(void) { return POLY_ABI_VERSION; }
 size_t poly_sizeof_pass_args(void) { return sizeof(PolyPassArgs); }
 size_t poly_sizeof_pass_bwd_args(void) { return sizeof(PolyPassBwdArgs); }
 size_t poly_sizeof_merge_args(void) { return sizeof(PolyMergeArgs); }
+size_t poly_sizeof_rotary_args(void) { return sizeof(PolyRotaryArgs); }
 
 size_t poly_pass_fwd_workspace_size(const PolyPassArgs* a) {
   if (check_pass(a) != POLY_OK) return 0;
@@ -129,6 +130,8 @@ int poly_pass_fwd(const PolyPassArgs* a, void* stream) {
 int poly_head_rmsnorm(const PolyHeadNorm* norms, int n, void* stream) {
   return head_rmsnorm(norms, n, (cudaStream_t)stream);
 }
+
+int poly_rotary(const PolyRotaryArgs* args, void* stream) { return rotary(args, (cudaStream_t)stream); }
 
 int poly_copy_rows(const PolyRowCopy* copies, int n, void* stream) {
   return copy_rows(copies, n, (cudaStream_t)stream);

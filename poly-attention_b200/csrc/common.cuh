@@ -86,5 +86,6 @@ int launch_pass_decode(const PolyPassArgs& a, cudaStream_t s, bool dependent = f
 size_t pass_decode_workspace(const PolyPassArgs& a);
 int copy_rows(const PolyRowCopy* copies, int n, cudaStream_t s);
 int head_rmsnorm(const PolyHeadNorm* norms, int n, cudaStream_t s);
+int rotary(const PolyRotaryArgs* args, cudaStream_t s);
 
 }  // namespace poly

@@ -1,0 +1,51 @@
+// Finding a row or a tile in a batch of sequences packed end to end.
+//
+// cu_seqlens[s] is sequence s's first row, cu_seqlens[s + 1] the row behind it.
+// The kernels that split every sequence into tiles of B rows number the tiles
+// without a prefix sum: sequence s owns the slots floor(cu[s] / B) + s and up to
+// (not including) floor(cu[s + 1] / B) + s + 1, which are at least ceil(len / B)
+// of them, and total / B + seqs slots cover every sequence. So a CTA finds its
+// sequence by one search over cu_seqlens; a slot past its sequence's last tile
+// is empty. Offsets are clamped to [0, total]: offsets outside it or running
+// backwards select wrong rows, never rows outside the tensors.
+#pragma once
+
+#include <stdint.h>
+
+namespace poly {
+
+__device__ __forceinline__ int packed_at(const int* cu, int s, int total) { return min(max(cu[s], 0), total); }
+
+// first row of the sequence that row i belongs to
+__device__ __forceinline__ int packed_start(const int* cu, int seqs, int total, int i) {
+  int lo = 0, hi = seqs;   // the last s with cu[s] <= i
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (packed_at(cu, mid, total) <= i) lo = mid; else hi = mid;
+  }
+  return packed_at(cu, lo, total);
+}
+
+struct PackedTile {
+  int seq, start, len;   // the sequence, its first row and its length
+  int tile;              // tile of the sequence
+  int slot0;             // the sequence's first slot
+};
+
+// The tile of slot `slot` (B rows a tile); false: the slot is empty.
+template <int B>
+__device__ __forceinline__ bool packed_tile(const int* cu, int seqs, int total, int slot, PackedTile& t) {
+  int lo = 0, hi = seqs;   // the last s with cu[s] / B + s <= slot
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (packed_at(cu, mid, total) / B + mid <= slot) lo = mid; else hi = mid;
+  }
+  t.seq = lo;
+  t.start = packed_at(cu, lo, total);
+  t.len = packed_at(cu, lo + 1, total) - t.start;
+  t.slot0 = t.start / B + lo;
+  t.tile = slot - t.slot0;
+  return t.tile >= 0 && t.tile * B < t.len;
+}
+
+}  // namespace poly

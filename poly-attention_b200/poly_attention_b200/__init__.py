@@ -7,9 +7,11 @@ from .n_poly_attention import NPolyAttention
 from .ops import kernel_names, lse_merge, pass_bwd, pass_fwd
 from .poly_attention import Order2PolyAttention, PolyAttention
 from .poly_vit import PolyViT
+from .rotary import RotaryEmbedding, apply_rotary, rotary_frequencies
 
 __all__ = [
     "PolyAttention", "Order2PolyAttention", "NPolyAttention", "PolyViT", "flash_poly_attention",
     "poly_attention_order2", "poly_attention_order2_cached", "poly_attention_chain", "poly_attention_chain_cached",
     "pass_fwd", "pass_bwd", "lse_merge", "kernel_names", "HostStreamedOrder2",
+    "apply_rotary", "rotary_frequencies", "RotaryEmbedding",
 ]

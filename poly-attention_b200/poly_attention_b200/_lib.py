@@ -79,6 +79,26 @@ class PolyHeadNorm(ctypes.Structure):
 
 MAX_NORMS = 4
 
+
+class PolyRotaryTensor(ctypes.Structure):
+    _fields_ = [("src", c_vp), ("dst", c_vp), ("heads", c_i32), ("reserved", c_i32),
+                ("src_stride", I64x3), ("dst_stride", I64x3)]
+
+
+MAX_ROTARY = 8
+
+
+class PolyRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("rows", c_i32), ("dim", c_i32), ("rot", c_i32), ("dtype", c_i32), ("interleaved", c_i32),
+        ("inverse", c_i32), ("n", c_i32), ("factor", c_f32), ("pos_wide", c_i32),
+        ("positions", c_vp), ("pos_stride", I64x2), ("pos_start", c_i64),
+        ("inv_freq", c_vp), ("angles", c_vp), ("angle_stride", I64x2),
+        ("cu_seqlens", c_vp), ("seqs", c_i32), ("reserved", c_i32),
+        ("t", PolyRotaryTensor * MAX_ROTARY),
+    ]
+
+
 EXPORTS = {
     "poly_pass_fwd": (ctypes.c_int, [ctypes.POINTER(PolyPassArgs), c_vp]),
     "poly_pass_fwd_workspace_size": (c_sz, [ctypes.POINTER(PolyPassArgs)]),
@@ -88,6 +108,7 @@ EXPORTS = {
     "poly_decode_chain": (ctypes.c_int, [ctypes.POINTER(PolyPassArgs), ctypes.c_int, c_vp]),
     "poly_copy_rows": (ctypes.c_int, [ctypes.POINTER(PolyRowCopy), ctypes.c_int, c_vp]),
     "poly_head_rmsnorm": (ctypes.c_int, [ctypes.POINTER(PolyHeadNorm), ctypes.c_int, c_vp]),
+    "poly_rotary": (ctypes.c_int, [ctypes.POINTER(PolyRotaryArgs), c_vp]),
     "poly_pass_bwd_noalloc": (ctypes.c_int, [ctypes.POINTER(PolyPassBwdArgs), c_vp]),
     "poly_noalloc_scratch_bytes": (c_sz, []),
     "poly_pass_fwd_kernel_name": (ctypes.c_char_p, [ctypes.POINTER(PolyPassArgs)]),
@@ -100,6 +121,7 @@ EXPORTS = {
     "poly_sizeof_pass_args": (c_sz, []),
     "poly_sizeof_pass_bwd_args": (c_sz, []),
     "poly_sizeof_merge_args": (c_sz, []),
+    "poly_sizeof_rotary_args": (c_sz, []),
 }
 
 
@@ -115,7 +137,7 @@ def _load():
     if lib.poly_abi_version() != ABI_VERSION:
         raise ImportError("libpolyattn.so ABI version mismatch")
     for fn, st in (("poly_sizeof_pass_args", PolyPassArgs), ("poly_sizeof_pass_bwd_args", PolyPassBwdArgs),
-                   ("poly_sizeof_merge_args", PolyMergeArgs)):
+                   ("poly_sizeof_merge_args", PolyMergeArgs), ("poly_sizeof_rotary_args", PolyRotaryArgs)):
         if getattr(lib, fn)() != ctypes.sizeof(st):
             raise ImportError(f"libpolyattn.so struct layout mismatch ({st.__name__})")
     return lib

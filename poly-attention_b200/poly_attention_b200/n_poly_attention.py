@@ -14,7 +14,8 @@ from torch.nn import Module, RMSNorm
 from .core import poly_attention_chain, poly_attention_chain_cached
 from .head_norm import head_rmsnorm
 from .kv_cache import ModuleKVCache, usable as _inplace_usable
-from .poly_attention import _rotary, cast_tuple, default, exists, merge_heads, split_heads
+from .poly_attention import cast_tuple, default, exists, merge_heads, rotate_by_angles, split_heads
+from .rotary import RotaryEmbedding
 
 LinearNoBias = partial(nn.Linear, bias=False)
 
@@ -53,7 +54,7 @@ class NPolyAttention(Module):
             *[LinearNoBias(dim, dim_inner_kv * (1 if shared_kv else 2)) for _ in range(order - 1)],
         ])
         self.q_norms = nn.ModuleList([RMSNorm(dim_head) for _ in range(order + 1)])
-        self.rotary_emb = _rotary().RotaryEmbedding(dim_head) if use_rotary_embed else None
+        self.rotary_emb = RotaryEmbedding(dim_head) if use_rotary_embed else None
         self.to_out = nn.Linear(dim_inner, dim)
         # buffers behind the cache tuple returned last (in-place decoding steps)
         self._kv_cache = None
@@ -118,8 +119,7 @@ class NPolyAttention(Module):
             root_value = kv1[1] if self.has_root_v else None
         qs = tuple(head_rmsnorm(self.q_norms, (q1, *qs_rest)))
         if exists(rotary_pos_emb):
-            r = _rotary()
-            qs = tuple(r.apply_rotary_emb(rotary_pos_emb, q) for q in qs)
+            qs = tuple(rotate_by_angles(rotary_pos_emb, [q])[0] for q in qs)
         q1, qs_rest = qs[0], qs[1:]
 
         inplace = (_inplace_usable(q1.dtype, q1.device, self.dim_head, exists(mask) or any(exists(m) for m in context_mask),
@@ -153,8 +153,13 @@ class NPolyAttention(Module):
         q_left = [q1, *qs_rest[:-1]]
         q_right = list(qs_rest_cache)
         if not exists(rotary_pos_emb) and exists(self.rotary_emb):
-            rot = [self.rotary_emb.rotate_queries_with_cached_keys(ql, qr) for ql, qr in zip(q_left, q_right)]
-            q_left, q_right = (list(t) for t in zip(*rot))
+            if not has_cache and len({q.shape[-2] for q in qs}) == 1:
+                # every row at its own position: a tensor turns the same way as keys and as queries
+                qs = self.rotary_emb(list(qs))
+                q_left, q_right = list(qs[:-1]), list(qs[1:])
+            else:
+                rot = [self.rotary_emb.rotate_queries_with_cached_keys(ql, qr) for ql, qr in zip(q_left, q_right)]
+                q_left, q_right = (list(t) for t in zip(*rot))
 
         if has_cache:
             out, lse_steps, msg_steps = poly_attention_chain_cached(

@@ -15,6 +15,7 @@ from torch.nn import Module, RMSNorm
 from .core import poly_attention_order2, poly_attention_order2_cached
 from .head_norm import head_rmsnorm
 from .kv_cache import ModuleKVCache, usable as _inplace_usable
+from .rotary import RotaryEmbedding, apply_rotary
 
 LinearNoBias = partial(nn.Linear, bias=False)
 
@@ -44,12 +45,11 @@ def merge_heads(t):
     return t.transpose(1, 2).reshape(b, n, h * d)
 
 
-def _rotary():
-    try:
-        import rotary_embedding_torch as r
-    except ImportError as e:  # pragma: no cover - depends on the environment
-        raise ImportError("rotary embeddings need the rotary-embedding-torch package") from e
-    return r
+def rotate_by_angles(rotary_pos_emb, qs):
+    """The modules' ``rotary_pos_emb``: angles [n, rot] or [b, n, rot] of the features,
+    both features (2i, 2i + 1) of a pair holding the pair's angle
+    (poly_attention/poly_attention.py:276-277)."""
+    return apply_rotary(qs, angles=rotary_pos_emb[..., ::2])
 
 
 class Order2PolyAttention(Module):
@@ -86,7 +86,7 @@ class Order2PolyAttention(Module):
             LinearNoBias(dim, dim_inner_kv * (1 if shared_kv else 2)),
         ])
         self.q_norms = nn.ModuleList([RMSNorm(dim_head), RMSNorm(dim_head), RMSNorm(dim_head)])
-        self.rotary_emb = _rotary().RotaryEmbedding(dim_head) if use_rotary_embed else None
+        self.rotary_emb = RotaryEmbedding(dim_head) if use_rotary_embed else None
         self.to_out = nn.Linear(dim_inner, dim)
         # buffers behind the cache tuple returned last (in-place decoding steps)
         self._kv_cache = None
@@ -152,8 +152,7 @@ class Order2PolyAttention(Module):
             q3, v3 = kv2[0], kv2[1]
         q1, q2, q3 = head_rmsnorm(self.q_norms, (q1, q2, q3))
         if exists(rotary_pos_emb):
-            r = _rotary()
-            q1, q2, q3 = (r.apply_rotary_emb(rotary_pos_emb, q) for q in (q1, q2, q3))
+            q1, q2, q3 = (rotate_by_angles(rotary_pos_emb, [q])[0] for q in (q1, q2, q3))
 
         cq2, cq3, cv3, clse23, cmsg = cache if has_cache else (None,) * 5
         inplace = (_inplace_usable(q1.dtype, q1.device, self.dim_head,
@@ -182,9 +181,13 @@ class Order2PolyAttention(Module):
         q2_left, q2_right, q3_full = q2, q2_cache, q3_cache
         q2_pass1 = None
         if not exists(rotary_pos_emb) and exists(self.rotary_emb):
-            q1, q2_right = self.rotary_emb.rotate_queries_with_cached_keys(q1, q2_right)
-            q2_left, q3_full = self.rotary_emb.rotate_queries_with_cached_keys(q2_left, q3_full)
-            q2_pass1 = q2_left
+            if not has_cache and q1.shape[-2] == q2.shape[-2] == q3.shape[-2]:
+                # every row at its own position: q2 turns the same way as a key and as a query
+                q1, q2_right, q3_full = self.rotary_emb([q1, q2, q3])
+            else:
+                q1, q2_right = self.rotary_emb.rotate_queries_with_cached_keys(q1, q2_right)
+                q2_left, q3_full = self.rotary_emb.rotate_queries_with_cached_keys(q2_left, q3_full)
+                q2_pass1 = q2_left
 
         if has_cache:
             out, lse_step, msg_step = poly_attention_order2_cached(

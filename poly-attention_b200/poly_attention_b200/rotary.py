@@ -1,0 +1,280 @@
+"""Rotary positions (``poly_rotary``): queries and keys of a layer rotated in one
+launch, straight from the strided head-split views, with gradients.
+
+``apply_rotary`` is the operator, ``rotary_frequencies`` its frequencies (with
+the usual scalings for contexts longer than a model was trained on) and
+``RotaryEmbedding`` the module that ``use_rotary_embed=True`` puts into the
+attention modules (``rotary_emb``, poly_attention/poly_attention.py:202,
+302-304; n_poly_attention.py:118, 226).
+
+There is no CPU implementation: CPU tensors raise.
+"""
+from __future__ import annotations
+
+import math
+from typing import List, Optional
+
+import torch
+from torch import nn
+
+from . import _lib
+from ._lib import PolyRotaryArgs, check, lib
+from .ops import _DTYPES, _require_cuda, _stream
+
+
+def rotary_frequencies(dim, *, theta=10000.0, scaling=None, factor=1.0, original_length=None, fast_turns=32.0,
+                       slow_turns=1.0):
+    """Inverse frequencies [dim / 2] (fp32) and the attention factor that goes with them.
+
+    ``theta ** (-2 i / dim)``, computed in 64 bits. ``scaling`` stretches the
+    context by ``factor``: "linear" divides every frequency by it, "ntk" raises
+    theta to ``theta * factor ** (dim / (dim - 2))``, "yarn" divides only the
+    frequencies that turn less than ``slow_turns`` times in ``original_length``
+    positions, keeps those that turn more than ``fast_turns`` times, mixes the
+    ones between, and returns the attention factor ``0.1 ln(factor) + 1``.
+    """
+    if dim <= 0 or dim % 2:
+        raise ValueError(f"rotary dim must be positive and even, got {dim}")
+    if not (theta > 0 and factor >= 1.0):
+        raise ValueError("theta must be positive and factor at least 1")
+    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    if scaling == "ntk":
+        theta = theta * factor ** (dim / max(dim - 2, 1))
+    elif scaling not in (None, "linear", "yarn"):
+        raise ValueError(f"unknown rotary scaling {scaling!r}")
+    inv = theta ** (-i / dim)
+    if scaling == "linear":
+        return (inv / factor).float(), 1.0
+    if scaling == "yarn":
+        if not original_length or not fast_turns > slow_turns:
+            raise ValueError("yarn scaling needs original_length and fast_turns > slow_turns")
+        turns = inv * (original_length / (2.0 * math.pi))
+        keep = ((turns - slow_turns) / (fast_turns - slow_turns)).clamp(0.0, 1.0)
+        return (inv * keep + inv / factor * (1.0 - keep)).float(), 0.1 * math.log(factor) + 1.0
+    return inv.float(), 1.0
+
+
+def _empty_like(x):
+    """Output with x's axis order in memory (token-major views stay token-major), dense."""
+    b, h, n, d = x.shape
+    if x.stride(1) <= x.stride(2):
+        return x.new_empty((b, n, h, d)).permute(0, 2, 1, 3)
+    return x.new_empty((b, h, n, d))
+
+
+def _launch(xs, outs, inv_freq, positions, start, cu_seqlens, angles, interleaved, factor, inverse):
+    x0 = xs[0]
+    a = PolyRotaryArgs()
+    a.batch, _, a.rows, a.dim = x0.shape
+    a.dtype, a.interleaved, a.inverse, a.factor = _DTYPES[x0.dtype], interleaved, inverse, factor
+    a.pos_start = start
+    if angles is not None:
+        a.rot, a.angles = 2 * angles.shape[-1], angles.data_ptr()
+        a.angle_stride[0], a.angle_stride[1] = angles.stride(0), angles.stride(1)
+    else:
+        a.rot, a.inv_freq = 2 * inv_freq.shape[0], inv_freq.data_ptr()
+    if cu_seqlens is not None:
+        a.cu_seqlens, a.seqs = cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1
+    elif positions is not None:
+        a.positions, a.pos_wide = positions.data_ptr(), positions.dtype == torch.int64
+        a.pos_stride[0], a.pos_stride[1] = positions.stride(0), positions.stride(1)
+    with torch.cuda.device(x0.device):
+        stream = _stream(x0.device)
+        for i0 in range(0, len(xs), _lib.MAX_ROTARY):
+            part = range(i0, min(len(xs), i0 + _lib.MAX_ROTARY))
+            a.n = len(part)
+            for t, i in zip(a.t, part):
+                x, y = xs[i], outs[i]
+                t.src, t.dst, t.heads = x.data_ptr(), y.data_ptr(), x.shape[1]
+                s, d = x.stride(), y.stride()
+                t.src_stride[0], t.src_stride[1], t.src_stride[2] = s[0], s[1], s[2]
+                t.dst_stride[0], t.dst_stride[1], t.dst_stride[2] = d[0], d[1], d[2]
+            check(lib.poly_rotary(a, stream), "poly_rotary")
+
+
+def _rotate(xs, inv_freq, positions, start, cu_seqlens, angles, interleaved, factor, inverse):
+    xs = [x if x.stride(-1) == 1 else x.contiguous() for x in xs]
+    outs = [_empty_like(x) for x in xs]
+    _launch(xs, outs, inv_freq, positions, start, cu_seqlens, angles, interleaved, factor, inverse)
+    return outs
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, args, *xs):
+        ctx.args = args
+        ctx.like = [(x.shape, x.dtype) for x in xs]
+        ctx.set_materialize_grads(False)
+        return tuple(_rotate(xs, *args, False))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *dys):
+        # the rotation's transpose: the same launch with sin negated
+        live = [i for i, g in enumerate(dys) if g is not None]
+        out = [None] * len(dys)
+        if live:
+            for i, g in zip(live, _rotate([dys[i].to(ctx.like[i][1]) for i in live], *ctx.args, True)):
+                out[i] = g
+        return (None, *out)
+
+
+# Under torch.compile the rotation is one opaque node with a shape function;
+# eager calls skip the dispatcher.
+@torch.library.custom_op("poly_b200::rotary", mutates_args=())
+def _rotary_op(xs: List[torch.Tensor], inv_freq: Optional[torch.Tensor], positions: Optional[torch.Tensor], start: int,
+               cu_seqlens: Optional[torch.Tensor], angles: Optional[torch.Tensor], interleaved: bool, factor: float,
+               inverse: bool) -> List[torch.Tensor]:
+    return _rotate(xs, inv_freq, positions, start, cu_seqlens, angles, interleaved, factor, inverse)
+
+
+@_rotary_op.register_fake
+def _(xs, inv_freq, positions, start, cu_seqlens, angles, interleaved, factor, inverse):
+    return [_empty_like(x) for x in xs]
+
+
+def _op_setup(ctx, inputs, output):
+    xs, inv_freq, positions, ctx.start, cu_seqlens, angles, ctx.interleaved, ctx.factor, ctx.inverse = inputs
+    ctx.save_for_backward(inv_freq, positions, cu_seqlens, angles)
+    ctx.shapes = [x.shape for x in xs]
+
+
+def _op_backward(ctx, grads):
+    inv_freq, positions, cu_seqlens, angles = ctx.saved_tensors
+    live = [i for i, g in enumerate(grads) if g is not None]
+    out = [None] * len(grads)
+    if live:
+        res = _rotary_op([grads[i] for i in live], inv_freq, positions, ctx.start, cu_seqlens, angles, ctx.interleaved,
+                         ctx.factor, not ctx.inverse)
+        for i, g in zip(live, res):
+            out[i] = g
+    return out, None, None, None, None, None, None, None, None
+
+
+_rotary_op.register_autograd(_op_backward, setup_context=_op_setup)
+
+
+def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None, interleaved=True, attention_factor=1.0):
+    """Rotate queries / keys by their positions; a tensor gives a tensor, a list a list.
+
+    xs: tensors [b, h, n, d] (any strides with a contiguous feature axis; heads
+    may differ) or packed [total, h, d], of one dtype, batch and length. The
+    first ``rot`` features are rotated, the rest copied.
+
+    The angles are ``position * inv_freq`` (fp32 [rot / 2]; the product is taken
+    in 64 bits, so far positions keep their angle) or ``angles`` (fp32 [n, rot / 2] or
+    [b, n, rot / 2]). ``positions`` is the first row's position (rows count up from
+    it), or an int32 / int64 tensor [n] or [b, n]; with ``cu_seqlens`` (int32 [s + 1],
+    packed sequences, batch 1) every sequence counts from 0. ``interleaved`` pairs
+    features (2i, 2i + 1), otherwise (i, i + rot / 2). ``attention_factor``
+    multiplies cos and sin. Gradients reach xs; frequencies and angles get none.
+    """
+    single = torch.is_tensor(xs)
+    xs = [xs] if single else list(xs)
+    if not xs:
+        return []
+    x0 = xs[0]
+    packed = x0.dim() == 3
+    if packed:
+        xs = [x.transpose(0, 1).unsqueeze(0) if x.dim() == 3 else x for x in xs]
+        x0 = xs[0]
+    if any(x.dim() != 4 for x in xs):
+        raise ValueError("apply_rotary takes tensors [b, h, n, d] or [total, h, d]")
+    b, _, n, d = x0.shape
+    _require_cuda(*xs, inv_freq, angles, cu_seqlens)
+    if x0.dtype not in _DTYPES or any(x.dtype != x0.dtype for x in xs):
+        raise TypeError(f"rotary tensors must share one of {list(_DTYPES)}; got {[x.dtype for x in xs]}")
+    if any((x.shape[0], x.shape[2], x.shape[3]) != (b, n, d) or x.device != x0.device for x in xs):
+        raise ValueError("rotary tensors must share batch, length, features and device")
+    if (inv_freq is None) == (angles is None):
+        raise ValueError("give either inv_freq or angles")
+    table = inv_freq if angles is None else angles
+    if table.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("rotary frequencies and angles have no gradient")
+    rot = 2 * table.shape[-1]
+    if rot == 0 or rot > d or d > 256:
+        raise ValueError(f"rotary features ({rot}) must be in [2, {d}] and the head at most 256")
+    if table.device != x0.device:
+        raise ValueError("rotary frequencies must be on the tensors' device")
+    start = 0
+    if angles is not None:
+        if cu_seqlens is not None or torch.is_tensor(positions) or positions != 0:
+            raise ValueError("angles already hold the positions")
+        angles = angles.float()
+        if angles.dim() == 2:
+            angles = angles.unsqueeze(0)
+        if angles.dim() != 3 or angles.shape[0] not in (1, b) or angles.shape[1] != n:
+            raise ValueError(f"angles must be [{n}, rot / 2] or [{b}, {n}, rot / 2], got {tuple(angles.shape)}")
+        if angles.stride(-1) != 1:
+            angles = angles.contiguous()
+        angles = angles.expand(b, -1, -1)
+        positions = None
+    else:
+        if inv_freq.dim() != 1:
+            raise ValueError("inv_freq must be [rot / 2]")
+        inv_freq = inv_freq.float().contiguous()
+        if cu_seqlens is not None:
+            if torch.is_tensor(positions) or positions != 0:
+                raise ValueError("positions and cu_seqlens exclude one another")
+            if b != 1 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2 or cu_seqlens.device != x0.device:
+                raise ValueError("cu_seqlens must be int32 [s + 1] on the tensors' device, with batch 1")
+            cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+            positions = None
+        elif torch.is_tensor(positions):
+            _require_cuda(positions)
+            if positions.dtype not in (torch.int32, torch.int64) or positions.device != x0.device:
+                raise TypeError("positions must be an int or an int32 / int64 tensor on the tensors' device")
+            if positions.dim() == 1:
+                positions = positions.unsqueeze(0)
+            if positions.dim() != 2 or positions.shape[0] not in (1, b) or positions.shape[1] != n:
+                raise ValueError(f"positions must be [{n}] or [{b}, {n}], got {tuple(positions.shape)}")
+            positions = positions.expand(b, -1)
+        else:
+            start, positions = int(positions), None
+    args = (inv_freq, positions, start, cu_seqlens, angles, bool(interleaved), float(attention_factor))
+    if x0.numel() == 0 and all(x.numel() == 0 for x in xs):
+        ys = [x.clone() for x in xs]
+    elif torch.compiler.is_compiling():
+        ys = _rotary_op(xs, *args, False)
+    elif torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        ys = _Rotary.apply(args, *xs)
+    else:
+        ys = _rotate(xs, *args, False)
+    if packed:
+        ys = [y.squeeze(0).transpose(0, 1) for y in ys]
+    return ys[0] if single else list(ys)
+
+
+class RotaryEmbedding(nn.Module):
+    """Rotary positions of one head size; ``freqs`` [dim / 2] is kept in fp32
+    whatever dtype the surrounding module is cast to (a frequency rounded to 16
+    bits is off by whole turns after a few hundred positions)."""
+
+    def __init__(self, dim, *, theta=10000.0, interleaved=True, scaling=None, factor=1.0, original_length=None):
+        super().__init__()
+        freqs, self.attention_factor = rotary_frequencies(dim, theta=theta, scaling=scaling, factor=factor,
+                                                          original_length=original_length)
+        self.freqs = nn.Parameter(freqs, requires_grad=False)
+        self.interleaved = interleaved
+
+    def _apply(self, fn, recurse=True):
+        keep = self.freqs.detach()
+        super()._apply(fn, recurse)
+        if self.freqs.dtype != torch.float32:
+            self.freqs = nn.Parameter(keep.float().to(self.freqs.device), requires_grad=False)
+        return self
+
+    def forward(self, xs, positions=0, cu_seqlens=None):
+        return apply_rotary(xs, self.freqs, positions=positions, cu_seqlens=cu_seqlens, interleaved=self.interleaved,
+                            attention_factor=self.attention_factor)
+
+    def rotate_queries_with_cached_keys(self, q, k):
+        """Queries are the last rows of the keys' sequence."""
+        if q.shape[-2] == k.shape[-2]:
+            return tuple(self([q, k]))
+        if q.shape[-2] > k.shape[-2]:
+            raise ValueError("more queries than keys")
+        return self(q, positions=k.shape[-2] - q.shape[-2]), self(k)
+
+
+__all__ = ["apply_rotary", "rotary_frequencies", "RotaryEmbedding"]
