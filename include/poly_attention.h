@@ -238,6 +238,46 @@ typedef struct {
 POLY_API int poly_head_rmsnorm(const PolyHeadNorm* norms, int n, void* stream);
 
 /*
+ * The pass over sequences packed end to end: pass.seq_q = pass.seq_k = the
+ * rows of all of them (pass.batch 1, batch strides ignored), sequence s is
+ * rows [cu_seqlens[s], cu_seqlens[s + 1]) and its queries see its own keys only
+ * (with causal, those at or before them). cu_seqlens is device memory: int32
+ * [seqs + 1], not decreasing, within [0, seq_q]; lengths may be 0, and rows
+ * outside every sequence are neither read into a result nor written. Offsets
+ * that break this give wrong rows, never an access outside the tensors.
+ * max_len: an upper bound of the lengths if the caller has one, else 0; rows
+ * of a longer sequence are then undefined. Up to 128 it selects kernels that hold a
+ * whole sequence per CTA. Bias, softclamp, grouped heads and the epilogue
+ * product as in poly_pass_fwd; masks, v_mul and causal_offset are
+ * POLY_EUNSUPPORTED. A row whose every key is dead (bias <= -FLT_MAX / 2) gets
+ * out = 0 and lse = -FLT_MAX, and no gradient.
+ */
+typedef struct PolyPackedArgs {
+  PolyPassArgs pass;
+  const int32_t* cu_seqlens;
+  int32_t seqs;
+  int32_t max_len;
+  int32_t zero_rest;
+  int32_t reserved;
+} PolyPackedArgs;
+
+typedef struct PolyPackedBwdArgs {
+  PolyPassBwdArgs bwd;
+  const int32_t* cu_seqlens;
+  int32_t seqs;
+  int32_t max_len;
+  int32_t zero_rest;
+  int32_t reserved;
+} PolyPackedBwdArgs;
+
+POLY_API int poly_packed_pass_fwd(const PolyPackedArgs* args, void* stream);
+POLY_API int poly_packed_pass_bwd(const PolyPackedBwdArgs* args, void* stream);
+POLY_API size_t poly_packed_pass_bwd_workspace_size(const PolyPackedBwdArgs* args);
+/* "small", "tc100", "tf32x3" or "simt" ("invalid" if validation fails) */
+POLY_API const char* poly_packed_pass_fwd_kernel_name(const PolyPackedArgs* args);
+POLY_API const char* poly_packed_pass_bwd_kernel_name(const PolyPackedBwdArgs* args);
+
+/*
  * Rotary positions of up to 8 query / key tensors in ONE launch. Over the
  * first rot features of a row, in pairs (a, b) = (2i, 2i + 1) (interleaved) or
  * (i, i + rot / 2):
@@ -334,6 +374,8 @@ POLY_API size_t poly_sizeof_pass_args(void);
 POLY_API size_t poly_sizeof_pass_bwd_args(void);
 POLY_API size_t poly_sizeof_merge_args(void);
 POLY_API size_t poly_sizeof_rotary_args(void);
+POLY_API size_t poly_sizeof_packed_args(void);
+POLY_API size_t poly_sizeof_packed_bwd_args(void);
 
 #ifdef __cplusplus
 }

@@ -88,4 +88,13 @@ int copy_rows(const PolyRowCopy* copies, int n, cudaStream_t s);
 int head_rmsnorm(const PolyHeadNorm* norms, int n, cudaStream_t s);
 int rotary(const PolyRotaryArgs* args, cudaStream_t s);
 
+// Sequences packed end to end (packed.cuh): device offsets, their number, rows in all.
+struct PackedSeqs {
+  const int* cu;
+  int seqs, total, max_len;
+};
+int launch_packed_fwd_simt(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s);
+int launch_packed_bwd_simt(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s);
+size_t packed_bwd_simt_workspace(const PolyPassBwdArgs& a);
+
 }  // namespace poly

@@ -1,0 +1,158 @@
+// Entry points of the passes over packed sequences: argument checks and kernel
+// choice. The kernels are the pass kernels of their own files, instantiated for
+// slots of packed sequences (packed.cuh).
+#include <string>
+
+#include "common.cuh"
+
+namespace poly {
+namespace {
+
+int fail(int code, const std::string& m) {
+  set_error(m);
+  return code;
+}
+
+// The checks of poly_pass_fwd that apply, then those of the packed layout.
+int check_packed(const PolyPassArgs& a, const int32_t* cu, int seqs, int max_len) {
+  if (a.batch != 1) return fail(POLY_EINVAL, "packed passes have batch 1");
+  if (a.heads <= 0 || a.kv_heads <= 0 || a.seq_q < 0 || a.head_dim <= 0)
+    return fail(POLY_EINVAL, "heads, kv_heads and head_dim must be positive, seq_q non-negative");
+  if (a.seq_q != a.seq_k) return fail(POLY_EINVAL, "packed passes have seq_q == seq_k (the rows of all sequences)");
+  if (a.heads % a.kv_heads != 0) return fail(POLY_EINVAL, "heads must be divisible by kv_heads");
+  if (a.dtype != POLY_F32 && a.dtype != POLY_F16 && a.dtype != POLY_BF16) return fail(POLY_EINVAL, "unknown dtype");
+  if (a.head_dim > 128) return fail(POLY_EUNSUPPORTED, "head_dim > 128 is not supported");
+  if (a.key_mask || a.query_mask || a.v_mul || a.causal_offset)
+    return fail(POLY_EUNSUPPORTED, "packed passes take no masks, v_mul or causal_offset");
+  if (seqs < 0 || max_len < 0) return fail(POLY_EINVAL, "seqs and max_len must be non-negative");
+  if (a.seq_q > 0 && seqs > 0 && (!a.q || !a.k || !a.v || !a.out || !cu))
+    return fail(POLY_EINVAL, "q, k, v, out and cu_seqlens are required");
+  if (a.epi_out && !a.epi_mul) return fail(POLY_EINVAL, "epi_out requires epi_mul");
+  if (!(a.scale == a.scale)) return fail(POLY_EINVAL, "scale is NaN");
+  // 16-row slots of every head fit the grid, rows the 32-bit tile arithmetic
+  if (a.seq_q > (1 << 30) || seqs > (1 << 28) || (int64_t)(a.seq_q / 8 + seqs) > 0x7fffffff / a.heads)
+    return fail(POLY_EUNSUPPORTED, "too many rows or sequences for one call");
+  return POLY_OK;
+}
+
+// Rows before the first and behind the last sequence of up to 5 outputs, as
+// zeros. Usually there are none: the CTAs read two offsets and leave.
+struct ZeroRest {
+  struct {
+    char* p;
+    int heads, row_bytes;
+    int64_t head_stride, row_stride;   // bytes
+  } t[5];
+  int n;
+};
+
+__global__ void __launch_bounds__(128) packed_zero_rest_kernel(const ZeroRest z, const int* cu, int seqs, int total) {
+  const int lo = min(max(cu[0], 0), total), hi = min(max(cu[seqs], lo), total);
+  const int rest = lo + (total - hi);
+  for (int r = blockIdx.x; r < rest; r += gridDim.x) {
+    const int64_t row = r < lo ? r : hi + (r - lo);
+    for (int k = 0; k < z.n; ++k) {
+      const int words = z.t[k].row_bytes >> 1;   // 16-bit words: rows need no more than their type's alignment
+      for (int i = threadIdx.x; i < z.t[k].heads * words; i += blockDim.x) {
+        const int h = i / words, w = i - h * words;
+        *reinterpret_cast<uint16_t*>(z.t[k].p + h * z.t[k].head_stride + row * z.t[k].row_stride + 2 * w) = 0;
+      }
+    }
+  }
+}
+
+void zero_add(ZeroRest& z, void* p, int heads, int dim, int es, int64_t head_stride, int64_t row_stride) {
+  if (!p) return;
+  auto& t = z.t[z.n++];
+  t.p = (char*)p;
+  t.heads = heads;
+  t.row_bytes = dim * es;
+  t.head_stride = head_stride * es;
+  t.row_stride = row_stride * es;
+}
+
+int zero_rest(const ZeroRest& z, const PackedSeqs& q, cudaStream_t s) {
+  packed_zero_rest_kernel<<<64, 128, 0, s>>>(z, q.cu, q.seqs, q.total);
+  note_launch(1);
+  return cuda_status(cudaGetLastError(), "packed_zero_rest launch");
+}
+
+int check_fwd(const PolyPackedArgs* a) {
+  if (!a) return fail(POLY_EINVAL, "null args");
+  return check_packed(a->pass, a->cu_seqlens, a->seqs, a->max_len);
+}
+
+int check_bwd(const PolyPackedBwdArgs* a) {
+  if (!a) return fail(POLY_EINVAL, "null args");
+  return check_packed(a->bwd.fwd, a->cu_seqlens, a->seqs, a->max_len);
+}
+
+}  // namespace
+}  // namespace poly
+
+using namespace poly;
+
+extern "C" {
+
+size_t poly_sizeof_packed_args(void) { return sizeof(PolyPackedArgs); }
+size_t poly_sizeof_packed_bwd_args(void) { return sizeof(PolyPackedBwdArgs); }
+
+const char* poly_packed_pass_fwd_kernel_name(const PolyPackedArgs* a) {
+  if (check_fwd(a) != POLY_OK) return "invalid";
+  return "simt";
+}
+
+const char* poly_packed_pass_bwd_kernel_name(const PolyPackedBwdArgs* a) {
+  if (check_bwd(a) != POLY_OK) return "invalid";
+  return "simt";
+}
+
+int poly_packed_pass_fwd(const PolyPackedArgs* a, void* stream) {
+  const int rc = check_fwd(a);
+  if (rc) return rc;
+  if (a->pass.seq_q == 0 || a->seqs == 0) return POLY_OK;
+  const PackedSeqs q{a->cu_seqlens, a->seqs, a->pass.seq_q, a->max_len};
+  if (a->zero_rest) {
+    const PolyPassArgs& f = a->pass;
+    const int es = f.dtype == POLY_F32 ? 4 : 2;
+    ZeroRest z{};
+    zero_add(z, f.out, f.heads, f.head_dim, es, f.out_stride[1], f.out_stride[2]);
+    zero_add(z, f.epi_out, f.heads, f.head_dim, es, f.epi_out_stride[1], f.epi_out_stride[2]);
+    zero_add(z, f.lse, f.heads, 1, 4, f.lse_stride[1], 1);
+    const int rz = zero_rest(z, q, (cudaStream_t)stream);
+    if (rz) return rz;
+  }
+  return launch_packed_fwd_simt(a->pass, q, (cudaStream_t)stream);
+}
+
+size_t poly_packed_pass_bwd_workspace_size(const PolyPackedBwdArgs* a) {
+  if (check_bwd(a) != POLY_OK) return 0;
+  return packed_bwd_simt_workspace(a->bwd);
+}
+
+int poly_packed_pass_bwd(const PolyPackedBwdArgs* a, void* stream) {
+  const int rc = check_bwd(a);
+  if (rc) return rc;
+  const PolyPassBwdArgs& b = a->bwd;
+  if (b.fwd.seq_q == 0 || a->seqs == 0) return POLY_OK;
+  if (!b.fwd.lse || !b.dout || !b.dq || !b.dk || !b.dv)
+    return fail(POLY_EINVAL, "backward needs fwd.out, fwd.lse, dout, dq, dk and dv");
+  const PackedSeqs q{a->cu_seqlens, a->seqs, b.fwd.seq_q, a->max_len};
+  const size_t need = poly_packed_pass_bwd_workspace_size(a);
+  if (need && (!b.workspace || b.workspace_bytes < need))
+    return fail(POLY_EINVAL, "workspace too small: need " + std::to_string(need) + " bytes");
+  if (a->zero_rest) {
+    const PolyPassArgs& f = b.fwd;
+    const int es = f.dtype == POLY_F32 ? 4 : 2;
+    ZeroRest z{};
+    if (!b.dq_accumulate) zero_add(z, b.dq, f.heads, f.head_dim, es, b.dq_stride[1], b.dq_stride[2]);
+    zero_add(z, b.dk, f.kv_heads, f.head_dim, es, b.dk_stride[1], b.dk_stride[2]);
+    zero_add(z, b.dv, f.kv_heads, f.head_dim, es, b.dv_stride[1], b.dv_stride[2]);
+    zero_add(z, b.dbias, f.kv_heads, 1, 4, b.dbias_stride[1], 1);
+    const int rz = zero_rest(z, q, (cudaStream_t)stream);
+    if (rz) return rz;
+  }
+  return launch_packed_bwd_simt(b, q, (cudaStream_t)stream);
+}
+
+}  // extern "C"

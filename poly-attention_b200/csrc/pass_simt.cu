@@ -7,7 +7,11 @@
 // (poly_attention/poly_attention.py:63-114): softclamp, causal triu(1), key
 // mask, query mask, then the additive per-key bias; a fully excluded row is the
 // uniform average over all keys (the -finfo.max masking of :68).
+//
+// PACKED: the rows of many sequences laid end to end; a CTA finds the 8 rows of
+// its slot (packed.cuh) and works on that sequence alone, from its first row.
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace poly {
 namespace {
@@ -49,8 +53,8 @@ __device__ __forceinline__ bool fallback_key(const PolyPassArgs& a, int i, int j
   return !(masked && dead);
 }
 
-template <typename T, int DMAX>
-__global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(const PolyPassArgs a) {
+template <typename T, int DMAX, bool PACKED>
+__global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(PolyPassArgs a, const PackedSeqs pk) {
   constexpr int NT = DMAX / 32;
   __shared__ float Ks[kTile][DMAX + 1];
   __shared__ float Vs[kTile][DMAX + 1];
@@ -58,16 +62,24 @@ __global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(const PolyPa
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const RowCtx c = bh_ctx(blockIdx.y, a.heads, a.kv_heads);
-  const int row0 = blockIdx.x * kWarps;
+  int row0 = blockIdx.x * kWarps;
+  int64_t first = 0;   // the sequence's first row
+  if constexpr (PACKED) {
+    PackedTile t;
+    if (!packed_tile<kWarps>(pk.cu, pk.seqs, pk.total, blockIdx.x, t)) return;
+    row0 = t.tile * kWarps;
+    first = t.start;
+    a.seq_q = a.seq_k = t.len;
+  }
   const int i = row0 + warp;
   const int d = a.head_dim;
   const bool row_ok = i < a.seq_q;
 
-  const T* q = (const T*)a.q + c.b * a.q_stride[0] + c.h * a.q_stride[1];
-  const T* k = (const T*)a.k + c.b * a.k_stride[0] + c.kvh * a.k_stride[1];
-  const T* v = (const T*)a.v + c.b * a.v_stride[0] + c.kvh * a.v_stride[1];
+  const T* q = (const T*)a.q + c.b * a.q_stride[0] + c.h * a.q_stride[1] + first * a.q_stride[2];
+  const T* k = (const T*)a.k + c.b * a.k_stride[0] + c.kvh * a.k_stride[1] + first * a.k_stride[2];
+  const T* v = (const T*)a.v + c.b * a.v_stride[0] + c.kvh * a.v_stride[1] + first * a.v_stride[2];
   const T* vmk = a.v_mul ? (const T*)a.v_mul + c.b * a.v_mul_stride[0] + c.kvh * a.v_mul_stride[1] : nullptr;
-  const float* bias = a.bias ? a.bias + c.b * a.bias_stride[0] + c.kvh * a.bias_stride[1] : nullptr;
+  const float* bias = a.bias ? a.bias + c.b * a.bias_stride[0] + c.kvh * a.bias_stride[1] + first : nullptr;
   const uint8_t* km = a.key_mask ? a.key_mask + c.b * a.key_mask_stride : nullptr;
   const bool q_masked = row_ok && a.query_mask && a.query_mask[c.b * a.query_mask_stride + i] == 0;
 
@@ -126,11 +138,12 @@ __global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(const PolyPa
   if (m == -INFINITY) {
     // Every entry excluded: the reference's -finfo.max fill makes the row a
     // uniform average over its keys, except keys that are both masked and
-    // dead (-max + -max overflows to -inf there).
+    // dead (-max + -max overflows to -inf there). Packed rows, which have no
+    // masks and no counterpart there, are zero.
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] = 0.f;
     int count = 0;
-    for (int j = 0; j < a.seq_k; ++j) {
+    for (int j = 0; j < (PACKED ? 0 : a.seq_k); ++j) {
       if (!fallback_key(a, i, j, q_masked, km, bias, a.seq_k)) continue;
       ++count;
 #pragma unroll
@@ -154,9 +167,10 @@ __global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(const PolyPa
     lse = m + logf(l);
   }
 
-  T* out = (T*)a.out + c.b * a.out_stride[0] + c.h * a.out_stride[1] + (int64_t)i * a.out_stride[2];
-  const T* vm = a.epi_out ? (const T*)a.epi_mul + c.b * a.epi_mul_stride[0] + c.h * a.epi_mul_stride[1] + (int64_t)i * a.epi_mul_stride[2] : nullptr;
-  T* vo = a.epi_out ? (T*)a.epi_out + c.b * a.epi_out_stride[0] + c.h * a.epi_out_stride[1] + (int64_t)i * a.epi_out_stride[2] : nullptr;
+  const int64_t io = first + i;
+  T* out = (T*)a.out + c.b * a.out_stride[0] + c.h * a.out_stride[1] + io * a.out_stride[2];
+  const T* vm = a.epi_out ? (const T*)a.epi_mul + c.b * a.epi_mul_stride[0] + c.h * a.epi_mul_stride[1] + io * a.epi_mul_stride[2] : nullptr;
+  T* vo = a.epi_out ? (T*)a.epi_out + c.b * a.epi_out_stride[0] + c.h * a.epi_out_stride[1] + io * a.epi_out_stride[2] : nullptr;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int col = lane + 32 * t;
@@ -166,17 +180,19 @@ __global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(const PolyPa
       if (vo) vo[col] = from_f32<T>(to_f32(vm[col]) * to_f32(o));
     }
   }
-  if (a.lse && lane == 0) a.lse[c.b * a.lse_stride[0] + c.h * a.lse_stride[1] + i] = lse;
+  if (a.lse && lane == 0) a.lse[c.b * a.lse_stride[0] + c.h * a.lse_stride[1] + io] = lse;
 }
 
 // delta_i = dout_i . out_i - dlse_i  (the row term of ds; dlse folds in the
 // log-sum-exp gradient, poly_attention/flash_poly_attention.py:280-284)
-template <typename T>
+// (rows of packed sequences are the rows of one batch element here)
+template <typename T, bool PACKED>
 __global__ void bwd_delta_kernel(const PolyPassBwdArgs a, float* delta, int* fb_count) {
-  const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-  const int rows = a.fwd.batch * a.fwd.heads * a.fwd.seq_q;
+  const int64_t warp = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)a.fwd.batch * a.fwd.heads * a.fwd.seq_q;
   if (warp >= rows) return;
-  const int i = warp % a.fwd.seq_q, bh = warp / a.fwd.seq_q;
+  const int i = (int)(warp % a.fwd.seq_q), bh = (int)(warp / a.fwd.seq_q);
   const int b = bh / a.fwd.heads, h = bh - b * a.fwd.heads;
   const T* o = (const T*)a.fwd.out + b * a.fwd.out_stride[0] + h * a.fwd.out_stride[1] + (int64_t)i * a.fwd.out_stride[2];
   const T* g = (const T*)a.dout + b * a.dout_stride[0] + h * a.dout_stride[1] + (int64_t)i * a.dout_stride[2];
@@ -185,7 +201,7 @@ __global__ void bwd_delta_kernel(const PolyPassBwdArgs a, float* delta, int* fb_
   s = warp_sum(s);
   const float lse_i = a.fwd.lse[b * a.fwd.lse_stride[0] + h * a.fwd.lse_stride[1] + i];
   int count = 0;
-  if (lse_i <= kDeadBias) {
+  if (!PACKED && lse_i <= kDeadBias) {
     const int kvh = h / (a.fwd.heads / a.fwd.kv_heads);
     const float* bias = a.fwd.bias ? a.fwd.bias + b * a.fwd.bias_stride[0] + kvh * a.fwd.bias_stride[1] : nullptr;
     const uint8_t* km = a.fwd.key_mask ? a.fwd.key_mask + b * a.fwd.key_mask_stride : nullptr;
@@ -239,32 +255,43 @@ __device__ __forceinline__ Entry bwd_entry(const PolyPassArgs& a, float dot, int
   return e;
 }
 
-template <typename T, int DMAX>
-__global__ void __launch_bounds__(kWarps * 32) pass_bwd_dq_simt_kernel(const PolyPassBwdArgs ab, const float* delta, const int* fb_count) {
+template <typename T, int DMAX, bool PACKED>
+__global__ void __launch_bounds__(kWarps * 32) pass_bwd_dq_simt_kernel(PolyPassBwdArgs ab, const float* delta, const int* fb_count, const PackedSeqs pk) {
   constexpr int NT = DMAX / 32;
-  const PolyPassArgs& a = ab.fwd;
+  PolyPassArgs& a = ab.fwd;
+  const int rows = a.seq_q;   // of a (batch, head) in delta and fb_count
   __shared__ float Ks[kTile][DMAX + 1];
   __shared__ float Vs[kTile][DMAX + 1];
   __shared__ float Qs[kWarps][DMAX];
   __shared__ float Gs[kWarps][DMAX];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const RowCtx c = bh_ctx(blockIdx.y, a.heads, a.kv_heads);
-  const int row0 = blockIdx.x * kWarps, i = row0 + warp, d = a.head_dim;
+  int row0 = blockIdx.x * kWarps;
+  const int d = a.head_dim;
+  int64_t first = 0;
+  if constexpr (PACKED) {
+    PackedTile t;
+    if (!packed_tile<kWarps>(pk.cu, pk.seqs, pk.total, blockIdx.x, t)) return;
+    row0 = t.tile * kWarps;
+    first = t.start;
+    a.seq_q = a.seq_k = t.len;
+  }
+  const int i = row0 + warp;
   const bool row_ok = i < a.seq_q;
-  const T* q = (const T*)a.q + c.b * a.q_stride[0] + c.h * a.q_stride[1];
-  const T* g = (const T*)ab.dout + c.b * ab.dout_stride[0] + c.h * ab.dout_stride[1];
-  const T* k = (const T*)a.k + c.b * a.k_stride[0] + c.kvh * a.k_stride[1];
-  const T* v = (const T*)a.v + c.b * a.v_stride[0] + c.kvh * a.v_stride[1];
-  const float* bias = a.bias ? a.bias + c.b * a.bias_stride[0] + c.kvh * a.bias_stride[1] : nullptr;
+  const T* q = (const T*)a.q + c.b * a.q_stride[0] + c.h * a.q_stride[1] + first * a.q_stride[2];
+  const T* g = (const T*)ab.dout + c.b * ab.dout_stride[0] + c.h * ab.dout_stride[1] + first * ab.dout_stride[2];
+  const T* k = (const T*)a.k + c.b * a.k_stride[0] + c.kvh * a.k_stride[1] + first * a.k_stride[2];
+  const T* v = (const T*)a.v + c.b * a.v_stride[0] + c.kvh * a.v_stride[1] + first * a.v_stride[2];
+  const float* bias = a.bias ? a.bias + c.b * a.bias_stride[0] + c.kvh * a.bias_stride[1] + first : nullptr;
   const uint8_t* km = a.key_mask ? a.key_mask + c.b * a.key_mask_stride : nullptr;
   const bool q_masked = row_ok && a.query_mask && a.query_mask[c.b * a.query_mask_stride + i] == 0;
   for (int t = lane; t < DMAX; t += 32) {
     Qs[warp][t] = (row_ok && t < d) ? to_f32(q[(int64_t)i * a.q_stride[2] + t]) : 0.f;
     Gs[warp][t] = (row_ok && t < d) ? to_f32(g[(int64_t)i * ab.dout_stride[2] + t]) : 0.f;
   }
-  const float lse_i = row_ok ? a.lse[c.b * a.lse_stride[0] + c.h * a.lse_stride[1] + i] : 0.f;
-  const float del = row_ok ? delta[((int64_t)blockIdx.y * a.seq_q) + i] : 0.f;
-  const int fbc = row_ok ? fb_count[((int64_t)blockIdx.y * a.seq_q) + i] : 0;
+  const float lse_i = row_ok ? a.lse[c.b * a.lse_stride[0] + c.h * a.lse_stride[1] + first + i] : 0.f;
+  const float del = row_ok ? delta[(int64_t)blockIdx.y * rows + first + i] : 0.f;
+  const int fbc = row_ok ? fb_count[(int64_t)blockIdx.y * rows + first + i] : 0;
   float acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = 0.f;
@@ -293,7 +320,7 @@ __global__ void __launch_bounds__(kWarps * 32) pass_bwd_dq_simt_kernel(const Pol
     }
   }
   if (!row_ok) return;
-  T* dq = (T*)ab.dq + c.b * ab.dq_stride[0] + c.h * ab.dq_stride[1] + (int64_t)i * ab.dq_stride[2];
+  T* dq = (T*)ab.dq + c.b * ab.dq_stride[0] + c.h * ab.dq_stride[1] + (first + i) * ab.dq_stride[2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int col = lane + 32 * t;
@@ -305,10 +332,11 @@ __global__ void __launch_bounds__(kWarps * 32) pass_bwd_dq_simt_kernel(const Pol
   }
 }
 
-template <typename T, int DMAX>
-__global__ void __launch_bounds__(kWarps * 32) pass_bwd_dkv_simt_kernel(const PolyPassBwdArgs ab, const float* delta, const int* fb_count) {
+template <typename T, int DMAX, bool PACKED>
+__global__ void __launch_bounds__(kWarps * 32) pass_bwd_dkv_simt_kernel(PolyPassBwdArgs ab, const float* delta, const int* fb_count, const PackedSeqs pk) {
   constexpr int NT = DMAX / 32;
-  const PolyPassArgs& a = ab.fwd;
+  PolyPassArgs& a = ab.fwd;
+  const int rows = a.seq_q;
   __shared__ float Qt[kTile][DMAX + 1];
   __shared__ float Gt[kTile][DMAX + 1];
   __shared__ float Kr[kWarps][DMAX];
@@ -319,11 +347,21 @@ __global__ void __launch_bounds__(kWarps * 32) pass_bwd_dkv_simt_kernel(const Po
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y - b * a.kv_heads;
   const int rep = a.heads / a.kv_heads;
-  const int row0 = blockIdx.x * kWarps, j = row0 + warp, d = a.head_dim;
+  int row0 = blockIdx.x * kWarps;
+  const int d = a.head_dim;
+  int64_t first = 0;
+  if constexpr (PACKED) {
+    PackedTile t;
+    if (!packed_tile<kWarps>(pk.cu, pk.seqs, pk.total, blockIdx.x, t)) return;
+    row0 = t.tile * kWarps;
+    first = t.start;
+    a.seq_q = a.seq_k = t.len;
+  }
+  const int j = row0 + warp;
   const bool row_ok = j < a.seq_k;
-  const T* k = (const T*)a.k + b * a.k_stride[0] + kvh * a.k_stride[1];
-  const T* v = (const T*)a.v + b * a.v_stride[0] + kvh * a.v_stride[1];
-  const float* bias = a.bias ? a.bias + b * a.bias_stride[0] + kvh * a.bias_stride[1] : nullptr;
+  const T* k = (const T*)a.k + b * a.k_stride[0] + kvh * a.k_stride[1] + first * a.k_stride[2];
+  const T* v = (const T*)a.v + b * a.v_stride[0] + kvh * a.v_stride[1] + first * a.v_stride[2];
+  const float* bias = a.bias ? a.bias + b * a.bias_stride[0] + kvh * a.bias_stride[1] + first : nullptr;
   const bool k_masked = row_ok && a.key_mask && a.key_mask[b * a.key_mask_stride + j] == 0;
   for (int t = lane; t < DMAX; t += 32) {
     Kr[warp][t] = (row_ok && t < d) ? to_f32(k[(int64_t)j * a.k_stride[2] + t]) : 0.f;
@@ -332,12 +370,12 @@ __global__ void __launch_bounds__(kWarps * 32) pass_bwd_dkv_simt_kernel(const Po
   float dk[NT], dv[NT], db = 0.f;
 #pragma unroll
   for (int t = 0; t < NT; ++t) dk[t] = dv[t] = 0.f;
-  const bool may_dead = a.key_mask || a.query_mask || a.bias;
+  const bool may_dead = !PACKED && (a.key_mask || a.query_mask || a.bias);
   const int istart = (a.causal && !may_dead) ? row0 : 0;
   for (int hr = 0; hr < rep; ++hr) {
     const int h = kvh * rep + hr;
-    const T* q = (const T*)a.q + b * a.q_stride[0] + h * a.q_stride[1];
-    const T* g = (const T*)ab.dout + b * ab.dout_stride[0] + h * ab.dout_stride[1];
+    const T* q = (const T*)a.q + b * a.q_stride[0] + h * a.q_stride[1] + first * a.q_stride[2];
+    const T* g = (const T*)ab.dout + b * ab.dout_stride[0] + h * ab.dout_stride[1] + first * ab.dout_stride[2];
     for (int i0 = istart; i0 < a.seq_q; i0 += kTile) {
       __syncthreads();
       load_tile<T, DMAX>(Qt, q, a.q_stride[2], i0, a.seq_q, d);
@@ -345,9 +383,9 @@ __global__ void __launch_bounds__(kWarps * 32) pass_bwd_dkv_simt_kernel(const Po
       if (threadIdx.x < kTile) {
         const int ii = i0 + threadIdx.x;
         const bool ok = ii < a.seq_q;
-        lse_t[threadIdx.x] = ok ? a.lse[b * a.lse_stride[0] + h * a.lse_stride[1] + ii] : 0.f;
-        del_t[threadIdx.x] = ok ? delta[((int64_t)(b * a.heads + h) * a.seq_q) + ii] : 0.f;
-        fb_t[threadIdx.x] = ok ? fb_count[((int64_t)(b * a.heads + h) * a.seq_q) + ii] : 0;
+        lse_t[threadIdx.x] = ok ? a.lse[b * a.lse_stride[0] + h * a.lse_stride[1] + first + ii] : 0.f;
+        del_t[threadIdx.x] = ok ? delta[(int64_t)(b * a.heads + h) * rows + first + ii] : 0.f;
+        fb_t[threadIdx.x] = ok ? fb_count[(int64_t)(b * a.heads + h) * rows + first + ii] : 0;
         qm_t[threadIdx.x] = (ok && a.query_mask) ? (a.query_mask[b * a.query_mask_stride + ii] == 0) : 0;
       }
       __syncthreads();
@@ -377,8 +415,8 @@ __global__ void __launch_bounds__(kWarps * 32) pass_bwd_dkv_simt_kernel(const Po
   }
   if (!row_ok) return;
   db = warp_sum(db);
-  T* dkp = (T*)ab.dk + b * ab.dk_stride[0] + kvh * ab.dk_stride[1] + (int64_t)j * ab.dk_stride[2];
-  T* dvp = (T*)ab.dv + b * ab.dv_stride[0] + kvh * ab.dv_stride[1] + (int64_t)j * ab.dv_stride[2];
+  T* dkp = (T*)ab.dk + b * ab.dk_stride[0] + kvh * ab.dk_stride[1] + (first + j) * ab.dk_stride[2];
+  T* dvp = (T*)ab.dv + b * ab.dv_stride[0] + kvh * ab.dv_stride[1] + (first + j) * ab.dv_stride[2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int col = lane + 32 * t;
@@ -387,61 +425,86 @@ __global__ void __launch_bounds__(kWarps * 32) pass_bwd_dkv_simt_kernel(const Po
       dvp[col] = from_f32<T>(dv[t]);
     }
   }
-  if (ab.dbias && lane == 0) ab.dbias[b * ab.dbias_stride[0] + kvh * ab.dbias_stride[1] + j] = db;
+  if (ab.dbias && lane == 0) ab.dbias[b * ab.dbias_stride[0] + kvh * ab.dbias_stride[1] + first + j] = db;
+}
+
+// CTAs along the rows: one per 8 rows, or one per slot of the packed sequences
+unsigned row_ctas(int rows, const PackedSeqs* pk) {
+  return pk ? (unsigned)(rows / kWarps + pk->seqs) : (unsigned)((rows + kWarps - 1) / kWarps);
 }
 
 template <typename T, int DMAX>
-int launch_fwd_t(const PolyPassArgs& a, cudaStream_t s) {
-  dim3 grid((a.seq_q + kWarps - 1) / kWarps, a.batch * a.heads);
-  pass_fwd_simt_kernel<T, DMAX><<<grid, kWarps * 32, 0, s>>>(a);
+int launch_fwd_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
+  dim3 grid(row_ctas(a.seq_q, pk), a.batch * a.heads);
+  if (pk)
+    pass_fwd_simt_kernel<T, DMAX, true><<<grid, kWarps * 32, 0, s>>>(a, *pk);
+  else
+    pass_fwd_simt_kernel<T, DMAX, false><<<grid, kWarps * 32, 0, s>>>(a, PackedSeqs{});
   note_launch(1);
   return cuda_status(cudaGetLastError(), "pass_fwd_simt launch");
 }
 
 template <typename T, int DMAX>
-int launch_bwd_t(const PolyPassBwdArgs& a, cudaStream_t s) {
-  const int rows = a.fwd.batch * a.fwd.heads * a.fwd.seq_q;
+int launch_bwd_t(const PolyPassBwdArgs& a, const PackedSeqs* pk, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.fwd.batch * a.fwd.heads * a.fwd.seq_q;
   float* delta = (float*)a.workspace;
   int* fb_count = (int*)(delta + rows);
-  bwd_delta_kernel<T><<<(rows + 7) / 8, 256, 0, s>>>(a, delta, fb_count);
-  dim3 gq((a.fwd.seq_q + kWarps - 1) / kWarps, a.fwd.batch * a.fwd.heads);
-  pass_bwd_dq_simt_kernel<T, DMAX><<<gq, kWarps * 32, 0, s>>>(a, delta, fb_count);
-  dim3 gk((a.fwd.seq_k + kWarps - 1) / kWarps, a.fwd.batch * a.fwd.kv_heads);
-  pass_bwd_dkv_simt_kernel<T, DMAX><<<gk, kWarps * 32, 0, s>>>(a, delta, fb_count);
+  dim3 gq(row_ctas(a.fwd.seq_q, pk), a.fwd.batch * a.fwd.heads);
+  dim3 gk(row_ctas(a.fwd.seq_k, pk), a.fwd.batch * a.fwd.kv_heads);
+  const unsigned gd = (unsigned)((rows + 7) / 8);
+  if (pk) {
+    bwd_delta_kernel<T, true><<<gd, 256, 0, s>>>(a, delta, fb_count);
+    pass_bwd_dq_simt_kernel<T, DMAX, true><<<gq, kWarps * 32, 0, s>>>(a, delta, fb_count, *pk);
+    pass_bwd_dkv_simt_kernel<T, DMAX, true><<<gk, kWarps * 32, 0, s>>>(a, delta, fb_count, *pk);
+  } else {
+    bwd_delta_kernel<T, false><<<gd, 256, 0, s>>>(a, delta, fb_count);
+    pass_bwd_dq_simt_kernel<T, DMAX, false><<<gq, kWarps * 32, 0, s>>>(a, delta, fb_count, PackedSeqs{});
+    pass_bwd_dkv_simt_kernel<T, DMAX, false><<<gk, kWarps * 32, 0, s>>>(a, delta, fb_count, PackedSeqs{});
+  }
   note_launch(3);
   return cuda_status(cudaGetLastError(), "pass_bwd_simt launch");
 }
 
 template <int DMAX>
-int fwd_by_dtype(const PolyPassArgs& a, cudaStream_t s) {
+int fwd_by_dtype(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   switch (a.dtype) {
-    case POLY_F32: return launch_fwd_t<float, DMAX>(a, s);
-    case POLY_F16: return launch_fwd_t<__half, DMAX>(a, s);
-    default: return launch_fwd_t<__nv_bfloat16, DMAX>(a, s);
+    case POLY_F32: return launch_fwd_t<float, DMAX>(a, pk, s);
+    case POLY_F16: return launch_fwd_t<__half, DMAX>(a, pk, s);
+    default: return launch_fwd_t<__nv_bfloat16, DMAX>(a, pk, s);
   }
 }
 
 template <int DMAX>
-int bwd_by_dtype(const PolyPassBwdArgs& a, cudaStream_t s) {
+int bwd_by_dtype(const PolyPassBwdArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   switch (a.fwd.dtype) {
-    case POLY_F32: return launch_bwd_t<float, DMAX>(a, s);
-    case POLY_F16: return launch_bwd_t<__half, DMAX>(a, s);
-    default: return launch_bwd_t<__nv_bfloat16, DMAX>(a, s);
+    case POLY_F32: return launch_bwd_t<float, DMAX>(a, pk, s);
+    case POLY_F16: return launch_bwd_t<__half, DMAX>(a, pk, s);
+    default: return launch_bwd_t<__nv_bfloat16, DMAX>(a, pk, s);
   }
+}
+
+int fwd_by_dim(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
+  if (a.head_dim <= 32) return fwd_by_dtype<32>(a, pk, s);
+  if (a.head_dim <= 64) return fwd_by_dtype<64>(a, pk, s);
+  return fwd_by_dtype<128>(a, pk, s);
+}
+
+int bwd_by_dim(const PolyPassBwdArgs& a, const PackedSeqs* pk, cudaStream_t s) {
+  if (a.fwd.head_dim <= 32) return bwd_by_dtype<32>(a, pk, s);
+  if (a.fwd.head_dim <= 64) return bwd_by_dtype<64>(a, pk, s);
+  return bwd_by_dtype<128>(a, pk, s);
 }
 
 }  // namespace
 
-int launch_pass_fwd_simt(const PolyPassArgs& a, cudaStream_t s) {
-  if (a.head_dim <= 32) return fwd_by_dtype<32>(a, s);
-  if (a.head_dim <= 64) return fwd_by_dtype<64>(a, s);
-  return fwd_by_dtype<128>(a, s);
+int launch_pass_fwd_simt(const PolyPassArgs& a, cudaStream_t s) { return fwd_by_dim(a, nullptr, s); }
+int launch_pass_bwd_simt(const PolyPassBwdArgs& a, cudaStream_t s) { return bwd_by_dim(a, nullptr, s); }
+int launch_packed_fwd_simt(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s) { return fwd_by_dim(a, &q, s); }
+int launch_packed_bwd_simt(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s) {
+  return bwd_by_dim(a, &q, s);
 }
-
-int launch_pass_bwd_simt(const PolyPassBwdArgs& a, cudaStream_t s) {
-  if (a.fwd.head_dim <= 32) return bwd_by_dtype<32>(a, s);
-  if (a.fwd.head_dim <= 64) return bwd_by_dtype<64>(a, s);
-  return bwd_by_dtype<128>(a, s);
+size_t packed_bwd_simt_workspace(const PolyPassBwdArgs& a) {
+  return (size_t)a.fwd.heads * (size_t)a.fwd.seq_q * (sizeof(float) + sizeof(int));
 }
 
 }  // namespace poly

@@ -80,6 +80,16 @@ class PolyHeadNorm(ctypes.Structure):
 MAX_NORMS = 4
 
 
+class PolyPackedArgs(ctypes.Structure):
+    _fields_ = [("fwd", PolyPassArgs), ("cu_seqlens", c_vp), ("seqs", c_i32), ("max_len", c_i32),
+                ("zero_rest", c_i32), ("reserved", c_i32)]
+
+
+class PolyPackedBwdArgs(ctypes.Structure):
+    _fields_ = [("bwd", PolyPassBwdArgs), ("cu_seqlens", c_vp), ("seqs", c_i32), ("max_len", c_i32),
+                ("zero_rest", c_i32), ("reserved", c_i32)]
+
+
 class PolyRotaryTensor(ctypes.Structure):
     _fields_ = [("src", c_vp), ("dst", c_vp), ("heads", c_i32), ("reserved", c_i32),
                 ("src_stride", I64x3), ("dst_stride", I64x3)]
@@ -108,6 +118,11 @@ EXPORTS = {
     "poly_decode_chain": (ctypes.c_int, [ctypes.POINTER(PolyPassArgs), ctypes.c_int, c_vp]),
     "poly_copy_rows": (ctypes.c_int, [ctypes.POINTER(PolyRowCopy), ctypes.c_int, c_vp]),
     "poly_head_rmsnorm": (ctypes.c_int, [ctypes.POINTER(PolyHeadNorm), ctypes.c_int, c_vp]),
+    "poly_packed_pass_fwd": (ctypes.c_int, [ctypes.POINTER(PolyPackedArgs), c_vp]),
+    "poly_packed_pass_bwd": (ctypes.c_int, [ctypes.POINTER(PolyPackedBwdArgs), c_vp]),
+    "poly_packed_pass_bwd_workspace_size": (c_sz, [ctypes.POINTER(PolyPackedBwdArgs)]),
+    "poly_packed_pass_fwd_kernel_name": (ctypes.c_char_p, [ctypes.POINTER(PolyPackedArgs)]),
+    "poly_packed_pass_bwd_kernel_name": (ctypes.c_char_p, [ctypes.POINTER(PolyPackedBwdArgs)]),
     "poly_rotary": (ctypes.c_int, [ctypes.POINTER(PolyRotaryArgs), c_vp]),
     "poly_pass_bwd_noalloc": (ctypes.c_int, [ctypes.POINTER(PolyPassBwdArgs), c_vp]),
     "poly_noalloc_scratch_bytes": (c_sz, []),
@@ -122,6 +137,8 @@ EXPORTS = {
     "poly_sizeof_pass_bwd_args": (c_sz, []),
     "poly_sizeof_merge_args": (c_sz, []),
     "poly_sizeof_rotary_args": (c_sz, []),
+    "poly_sizeof_packed_args": (c_sz, []),
+    "poly_sizeof_packed_bwd_args": (c_sz, []),
 }
 
 
@@ -137,7 +154,8 @@ def _load():
     if lib.poly_abi_version() != ABI_VERSION:
         raise ImportError("libpolyattn.so ABI version mismatch")
     for fn, st in (("poly_sizeof_pass_args", PolyPassArgs), ("poly_sizeof_pass_bwd_args", PolyPassBwdArgs),
-                   ("poly_sizeof_merge_args", PolyMergeArgs), ("poly_sizeof_rotary_args", PolyRotaryArgs)):
+                   ("poly_sizeof_merge_args", PolyMergeArgs), ("poly_sizeof_rotary_args", PolyRotaryArgs),
+                   ("poly_sizeof_packed_args", PolyPackedArgs), ("poly_sizeof_packed_bwd_args", PolyPackedBwdArgs)):
         if getattr(lib, fn)() != ctypes.sizeof(st):
             raise ImportError(f"libpolyattn.so struct layout mismatch ({st.__name__})")
     return lib

@@ -14,7 +14,9 @@ from torch.nn import Module, RMSNorm
 from .core import poly_attention_chain, poly_attention_chain_cached
 from .head_norm import head_rmsnorm
 from .kv_cache import ModuleKVCache, usable as _inplace_usable
-from .poly_attention import cast_tuple, default, exists, merge_heads, rotate_by_angles, split_heads
+from .packed import poly_attention_chain_packed
+from .poly_attention import (cast_tuple, check_packed, default, exists, merge_heads, rotate_by_angles, split_heads,
+                             token_rows)
 from .rotary import RotaryEmbedding
 
 LinearNoBias = partial(nn.Linear, bias=False)
@@ -78,8 +80,11 @@ class NPolyAttention(Module):
 
     def forward(self, x, context: Tensor | tuple[Tensor, ...] | None = None, mask=None,
                 context_mask: Tensor | tuple[Tensor | None, ...] | None = None, rotary_pos_emb=None, cache=None,
-                return_cache=False):
+                return_cache=False, cu_seqlens=None, max_seqlen=None):
         order = self.order
+        if exists(cu_seqlens):
+            # sequences laid end to end in one row [1, total, dim]; each attends itself alone
+            check_packed(x, context, mask, context_mask, cache, return_cache)
         seq_len = x.shape[-2]
         has_cache = exists(cache)
         if has_cache:
@@ -155,12 +160,19 @@ class NPolyAttention(Module):
         if not exists(rotary_pos_emb) and exists(self.rotary_emb):
             if not has_cache and len({q.shape[-2] for q in qs}) == 1:
                 # every row at its own position: a tensor turns the same way as keys and as queries
-                qs = self.rotary_emb(list(qs))
+                qs = self.rotary_emb(list(qs), cu_seqlens=cu_seqlens)
                 q_left, q_right = list(qs[:-1]), list(qs[1:])
             else:
                 rot = [self.rotary_emb.rotate_queries_with_cached_keys(ql, qr) for ql, qr in zip(q_left, q_right)]
                 q_left, q_right = (list(t) for t in zip(*rot))
 
+        if exists(cu_seqlens):
+            keys = [token_rows(q) for q in q_right]
+            # below the first level the queries are the keys of the level above
+            out = poly_attention_chain_packed([token_rows(q_left[0]), *keys[:-1]], keys, [token_rows(v) for v in vs],
+                                              cu_seqlens, softclamp_value=self.softclamp_value, causal=self.causal,
+                                              max_seqlen=max_seqlen)[0]
+            return self._finish(out.transpose(0, 1).unsqueeze(0), root_value, gates)
         if has_cache:
             out, lse_steps, msg_steps = poly_attention_chain_cached(
                 q_left, q_right, list(vs_cache), [self._squeeze(t) for t in c_lses],

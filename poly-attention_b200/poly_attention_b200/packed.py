@@ -1,0 +1,266 @@
+"""Poly attention over sequences of different lengths packed end to end.
+
+Tensors are [total, heads, d] (tokens of all sequences, no batch axis) and
+``cu_seqlens`` (int32 [s + 1] on the device) holds each sequence's first row and
+the row behind the last. A sequence's tokens attend that sequence alone, so the
+result of each is that of ``poly_attention_order2`` / ``poly_attention_chain`` on
+it by itself (poly_attention/poly_attention.py:48-116,
+n_poly_attention.py:263-313), without the padding that a [b, n, ...] batch of
+unequal lengths needs. Rows outside every sequence come out as zeros and get
+zero gradients.
+
+The offsets stay on the device and are not checked there: they must not
+decrease and must lie in [0, total] (others give wrong rows, never an access
+outside the tensors). ``max_seqlen`` is an upper bound of the lengths, if the
+caller has one: up to 128 it selects kernels that hold a whole sequence per CTA.
+"""
+from __future__ import annotations
+
+import torch
+
+from ._lib import PolyPackedArgs, PolyPackedBwdArgs, check, lib
+from .core import _autocast, _sc
+from .ops import _DTYPES, _require_cuda, _stream
+
+
+def packed_offsets(lengths, device="cuda"):
+    """(cu_seqlens, max_seqlen) of a list of sequence lengths."""
+    lengths = [int(n) for n in lengths]
+    if any(n < 0 for n in lengths):
+        raise ValueError("sequence lengths must be non-negative")
+    cu = [0]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    return torch.tensor(cu, dtype=torch.int32).to(device), max(lengths, default=0)
+
+
+def _offsets(cu_seqlens, like):
+    _require_cuda(cu_seqlens)
+    if (cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64)
+            or cu_seqlens.device != like.device):
+        raise ValueError("cu_seqlens must be an int32 / int64 tensor [s + 1] on the tensors' device")
+    return cu_seqlens.to(torch.int32).contiguous()
+
+
+def _tensors(q, k, v, *same):
+    _require_cuda(q, k, v, *same)
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k, v must share one of {list(_DTYPES)}; got {q.dtype}, {k.dtype}, {v.dtype}")
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[::2] != k.shape[::2]:
+        raise ValueError(f"packed tensors are q [total, h, d] and k, v [total, g, d]; got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    for t in (k, v, *same):
+        if t is not None and t.device != q.device:
+            raise ValueError("packed tensors must be on one device")
+
+
+def _rows(t):
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _set(a, name, t):
+    """A [total, heads, d] tensor (or [heads, total] fp32 vector) into its pointer and (batch, head, row) strides."""
+    setattr(a, name, t.data_ptr())
+    st = getattr(a, name + "_stride")
+    if t.dim() == 3:
+        st[0], st[1], st[2] = 0, t.stride(1), t.stride(0)
+    else:
+        st[0], st[1] = 0, t.stride(0)
+
+
+def _vec(t, heads, total, what):
+    if t.shape != (heads, total):
+        raise ValueError(f"{what} must be [{heads}, {total}], got {tuple(t.shape)}")
+    return _rows(t.float())
+
+
+def _fill(a, q, k, v, bias, causal, softclamp, scale):
+    a.batch, a.heads, a.kv_heads, a.head_dim = 1, q.shape[1], k.shape[1], q.shape[2]
+    a.seq_q = a.seq_k = q.shape[0]
+    a.dtype, a.causal = _DTYPES[q.dtype], int(bool(causal))
+    a.scale = float(q.shape[2] ** -0.5 if scale is None else scale)
+    a.softclamp = _sc(softclamp)
+    _set(a, "q", q)
+    _set(a, "k", k)
+    _set(a, "v", v)
+    if bias is not None:
+        _set(a, "bias", bias)
+
+
+@torch.compiler.disable   # library calls through ctypes: dynamo runs them eagerly
+def pass_fwd_packed(q, k, v, cu_seqlens, *, causal=False, softclamp=None, scale=None, bias=None, epi_mul=None,
+                    max_seqlen=None):
+    """One attention pass over packed sequences (see PolyPackedArgs in include/poly_attention.h).
+
+    q [total, h, d]; k, v [total, g, d] with g | h; bias [g, total] fp32; epi_mul
+    [total, h, d]. Returns (out, lse[, epi_mul * out]) with out like q and lse fp32 [h, total].
+    """
+    _tensors(q, k, v, bias, epi_mul)
+    cu = _offsets(cu_seqlens, q)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    total, h, d = q.shape
+    a = PolyPackedArgs()
+    if bias is not None:
+        bias = _vec(bias, k.shape[1], total, "bias")
+    if h % max(k.shape[1], 1):
+        raise ValueError("heads must be divisible by kv_heads")
+    _fill(a.fwd, q, k, v, bias, causal, softclamp, scale)
+    out = q.new_empty(total, h, d)
+    lse = q.new_empty(h, total, dtype=torch.float32)
+    _set(a.fwd, "out", out)
+    _set(a.fwd, "lse", lse)
+    epi = None
+    if epi_mul is not None:
+        if epi_mul.shape != q.shape or epi_mul.dtype != q.dtype:
+            raise ValueError("epi_mul must have q's shape and dtype")
+        epi_mul, epi = _rows(epi_mul), torch.empty_like(out)
+        _set(a.fwd, "epi_mul", epi_mul)
+        _set(a.fwd, "epi_out", epi)
+    a.cu_seqlens, a.seqs, a.max_len, a.zero_rest = cu.data_ptr(), cu.shape[0] - 1, int(max_seqlen or 0), 1
+    if a.seqs == 0 and total:
+        out.zero_(), lse.zero_()
+        if epi is not None:
+            epi.zero_()
+    with torch.cuda.device(q.device):
+        check(lib.poly_packed_pass_fwd(a, _stream(q.device)), "poly_packed_pass_fwd")
+    return (out, lse) if epi is None else (out, lse, epi)
+
+
+@torch.compiler.disable
+def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softclamp=None, scale=None, bias=None,
+                    dlse=None, dq=None, want_dbias=False, max_seqlen=None):
+    """Backward of ``pass_fwd_packed``. Returns (dq, dk, dv, dbias-or-None). With ``dq`` given the
+    query gradient is added to it in place."""
+    _tensors(q, k, v, out, lse, dout, bias, dlse, dq)
+    cu = _offsets(cu_seqlens, q)
+    q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout.to(q.dtype))
+    total, h, d = q.shape
+    g = k.shape[1]
+    if h % max(g, 1):
+        raise ValueError("heads must be divisible by kv_heads")
+    if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out and dout must have q's shape, out its dtype")
+    if any(st <= 0 for st in dout.stride()):
+        dout = dout.contiguous()        # broadcast gradients (out.sum().backward())
+    if dq is not None and (dq.shape != q.shape or dq.dtype != q.dtype or dq.stride(-1) != 1):
+        raise ValueError("dq must have q's shape and dtype and a contiguous last dim")
+    lse = _vec(lse, h, total, "lse")
+    a = PolyPackedBwdArgs()
+    b = a.bwd
+    if bias is not None:
+        bias = _vec(bias, g, total, "bias")
+    _fill(b.fwd, q, k, v, bias, causal, softclamp, scale)
+    _set(b.fwd, "out", out)
+    _set(b.fwd, "lse", lse)
+    _set(b, "dout", dout)
+    if dlse is not None:
+        dlse = _vec(dlse, h, total, "dlse")
+        _set(b, "dlse", dlse)
+    b.dq_accumulate = int(dq is not None)
+    if dq is None:
+        dq = q.new_empty(total, h, d)
+    dk, dv = k.new_empty(total, g, d), v.new_empty(total, g, d)
+    dbias = q.new_empty(g, total, dtype=torch.float32) if want_dbias else None
+    _set(b, "dq", dq)
+    _set(b, "dk", dk)
+    _set(b, "dv", dv)
+    if want_dbias:
+        _set(b, "dbias", dbias)
+    a.cu_seqlens, a.seqs, a.max_len, a.zero_rest = cu.data_ptr(), cu.shape[0] - 1, int(max_seqlen or 0), 1
+    if a.seqs == 0 and total:
+        for t in (dk, dv, dbias, None if b.dq_accumulate else dq):
+            if t is not None:
+                t.zero_()
+    with torch.cuda.device(q.device):
+        need = lib.poly_packed_pass_bwd_workspace_size(a)
+        ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+        if need:
+            b.workspace, b.workspace_bytes = ws.data_ptr(), need
+        check(lib.poly_packed_pass_bwd(a, _stream(q.device)), "poly_packed_pass_bwd")
+    return dq, dk, dv, dbias
+
+
+class _PackedChain(torch.autograd.Function):
+    """The order-n chain. Inputs: order queries ql, order keys qr and order - 1 values; shared[t] says
+    that ql[t] is qr[t - 1], whose two gradients are then summed inside the kernel."""
+
+    @staticmethod
+    def forward(ctx, order, shared, cu, opts, *tensors):
+        ql, qr, vs = tensors[:order], tensors[order:2 * order], tensors[2 * order:]
+        vals, biases, msgs, lses = [None] * order, [None] * order, [None] * order, [None] * order
+        val, bias = vs[-1], None
+        for t in range(order - 1, -1, -1):
+            vals[t], biases[t] = val, bias
+            # V' = v * msg is written by the pass that makes msg (n_poly_attention.py:287)
+            res = pass_fwd_packed(ql[t], qr[t], val, cu, bias=bias, epi_mul=vs[t - 2] if t >= 2 else None, **opts)
+            msgs[t], lses[t] = res[:2]
+            val, bias = res[-1] if t >= 2 else msgs[t], lses[t]
+        ctx.order, ctx.shared, ctx.opts = order, shared, opts
+        ctx.has = [b is not None for b in biases]
+        ctx.save_for_backward(cu, *tensors, *vals, *msgs, *lses, *[b for b in biases if b is not None])
+        extra = (*lses[:0:-1], *msgs[:0:-1])        # level order - 1 first, as in the caches
+        ctx.mark_non_differentiable(*extra)
+        return (msgs[0], *extra)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, *_unused):
+        n, saved = ctx.order, list(ctx.saved_tensors)
+        take = lambda k: [saved.pop(0) for _ in range(k)]   # noqa: E731
+        cu, = take(1)
+        ql, qr, vs, vals, msgs, lses = take(n), take(n), take(n - 1), take(n), take(n), take(n)
+        biases = [saved.pop(0) if has else None for has in ctx.has]
+        dql, dqr, dvs = [None] * n, [None] * n, [None] * (n - 1)
+        g_out, g_lse = dout, None
+        for t in range(n):
+            # a key tensor that is the next level's query keeps one gradient: the second part is added in the
+            # kernel to the first, which was rounded once to the tensors' type
+            dq, dqr[t], dv, g_lse = pass_bwd_packed(ql[t], qr[t], vals[t], cu, msgs[t], lses[t], g_out, bias=biases[t],
+                                                    dlse=g_lse, dq=dqr[t - 1] if ctx.shared[t] else None,
+                                                    want_dbias=t < n - 1, **ctx.opts)
+            if not ctx.shared[t]:
+                dql[t] = dq
+            if t == n - 1:
+                dvs[-1] = dv
+            elif t == 0:
+                g_out = dv
+            else:
+                dvs[t - 1] = dv * msgs[t + 1]
+                g_out = dv * vs[t - 1]
+        return (None, None, None, None, *dql, *dqr, *dvs)
+
+
+@torch.compiler.disable
+def poly_attention_chain_packed(q_left, q_right, vs, cu_seqlens, *, softclamp_value=None, causal=False, max_seqlen=None):
+    """Order-n chain over packed sequences (n = len(q_left)), as ``poly_attention_chain``.
+
+    q_left[0] = q1 [total, h, d]; q_left[t >= 1], q_right[t] and vs[t] are [total, g, d]. Returns
+    (out [total, h, d], lses [g, total], msgs [total, g, d]), lses / msgs in the caches' order.
+    """
+    order = len(q_left)
+    if order < 2 or len(q_right) != order or len(vs) != order - 1:
+        raise ValueError("a chain of order n >= 2 takes n queries, n keys and n - 1 values")
+    shared = tuple(t >= 1 and q_left[t] is q_right[t - 1] for t in range(order))
+    ql, qr, vv = list(_autocast(*q_left)), list(_autocast(*q_right)), list(_autocast(*vs))
+    ql = [qr[t - 1] if shared[t] else ql[t] for t in range(order)]
+    for t in range(order):
+        _tensors(ql[t], qr[t], vv[t - 1 if t else 0])
+        if t and ql[t].shape != qr[t].shape:
+            raise ValueError("levels below the last have as many query as key heads")
+    cu = _offsets(cu_seqlens, ql[0])
+    opts = dict(causal=bool(causal), softclamp=softclamp_value, max_seqlen=max_seqlen)
+    res = _PackedChain.apply(order, shared, cu, opts, *ql, *qr, *vv)
+    return res[0], res[1:order], res[order:]
+
+
+def poly_attention_order2_packed(q1, q2, q3, v3, cu_seqlens, *, q2_pass1=None, softclamp_value=None, causal=False,
+                                 max_seqlen=None):
+    """Order-2 poly attention over packed sequences, as ``poly_attention_order2``: q1 [total, h, d];
+    q2, q3, v3 [total, g, d]. Returns (out, lse23 [g, total], msg [total, g, d])."""
+    out, lses, msgs = poly_attention_chain_packed([q1, q2 if q2_pass1 is None else q2_pass1], [q2, q3], [v3], cu_seqlens,
+                                                  softclamp_value=softclamp_value, causal=causal, max_seqlen=max_seqlen)
+    return out, lses[0], msgs[0]
+
+
+__all__ = ["packed_offsets", "pass_fwd_packed", "pass_bwd_packed", "poly_attention_order2_packed",
+           "poly_attention_chain_packed"]

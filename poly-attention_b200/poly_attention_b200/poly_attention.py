@@ -15,6 +15,7 @@ from torch.nn import Module, RMSNorm
 from .core import poly_attention_order2, poly_attention_order2_cached
 from .head_norm import head_rmsnorm
 from .kv_cache import ModuleKVCache, usable as _inplace_usable
+from .packed import poly_attention_order2_packed
 from .rotary import RotaryEmbedding, apply_rotary
 
 LinearNoBias = partial(nn.Linear, bias=False)
@@ -50,6 +51,18 @@ def rotate_by_angles(rotary_pos_emb, qs):
     both features (2i, 2i + 1) of a pair holding the pair's angle
     (poly_attention/poly_attention.py:276-277)."""
     return apply_rotary(qs, angles=rotary_pos_emb[..., ::2])
+
+
+def check_packed(x, context, mask, context_mask, cache, return_cache):
+    if x.dim() != 3 or x.shape[0] != 1:
+        raise ValueError("packed sequences (cu_seqlens) come as one row: x [1, total, dim]")
+    if any(exists(t) for t in (context, mask, context_mask, cache)) or return_cache:
+        raise ValueError("packed sequences (cu_seqlens) take no context, masks or cache")
+
+
+def token_rows(t):
+    """[1, heads, total, d] -> [total, heads, d] (a view)."""
+    return t.squeeze(0).transpose(0, 1)
 
 
 class Order2PolyAttention(Module):
@@ -112,9 +125,13 @@ class Order2PolyAttention(Module):
 
     def forward(self, x, context: Tensor | tuple[Tensor, ...] | None = None, mask=None,
                 context_mask: Tensor | tuple[Tensor | None, ...] | None = None, rotary_pos_emb=None, cache=None,
-                return_cache=False):
+                return_cache=False, cu_seqlens=None, max_seqlen=None):
         seq_len = x.shape[-2]
         has_cache = exists(cache)
+        packed = exists(cu_seqlens)
+        if packed:
+            # sequences laid end to end in one row [1, total, dim]; each attends itself alone
+            check_packed(x, context, mask, context_mask, cache, return_cache)
         if has_cache:
             assert seq_len == 1, 'sequence length must be 1 when using kv cache'
         orig_x = x
@@ -183,12 +200,17 @@ class Order2PolyAttention(Module):
         if not exists(rotary_pos_emb) and exists(self.rotary_emb):
             if not has_cache and q1.shape[-2] == q2.shape[-2] == q3.shape[-2]:
                 # every row at its own position: q2 turns the same way as a key and as a query
-                q1, q2_right, q3_full = self.rotary_emb([q1, q2, q3])
+                q1, q2_right, q3_full = self.rotary_emb([q1, q2, q3], cu_seqlens=cu_seqlens)
             else:
                 q1, q2_right = self.rotary_emb.rotate_queries_with_cached_keys(q1, q2_right)
                 q2_left, q3_full = self.rotary_emb.rotate_queries_with_cached_keys(q2_left, q3_full)
                 q2_pass1 = q2_left
 
+        if packed:
+            out = poly_attention_order2_packed(*(token_rows(t) for t in (q1, q2_right, q3_full, v3_cache)), cu_seqlens,
+                                               softclamp_value=self.softclamp_value, causal=self.causal,
+                                               max_seqlen=max_seqlen)[0]
+            return self._finish(out.transpose(0, 1).unsqueeze(0), v2, gates)
         if has_cache:
             out, lse_step, msg_step = poly_attention_order2_cached(
                 q1, q2_left, q2_right, q3_full, v3_cache, self._squeeze(clse23), self._squeeze(cmsg),

@@ -1,0 +1,100 @@
+"""Packed passes without a GPU: offsets, refusals, the C entries' checks, the slot numbering."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+
+def test_offsets():
+    import poly_attention_b200 as P
+    cu, longest = P.packed_offsets([3, 0, 5], device="cpu")
+    assert cu.tolist() == [0, 3, 3, 8] and cu.dtype == torch.int32 and longest == 5
+    assert P.packed_offsets([], device="cpu")[0].tolist() == [0]
+    with pytest.raises(ValueError):
+        P.packed_offsets([3, -1], device="cpu")
+
+
+def test_cpu_tensors_are_refused():
+    import poly_attention_b200 as P
+    t = torch.randn(8, 2, 64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        P.pass_fwd_packed(t, t, t, torch.tensor([0, 8], dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        P.poly_attention_order2_packed(t, t, t, t, torch.tensor([0, 8], dtype=torch.int32))
+    attn = P.PolyAttention(dim=16, heads=2, dim_head=8)
+    with pytest.raises(ValueError, match="packed"):
+        attn(torch.randn(2, 4, 16), cu_seqlens=torch.tensor([0, 4]))
+
+
+def test_c_entries_check_before_launching():
+    from poly_attention_b200 import _lib
+    lib = _lib.lib
+    assert lib.poly_sizeof_packed_args() == ctypes.sizeof(_lib.PolyPackedArgs)
+    assert lib.poly_sizeof_packed_bwd_args() == ctypes.sizeof(_lib.PolyPackedBwdArgs)
+    assert lib.poly_packed_pass_fwd(None, None) == _lib.POLY_EINVAL
+    assert lib.poly_packed_pass_bwd(None, None) == _lib.POLY_EINVAL
+    assert lib.poly_packed_pass_bwd_workspace_size(None) == 0
+
+    def args(cls, **kw):
+        a = cls()
+        f = a.fwd if cls is _lib.PolyPackedArgs else a.bwd.fwd
+        f.batch, f.heads, f.kv_heads, f.seq_q, f.seq_k, f.head_dim, f.scale = 1, 2, 1, 16, 16, 64, 0.1
+        f.q = f.k = f.v = f.out = 256
+        a.cu_seqlens, a.seqs = 256, 2
+        for k, v in kw.items():
+            setattr(f if hasattr(f, k) else a, k, v)
+        return a
+
+    for cls, call in ((_lib.PolyPackedArgs, lib.poly_packed_pass_fwd), (_lib.PolyPackedBwdArgs, lib.poly_packed_pass_bwd)):
+        for kw, rc in ((dict(batch=2), _lib.POLY_EINVAL), (dict(seq_k=8), _lib.POLY_EINVAL), (dict(heads=3, kv_heads=2), _lib.POLY_EINVAL),
+                       (dict(dtype=7), _lib.POLY_EINVAL), (dict(head_dim=129), _lib.POLY_EUNSUPPORTED),
+                       (dict(key_mask=256), _lib.POLY_EUNSUPPORTED), (dict(query_mask=256), _lib.POLY_EUNSUPPORTED),
+                       (dict(v_mul=256), _lib.POLY_EUNSUPPORTED), (dict(causal_offset=128), _lib.POLY_EUNSUPPORTED),
+                       (dict(seqs=-1), _lib.POLY_EINVAL), (dict(max_len=-1), _lib.POLY_EINVAL), (dict(cu_seqlens=None), _lib.POLY_EINVAL),
+                       (dict(q=None), _lib.POLY_EINVAL), (dict(scale=float("nan")), _lib.POLY_EINVAL),
+                       (dict(epi_out=256), _lib.POLY_EINVAL), (dict(seq_q=2 ** 31 - 1, seq_k=2 ** 31 - 1), _lib.POLY_EUNSUPPORTED)):
+            assert call(args(cls, **kw), None) == rc, kw
+        assert call(args(cls, seq_q=0, seq_k=0), None) == _lib.POLY_OK
+        assert call(args(cls, seqs=0), None) == _lib.POLY_OK
+    # the backward's own needs: its tensors, then its workspace
+    assert lib.poly_packed_pass_bwd(args(_lib.PolyPackedBwdArgs), None) == _lib.POLY_EINVAL
+    b = args(_lib.PolyPackedBwdArgs, lse=256)
+    b.bwd.dout = b.bwd.dq = b.bwd.dk = b.bwd.dv = 256
+    assert lib.poly_packed_pass_bwd(b, None) == _lib.POLY_EINVAL
+    assert "workspace" in lib.poly_last_error().decode()
+
+
+@pytest.mark.parametrize("block", [8, 64, 128, 256])
+def test_slot_numbering_covers_every_tile_once(block):
+    """The search of csrc/packed.cuh restated: every tile of every sequence has one slot, every slot stays inside."""
+    def locate(cu, total, slot):
+        at = lambda s: min(max(cu[s], 0), total)   # noqa: E731
+        lo, hi = 0, len(cu) - 1
+        while hi - lo > 1:
+            mid = (lo + hi) >> 1
+            if at(mid) // block + mid <= slot:
+                lo = mid
+            else:
+                hi = mid
+        start, length = at(lo), at(lo + 1) - at(lo)
+        tile = slot - (start // block + lo)
+        return (lo, start, length, tile) if tile >= 0 and tile * block < length else None
+
+    rng = random.Random(block)
+    for _ in range(300):
+        lens = [rng.choice([0, 1, rng.randrange(3 * block), block, block - 1, block + 1]) for _ in range(rng.randrange(1, 12))]
+        lead = rng.choice([0, 0, 5, 300])
+        cu = [lead]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        total = cu[-1] + rng.choice([0, 0, 7, 500])
+        found = [t for t in (locate(cu, total, s) for s in range(total // block + len(lens))) if t]
+        want = [(s, cu[s], n, t) for s, n in enumerate(lens) for t in range((n + block - 1) // block)]
+        assert sorted((a, b, c, d) for a, b, c, d in found) == sorted(want)
+        # tiles of different sequences never share a slot, so slot-addressed rows do not overlap
+        wild = [rng.randrange(-1000, 2000) for _ in range(len(cu))]
+        for s in range(total // block + len(lens)):
+            t = locate(wild, total, s)
+            if t:
+                assert 0 <= t[1] and t[1] + t[2] <= total and t[1] + t[3] * block < total
