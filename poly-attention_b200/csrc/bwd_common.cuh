@@ -5,6 +5,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "packed.cuh"
 #include "tc_ptx.cuh"
 
 namespace poly {
@@ -21,6 +22,7 @@ struct BwdParams {
   void* dk; int64_t dk_stride[3];
   void* dv; int64_t dv_stride[3];
   float* dbias; int64_t dbias_stride[2];
+  PackedSeqs pk;                 // packed sequences: rows of slots of 128 in dq_acc, lse2 and delta
 };
 
 template <typename T>
@@ -173,6 +175,92 @@ __global__ void bwd_dq_convert_kernel(const PolyPassBwdArgs a, const float* dq_a
   *reinterpret_cast<uint4*>(dst) = out;
 }
 
+// Packed sequences. The kernels' row statistics and the dQ accumulator are laid
+// out by slots of 128 rows (packed.cuh), so every sequence owns whole tiles: a
+// tile's rows past its sequence's end add to rows that nobody reads, not to the
+// next sequence's (0 * NaN), and the statistics are 16-byte aligned.
+// One block per 32 rows of a slot and head: delta and -log2 lse as above, and
+// the accumulator's rows as zeros. A row that saw no live key gets p = 0.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) packed_bwd_prep_kernel(const PolyPassBwdArgs a, const PackedSeqs q, float* dq_acc,
+                                                              float* lse2, float* delta, int64_t nq_pad) {
+  PackedTile t;
+  const int slot = blockIdx.x >> 2;
+  if (!packed_tile<128>(q.cu, q.seqs, q.total, slot, t)) return;
+  const int h = blockIdx.y, sub = threadIdx.x & 7;
+  const int r = (blockIdx.x & 3) * 32 + (threadIdx.x >> 3);   // row of the slot
+  const int i = t.tile * 128 + r;                              // row of the sequence
+  const int64_t w = h * nq_pad + (int64_t)slot * 128 + r;
+  const bool live = i < t.len;
+  const int64_t row = (int64_t)t.start + i;
+  float s = 0.f;
+  float* acc = dq_acc + w * D + sub * (D / 8);
+#pragma unroll
+  for (int v4 = 0; v4 < D / 32; ++v4) *reinterpret_cast<float4*>(acc + v4 * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+    const T* o = (const T*)a.fwd.out + h * a.fwd.out_stride[1] + row * a.fwd.out_stride[2] + sub * (D / 8);
+    const T* g = (const T*)a.dout + h * a.dout_stride[1] + row * a.dout_stride[2] + sub * (D / 8);
+#pragma unroll
+    for (int v8 = 0; v8 < D / 64; ++v8) {
+      const uint4 ov = *reinterpret_cast<const uint4*>(o + v8 * 8);
+      const uint4 gv = *reinterpret_cast<const uint4*>(g + v8 * 8);
+      const T* op = reinterpret_cast<const T*>(&ov);
+      const T* gp = reinterpret_cast<const T*>(&gv);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += to_f32(op[e]) * to_f32(gp[e]);
+    }
+  }
+  s += __shfl_xor_sync(0xffffffffu, s, 1);
+  s += __shfl_xor_sync(0xffffffffu, s, 2);
+  s += __shfl_xor_sync(0xffffffffu, s, 4);
+  if (sub == 0) {
+    const float l = live ? a.fwd.lse[h * a.fwd.lse_stride[1] + row] : -FLT_MAX;
+    if (l <= kDeadBias) {
+      lse2[w] = -INFINITY;
+      delta[w] = 0.f;
+    } else {
+      if (a.dlse) s -= a.dlse[h * a.dlse_stride[1] + row];
+      delta[w] = s;
+      lse2[w] = -l * kLog2e;
+    }
+  }
+}
+
+// dq = scale * dq_acc (+ dq), from slot rows to the sequences' rows.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) packed_bwd_dq_kernel(const PolyPassBwdArgs a, const PackedSeqs q,
+                                                            const float* dq_acc, int64_t nq_pad) {
+  PackedTile t;
+  const int slot = blockIdx.x >> 2;
+  if (!packed_tile<128>(q.cu, q.seqs, q.total, slot, t)) return;
+  const int h = blockIdx.y, r0 = (blockIdx.x & 3) * 32;
+  const float sc = a.fwd.scale;
+  for (int idx = threadIdx.x; idx < 32 * (D / 8); idx += 256) {
+    const int r = r0 + idx / (D / 8), c = (idx % (D / 8)) * 8;
+    const int i = t.tile * 128 + r;
+    if (i >= t.len) return;
+    const float* src = dq_acc + (h * nq_pad + (int64_t)slot * 128 + r) * D + c;
+    T* dst = (T*)a.dq + h * a.dq_stride[1] + ((int64_t)t.start + i) * a.dq_stride[2] + c;
+    const float4 x0 = *reinterpret_cast<const float4*>(src);
+    const float4 x1 = *reinterpret_cast<const float4*>(src + 4);
+    float v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+    if (a.dq_accumulate) {
+      const uint4 old = *reinterpret_cast<const uint4*>(dst);
+      const T* pr = reinterpret_cast<const T*>(&old);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * sc + to_f32(pr[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= sc;
+    }
+    uint4 out;
+    uint32_t* w = &out.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pk<T>(v[2 * e], v[2 * e + 1]);
+    *reinterpret_cast<uint4*>(dst) = out;
+  }
+}
+
 struct BwdWs {
   float* dq_acc;
   float* lse2;
@@ -195,6 +283,28 @@ BwdWs bwd_ws(const PolyPassBwdArgs& a) {
   w.dq_acc = (float*)base;
   w.lse2 = (float*)(base + acc);
   w.delta = (float*)(base + acc + vec);
+  return w;
+}
+
+// The same for packed sequences: nq_pad rows of slots per head.
+struct PackedBwdWs {
+  float* dq_acc;
+  float* lse2;
+  float* delta;
+  int slots;
+  int64_t nq_pad;
+  size_t bytes;
+};
+
+inline PackedBwdWs packed_bwd_ws(const PolyPassBwdArgs& a, int seqs) {
+  PackedBwdWs w{};
+  w.slots = a.fwd.seq_q / 128 + seqs;
+  w.nq_pad = (int64_t)w.slots * 128;
+  const size_t rows = (size_t)a.fwd.heads * w.nq_pad;
+  w.bytes = rows * (a.fwd.head_dim + 2) * 4;
+  w.dq_acc = (float*)a.workspace;
+  w.lse2 = w.dq_acc + rows * a.fwd.head_dim;
+  w.delta = w.lse2 + rows;
   return w;
 }
 

@@ -69,7 +69,7 @@ struct BwdLayout {
   static constexpr int kDel = kLse + kStages * BQ * 4;
   static constexpr int kDb = kDel + kStages * BQ * 4;   // d-bias partials of warpgroup 1
   static constexpr int kBar = kDb + BK * 4;
-  static constexpr int kNumBars = 16;
+  static constexpr int kNumBars = 20;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kBytes = kMisc + 16;
   static constexpr int kAlloc = kBytes + 1024;
@@ -78,7 +78,7 @@ struct BwdLayout {
   static constexpr uint32_t kS = 0, kDP = 128, kDV = 256, kDK = 320, kDQ = 384, kPT = 448;
 };
 
-template <typename T, bool SOFTCLAMP, bool HAS_BIAS, bool DB>
+template <typename T, bool SOFTCLAMP, bool HAS_BIAS, bool DB, bool PACKED>
 __global__ void __launch_bounds__(kThreads, 1)
     pass_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                        const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -110,6 +110,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* dq_free = bars + 12;
   uint64_t* dkv_done = bars + 13;
   uint64_t* drain = bars + 14;
+  uint64_t* kv_clean = bars + 15;  // PACKED: the tiles hold no other sequence's rows
+  uint64_t* q_clean = bars + 16;   // [QS]
   uint32_t* tmem_slot = (uint32_t*)(smem + L::kMisc);
   volatile int* abort_flag = (volatile int*)(smem + L::kMisc + 4);
   int* err = g_poly_device_error;
@@ -131,8 +133,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int b = bh / p.kv_heads, kvh = bh - b * p.kv_heads;
   const int rep = p.heads / p.kv_heads;
+  int first = 0, slot_row = 0;   // PACKED: the sequence's first row, and its first row of slots
+  int seq_k = p.seq_k, q_tiles = p.q_tiles;
+  if constexpr (PACKED) {
+    PackedTile t;
+    if (!packed_tile<BK>(p.pk.cu, p.pk.seqs, p.pk.total, kt, t)) return;
+    kt = t.tile;
+    first = t.start;
+    slot_row = t.slot0 * BK;
+    seq_k = t.len;
+    q_tiles = (t.len + BQ - 1) / BQ;
+  }
   const int qt0 = p.causal ? kt : 0;
-  const int nqt = max(0, p.q_tiles - qt0);
+  const int nqt = max(0, q_tiles - qt0);
+  // PACKED: key rows of this tile, and query rows of the last tile, if cut by the sequence's end
+  const int k_cut = PACKED && seq_k - kt * BK < BK ? seq_k - kt * BK : 0;
+  const int q_cut = PACKED ? seq_k % BQ : 0;
   const int NT = rep * nqt;
 
   if (threadIdx.x == 0) {
@@ -149,6 +165,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(mma_done, 1);
     mbar_init(dkv_done, 1);
     mbar_init(drain, 1);
+    if (PACKED) {
+      mbar_init(kv_clean, 64);
+      for (int s = 0; s < QS; ++s) mbar_init(&q_clean[s], 64);
+    }
     tc::abort_init(abort_flag, err);
     fence_barrier_init();
   }
@@ -199,8 +219,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     named_bar_sync(2, 128);
     if (lane == 0 && warp == 4) {
       const int plane = b * p.heads + h;
-      tma_reduce_add_3d(&tm_dq, sDQ, 0, qt * BQ, plane);
-      tma_reduce_add_3d(&tm_dq, sDQ + 128 * 128, 32, qt * BQ, plane);
+      tma_reduce_add_3d(&tm_dq, sDQ, 0, slot_row + qt * BQ, plane);
+      tma_reduce_add_3d(&tm_dq, sDQ + 128 * 128, 32, slot_row + qt * BQ, plane);
       bulk_commit_group();
     }
     return true;
@@ -212,18 +232,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_do);
       mbar_arrive_expect_tx(kv_full, 2 * L::kTile);
-      tma_load_4d(sK, &tm_k, kv_full, 0, kt * BK, kvh, b);
-      tma_load_4d(sV, &tm_v, kv_full, 0, kt * BK, kvh, b);
+      tma_load_4d(sK, &tm_k, kv_full, 0, first + kt * BK, kvh, b);
+      tma_load_4d(sV, &tm_v, kv_full, 0, first + kt * BK, kvh, b);
       int issued = 0;
       for (int t = 0; t < NT; ++t) {
         const int s = t % QS;
         if (t >= QS && !mbar_wait(&q_empty[s], ((t / QS) - 1) & 1, abort_flag, err, 1)) break;
         int h, qt;
         tile_of(t, h, qt);
-        const int64_t row = (int64_t)(b * p.heads + h) * p.nq_pad + qt * BQ;
+        const int64_t row = (int64_t)(b * p.heads + h) * p.nq_pad + slot_row + qt * BQ;
         mbar_arrive_expect_tx(&q_full[s], 2 * L::kTile + 2 * BQ * 4);
-        tma_load_4d(sQ + s * L::kTile, &tm_q, &q_full[s], 0, qt * BQ, h, b);
-        tma_load_4d(sDO + s * L::kTile, &tm_do, &q_full[s], 0, qt * BQ, h, b);
+        tma_load_4d(sQ + s * L::kTile, &tm_q, &q_full[s], 0, first + qt * BQ, h, b);
+        tma_load_4d(sDO + s * L::kTile, &tm_do, &q_full[s], 0, first + qt * BQ, h, b);
         bulk_load(sLse + s * BQ, p.lse2 + row, BQ * 4, &q_full[s]);
         bulk_load(sDel + s * BQ, p.delta + row, BQ * 4, &q_full[s]);
         issued = t + 1;
@@ -252,6 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit(sdp_full);
       };
       bool ok = mbar_wait(kv_full, 0, abort_flag, err, 2) && mbar_wait(&q_full[0], 0, abort_flag, err, 3);
+      if (PACKED && ok && k_cut) ok = mbar_wait(kv_clean, 0, abort_flag, err, 12);
+      if (PACKED && ok && q_cut) ok = mbar_wait(&q_clean[0], 0, abort_flag, err, 13);
       if (ok) {
         tc_fence_after();
         issue_sdp(0);
@@ -263,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // buffers take tile t + 1 while the softmax still works on t
           if (!mbar_wait(sdp_free, t & 1, abort_flag, err, 11)) break;
           if (!mbar_wait(&q_full[(t + 1) % QS], ((t + 1) / QS) & 1, abort_flag, err, 5)) break;
+          if (PACKED && q_cut && !mbar_wait(&q_clean[(t + 1) % QS], ((t + 1) / QS) & 1, abort_flag, err, 14)) break;
           tc_fence_after();
           issue_sdp((t + 1) % QS);
         }
@@ -292,6 +315,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       mma_commit(drain);
       drain_wait(drain, 0);
     }
+  } else if (PACKED && warp < 4) {
+    // ---------------------------------------------------- rows behind the sequence's end
+    // A tile that runs over the end holds the next sequence's rows. Their
+    // probabilities are 0, but 0 * NaN or 0 * infinity in a product over keys
+    // (dQ) or queries (dK, dV) is not: such rows are zeroed before the MMAs read them.
+    const int tid = threadIdx.x - 64;
+    bool ok = true;
+    if (k_cut) {
+      ok = mbar_wait_warp(kv_full, 0, abort_flag, err, 15);
+      if (ok) {
+        zero_tile_rows<BK, D / 64>(sK, k_cut, tid, 64);
+        zero_tile_rows<BK, D / 64>(sV, k_cut, tid, 64);
+        fence_proxy_async_smem();
+        mbar_arrive(kv_clean);
+      }
+    }
+    for (int t = 0; ok && q_cut && t < NT; ++t) {
+      const int s = t % QS;
+      int h, qt;
+      tile_of(t, h, qt);
+      if (!mbar_wait_warp(&q_full[s], (t / QS) & 1, abort_flag, err, 16)) break;
+      if (qt == q_tiles - 1) {
+        zero_tile_rows<BQ, D / 64>(sQ + s * L::kTile, q_cut, tid, 64);
+        zero_tile_rows<BQ, D / 64>(sDO + s * L::kTile, q_cut, tid, 64);
+        fence_proxy_async_smem();
+      }
+      mbar_arrive(&q_clean[s]);
+    }
   } else if (warp >= 4 && warp < 12) {
     // -------------------------------------------------- softmax-backward
     // Two warpgroups: thread = key row r, warpgroup hw takes query columns
@@ -300,11 +351,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = (warp & 3) * 32 + lane;
     const int j = kt * BK + r;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const bool key_ok = j < p.seq_k;
+    const bool key_ok = j < seq_k;
     const bool key_ok_warp = __all_sync(0xffffffffu, key_ok);
     float b2 = 0.f;
     if (HAS_BIAS && key_ok) {
-      const float braw = p.bias[b * p.bias_stride[0] + kvh * p.bias_stride[1] + j];
+      const float braw = p.bias[b * p.bias_stride[0] + kvh * p.bias_stride[1] + first + j];
       b2 = braw <= kDeadBias ? -INFINITY : braw * kLog2e;
     }
     float dbias = 0.f;
@@ -361,8 +412,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool have = ok && NT > 0 && mbar_wait_warp(dkv_done, 0, abort_flag, err, 9);
     if (have) tc_fence_after();
     if (have || NT == 0) {
-      T* dst = hw == 0 ? (T*)p.dk + b * p.dk_stride[0] + kvh * p.dk_stride[1] + (int64_t)j * p.dk_stride[2]
-                       : (T*)p.dv + b * p.dv_stride[0] + kvh * p.dv_stride[1] + (int64_t)j * p.dv_stride[2];
+      T* dst = hw == 0 ? (T*)p.dk + b * p.dk_stride[0] + kvh * p.dk_stride[1] + ((int64_t)first + j) * p.dk_stride[2]
+                       : (T*)p.dv + b * p.dv_stride[0] + kvh * p.dv_stride[1] + ((int64_t)first + j) * p.dv_stride[2];
       const float mul = hw == 0 ? p.scale : 1.f;
       const uint32_t col = hw == 0 ? L::kDK : L::kDV;
 #pragma unroll
@@ -401,33 +452,46 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 4 && warp < 8 && p.dbias) {
     const int r = (warp & 3) * 32 + lane;
     const int j = kt * BK + r;
-    if (j < p.seq_k) p.dbias[b * p.dbias_stride[0] + kvh * p.dbias_stride[1] + j] = dbias_part + sDb[r];
+    if (j < seq_k) p.dbias[b * p.dbias_stride[0] + kvh * p.dbias_stride[1] + first + j] = dbias_part + sDb[r];
   }
 }
 
-template <typename T, bool SOFTCLAMP, bool HAS_BIAS, bool DB>
-int launch_bwd_t(const PolyPassBwdArgs& a, cudaStream_t s) {
+template <typename T, bool SOFTCLAMP, bool HAS_BIAS, bool DB, bool PACKED>
+int launch_bwd_t(const PolyPassBwdArgs& a, const PackedSeqs* seqs, cudaStream_t s) {
   using L = BwdLayout;
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(pass_bwd_tc_kernel<T, SOFTCLAMP, HAS_BIAS, DB>,
+    attr_err = cudaFuncSetAttribute(pass_bwd_tc_kernel<T, SOFTCLAMP, HAS_BIAS, DB, PACKED>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
   });
   if (attr_err != cudaSuccess) return cuda_status(attr_err, "cudaFuncSetAttribute(bwd tc)");
   const PolyPassArgs& f = a.fwd;
   BwdWs w = bwd_ws<D, BQ>(a);
+  PackedBwdWs pw{};
+  if (PACKED) {
+    pw = packed_bwd_ws(a, seqs->seqs);
+    w.dq_acc = pw.dq_acc;
+    w.lse2 = pw.lse2;
+    w.delta = pw.delta;
+    w.nq_pad = (int)pw.nq_pad;
+  }
   CUtensorMap tq, tdo, tk, tv, tdq;
   int rc = make_map(&tq, f.q, f.dtype, D, f.seq_q, f.heads, f.batch, f.q_stride, BQ);
   if (!rc) rc = make_map(&tdo, a.dout, f.dtype, D, f.seq_q, f.heads, f.batch, a.dout_stride, BQ);
   if (!rc) rc = make_map(&tk, f.k, f.dtype, D, f.seq_k, f.kv_heads, f.batch, f.k_stride, BK);
   if (!rc) rc = make_map(&tv, f.v, f.dtype, D, f.seq_k, f.kv_heads, f.batch, f.v_stride, BK);
-  if (!rc) rc = make_map_f32_acc(&tdq, w.dq_acc, f.seq_q, f.batch * f.heads);
+  if (!rc) rc = make_map_f32_acc(&tdq, w.dq_acc, PACKED ? w.nq_pad : f.seq_q, f.batch * f.heads);
   if (rc) return rc;
-  rc = cuda_status(cudaMemsetAsync(w.dq_acc, 0, (size_t)f.batch * f.heads * f.seq_q * D * 4, s), "memset dq acc");
-  if (rc) return rc;
-  const int64_t prow = (int64_t)f.batch * f.heads * w.nq_pad;
-  bwd_prep_kernel<T, D><<<(unsigned)((prow * 8 + 255) / 256), 256, 0, s>>>(a, w.lse2, w.delta, w.nq_pad);
+  const dim3 pgrid((unsigned)(pw.slots * 4), (unsigned)f.heads);
+  if (PACKED) {
+    packed_bwd_prep_kernel<T, D><<<pgrid, 256, 0, s>>>(a, *seqs, w.dq_acc, w.lse2, w.delta, pw.nq_pad);
+  } else {
+    rc = cuda_status(cudaMemsetAsync(w.dq_acc, 0, (size_t)f.batch * f.heads * f.seq_q * D * 4, s), "memset dq acc");
+    if (rc) return rc;
+    const int64_t prow = (int64_t)f.batch * f.heads * w.nq_pad;
+    bwd_prep_kernel<T, D><<<(unsigned)((prow * 8 + 255) / 256), 256, 0, s>>>(a, w.lse2, w.delta, w.nq_pad);
+  }
   BwdParams p{};
   p.seq_q = f.seq_q;
   p.seq_k = f.seq_k;
@@ -455,24 +519,29 @@ int launch_bwd_t(const PolyPassBwdArgs& a, cudaStream_t s) {
   p.dbias = a.dbias;
   p.dbias_stride[0] = a.dbias_stride[0];
   p.dbias_stride[1] = a.dbias_stride[1];
-  p.k_tiles = (f.seq_k + BK - 1) / BK;
+  p.k_tiles = PACKED ? pw.slots : (f.seq_k + BK - 1) / BK;
+  if (PACKED) p.pk = *seqs;
   dim3 grid(p.k_tiles * f.batch * f.kv_heads);
-  pass_bwd_tc_kernel<T, SOFTCLAMP, HAS_BIAS, DB><<<grid, kThreads, L::kAlloc, s>>>(tq, tdo, tk, tv, tdq, p);
-  const int64_t cthreads = (int64_t)f.batch * f.heads * f.seq_q * (D / 8);
-  bwd_dq_convert_kernel<T, D><<<(unsigned)((cthreads + 255) / 256), 256, 0, s>>>(a, w.dq_acc);
+  pass_bwd_tc_kernel<T, SOFTCLAMP, HAS_BIAS, DB, PACKED><<<grid, kThreads, L::kAlloc, s>>>(tq, tdo, tk, tv, tdq, p);
+  if (PACKED) {
+    packed_bwd_dq_kernel<T, D><<<pgrid, 256, 0, s>>>(a, *seqs, w.dq_acc, pw.nq_pad);
+  } else {
+    const int64_t cthreads = (int64_t)f.batch * f.heads * f.seq_q * (D / 8);
+    bwd_dq_convert_kernel<T, D><<<(unsigned)((cthreads + 255) / 256), 256, 0, s>>>(a, w.dq_acc);
+  }
   note_launch(3);
   return cuda_status(cudaGetLastError(), "pass_bwd_tc launch");
 }
 
-template <typename T>
-int bwd_dispatch(const PolyPassBwdArgs& a, cudaStream_t s) {
+template <typename T, bool PACKED>
+int bwd_dispatch(const PolyPassBwdArgs& a, const PackedSeqs* q, cudaStream_t s) {
   const bool sc = a.fwd.softclamp > 0.f, bias = a.fwd.bias != nullptr, db = a.dbias != nullptr;
   if (db) {
-    if (sc) return bias ? launch_bwd_t<T, true, true, true>(a, s) : launch_bwd_t<T, true, false, true>(a, s);
-    return bias ? launch_bwd_t<T, false, true, true>(a, s) : launch_bwd_t<T, false, false, true>(a, s);
+    if (sc) return bias ? launch_bwd_t<T, true, true, true, PACKED>(a, q, s) : launch_bwd_t<T, true, false, true, PACKED>(a, q, s);
+    return bias ? launch_bwd_t<T, false, true, true, PACKED>(a, q, s) : launch_bwd_t<T, false, false, true, PACKED>(a, q, s);
   }
-  if (sc) return bias ? launch_bwd_t<T, true, true, false>(a, s) : launch_bwd_t<T, true, false, false>(a, s);
-  return bias ? launch_bwd_t<T, false, true, false>(a, s) : launch_bwd_t<T, false, false, false>(a, s);
+  if (sc) return bias ? launch_bwd_t<T, true, true, false, PACKED>(a, q, s) : launch_bwd_t<T, true, false, false, PACKED>(a, q, s);
+  return bias ? launch_bwd_t<T, false, true, false, PACKED>(a, q, s) : launch_bwd_t<T, false, false, false, PACKED>(a, q, s);
 }
 
 // Self-test of the bounded waits (poly_selftest_wait_timeout): one CTA holds
@@ -531,7 +600,32 @@ size_t pass_bwd_tc_workspace(const PolyPassBwdArgs& a) {
 
 int launch_pass_bwd_tc(const PolyPassBwdArgs& a, cudaStream_t s) {
   if (a.fwd.head_dim == 128) return launch_pass_bwd_tc128(a, s);
-  return a.fwd.dtype == POLY_BF16 ? bwd_dispatch<__nv_bfloat16>(a, s) : bwd_dispatch<__half>(a, s);
+  return a.fwd.dtype == POLY_BF16 ? bwd_dispatch<__nv_bfloat16, false>(a, nullptr, s) : bwd_dispatch<__half, false>(a, nullptr, s);
+}
+
+// Rows as packed_fwd_tc_eligible wants them (batch strides are not used), and
+// few enough slot rows for TMA's 32-bit coordinates.
+bool packed_bwd_tc_eligible(const PolyPassBwdArgs& a, int seqs) {
+  const PolyPassArgs& f = a.fwd;
+  if (f.dtype != POLY_BF16 && f.dtype != POLY_F16) return false;
+  if (f.head_dim != D && f.head_dim != 128) return false;
+  if (f.seq_q / BK + seqs >= (1 << 23)) return false;
+  const int64_t* st[8] = {f.q_stride, f.k_stride, f.v_stride, f.out_stride, a.dout_stride, a.dq_stride, a.dk_stride, a.dv_stride};
+  for (const int64_t* t : st)
+    if (!strides_ok(t + 1, 2)) return false;
+  return aligned16(f.q) && aligned16(f.k) && aligned16(f.v) && aligned16(f.out) && aligned16(a.dout) &&
+         aligned16(a.dq) && aligned16(a.dk) && aligned16(a.dv);
+}
+
+size_t packed_bwd_tc_workspace(const PolyPassBwdArgs& a, int seqs) { return packed_bwd_ws(a, seqs).bytes; }
+
+int launch_packed_bwd_tc(PolyPassBwdArgs a, const PackedSeqs& q, cudaStream_t s) {
+  PolyPassArgs& f = a.fwd;   // one batch element: any valid stride
+  f.q_stride[0] = f.k_stride[0] = f.v_stride[0] = a.dout_stride[0] = 8;
+  f.out_stride[0] = f.lse_stride[0] = f.bias_stride[0] = 0;
+  a.dq_stride[0] = a.dk_stride[0] = a.dv_stride[0] = a.dlse_stride[0] = a.dbias_stride[0] = 0;
+  if (f.head_dim == 128) return launch_packed_bwd_tc128(a, q, s);
+  return f.dtype == POLY_BF16 ? bwd_dispatch<__nv_bfloat16, true>(a, &q, s) : bwd_dispatch<__half, true>(a, &q, s);
 }
 
 }  // namespace poly

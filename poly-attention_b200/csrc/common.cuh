@@ -96,5 +96,11 @@ struct PackedSeqs {
 int launch_packed_fwd_simt(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s);
 int launch_packed_bwd_simt(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s);
 size_t packed_bwd_simt_workspace(const PolyPassBwdArgs& a);
+bool packed_fwd_tc_eligible(const PolyPassArgs& a);
+int launch_packed_fwd_tc(PolyPassArgs a, const PackedSeqs& q, cudaStream_t s);
+bool packed_bwd_tc_eligible(const PolyPassBwdArgs& a, int seqs);
+int launch_packed_bwd_tc(PolyPassBwdArgs a, const PackedSeqs& q, cudaStream_t s);
+int launch_packed_bwd_tc128(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s);
+size_t packed_bwd_tc_workspace(const PolyPassBwdArgs& a, int seqs);
 
 }  // namespace poly

@@ -12,12 +12,22 @@
 // O_B [320,384), P_A [384,448), P_B [448,512). P (16-bit, two per column)
 // stays in TMEM and is the A operand of the P V MMA, so no probability tile
 // crosses shared memory (shared-memory operand bandwidth bounds SS MMAs).
+//
+// PACKED: sequences laid end to end; a CTA takes the 256 rows of one slot
+// (packed.cuh) of one head. Three things differ from a batch of equal lengths,
+// and the warps that are idle there (2, 3) do two of them. TMA tiles run over
+// the end of a sequence into the next one: its keys are masked, and its values
+// (in the last tile only) are zeroed in shared memory, since 0 * NaN of a
+// neighbour would reach this sequence's rows. Bias rows start anywhere, which
+// TMA cannot load (16-byte boundary), so warp 2 stages them and drops the dead
+// keys there. Softclamp is done here too (tanh from one ex2 and one reciprocal).
 #include <algorithm>
 #include <mutex>
 #include <string>
 #include <type_traits>
 
 #include "common.cuh"
+#include "packed.cuh"
 #include "tc_host.cuh"
 #include "tc_ptx.cuh"
 
@@ -53,7 +63,7 @@ struct L2T {
   static constexpr int kV = kK + S * kTile;
   static constexpr int kB = kV + S * kTile;   // S x 128 fp32 bias
   static constexpr int kBar = kB + S * BN * 4;
-  static constexpr int kNumBars = 1 + 3 * S + 2 * 4 + 1;
+  static constexpr int kNumBars = 1 + 3 * S + 2 * 4 + 3;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kBytes = kMisc + 16;
   static constexpr int kAlloc = kBytes + 1024;
@@ -69,7 +79,17 @@ struct Fwd2Params {
   float* lse; int64_t lse_stride[2];
   const void* epi_mul; int64_t epi_mul_stride[3];
   void* epi_out; int64_t epi_out_stride[3];
+  // packed sequences
+  PackedSeqs pk;
+  const float* bias; int64_t bias_stride;   // per kv head
+  float sc_in, sc_out;                       // softclamp: x = sc_out tanh(s sc_in)
 };
+
+// tanh(z) = 1 - 2 / (e^2z + 1): off by about 2^-22 of 1, i.e. 2^-22 of the clamp
+// in a score, where tanhf's branches on 128 scores a thread would not fit.
+__device__ __forceinline__ float tanh_ex2(float z) {
+  return 1.f - __fdividef(2.f, ex2(fminf(z * (2.f * kLog2e), 126.f)) + 1.f);
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t pk2(float a, float b);
@@ -101,7 +121,7 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uin
       : "memory");
 }
 
-template <typename T, bool HAS_BIAS, int D>
+template <typename T, bool HAS_BIAS, int D, bool PACKED, bool SOFTCLAMP>
 __global__ void __launch_bounds__(kThreads, 1)
     pass_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_b,
@@ -127,6 +147,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* p_full = bars + 5 + 3 * S;    // [2]
   uint64_t* o_done = bars + 7 + 3 * S;    // [2]
   uint64_t* drain = bars + 9 + 3 * S;
+  // PACKED: a value tile cut by the sequence's end arrives on v_cut instead of
+  // its stage's v_full, and is without other sequences' rows at v_clean
+  uint64_t* v_cut = bars + 10 + 3 * S;
+  uint64_t* v_clean = bars + 11 + 3 * S;
   uint32_t* tmem_slot = (uint32_t*)(smem + L2::kMisc);
   volatile int* abort_flag = (volatile int*)(smem + L2::kMisc + 4);
   int* err = g_poly_device_error;
@@ -148,18 +172,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int b = bh / p.heads, h = bh - b * p.heads;
   const int kvh = h / (p.heads / p.kv_heads);
-  const int mt = p.causal ? (p.m_tiles - 1 - yi) : yi;
+  int mt = p.causal ? (p.m_tiles - 1 - yi) : yi;
+  int first = 0;   // PACKED: the sequence's first row
+  int seq_q = p.seq_q, seq_k = p.seq_k;
+  if constexpr (PACKED) {
+    PackedTile t;
+    if (!packed_tile<2 * BM>(p.pk.cu, p.pk.seqs, p.pk.total, mt, t)) return;
+    mt = t.tile;
+    first = t.start;
+    seq_q = seq_k = t.len;
+  }
   const int row0 = mt * 2 * BM;
-  const int kt_total = (p.seq_k + BN - 1) / BN;
+  const int kt_total = (seq_k + BN - 1) / BN;
   // key tiles seen by tile A (rows row0..) and tile B (rows row0 + 128..)
   const int ntA = p.causal ? min(kt_total, 2 * mt + 1 + p.off_tiles) : kt_total;
-  const int ntB = p.causal ? min(kt_total, 2 * mt + 2 + p.off_tiles) : kt_total;
-  const int ntMax = ntB;
+  const int ntB = PACKED && row0 + BM >= seq_q ? 0 : p.causal ? min(kt_total, 2 * mt + 2 + p.off_tiles) : kt_total;
+  const int ntMax = max(ntA, ntB);
+  // PACKED: the tile whose values need cleaning (-1: none visited)
+  const int clean_tile = PACKED && (seq_k % BN) != 0 && ntMax == kt_total ? kt_total - 1 : -1;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int s = 0; s < S; ++s) {
-      mbar_init(&k_full[s], 1);
+      mbar_init(&k_full[s], PACKED && HAS_BIAS ? 33 : 1);
       mbar_init(&v_full[s], 1);
       mbar_init(&kv_empty[s], 1);
     }
@@ -170,6 +205,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&o_done[x], 1);
     }
     mbar_init(drain, 1);
+    if (PACKED) {
+      mbar_init(v_cut, 1);
+      mbar_init(v_clean, 32);
+    }
     tc::abort_init(abort_flag, err);
     fence_barrier_init();
   }
@@ -185,29 +224,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive_expect_tx(q_full, 2 * L2::kTile);
 #pragma unroll
       for (int hf = 0; hf < D / 64; ++hf) {
-        tma_load_4d(sQ + hf * kAtom, &tm_q, q_full, hf * 64, row0, h, b);
-        tma_load_4d(sQ + L2::kTile + hf * kAtom, &tm_q, q_full, hf * 64, row0 + BM, h, b);
+        tma_load_4d(sQ + hf * kAtom, &tm_q, q_full, hf * 64, first + row0, h, b);
+        tma_load_4d(sQ + L2::kTile + hf * kAtom, &tm_q, q_full, hf * 64, first + row0 + BM, h, b);
       }
       int issued = 0;
       for (int j = 0; j < ntMax; ++j) {
         const int s = j % S;
         if (j >= S && !mbar_wait(&kv_empty[s], ((j / S) - 1) & 1, abort_flag, err, 41)) break;
-        mbar_arrive_expect_tx(&k_full[s], L2::kTile + (HAS_BIAS ? BN * 4 : 0));
+        mbar_arrive_expect_tx(&k_full[s], L2::kTile + (HAS_BIAS && !PACKED ? BN * 4 : 0));
 #pragma unroll
         for (int hf = 0; hf < D / 64; ++hf)
-          tma_load_4d(sK + s * L2::kTile + hf * kAtom, &tm_k, &k_full[s], hf * 64, j * BN, kvh, b);
-        if (HAS_BIAS) tma_load_3d(sB + s * BN, &tm_b, &k_full[s], j * BN, kvh, b);
-        mbar_arrive_expect_tx(&v_full[s], L2::kTile);
+          tma_load_4d(sK + s * L2::kTile + hf * kAtom, &tm_k, &k_full[s], hf * 64, first + j * BN, kvh, b);
+        if (HAS_BIAS && !PACKED) tma_load_3d(sB + s * BN, &tm_b, &k_full[s], j * BN, kvh, b);
+        uint64_t* v_bar = PACKED && j == clean_tile ? v_cut : &v_full[s];
+        mbar_arrive_expect_tx(v_bar, L2::kTile);
 #pragma unroll
         for (int hf = 0; hf < D / 64; ++hf)
-          tma_load_4d(sV + s * L2::kTile + hf * kAtom, &tm_v, &v_full[s], hf * 64, j * BN, kvh, b);
+          tma_load_4d(sV + s * L2::kTile + hf * kAtom, &tm_v, v_bar, hf * 64, first + j * BN, kvh, b);
         issued = j + 1;
       }
       if (*abort_flag) {
         drain_wait(q_full, 0);
         for (int j = max(0, issued - S); j < issued; ++j) {
           drain_wait(&k_full[j % S], (j / S) & 1);
-          drain_wait(&v_full[j % S], (j / S) & 1);
+          if (PACKED && j == clean_tile) drain_wait(v_cut, 0);
+          else drain_wait(&v_full[j % S], (j / S) & 1);
         }
       }
     }
@@ -239,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) {
         tc_fence_after();
         issue_s(0, 0);
-        issue_s(1, 0);
+        if (ntB > 0) issue_s(1, 0);
       }
       for (int j = 0; ok && j < ntMax; ++j) {
         const int s = j % S;
@@ -259,7 +300,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!(ok = mbar_wait(&p_full[x], j & 1, abort_flag, err, 46))) break;
           if (!v_ok) {
-            if (!(ok = mbar_wait(&v_full[s], (j / S) & 1, abort_flag, err, 47))) break;
+            ok = PACKED && j == clean_tile ? mbar_wait(v_clean, 0, abort_flag, err, 52)
+                                           : mbar_wait(&v_full[s], (j / S) & 1, abort_flag, err, 47);
+            if (!ok) break;
             v_ok = true;
           }
           tc_fence_after();
@@ -273,6 +316,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       mma_commit(drain);
       drain_wait(drain, 0);
+    }
+  } else if (PACKED && warp == 2) {
+    if (HAS_BIAS) {
+      // -------------------------------------------------- bias rows (k_full counts these 32 threads too)
+      const float* bias = p.bias + kvh * p.bias_stride + first;
+      for (int j = 0; j < ntMax; ++j) {
+        const int s = j % S;
+        float x[BN / 32];
+#pragma unroll
+        for (int e = 0; e < BN / 32; ++e) {
+          const int key = j * BN + e * 32 + lane;
+          x[e] = key < seq_k ? bias[key] : -INFINITY;
+        }
+        if (j >= S && !mbar_wait_warp(&kv_empty[s], ((j / S) - 1) & 1, abort_flag, err, 53)) break;
+#pragma unroll
+        for (int e = 0; e < BN / 32; ++e) sB[s * BN + e * 32 + lane] = x[e] <= kDeadBias ? -INFINITY : x[e];
+        mbar_arrive(&k_full[s]);
+      }
+    }
+  } else if (PACKED && warp == 3) {
+    if (clean_tile >= 0) {
+      // -------------------------------------------------- values behind the sequence's end
+      const int s = clean_tile % S;
+      if (mbar_wait_warp(v_cut, 0, abort_flag, err, 54)) {
+        zero_tile_rows<BN, D / 64>(sV + s * L2::kTile, seq_k - clean_tile * BN, lane, 32);
+        fence_proxy_async_smem();
+        mbar_arrive(v_clean);
+      }
     }
   } else if (warp >= 4) {
     // -------------------------------------------------- softmax (thread = query row)
@@ -299,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(&s_free[x]);                // S is in registers: the MMA may overwrite it
       }
-      const bool tail = (j == kt_total - 1) && (p.seq_k % BN) != 0;
+      const bool tail = (j == kt_total - 1) && (seq_k % BN) != 0;
       const bool diag = p.causal && (j == diag_tile);
       float tmax = -INFINITY;
       // Without a bias the row max is taken on the raw scores and the scale is
@@ -308,7 +379,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       // FFMA instead. Both end with v[] holding values whose 2^(v*mul - m) is
       // the unnormalised probability.
       float mul = p.sl2;
-      if (HAS_BIAS) {
+      if (SOFTCLAMP) {
+        mul = kLog2e;
+        const float4* b4 = reinterpret_cast<const float4*>(sB + s * BN);
+#pragma unroll
+        for (int q = 0; q < BN / 4; ++q) {
+          const float4 bb = HAS_BIAS ? b4[q] : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float be[4] = {bb.x, bb.y, bb.z, bb.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[4 * q + e] = __float_as_uint(fmaf(tanh_ex2(__uint_as_float(v[4 * q + e]) * p.sc_in), p.sc_out, be[e]));
+        }
+      } else if (HAS_BIAS) {
         mul = kLog2e;
         const float4* b4 = reinterpret_cast<const float4*>(sB + s * BN);
 #pragma unroll
@@ -321,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (tail) {
-        const int kvalid = p.seq_k - j * BN;
+        const int kvalid = seq_k - j * BN;
 #pragma unroll
         for (int c = 0; c < BN; ++c)
           if (c >= kvalid) v[c] = __float_as_uint(-INFINITY);
@@ -383,20 +465,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && nt > 0 && mbar_wait_warp(&o_done[x], (nt - 1) & 1, abort_flag, err, 51)) {
       tc_fence_after();
       const int row = row0 + x * BM + r;
+      const int64_t orow = PACKED ? (int64_t)first + row : (int64_t)row;
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-      T* out = (T*)p.out + b * p.out_stride[0] + h * p.out_stride[1] + (int64_t)row * p.out_stride[2];
+      T* out = (T*)p.out + b * p.out_stride[0] + h * p.out_stride[1] + orow * p.out_stride[2];
       const T* em = p.epi_out ? (const T*)p.epi_mul + b * p.epi_mul_stride[0] + h * p.epi_mul_stride[1] +
-                                    (int64_t)row * p.epi_mul_stride[2]
+                                    orow * p.epi_mul_stride[2]
                               : nullptr;
       T* eo = p.epi_out ? (T*)p.epi_out + b * p.epi_out_stride[0] + h * p.epi_out_stride[1] +
-                              (int64_t)row * p.epi_out_stride[2]
+                              orow * p.epi_out_stride[2]
                         : nullptr;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         tmem_ld32(o_addr + c * 32, o);
         tmem_wait_ld();
-        if (row < p.seq_q) {
+        if (row < seq_q) {
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
             uint4 val;
@@ -420,8 +503,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (p.lse && row < p.seq_q)
-        p.lse[b * p.lse_stride[0] + h * p.lse_stride[1] + row] = (m_run + __log2f(l_run)) * kLn2;
+      if (p.lse && row < seq_q)
+        p.lse[b * p.lse_stride[0] + h * p.lse_stride[1] + orow] =
+            PACKED && l_run == 0.f ? -FLT_MAX : (m_run + __log2f(l_run)) * kLn2;
     }
   }
   tc_fence_before();
@@ -430,14 +514,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, L2::kTmemCols);
 }
 
-template <typename T, bool HAS_BIAS, int D>
-int launch_t(const PolyPassArgs& a, cudaStream_t st) {
+template <typename T, bool HAS_BIAS, int D, bool PACKED, bool SOFTCLAMP>
+int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t st) {
   using L2 = L2T<D>;
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(pass_fwd_tc2_kernel<T, HAS_BIAS, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    L2::kAlloc);
+    attr_err = cudaFuncSetAttribute(pass_fwd_tc2_kernel<T, HAS_BIAS, D, PACKED, SOFTCLAMP>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, L2::kAlloc);
   });
   if (attr_err != cudaSuccess) return cuda_status(attr_err, "cudaFuncSetAttribute(fwd tc2)");
   CUtensorMap tq, tk, tv, tb;
@@ -446,7 +530,7 @@ int launch_t(const PolyPassArgs& a, cudaStream_t st) {
   if (!rc) rc = make_map(&tv, a.v, a.dtype, D, a.seq_k, a.kv_heads, a.batch, a.v_stride, BN);
   if (rc) return rc;
   memset(&tb, 0, sizeof(tb));
-  if (HAS_BIAS) {
+  if (HAS_BIAS && !PACKED) {
     EncodeTiledFn fn = encode_fn();
     const cuuint64_t dims[3] = {(cuuint64_t)a.seq_k, (cuuint64_t)a.kv_heads, (cuuint64_t)a.batch};
     const cuuint64_t strides[2] = {(cuuint64_t)a.bias_stride[1] * 4, (cuuint64_t)a.bias_stride[0] * 4};
@@ -465,7 +549,12 @@ int launch_t(const PolyPassArgs& a, cudaStream_t st) {
   p.seq_k = a.seq_k;
   p.heads = a.heads;
   p.kv_heads = a.kv_heads;
-  p.m_tiles = (a.seq_q + 2 * BM - 1) / (2 * BM);
+  p.m_tiles = PACKED ? a.seq_q / (2 * BM) + pk->seqs : (a.seq_q + 2 * BM - 1) / (2 * BM);   // pairs or slots of them
+  if (PACKED) p.pk = *pk;
+  p.bias = a.bias;
+  p.bias_stride = a.bias_stride[1];
+  p.sc_in = SOFTCLAMP ? a.scale / a.softclamp : 0.f;
+  p.sc_out = a.softclamp;
   p.causal = a.causal;
   p.off_tiles = a.causal ? a.causal_offset / BN : 0;
   p.sl2 = a.scale * kLog2e;
@@ -484,12 +573,13 @@ int launch_t(const PolyPassArgs& a, cudaStream_t st) {
   // dispatch groups: whole GQA groups whose K / V (2 x seq_k x D x 2 bytes per
   // kv head) fit in ~32 MB of L2
   const int rep_h = a.heads / a.kv_heads;
-  const size_t kv_bytes = (size_t)a.seq_k * D * 4;
+  const int kv_rows = PACKED && pk->max_len > 0 ? std::min(pk->max_len, a.seq_k) : a.seq_k;
+  const size_t kv_bytes = (size_t)kv_rows * D * 4;
   const int grp_kv = (int)std::max<size_t>(1, (32u << 20) / std::max<size_t>(kv_bytes, 1));
   p.n_bh = a.batch * a.heads;
   p.grp_bh = std::min(p.n_bh, grp_kv * rep_h);
   dim3 grid((unsigned)(p.n_bh * p.m_tiles));
-  pass_fwd_tc2_kernel<T, HAS_BIAS, D><<<grid, kThreads, L2::kAlloc, st>>>(tq, tk, tv, tb, p);
+  pass_fwd_tc2_kernel<T, HAS_BIAS, D, PACKED, SOFTCLAMP><<<grid, kThreads, L2::kAlloc, st>>>(tq, tk, tv, tb, p);
   note_launch(1);
   return cuda_status(cudaGetLastError(), "pass_fwd_tc2 launch");
 }
@@ -511,10 +601,40 @@ namespace {
 template <int D>
 int launch_d(const PolyPassArgs& a, cudaStream_t s) {
   if (a.dtype == POLY_BF16)
-    return a.bias ? launch_t<__nv_bfloat16, true, D>(a, s) : launch_t<__nv_bfloat16, false, D>(a, s);
-  return a.bias ? launch_t<__half, true, D>(a, s) : launch_t<__half, false, D>(a, s);
+    return a.bias ? launch_t<__nv_bfloat16, true, D, false, false>(a, nullptr, s)
+                  : launch_t<__nv_bfloat16, false, D, false, false>(a, nullptr, s);
+  return a.bias ? launch_t<__half, true, D, false, false>(a, nullptr, s)
+                : launch_t<__half, false, D, false, false>(a, nullptr, s);
+}
+
+template <typename T, int D>
+int launch_packed(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s) {
+  if (a.softclamp > 0.f)
+    return a.bias ? launch_t<T, true, D, true, true>(a, &q, s) : launch_t<T, false, D, true, true>(a, &q, s);
+  return a.bias ? launch_t<T, true, D, true, false>(a, &q, s) : launch_t<T, false, D, true, false>(a, &q, s);
 }
 }  // namespace
+
+// 16-bit, d = 64 or 128, every row 16-byte aligned and within TMA's strides
+// (the batch stride is not used: the maps get the rows of one batch element).
+bool packed_fwd_tc_eligible(const PolyPassArgs& a) {
+  if (a.dtype != POLY_BF16 && a.dtype != POLY_F16) return false;
+  if (a.head_dim != 64 && a.head_dim != 128) return false;
+  const int64_t* st[5] = {a.q_stride, a.k_stride, a.v_stride, a.out_stride, a.epi_out ? a.epi_out_stride : a.out_stride};
+  for (const int64_t* t : st)
+    if (!strides_ok(t + 1, 2)) return false;
+  if (a.epi_out && (!strides_ok(a.epi_mul_stride + 1, 2) || !aligned16(a.epi_mul) || !aligned16(a.epi_out))) return false;
+  return aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.out);
+}
+
+int launch_packed_fwd_tc(PolyPassArgs a, const PackedSeqs& q, cudaStream_t s) {
+  // one batch element: any valid stride
+  a.q_stride[0] = a.k_stride[0] = a.v_stride[0] = 8;
+  a.out_stride[0] = a.lse_stride[0] = a.bias_stride[0] = a.epi_mul_stride[0] = a.epi_out_stride[0] = 0;
+  if (a.head_dim == 128)
+    return a.dtype == POLY_BF16 ? launch_packed<__nv_bfloat16, 128>(a, q, s) : launch_packed<__half, 128>(a, q, s);
+  return a.dtype == POLY_BF16 ? launch_packed<__nv_bfloat16, 64>(a, q, s) : launch_packed<__half, 64>(a, q, s);
+}
 
 int launch_pass_fwd_tc2(const PolyPassArgs& a, cudaStream_t s) {
   return a.head_dim == 128 ? launch_d<128>(a, s) : launch_d<64>(a, s);

@@ -82,6 +82,17 @@ int check_fwd(const PolyPackedArgs* a) {
   return check_packed(a->pass, a->cu_seqlens, a->seqs, a->max_len);
 }
 
+enum class Kind { kSimt, kTc };
+
+// The tcgen05 kernels take the row maximum on unscaled scores: no negative scale.
+Kind choose_fwd(const PolyPackedArgs& a) {
+  return packed_fwd_tc_eligible(a.pass) && a.pass.scale >= 0.f ? Kind::kTc : Kind::kSimt;
+}
+
+const char* fwd_name(Kind k) { return k == Kind::kTc ? "tc100" : "simt"; }
+
+bool bwd_on_tc(const PolyPackedBwdArgs& a) { return packed_bwd_tc_eligible(a.bwd, a.seqs); }
+
 int check_bwd(const PolyPackedBwdArgs* a) {
   if (!a) return fail(POLY_EINVAL, "null args");
   return check_packed(a->bwd.fwd, a->cu_seqlens, a->seqs, a->max_len);
@@ -99,12 +110,12 @@ size_t poly_sizeof_packed_bwd_args(void) { return sizeof(PolyPackedBwdArgs); }
 
 const char* poly_packed_pass_fwd_kernel_name(const PolyPackedArgs* a) {
   if (check_fwd(a) != POLY_OK) return "invalid";
-  return "simt";
+  return fwd_name(choose_fwd(*a));
 }
 
 const char* poly_packed_pass_bwd_kernel_name(const PolyPackedBwdArgs* a) {
   if (check_bwd(a) != POLY_OK) return "invalid";
-  return "simt";
+  return bwd_on_tc(*a) ? "tc100" : "simt";
 }
 
 int poly_packed_pass_fwd(const PolyPackedArgs* a, void* stream) {
@@ -122,12 +133,13 @@ int poly_packed_pass_fwd(const PolyPackedArgs* a, void* stream) {
     const int rz = zero_rest(z, q, (cudaStream_t)stream);
     if (rz) return rz;
   }
+  if (choose_fwd(*a) == Kind::kTc) return launch_packed_fwd_tc(a->pass, q, (cudaStream_t)stream);
   return launch_packed_fwd_simt(a->pass, q, (cudaStream_t)stream);
 }
 
 size_t poly_packed_pass_bwd_workspace_size(const PolyPackedBwdArgs* a) {
   if (check_bwd(a) != POLY_OK) return 0;
-  return packed_bwd_simt_workspace(a->bwd);
+  return bwd_on_tc(*a) ? packed_bwd_tc_workspace(a->bwd, a->seqs) : packed_bwd_simt_workspace(a->bwd);
 }
 
 int poly_packed_pass_bwd(const PolyPackedBwdArgs* a, void* stream) {
@@ -152,6 +164,7 @@ int poly_packed_pass_bwd(const PolyPackedBwdArgs* a, void* stream) {
     const int rz = zero_rest(z, q, (cudaStream_t)stream);
     if (rz) return rz;
   }
+  if (bwd_on_tc(*a)) return launch_packed_bwd_tc(b, q, (cudaStream_t)stream);
   return launch_packed_bwd_simt(b, q, (cudaStream_t)stream);
 }
 

@@ -220,6 +220,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Rows from `from` on of a [ROWS][64 ATOMS] 16-bit tile in 128-byte-swizzled atoms
+// of 64 columns, as zeros (the swizzle stays inside a row). The caller's threads
+// tid = 0 .. n - 1 share the work; a proxy fence has to follow.
+template <int ROWS, int ATOMS>
+__device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int from, int tid, int n) {
+#pragma unroll
+  for (int at = 0; at < ATOMS; ++at)
+    for (int i = from * 8 + tid; i < ROWS * 8; i += n)
+      *reinterpret_cast<uint4*>(tile + at * (ROWS * 128) + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+}
+
 // ---------------------------------------------------------------- MMA
 // Shared-memory matrix descriptor, 128-byte swizzle (layout type 2), sm_100
 // descriptor version 1. lbo / sbo in bytes.
