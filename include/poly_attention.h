@@ -250,7 +250,17 @@ POLY_API int poly_head_rmsnorm(const PolyHeadNorm* norms, int n, void* stream);
  * whole sequence per CTA. Bias, softclamp, grouped heads and the epilogue
  * product as in poly_pass_fwd; masks, v_mul and causal_offset are
  * POLY_EUNSUPPORTED. A row whose every key is dead (bias <= -FLT_MAX / 2) gets
- * out = 0 and lse = -FLT_MAX, and no gradient.
+ * out = 0 and lse = -FLT_MAX, and no gradient. epi_out is epi_mul times the
+ * unrounded out.
+ *
+ * out_lo (optional, out's layout; 16-bit dtypes): what rounding took off out,
+ * rounded itself. The backward subtracts dout . out from every entry of a row of
+ * dP, so an error of out there is common to the row and does not average out
+ * over the keys: given out_lo it uses out + out_lo.
+ *
+ * v_left, v_right (backward, optional, dv's layout): the values were the product
+ * v_left * v_right (the chain's V' = v * msg). dv then receives the gradient of
+ * v_left and dv_right that of v_right, each rounded once.
  */
 typedef struct PolyPackedArgs {
   PolyPassArgs pass;
@@ -259,6 +269,7 @@ typedef struct PolyPackedArgs {
   int32_t max_len;
   int32_t zero_rest;
   int32_t reserved;
+  void* out_lo;
 } PolyPackedArgs;
 
 typedef struct PolyPackedBwdArgs {
@@ -268,6 +279,10 @@ typedef struct PolyPackedBwdArgs {
   int32_t max_len;
   int32_t zero_rest;
   int32_t reserved;
+  const void* out_lo;                                /* as bwd.fwd.out | NULL */
+  const void* v_left;   int64_t v_left_stride[2];    /* (head, row) elements | NULL */
+  const void* v_right;  int64_t v_right_stride[2];
+  void* dv_right;       int64_t dv_right_stride[2];
 } PolyPackedBwdArgs;
 
 POLY_API int poly_packed_pass_fwd(const PolyPackedArgs* args, void* stream);

@@ -200,14 +200,18 @@ __global__ void __launch_bounds__(256) packed_bwd_prep_kernel(const PolyPassBwdA
   if (live) {
     const T* o = (const T*)a.fwd.out + h * a.fwd.out_stride[1] + row * a.fwd.out_stride[2] + sub * (D / 8);
     const T* g = (const T*)a.dout + h * a.dout_stride[1] + row * a.dout_stride[2] + sub * (D / 8);
+    const T* ol = q.out_lo ? (const T*)q.out_lo + h * a.fwd.out_stride[1] + row * a.fwd.out_stride[2] + sub * (D / 8) : nullptr;
 #pragma unroll
     for (int v8 = 0; v8 < D / 64; ++v8) {
       const uint4 ov = *reinterpret_cast<const uint4*>(o + v8 * 8);
       const uint4 gv = *reinterpret_cast<const uint4*>(g + v8 * 8);
+      uint4 lv = make_uint4(0u, 0u, 0u, 0u);
+      if (ol) lv = *reinterpret_cast<const uint4*>(ol + v8 * 8);
       const T* op = reinterpret_cast<const T*>(&ov);
       const T* gp = reinterpret_cast<const T*>(&gv);
+      const T* lp = reinterpret_cast<const T*>(&lv);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += to_f32(op[e]) * to_f32(gp[e]);
+      for (int e = 0; e < 8; ++e) s += (to_f32(op[e]) + to_f32(lp[e])) * to_f32(gp[e]);
     }
   }
   s += __shfl_xor_sync(0xffffffffu, s, 1);
@@ -268,6 +272,32 @@ struct BwdWs {
   int nq_pad;
   size_t bytes;
 };
+
+// 32 features of dV = a[] as the gradients of a product's two factors (packed
+// sequences whose values were v_left * v_right): dv for v_left, dv_right for v_right.
+template <typename T>
+__device__ __forceinline__ void store_dv_factors(const PackedSeqs& q, int kvh, int64_t row, int col, const uint32_t (&a)[32],
+                                                 T* dv) {
+  const T* vl = (const T*)q.v_left + kvh * q.v_left_stride[0] + row * q.v_left_stride[1] + col;
+  const T* vr = (const T*)q.v_right + kvh * q.v_right_stride[0] + row * q.v_right_stride[1] + col;
+  T* dr = (T*)q.dv_right + kvh * q.dv_right_stride[0] + row * q.dv_right_stride[1] + col;
+#pragma unroll
+  for (int q8 = 0; q8 < 4; ++q8) {
+    const uint4 l4 = *reinterpret_cast<const uint4*>(vl + q8 * 8), r4 = *reinterpret_cast<const uint4*>(vr + q8 * 8);
+    const T* lp = reinterpret_cast<const T*>(&l4);
+    const T* rp = reinterpret_cast<const T*>(&r4);
+    uint4 x4, y4;
+    uint32_t *xp = &x4.x, *yp = &y4.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float g0 = __uint_as_float(a[q8 * 8 + 2 * e]), g1 = __uint_as_float(a[q8 * 8 + 2 * e + 1]);
+      xp[e] = pk<T>(g0 * to_f32(rp[2 * e]), g1 * to_f32(rp[2 * e + 1]));
+      yp[e] = pk<T>(g0 * to_f32(lp[2 * e]), g1 * to_f32(lp[2 * e + 1]));
+    }
+    *reinterpret_cast<uint4*>(dv + q8 * 8) = x4;
+    *reinterpret_cast<uint4*>(dr + q8 * 8) = y4;
+  }
+}
 
 // Workspace: fp32 dQ accumulator [b * heads][seq_q][D], then the log2-domain
 // lse and delta rows padded to the query tile BQ.

@@ -426,7 +426,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int u = 0; u < 32; ++u) a[u] = 0u;
         }
-        if (key_ok) {
+        if (PACKED && key_ok && hw == 1 && p.pk.v_left) {
+          store_dv_factors<T>(p.pk, kvh, (int64_t)first + j, half * 32, a, dst + half * 32);
+        } else if (key_ok) {
 #pragma unroll
           for (int q8 = 0; q8 < 4; ++q8) {
             uint4 w4;
@@ -605,15 +607,20 @@ int launch_pass_bwd_tc(const PolyPassBwdArgs& a, cudaStream_t s) {
 
 // Rows as packed_fwd_tc_eligible wants them (batch strides are not used), and
 // few enough slot rows for TMA's 32-bit coordinates.
-bool packed_bwd_tc_eligible(const PolyPassBwdArgs& a, int seqs) {
+bool packed_bwd_tc_eligible(const PolyPackedBwdArgs& pa) {
+  const PolyPassBwdArgs& a = pa.bwd;
   const PolyPassArgs& f = a.fwd;
   if (f.dtype != POLY_BF16 && f.dtype != POLY_F16) return false;
   if (f.head_dim != D && f.head_dim != 128) return false;
-  if (f.seq_q / BK + seqs >= (1 << 23)) return false;
+  if (f.seq_q / BK + pa.seqs >= (1 << 23)) return false;
   const int64_t* st[8] = {f.q_stride, f.k_stride, f.v_stride, f.out_stride, a.dout_stride, a.dq_stride, a.dk_stride, a.dv_stride};
   for (const int64_t* t : st)
     if (!strides_ok(t + 1, 2)) return false;
-  return aligned16(f.q) && aligned16(f.k) && aligned16(f.v) && aligned16(f.out) && aligned16(a.dout) &&
+  if (pa.v_left && (!strides_ok(pa.v_left_stride, 2) || !strides_ok(pa.v_right_stride, 2) ||
+                    !strides_ok(pa.dv_right_stride, 2) || !aligned16(pa.v_left) || !aligned16(pa.v_right) ||
+                    !aligned16(pa.dv_right)))
+    return false;
+  return aligned16(f.q) && aligned16(f.k) && aligned16(f.v) && aligned16(f.out) && aligned16(pa.out_lo) && aligned16(a.dout) &&
          aligned16(a.dq) && aligned16(a.dk) && aligned16(a.dv);
 }
 

@@ -416,7 +416,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int u = 0; u < 32; ++u) a[u] = 0u;
         }
-        if (key_ok) {
+        if (PACKED && key_ok && hw == 1 && p.pk.v_left) {
+          store_dv_factors<T>(p.pk, kvh, (int64_t)first + j, part * 32, a, dst + part * 32);
+        } else if (key_ok) {
 #pragma unroll
           for (int q8 = 0; q8 < 4; ++q8) {
             uint4 w4;

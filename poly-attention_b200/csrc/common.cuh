@@ -92,13 +92,20 @@ int rotary(const PolyRotaryArgs* args, cudaStream_t s);
 struct PackedSeqs {
   const int* cu;
   int seqs, total, max_len;
+  void* out_lo;         // rounding residue of out (forward: written, backward: read) | NULL
+  // backward of values that are a product: the factors and the second gradient | NULL
+  const void* v_left; int64_t v_left_stride[2];
+  const void* v_right; int64_t v_right_stride[2];
+  void* dv_right; int64_t dv_right_stride[2];
 };
 int launch_packed_fwd_simt(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s);
 int launch_packed_bwd_simt(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s);
 size_t packed_bwd_simt_workspace(const PolyPassBwdArgs& a);
-bool packed_fwd_tc_eligible(const PolyPassArgs& a);
+bool packed_fwd_tc_eligible(const PolyPassArgs& a, const void* out_lo);
 int launch_packed_fwd_tc(PolyPassArgs a, const PackedSeqs& q, cudaStream_t s);
-bool packed_bwd_tc_eligible(const PolyPassBwdArgs& a, int seqs);
+int launch_packed_fwd_small(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s);
+int launch_packed_bwd_small(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s);
+bool packed_bwd_tc_eligible(const PolyPackedBwdArgs& a);
 int launch_packed_bwd_tc(PolyPassBwdArgs a, const PackedSeqs& q, cudaStream_t s);
 int launch_packed_bwd_tc128(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s);
 size_t packed_bwd_tc_workspace(const PolyPassBwdArgs& a, int seqs);

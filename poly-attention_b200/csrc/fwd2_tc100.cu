@@ -488,6 +488,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int t = 0; t < 4; ++t)
               w[t] = pk2<T>(__uint_as_float(o[q4 * 8 + 2 * t]) * inv, __uint_as_float(o[q4 * 8 + 2 * t + 1]) * inv);
             *reinterpret_cast<uint4*>(out + c * 32 + q4 * 8) = val;
+            if (PACKED && p.pk.out_lo) {
+              uint4 lv;
+              uint32_t* lw = &lv.x;
+#pragma unroll
+              for (int t = 0; t < 4; ++t) {
+                const float2 a2 = up2<T>(w[t]);
+                lw[t] = pk2<T>(__uint_as_float(o[q4 * 8 + 2 * t]) * inv - a2.x,
+                               __uint_as_float(o[q4 * 8 + 2 * t + 1]) * inv - a2.y);
+              }
+              *reinterpret_cast<uint4*>((T*)p.pk.out_lo + h * p.out_stride[1] + orow * p.out_stride[2] + c * 32 +
+                                        q4 * 8) = lv;
+            }
             if (eo) {
               const uint4 mv = *reinterpret_cast<const uint4*>(em + c * 32 + q4 * 8);
               const uint32_t* mw = &mv.x;
@@ -495,7 +507,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               uint32_t* ew = &ev.x;
 #pragma unroll
               for (int t = 0; t < 4; ++t) {
-                const float2 a2 = up2<T>(w[t]), m2 = up2<T>(mw[t]);
+                const float2 m2 = up2<T>(mw[t]);
+                const float2 a2 = PACKED ? make_float2(__uint_as_float(o[q4 * 8 + 2 * t]) * inv,
+                                                       __uint_as_float(o[q4 * 8 + 2 * t + 1]) * inv)
+                                         : up2<T>(w[t]);
                 ew[t] = pk2<T>(a2.x * m2.x, a2.y * m2.y);
               }
               *reinterpret_cast<uint4*>(eo + c * 32 + q4 * 8) = ev;
@@ -617,14 +632,14 @@ int launch_packed(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s) {
 
 // 16-bit, d = 64 or 128, every row 16-byte aligned and within TMA's strides
 // (the batch stride is not used: the maps get the rows of one batch element).
-bool packed_fwd_tc_eligible(const PolyPassArgs& a) {
+bool packed_fwd_tc_eligible(const PolyPassArgs& a, const void* out_lo) {
   if (a.dtype != POLY_BF16 && a.dtype != POLY_F16) return false;
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   const int64_t* st[5] = {a.q_stride, a.k_stride, a.v_stride, a.out_stride, a.epi_out ? a.epi_out_stride : a.out_stride};
   for (const int64_t* t : st)
     if (!strides_ok(t + 1, 2)) return false;
   if (a.epi_out && (!strides_ok(a.epi_mul_stride + 1, 2) || !aligned16(a.epi_mul) || !aligned16(a.epi_out))) return false;
-  return aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.out);
+  return aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.out) && aligned16(out_lo);
 }
 
 int launch_packed_fwd_tc(PolyPassArgs a, const PackedSeqs& q, cudaStream_t s) {

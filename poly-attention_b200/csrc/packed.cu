@@ -29,7 +29,7 @@ int check_packed(const PolyPassArgs& a, const int32_t* cu, int seqs, int max_len
     return fail(POLY_EINVAL, "q, k, v, out and cu_seqlens are required");
   if (a.epi_out && !a.epi_mul) return fail(POLY_EINVAL, "epi_out requires epi_mul");
   if (!(a.scale == a.scale)) return fail(POLY_EINVAL, "scale is NaN");
-  // 16-row slots of every head fit the grid, rows the 32-bit tile arithmetic
+  // 8-row slots of every head fit the grid, rows the 32-bit tile arithmetic
   if (a.seq_q > (1 << 30) || seqs > (1 << 28) || (int64_t)(a.seq_q / 8 + seqs) > 0x7fffffff / a.heads)
     return fail(POLY_EUNSUPPORTED, "too many rows or sequences for one call");
   return POLY_OK;
@@ -82,16 +82,23 @@ int check_fwd(const PolyPackedArgs* a) {
   return check_packed(a->pass, a->cu_seqlens, a->seqs, a->max_len);
 }
 
-enum class Kind { kSimt, kTc };
+enum class Kind { kSimt, kTc, kSmall };
+
+bool short_sequences(int max_len) { return max_len > 0 && max_len <= 128; }
 
 // The tcgen05 kernels take the row maximum on unscaled scores: no negative scale.
 Kind choose_fwd(const PolyPackedArgs& a) {
-  return packed_fwd_tc_eligible(a.pass) && a.pass.scale >= 0.f ? Kind::kTc : Kind::kSimt;
+  if (!packed_fwd_tc_eligible(a.pass, a.out_lo)) return Kind::kSimt;   // the short kernel takes the same tensors
+  if (short_sequences(a.max_len)) return Kind::kSmall;
+  return a.pass.scale >= 0.f ? Kind::kTc : Kind::kSimt;
 }
 
-const char* fwd_name(Kind k) { return k == Kind::kTc ? "tc100" : "simt"; }
+Kind choose_bwd(const PolyPackedBwdArgs& a) {
+  if (!packed_bwd_tc_eligible(a)) return Kind::kSimt;
+  return short_sequences(a.max_len) ? Kind::kSmall : Kind::kTc;
+}
 
-bool bwd_on_tc(const PolyPackedBwdArgs& a) { return packed_bwd_tc_eligible(a.bwd, a.seqs); }
+const char* name_of(Kind k) { return k == Kind::kTc ? "tc100" : k == Kind::kSmall ? "small" : "simt"; }
 
 int check_bwd(const PolyPackedBwdArgs* a) {
   if (!a) return fail(POLY_EINVAL, "null args");
@@ -110,19 +117,24 @@ size_t poly_sizeof_packed_bwd_args(void) { return sizeof(PolyPackedBwdArgs); }
 
 const char* poly_packed_pass_fwd_kernel_name(const PolyPackedArgs* a) {
   if (check_fwd(a) != POLY_OK) return "invalid";
-  return fwd_name(choose_fwd(*a));
+  return name_of(choose_fwd(*a));
 }
 
 const char* poly_packed_pass_bwd_kernel_name(const PolyPackedBwdArgs* a) {
   if (check_bwd(a) != POLY_OK) return "invalid";
-  return bwd_on_tc(*a) ? "tc100" : "simt";
+  return name_of(choose_bwd(*a));
 }
 
 int poly_packed_pass_fwd(const PolyPackedArgs* a, void* stream) {
   const int rc = check_fwd(a);
   if (rc) return rc;
   if (a->pass.seq_q == 0 || a->seqs == 0) return POLY_OK;
-  const PackedSeqs q{a->cu_seqlens, a->seqs, a->pass.seq_q, a->max_len};
+  PackedSeqs q{};
+  q.cu = a->cu_seqlens;
+  q.seqs = a->seqs;
+  q.total = a->pass.seq_q;
+  q.max_len = a->max_len;
+  q.out_lo = a->out_lo;
   if (a->zero_rest) {
     const PolyPassArgs& f = a->pass;
     const int es = f.dtype == POLY_F32 ? 4 : 2;
@@ -130,16 +142,24 @@ int poly_packed_pass_fwd(const PolyPackedArgs* a, void* stream) {
     zero_add(z, f.out, f.heads, f.head_dim, es, f.out_stride[1], f.out_stride[2]);
     zero_add(z, f.epi_out, f.heads, f.head_dim, es, f.epi_out_stride[1], f.epi_out_stride[2]);
     zero_add(z, f.lse, f.heads, 1, 4, f.lse_stride[1], 1);
+    zero_add(z, a->out_lo, f.heads, f.head_dim, es, f.out_stride[1], f.out_stride[2]);
     const int rz = zero_rest(z, q, (cudaStream_t)stream);
     if (rz) return rz;
   }
-  if (choose_fwd(*a) == Kind::kTc) return launch_packed_fwd_tc(a->pass, q, (cudaStream_t)stream);
-  return launch_packed_fwd_simt(a->pass, q, (cudaStream_t)stream);
+  switch (choose_fwd(*a)) {
+    case Kind::kTc: return launch_packed_fwd_tc(a->pass, q, (cudaStream_t)stream);
+    case Kind::kSmall: return launch_packed_fwd_small(a->pass, q, (cudaStream_t)stream);
+    default: return launch_packed_fwd_simt(a->pass, q, (cudaStream_t)stream);
+  }
 }
 
 size_t poly_packed_pass_bwd_workspace_size(const PolyPackedBwdArgs* a) {
   if (check_bwd(a) != POLY_OK) return 0;
-  return bwd_on_tc(*a) ? packed_bwd_tc_workspace(a->bwd, a->seqs) : packed_bwd_simt_workspace(a->bwd);
+  switch (choose_bwd(*a)) {
+    case Kind::kTc: return packed_bwd_tc_workspace(a->bwd, a->seqs);
+    case Kind::kSmall: return 0;
+    default: return packed_bwd_simt_workspace(a->bwd);
+  }
 }
 
 int poly_packed_pass_bwd(const PolyPackedBwdArgs* a, void* stream) {
@@ -149,7 +169,22 @@ int poly_packed_pass_bwd(const PolyPackedBwdArgs* a, void* stream) {
   if (b.fwd.seq_q == 0 || a->seqs == 0) return POLY_OK;
   if (!b.fwd.lse || !b.dout || !b.dq || !b.dk || !b.dv)
     return fail(POLY_EINVAL, "backward needs fwd.out, fwd.lse, dout, dq, dk and dv");
-  const PackedSeqs q{a->cu_seqlens, a->seqs, b.fwd.seq_q, a->max_len};
+  if (!a->v_left != !a->v_right || !a->v_left != !a->dv_right)
+    return fail(POLY_EINVAL, "v_left, v_right and dv_right come together");
+  PackedSeqs q{};
+  q.cu = a->cu_seqlens;
+  q.seqs = a->seqs;
+  q.total = b.fwd.seq_q;
+  q.max_len = a->max_len;
+  q.out_lo = const_cast<void*>(a->out_lo);
+  q.v_left = a->v_left;
+  q.v_right = a->v_right;
+  q.dv_right = a->dv_right;
+  for (int i = 0; i < 2; ++i) {
+    q.v_left_stride[i] = a->v_left_stride[i];
+    q.v_right_stride[i] = a->v_right_stride[i];
+    q.dv_right_stride[i] = a->dv_right_stride[i];
+  }
   const size_t need = poly_packed_pass_bwd_workspace_size(a);
   if (need && (!b.workspace || b.workspace_bytes < need))
     return fail(POLY_EINVAL, "workspace too small: need " + std::to_string(need) + " bytes");
@@ -161,11 +196,15 @@ int poly_packed_pass_bwd(const PolyPackedBwdArgs* a, void* stream) {
     zero_add(z, b.dk, f.kv_heads, f.head_dim, es, b.dk_stride[1], b.dk_stride[2]);
     zero_add(z, b.dv, f.kv_heads, f.head_dim, es, b.dv_stride[1], b.dv_stride[2]);
     zero_add(z, b.dbias, f.kv_heads, 1, 4, b.dbias_stride[1], 1);
+    zero_add(z, a->dv_right, f.kv_heads, f.head_dim, es, a->dv_right_stride[0], a->dv_right_stride[1]);
     const int rz = zero_rest(z, q, (cudaStream_t)stream);
     if (rz) return rz;
   }
-  if (bwd_on_tc(*a)) return launch_packed_bwd_tc(b, q, (cudaStream_t)stream);
-  return launch_packed_bwd_simt(b, q, (cudaStream_t)stream);
+  switch (choose_bwd(*a)) {
+    case Kind::kTc: return launch_packed_bwd_tc(b, q, (cudaStream_t)stream);
+    case Kind::kSmall: return launch_packed_bwd_small(b, q, (cudaStream_t)stream);
+    default: return launch_packed_bwd_simt(b, q, (cudaStream_t)stream);
+  }
 }
 
 }  // extern "C"

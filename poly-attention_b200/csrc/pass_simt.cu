@@ -177,7 +177,9 @@ __global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(PolyPassArgs
     if (col < d) {
       const T o = from_f32<T>(acc[t]);
       out[col] = o;
-      if (vo) vo[col] = from_f32<T>(to_f32(vm[col]) * to_f32(o));
+      if (vo) vo[col] = from_f32<T>(to_f32(vm[col]) * (PACKED ? acc[t] : to_f32(o)));
+      if (PACKED && pk.out_lo)
+        ((T*)pk.out_lo + c.h * a.out_stride[1] + io * a.out_stride[2])[col] = from_f32<T>(acc[t] - to_f32(o));
     }
   }
   if (a.lse && lane == 0) a.lse[c.b * a.lse_stride[0] + c.h * a.lse_stride[1] + io] = lse;
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(PolyPassArgs
 // log-sum-exp gradient, poly_attention/flash_poly_attention.py:280-284)
 // (rows of packed sequences are the rows of one batch element here)
 template <typename T, bool PACKED>
-__global__ void bwd_delta_kernel(const PolyPassBwdArgs a, float* delta, int* fb_count) {
+__global__ void bwd_delta_kernel(const PolyPassBwdArgs a, float* delta, int* fb_count, const void* out_lo) {
   const int64_t warp = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   const int64_t rows = (int64_t)a.fwd.batch * a.fwd.heads * a.fwd.seq_q;
@@ -197,7 +199,8 @@ __global__ void bwd_delta_kernel(const PolyPassBwdArgs a, float* delta, int* fb_
   const T* o = (const T*)a.fwd.out + b * a.fwd.out_stride[0] + h * a.fwd.out_stride[1] + (int64_t)i * a.fwd.out_stride[2];
   const T* g = (const T*)a.dout + b * a.dout_stride[0] + h * a.dout_stride[1] + (int64_t)i * a.dout_stride[2];
   float s = 0.f;
-  for (int t = lane; t < a.fwd.head_dim; t += 32) s += to_f32(o[t]) * to_f32(g[t]);
+  const T* ol = PACKED && out_lo ? (const T*)out_lo + h * a.fwd.out_stride[1] + (int64_t)i * a.fwd.out_stride[2] : nullptr;
+  for (int t = lane; t < a.fwd.head_dim; t += 32) s += (to_f32(o[t]) + (ol ? to_f32(ol[t]) : 0.f)) * to_f32(g[t]);
   s = warp_sum(s);
   const float lse_i = a.fwd.lse[b * a.fwd.lse_stride[0] + h * a.fwd.lse_stride[1] + i];
   int count = 0;
@@ -422,7 +425,16 @@ __global__ void __launch_bounds__(kWarps * 32) pass_bwd_dkv_simt_kernel(PolyPass
     const int col = lane + 32 * t;
     if (col < d) {
       dkp[col] = from_f32<T>(dk[t] * a.scale);
-      dvp[col] = from_f32<T>(dv[t]);
+      if (PACKED && pk.v_left) {
+        const int64_t row = first + j;
+        const T* vl = (const T*)pk.v_left + kvh * pk.v_left_stride[0] + row * pk.v_left_stride[1];
+        const T* vr = (const T*)pk.v_right + kvh * pk.v_right_stride[0] + row * pk.v_right_stride[1];
+        dvp[col] = from_f32<T>(dv[t] * to_f32(vr[col]));
+        ((T*)pk.dv_right + kvh * pk.dv_right_stride[0] + row * pk.dv_right_stride[1])[col] =
+            from_f32<T>(dv[t] * to_f32(vl[col]));
+      } else {
+        dvp[col] = from_f32<T>(dv[t]);
+      }
     }
   }
   if (ab.dbias && lane == 0) ab.dbias[b * ab.dbias_stride[0] + kvh * ab.dbias_stride[1] + first + j] = db;
@@ -453,11 +465,11 @@ int launch_bwd_t(const PolyPassBwdArgs& a, const PackedSeqs* pk, cudaStream_t s)
   dim3 gk(row_ctas(a.fwd.seq_k, pk), a.fwd.batch * a.fwd.kv_heads);
   const unsigned gd = (unsigned)((rows + 7) / 8);
   if (pk) {
-    bwd_delta_kernel<T, true><<<gd, 256, 0, s>>>(a, delta, fb_count);
+    bwd_delta_kernel<T, true><<<gd, 256, 0, s>>>(a, delta, fb_count, pk->out_lo);
     pass_bwd_dq_simt_kernel<T, DMAX, true><<<gq, kWarps * 32, 0, s>>>(a, delta, fb_count, *pk);
     pass_bwd_dkv_simt_kernel<T, DMAX, true><<<gk, kWarps * 32, 0, s>>>(a, delta, fb_count, *pk);
   } else {
-    bwd_delta_kernel<T, false><<<gd, 256, 0, s>>>(a, delta, fb_count);
+    bwd_delta_kernel<T, false><<<gd, 256, 0, s>>>(a, delta, fb_count, nullptr);
     pass_bwd_dq_simt_kernel<T, DMAX, false><<<gq, kWarps * 32, 0, s>>>(a, delta, fb_count, PackedSeqs{});
     pass_bwd_dkv_simt_kernel<T, DMAX, false><<<gk, kWarps * 32, 0, s>>>(a, delta, fb_count, PackedSeqs{});
   }

@@ -9,70 +9,75 @@
 // pass kernels: scale, softclamp, causal (top-left aligned), per-key bias in
 // the log2 domain with dead keys (bias <= -FLT_MAX / 2) dropped, lse in
 // natural-log units.
+//
+// PACKED: one CTA per (packed sequence, head) where the caller bounds the
+// lengths by 128; the CTA takes the rows of its sequence.
 #include <cfloat>
 #include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
+#include "mma_sync.cuh"
+#include "packed.cuh"
 #include "tc_ptx.cuh"
 
 namespace poly {
 namespace {
+using namespace ms;
 
 constexpr int kMaxN = 128;
 
-__device__ __forceinline__ void cp16(uint32_t sa, const void* g, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sa), "l"(g), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(a));
-}
-__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(a));
-}
+// Two neighbouring features of a packed sequence's output row (a's pointers are
+// at the sequence): out, its rounding residue, the epilogue's product.
 template <typename T>
-__device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pk2(float lo, float hi) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) return tc::pack_bf16(lo, hi);
-  else return tc::pack_f16(lo, hi);
+__device__ __forceinline__ void store_packed(const PolyPassArgs& a, const PackedSeqs& pk, int h, int row, int c, float x,
+                                             float y) {
+  const int64_t at = h * a.out_stride[1] + (int64_t)row * a.out_stride[2] + c;
+  const uint32_t w = pk2<T>(x, y);
+  *reinterpret_cast<uint32_t*>((T*)a.out + at) = w;
+  if (pk.out_lo) {
+    const T* e = reinterpret_cast<const T*>(&w);
+    const int64_t first = (int64_t)packed_at(pk.cu, blockIdx.x / a.heads, pk.total) * a.out_stride[2];
+    *reinterpret_cast<uint32_t*>((T*)pk.out_lo + first + at) = pk2<T>(x - to_f32(e[0]), y - to_f32(e[1]));
+  }
+  if (a.epi_out) {
+    const uint32_t mw = *reinterpret_cast<const uint32_t*>((const T*)a.epi_mul + h * a.epi_mul_stride[1] +
+                                                           (int64_t)row * a.epi_mul_stride[2] + c);
+    const T* m = reinterpret_cast<const T*>(&mw);
+    *reinterpret_cast<uint32_t*>((T*)a.epi_out + h * a.epi_out_stride[1] + (int64_t)row * a.epi_out_stride[2] + c) =
+        pk2<T>(x * to_f32(m[0]), y * to_f32(m[1]));
+  }
 }
 
-// byte offset of 16-byte chunk ch of row r in a [kMaxN][D] tile
-template <int D>
-__device__ __forceinline__ uint32_t soff(int r, int ch) {
-  return (uint32_t)(r * (D * 2) + ((ch ^ (r & 7)) << 4));
-}
-
-template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP>
-__global__ void __launch_bounds__(256) pass_small_kernel(const PolyPassArgs a) {
+template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP, bool PACKED>
+__global__ void __launch_bounds__(256) pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
   constexpr int KS = D / 16, NB = D / 8, CH = D / 8;
   constexpr int KNB = kMaxN / 8;   // key n-blocks
-  const int nq = a.seq_q, nk = a.seq_k;
+  const int bh = blockIdx.x;
+  const int b = PACKED ? 0 : bh / a.heads, h = bh - (PACKED ? bh / a.heads : b) * a.heads;
+  int nq = a.seq_q, nk = a.seq_k;
+  if constexpr (PACKED) {
+    const int first = packed_at(pk.cu, bh / a.heads, pk.total);
+    nq = nk = min(packed_at(pk.cu, bh / a.heads + 1, pk.total) - first, pk.max_len);
+    if (nk <= 0) return;
+    const int64_t f = first;
+    a.q = (const T*)a.q + f * a.q_stride[2];
+    a.k = (const T*)a.k + f * a.k_stride[2];
+    a.v = (const T*)a.v + f * a.v_stride[2];
+    a.out = (T*)a.out + f * a.out_stride[2];
+    if (HAS_BIAS) a.bias += f;
+    if (a.lse) a.lse += f;
+    if (a.epi_out) {
+      a.epi_mul = (const T*)a.epi_mul + f * a.epi_mul_stride[2];
+      a.epi_out = (T*)a.epi_out + f * a.epi_out_stride[2];
+    }
+  }
   const int kp = (nk + 15) & ~15;   // keys padded to the P.V K step
   // shared memory sized to the keys present: K [kp][D], V [kp][D], bias [kp]
   extern __shared__ __align__(16) uint8_t sm[];
   const uint32_t sK = tc::smem_u32(sm), sV = sK + kp * D * 2;
   float* sB = reinterpret_cast<float*>(sm + 2 * kp * D * 2);
 
-  const int bh = blockIdx.x;
-  const int b = bh / a.heads, h = bh - b * a.heads;
   const int g = h / (a.heads / a.kv_heads);
   const T* kg = (const T*)a.k + b * a.k_stride[0] + g * a.k_stride[1];
   const T* vg = (const T*)a.v + b * a.v_stride[0] + g * a.v_stride[1];
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(256) pass_small_kernel(const PolyPassArgs a) {
   // A row whose every key is excluded (only dead keys can do that here) gets
   // the reference's -finfo.max result: the uniform average over the keys that
   // are not both causally masked and dead, lse = -FLT_MAX.
-  if (HAS_BIAS && (m0 == -INFINITY || m1 == -INFINITY)) {
+  if (!PACKED && HAS_BIAS && (m0 == -INFINITY || m1 == -INFINITY)) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int row = hf ? r1 : r0;
@@ -219,38 +224,52 @@ __global__ void __launch_bounds__(256) pass_small_kernel(const PolyPassArgs a) {
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const int c = n * 8 + 2 * tq;
-    if (r0 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r0 * a.out_stride[2] + c) = pk2<T>(o[n][0] * j0, o[n][1] * j0);
-    if (r1 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r1 * a.out_stride[2] + c) = pk2<T>(o[n][2] * j1, o[n][3] * j1);
+    if constexpr (PACKED) {
+      if (r0 < nq) store_packed<T>(a, pk, h, r0, c, o[n][0] * j0, o[n][1] * j0);
+      if (r1 < nq) store_packed<T>(a, pk, h, r1, c, o[n][2] * j1, o[n][3] * j1);
+    } else {
+      if (r0 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r0 * a.out_stride[2] + c) = pk2<T>(o[n][0] * j0, o[n][1] * j0);
+      if (r1 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r1 * a.out_stride[2] + c) = pk2<T>(o[n][2] * j1, o[n][3] * j1);
+    }
   }
   if (a.lse && tq == 0) {
     float* lb = a.lse + b * a.lse_stride[0] + h * a.lse_stride[1];
-    if (r0 < nq) lb[r0] = fb0 ? -FLT_MAX : (m0 + __log2f(l0)) * kLn2;
-    if (r1 < nq) lb[r1] = fb1 ? -FLT_MAX : (m1 + __log2f(l1)) * kLn2;
+    if (r0 < nq) lb[r0] = fb0 || (PACKED && l0 == 0.f) ? -FLT_MAX : (m0 + __log2f(l0)) * kLn2;
+    if (r1 < nq) lb[r1] = fb1 || (PACKED && l1 == 0.f) ? -FLT_MAX : (m1 + __log2f(l1)) * kLn2;
   }
 }
 
-template <typename T, int D, bool B, bool C>
-int launch_t(const PolyPassArgs& a, cudaStream_t s) {
+template <typename T, int D, bool B, bool C, bool PACKED>
+int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   constexpr int smem = 2 * kMaxN * D * 2 + kMaxN * 4;
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
   std::call_once(once, [] {
-    err = cudaFuncSetAttribute(pass_small_kernel<T, D, B, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    err = cudaFuncSetAttribute(pass_small_kernel<T, D, B, C, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(small)");
-  const int threads = 32 * ((a.seq_q + 15) / 16);
-  const int kp = (a.seq_k + 15) & ~15;
+  const int nq = PACKED ? pk->max_len : a.seq_q, nk = PACKED ? pk->max_len : a.seq_k;
+  const int threads = 32 * ((nq + 15) / 16);
+  const int kp = (nk + 15) & ~15;
   const int bytes = 2 * kp * D * 2 + kp * 4;   // <= smem (the attribute's maximum)
-  pass_small_kernel<T, D, B, C><<<a.batch * a.heads, threads, bytes, s>>>(a);
+  const unsigned grid = (unsigned)((PACKED ? pk->seqs : a.batch) * a.heads);
+  pass_small_kernel<T, D, B, C, PACKED><<<grid, threads, bytes, s>>>(a, PACKED ? *pk : PackedSeqs{});
   note_launch(1);
   return cuda_status(cudaGetLastError(), "pass_small launch");
 }
 
-template <typename T, int D>
-int launch_d(const PolyPassArgs& a, cudaStream_t s) {
+template <typename T, int D, bool PACKED>
+int launch_d(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   const bool bias = a.bias != nullptr, sc = a.softclamp > 0.f;
-  if (sc) return bias ? launch_t<T, D, true, true>(a, s) : launch_t<T, D, false, true>(a, s);
-  return bias ? launch_t<T, D, true, false>(a, s) : launch_t<T, D, false, false>(a, s);
+  if (sc) return bias ? launch_t<T, D, true, true, PACKED>(a, pk, s) : launch_t<T, D, false, true, PACKED>(a, pk, s);
+  return bias ? launch_t<T, D, true, false, PACKED>(a, pk, s) : launch_t<T, D, false, false, PACKED>(a, pk, s);
+}
+
+template <bool PACKED>
+int launch_any(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
+  if (a.dtype == POLY_BF16)
+    return a.head_dim == 64 ? launch_d<__nv_bfloat16, 64, PACKED>(a, pk, s) : launch_d<__nv_bfloat16, 128, PACKED>(a, pk, s);
+  return a.head_dim == 64 ? launch_d<__half, 64, PACKED>(a, pk, s) : launch_d<__half, 128, PACKED>(a, pk, s);
 }
 
 bool al(const void* p, int bytes) { return ((uintptr_t)p % bytes) == 0; }
@@ -270,10 +289,9 @@ bool pass_small_eligible(const PolyPassArgs& a) {
   return true;
 }
 
-int launch_pass_small(const PolyPassArgs& a, cudaStream_t s) {
-  if (a.dtype == POLY_BF16)
-    return a.head_dim == 64 ? launch_d<__nv_bfloat16, 64>(a, s) : launch_d<__nv_bfloat16, 128>(a, s);
-  return a.head_dim == 64 ? launch_d<__half, 64>(a, s) : launch_d<__half, 128>(a, s);
+int launch_pass_small(const PolyPassArgs& a, cudaStream_t s) { return launch_any<false>(a, nullptr, s); }
+int launch_packed_fwd_small(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s) {
+  return launch_any<true>(a, &q, s);
 }
 
 }  // namespace poly

@@ -82,12 +82,14 @@ MAX_NORMS = 4
 
 class PolyPackedArgs(ctypes.Structure):
     _fields_ = [("fwd", PolyPassArgs), ("cu_seqlens", c_vp), ("seqs", c_i32), ("max_len", c_i32),
-                ("zero_rest", c_i32), ("reserved", c_i32)]
+                ("zero_rest", c_i32), ("reserved", c_i32), ("out_lo", c_vp)]
 
 
 class PolyPackedBwdArgs(ctypes.Structure):
     _fields_ = [("bwd", PolyPassBwdArgs), ("cu_seqlens", c_vp), ("seqs", c_i32), ("max_len", c_i32),
-                ("zero_rest", c_i32), ("reserved", c_i32)]
+                ("zero_rest", c_i32), ("reserved", c_i32), ("out_lo", c_vp),
+                ("v_left", c_vp), ("v_left_stride", I64x2), ("v_right", c_vp), ("v_right_stride", I64x2),
+                ("dv_right", c_vp), ("dv_right_stride", I64x2)]
 
 
 class PolyRotaryTensor(ctypes.Structure):

@@ -62,8 +62,10 @@ def _set(a, name, t):
     """A [total, heads, d] tensor (or [heads, total] fp32 vector) into its pointer and (batch, head, row) strides."""
     setattr(a, name, t.data_ptr())
     st = getattr(a, name + "_stride")
-    if t.dim() == 3:
+    if t.dim() == 3 and len(st) == 3:
         st[0], st[1], st[2] = 0, t.stride(1), t.stride(0)
+    elif t.dim() == 3:
+        st[0], st[1] = t.stride(1), t.stride(0)
     else:
         st[0], st[1] = 0, t.stride(0)
 
@@ -89,11 +91,13 @@ def _fill(a, q, k, v, bias, causal, softclamp, scale):
 
 @torch.compiler.disable   # library calls through ctypes: dynamo runs them eagerly
 def pass_fwd_packed(q, k, v, cu_seqlens, *, causal=False, softclamp=None, scale=None, bias=None, epi_mul=None,
-                    max_seqlen=None):
+                    max_seqlen=None, out_lo=False):
     """One attention pass over packed sequences (see PolyPackedArgs in include/poly_attention.h).
 
     q [total, h, d]; k, v [total, g, d] with g | h; bias [g, total] fp32; epi_mul
-    [total, h, d]. Returns (out, lse[, epi_mul * out]) with out like q and lse fp32 [h, total].
+    [total, h, d]. Returns (out, lse[, epi_mul * out][, out_lo]) with out like q and lse
+    fp32 [h, total]; out_lo is what rounding took off out, which ``pass_bwd_packed`` takes
+    (None for float32).
     """
     _tensors(q, k, v, bias, epi_mul)
     cu = _offsets(cu_seqlens, q)
@@ -116,22 +120,26 @@ def pass_fwd_packed(q, k, v, cu_seqlens, *, causal=False, softclamp=None, scale=
         epi_mul, epi = _rows(epi_mul), torch.empty_like(out)
         _set(a.fwd, "epi_mul", epi_mul)
         _set(a.fwd, "epi_out", epi)
+    lo = torch.empty_like(out) if out_lo and q.dtype != torch.float32 else None
+    if lo is not None:
+        a.out_lo = lo.data_ptr()
     a.cu_seqlens, a.seqs, a.max_len, a.zero_rest = cu.data_ptr(), cu.shape[0] - 1, int(max_seqlen or 0), 1
     if a.seqs == 0 and total:
-        out.zero_(), lse.zero_()
-        if epi is not None:
-            epi.zero_()
+        for t in (out, lse, epi, lo):
+            if t is not None:
+                t.zero_()
     with torch.cuda.device(q.device):
         check(lib.poly_packed_pass_fwd(a, _stream(q.device)), "poly_packed_pass_fwd")
-    return (out, lse) if epi is None else (out, lse, epi)
+    return (out, lse) + ((epi,) if epi is not None else ()) + ((lo,) if out_lo else ())
 
 
 @torch.compiler.disable
 def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softclamp=None, scale=None, bias=None,
-                    dlse=None, dq=None, want_dbias=False, max_seqlen=None):
+                    dlse=None, dq=None, want_dbias=False, max_seqlen=None, out_lo=None, factors=None):
     """Backward of ``pass_fwd_packed``. Returns (dq, dk, dv, dbias-or-None). With ``dq`` given the
-    query gradient is added to it in place."""
-    _tensors(q, k, v, out, lse, dout, bias, dlse, dq)
+    query gradient is added to it in place. With ``factors`` = (left, right), whose product the
+    values were, dv is the pair of their gradients."""
+    _tensors(q, k, v, out, lse, dout, bias, dlse, dq, out_lo, *(factors or ()))
     cu = _offsets(cu_seqlens, q)
     q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout.to(q.dtype))
     total, h, d = q.shape
@@ -156,6 +164,19 @@ def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softcl
     if dlse is not None:
         dlse = _vec(dlse, h, total, "dlse")
         _set(b, "dlse", dlse)
+    if out_lo is not None:
+        if out_lo.shape != out.shape or out_lo.dtype != out.dtype or out_lo.stride() != out.stride():
+            raise ValueError("out_lo must have out's shape, dtype and strides")
+        a.out_lo = out_lo.data_ptr()
+    dright = None
+    if factors is not None:
+        if any(t.shape != v.shape or t.dtype != v.dtype for t in factors):
+            raise ValueError("the values' factors must have their shape and dtype")
+        factors = tuple(_rows(t) for t in factors)
+        dright = v.new_empty(total, g, d)
+        _set(a, "v_left", factors[0])
+        _set(a, "v_right", factors[1])
+        _set(a, "dv_right", dright)
     b.dq_accumulate = int(dq is not None)
     if dq is None:
         dq = q.new_empty(total, h, d)
@@ -168,7 +189,7 @@ def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softcl
         _set(b, "dbias", dbias)
     a.cu_seqlens, a.seqs, a.max_len, a.zero_rest = cu.data_ptr(), cu.shape[0] - 1, int(max_seqlen or 0), 1
     if a.seqs == 0 and total:
-        for t in (dk, dv, dbias, None if b.dq_accumulate else dq):
+        for t in (dk, dv, dbias, dright, None if b.dq_accumulate else dq):
             if t is not None:
                 t.zero_()
     with torch.cuda.device(q.device):
@@ -177,7 +198,7 @@ def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softcl
         if need:
             b.workspace, b.workspace_bytes = ws.data_ptr(), need
         check(lib.poly_packed_pass_bwd(a, _stream(q.device)), "poly_packed_pass_bwd")
-    return dq, dk, dv, dbias
+    return dq, dk, dv if dright is None else (dv, dright), dbias
 
 
 class _PackedChain(torch.autograd.Function):
@@ -187,17 +208,22 @@ class _PackedChain(torch.autograd.Function):
     @staticmethod
     def forward(ctx, order, shared, cu, opts, *tensors):
         ql, qr, vs = tensors[:order], tensors[order:2 * order], tensors[2 * order:]
-        vals, biases, msgs, lses = [None] * order, [None] * order, [None] * order, [None] * order
+        vals, biases, msgs, lses, los = ([None] * order for _ in range(5))
         val, bias = vs[-1], None
+        keep = any(ctx.needs_input_grad)
         for t in range(order - 1, -1, -1):
             vals[t], biases[t] = val, bias
             # V' = v * msg is written by the pass that makes msg (n_poly_attention.py:287)
-            res = pass_fwd_packed(ql[t], qr[t], val, cu, bias=bias, epi_mul=vs[t - 2] if t >= 2 else None, **opts)
+            res = pass_fwd_packed(ql[t], qr[t], val, cu, bias=bias, epi_mul=vs[t - 2] if t >= 2 else None, out_lo=keep,
+                                  **opts)
             msgs[t], lses[t] = res[:2]
-            val, bias = res[-1] if t >= 2 else msgs[t], lses[t]
+            if keep:
+                los[t] = res[-1]
+            val, bias = res[2] if t >= 2 else msgs[t], lses[t]
         ctx.order, ctx.shared, ctx.opts = order, shared, opts
-        ctx.has = [b is not None for b in biases]
-        ctx.save_for_backward(cu, *tensors, *vals, *msgs, *lses, *[b for b in biases if b is not None])
+        if keep:
+            ctx.has = [[x is not None for x in xs] for xs in (biases, los)]
+            ctx.save_for_backward(cu, *tensors, *vals, *msgs, *lses, *(x for x in (*biases, *los) if x is not None))
         extra = (*lses[:0:-1], *msgs[:0:-1])        # level order - 1 first, as in the caches
         ctx.mark_non_differentiable(*extra)
         return (msgs[0], *extra)
@@ -209,7 +235,7 @@ class _PackedChain(torch.autograd.Function):
         take = lambda k: [saved.pop(0) for _ in range(k)]   # noqa: E731
         cu, = take(1)
         ql, qr, vs, vals, msgs, lses = take(n), take(n), take(n - 1), take(n), take(n), take(n)
-        biases = [saved.pop(0) if has else None for has in ctx.has]
+        biases, los = ([saved.pop(0) if x else None for x in has] for has in ctx.has)
         dql, dqr, dvs = [None] * n, [None] * n, [None] * (n - 1)
         g_out, g_lse = dout, None
         for t in range(n):
@@ -217,7 +243,8 @@ class _PackedChain(torch.autograd.Function):
             # kernel to the first, which was rounded once to the tensors' type
             dq, dqr[t], dv, g_lse = pass_bwd_packed(ql[t], qr[t], vals[t], cu, msgs[t], lses[t], g_out, bias=biases[t],
                                                     dlse=g_lse, dq=dqr[t - 1] if ctx.shared[t] else None,
-                                                    want_dbias=t < n - 1, **ctx.opts)
+                                                    want_dbias=t < n - 1, out_lo=los[t],
+                                                    factors=(vs[t - 1], msgs[t + 1]) if 0 < t < n - 1 else None, **ctx.opts)
             if not ctx.shared[t]:
                 dql[t] = dq
             if t == n - 1:
@@ -225,8 +252,7 @@ class _PackedChain(torch.autograd.Function):
             elif t == 0:
                 g_out = dv
             else:
-                dvs[t - 1] = dv * msgs[t + 1]
-                g_out = dv * vs[t - 1]
+                dvs[t - 1], g_out = dv
         return (None, None, None, None, *dql, *dqr, *dvs)
 
 

@@ -292,24 +292,42 @@ def test_chain_is_its_passes(dtype, d, bound, order):
     with torch.no_grad():
         val, bias, st = vs[-1], None, {}
         for t in range(order - 1, -1, -1):
-            res = P.pass_fwd_packed(qs[t], qs[t + 1], val, cu, bias=bias, epi_mul=vs[t - 2] if t >= 2 else None, **kw)
-            st[t] = (val, bias, *res[:2])
+            res = P.pass_fwd_packed(qs[t], qs[t + 1], val, cu, bias=bias, epi_mul=vs[t - 2] if t >= 2 else None, out_lo=True, **kw)
+            st[t] = (val, bias, res[0], res[1], res[-1])
+            # out + out_lo is out in more bits, and the epilogue's product is made from it
+            wide = res[0].double() + res[-1].double()
+            half = torch.finfo(dtype).eps / 2 * res[0].double().abs() + 2.0 ** -25
+            assert (res[-1].double().abs() <= half).all() and (res[-1] != 0).any()
             if t >= 2:
-                assert torch.equal(res[2], (vs[t - 2] * res[0]))
-            val, bias = res[-1] if t >= 2 else res[0], res[1]
+                step = torch.finfo(dtype).eps / 2
+                want = vs[t - 2].double() * wide
+                tol = (step + 2 * step ** 2) * want.abs() + (2.0 ** -24 * (1 + vs[t - 2].double().abs()) if dtype == torch.float16 else 0)
+                assert ((res[2].double() - want).abs() <= tol).all()
+            val, bias = res[2] if t >= 2 else res[0], res[1]
         assert torch.equal(out, st[0][2])
         for i, t in enumerate(range(order - 1, 0, -1)):
             assert torch.equal(msgs[i], st[t][2]) and torch.equal(lses[i], st[t][3])
         g_out, g_lse, dk = do, None, None
         for t in range(order):
+            fac = (vs[t - 1], st[t + 1][2]) if 0 < t < order - 1 else None
             dq, dkn, dv, db = P.pass_bwd_packed(qs[t], qs[t + 1], st[t][0], cu, st[t][2], st[t][3], g_out, bias=st[t][1],
-                                                dlse=g_lse, dq=dk, want_dbias=True, **kw)
+                                                dlse=g_lse, dq=dk, want_dbias=True, out_lo=st[t][4], factors=fac, **kw)
+            if fac is not None:
+                # the factors' gradients are the values' times the other factor, rounded once more
+                plain = P.pass_bwd_packed(qs[t], qs[t + 1], st[t][0], cu, st[t][2], st[t][3], g_out, bias=st[t][1],
+                                          dlse=g_lse, want_dbias=True, out_lo=st[t][4], **kw)[2].double()
+                for got, other in zip(dv, (fac[1], fac[0])):
+                    want = plain * other.double()
+                    floor = 2.0 ** -24 * (1 + other.double().abs()) if dtype == torch.float16 else 0
+                    assert ((got.double() - want).abs() <= 1.01 * torch.finfo(dtype).eps * want.abs() + floor).all()
             # dq sums its key tiles in 32 bits in any order: one step of the type
             near = lambda a, b: bool(((a.float() - b.float()).abs() <= 2 * torch.finfo(dtype).eps * b.float().abs() + 1e-3).all())   # noqa: E731
             assert near(grads[t], dq)
             if t == order - 1:
                 assert near(grads[t + 1], dkn) and near(grads[2 * order - 1], dv)
-            g_out, g_lse, dk = (dv if t == 0 else dv * vs[t - 1]), db, dkn
+            if fac is not None:
+                assert near(grads[order + 1 + t - 1], dv[0])
+            g_out, g_lse, dk = (dv if fac is None else dv[1]), db, dkn
 
 
 @pytest.mark.parametrize("kind", ["order2", "order3"])
