@@ -103,6 +103,8 @@ int launch_packed_bwd_simt(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaSt
 size_t packed_bwd_simt_workspace(const PolyPassBwdArgs& a);
 bool packed_fwd_tc_eligible(const PolyPassArgs& a, const void* out_lo);
 int launch_packed_fwd_tc(PolyPassArgs a, const PackedSeqs& q, cudaStream_t s);
+bool packed_f32_eligible(const PolyPackedArgs& a);
+int launch_packed_fwd_f32(PolyPassArgs a, const PackedSeqs& q, cudaStream_t s);
 int launch_packed_fwd_small(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s);
 int launch_packed_bwd_small(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s);
 bool packed_bwd_tc_eligible(const PolyPackedBwdArgs& a);

@@ -82,12 +82,13 @@ int check_fwd(const PolyPackedArgs* a) {
   return check_packed(a->pass, a->cu_seqlens, a->seqs, a->max_len);
 }
 
-enum class Kind { kSimt, kTc, kSmall };
+enum class Kind { kSimt, kTc, kSmall, kF32 };
 
 bool short_sequences(int max_len) { return max_len > 0 && max_len <= 128; }
 
 // The tcgen05 kernels take the row maximum on unscaled scores: no negative scale.
 Kind choose_fwd(const PolyPackedArgs& a) {
+  if (packed_f32_eligible(a)) return Kind::kF32;
   if (!packed_fwd_tc_eligible(a.pass, a.out_lo)) return Kind::kSimt;   // the short kernel takes the same tensors
   if (short_sequences(a.max_len)) return Kind::kSmall;
   return a.pass.scale >= 0.f ? Kind::kTc : Kind::kSimt;
@@ -98,7 +99,14 @@ Kind choose_bwd(const PolyPackedBwdArgs& a) {
   return short_sequences(a.max_len) ? Kind::kSmall : Kind::kTc;
 }
 
-const char* name_of(Kind k) { return k == Kind::kTc ? "tc100" : k == Kind::kSmall ? "small" : "simt"; }
+const char* name_of(Kind k) {
+  switch (k) {
+    case Kind::kTc: return "tc100";
+    case Kind::kSmall: return "small";
+    case Kind::kF32: return "tf32x3";
+    default: return "simt";
+  }
+}
 
 int check_bwd(const PolyPackedBwdArgs* a) {
   if (!a) return fail(POLY_EINVAL, "null args");
@@ -149,6 +157,7 @@ int poly_packed_pass_fwd(const PolyPackedArgs* a, void* stream) {
   switch (choose_fwd(*a)) {
     case Kind::kTc: return launch_packed_fwd_tc(a->pass, q, (cudaStream_t)stream);
     case Kind::kSmall: return launch_packed_fwd_small(a->pass, q, (cudaStream_t)stream);
+    case Kind::kF32: return launch_packed_fwd_f32(a->pass, q, (cudaStream_t)stream);
     default: return launch_packed_fwd_simt(a->pass, q, (cudaStream_t)stream);
   }
 }

@@ -12,10 +12,15 @@
 // Online softmax in the log2 domain. Rows whose every key is excluded get the
 // reference's -finfo.max result: a uniform average over the keys that are not
 // both masked (causal) and dead (bias <= -FLT_MAX / 2), lse = -FLT_MAX.
+//
+// PACKED: sequences laid end to end, one CTA per 64-row slot (packed.cuh) and
+// head; slots are taken from the last to the first, so that of a causal sequence
+// the rows with the most keys start first.
 #include <cfloat>
 #include <mutex>
 
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace poly {
 namespace {
@@ -50,21 +55,40 @@ __device__ __forceinline__ void cp16(uint32_t sa, const void* g, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sa), "l"(g), "r"(ok ? 16 : 0) : "memory");
 }
 
-template <bool HAS_BIAS, bool SOFTCLAMP>
-__global__ void __launch_bounds__(128) pass_f32_kernel(const PolyPassArgs a) {
+template <bool HAS_BIAS, bool SOFTCLAMP, bool PACKED>
+__global__ void __launch_bounds__(128) pass_f32_kernel(PolyPassArgs a, const PackedSeqs pk) {
   extern __shared__ __align__(16) float smf[];
   float(*sK)[BN * LD] = reinterpret_cast<float(*)[BN * LD]>(smf);
   float(*sV)[BN * LD] = reinterpret_cast<float(*)[BN * LD]>(smf + 2 * BN * LD);
   float(*sB)[BN] = reinterpret_cast<float(*)[BN]>(smf + 4 * BN * LD);
-  const int bh = blockIdx.y;
-  const int b = bh / a.heads, h = bh - b * a.heads, g = h / (a.heads / a.kv_heads);
+  // packed: heads fastest, so that CTAs running together share a sequence's keys
+  const int bh = PACKED ? blockIdx.x : blockIdx.y;
+  const int b = PACKED ? 0 : bh / a.heads, h = bh - b * a.heads, g = h / (a.heads / a.kv_heads);
+  int tile = blockIdx.x;
+  if constexpr (PACKED) {
+    PackedTile t;
+    if (!packed_tile<BM>(pk.cu, pk.seqs, pk.total, gridDim.y - 1 - blockIdx.y, t)) return;
+    tile = t.tile;
+    a.seq_q = a.seq_k = t.len;
+    const int64_t f = t.start;
+    a.q = (const float*)a.q + f * a.q_stride[2];
+    a.k = (const float*)a.k + f * a.k_stride[2];
+    a.v = (const float*)a.v + f * a.v_stride[2];
+    a.out = (float*)a.out + f * a.out_stride[2];
+    if (HAS_BIAS) a.bias += f;
+    if (a.lse) a.lse += f;
+    if (a.epi_out) {
+      a.epi_mul = (const float*)a.epi_mul + f * a.epi_mul_stride[2];
+      a.epi_out = (float*)a.epi_out + f * a.epi_out_stride[2];
+    }
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
-  const int i0 = blockIdx.x * BM + warp * 16 + gq, i1 = i0 + 8;   // this thread's two rows
+  const int i0 = tile * BM + warp * 16 + gq, i1 = i0 + 8;   // this thread's two rows
   const int nq = a.seq_q, nk = a.seq_k;
   const float* kg = (const float*)a.k + b * a.k_stride[0] + g * a.k_stride[1];
   const float* vg = (const float*)a.v + b * a.v_stride[0] + g * a.v_stride[1];
   const float* bg = HAS_BIAS ? a.bias + b * a.bias_stride[0] + g * a.bias_stride[1] : nullptr;
-  const int kend = a.causal ? min(nk, (int)blockIdx.x * BM + BM) : nk;
+  const int kend = a.causal ? min(nk, tile * BM + BM) : nk;
   const int ntile = (kend + BN - 1) / BN;
 
   auto issue = [&](int t) {
@@ -209,10 +233,11 @@ __global__ void __launch_bounds__(128) pass_f32_kernel(const PolyPassArgs a) {
     float r[D / 8][2];
     if (m == -INFINITY) {
       // every key excluded: uniform average over keys not both masked and dead
+      // (packed rows: zero)
       int count = 0;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) r[n][0] = r[n][1] = 0.f;
-      for (int j = 0; j < nk; ++j) {
+      for (int j = 0; j < (PACKED ? 0 : nk); ++j) {
         const bool masked = a.causal && j > row;
         const bool dead = HAS_BIAS && bg[j] <= kDeadBias;
         if (masked && dead) continue;
@@ -244,6 +269,16 @@ __global__ void __launch_bounds__(128) pass_f32_kernel(const PolyPassArgs a) {
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
       *reinterpret_cast<float2*>(orow + n * 8 + 2 * tq) = make_float2(r[n][0], r[n][1]);
+    if (PACKED && a.epi_out) {
+      const float* em = (const float*)a.epi_mul + h * a.epi_mul_stride[1] + (int64_t)row * a.epi_mul_stride[2];
+      float* eo = (float*)a.epi_out + h * a.epi_out_stride[1] + (int64_t)row * a.epi_out_stride[2];
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        const int c = n * 8 + 2 * tq;
+        eo[c] = em[c] * r[n][0];
+        eo[c + 1] = em[c + 1] * r[n][1];
+      }
+    }
     if (a.lse && tq == 0) a.lse[b * a.lse_stride[0] + h * a.lse_stride[1] + row] = lse;
   }
 }
@@ -264,28 +299,39 @@ bool pass_f32_eligible(const PolyPassArgs& a) {
 namespace {
 constexpr int kSmem = (4 * BN * LD + 2 * BN) * 4;
 
-template <bool B, bool C>
-int launch_t(const PolyPassArgs& a, cudaStream_t s) {
+template <bool B, bool C, bool PACKED>
+int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
   std::call_once(once, [] {
-    err = cudaFuncSetAttribute(pass_f32_kernel<B, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    err = cudaFuncSetAttribute(pass_f32_kernel<B, C, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(f32)");
-  const dim3 grid((a.seq_q + BM - 1) / BM, a.batch * a.heads);
-  pass_f32_kernel<B, C><<<grid, 128, kSmem, s>>>(a);
-  return POLY_OK;
+  const dim3 grid = PACKED ? dim3(a.heads, a.seq_q / BM + pk->seqs) : dim3((a.seq_q + BM - 1) / BM, a.batch * a.heads);
+  pass_f32_kernel<B, C, PACKED><<<grid, 128, kSmem, s>>>(a, PACKED ? *pk : PackedSeqs{});
+  note_launch(1);
+  return cuda_status(cudaGetLastError(), "pass_f32 launch");
+}
+
+template <bool PACKED>
+int launch_any(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
+  const bool bias = a.bias != nullptr, sc = a.softclamp > 0.f;
+  if (sc) return bias ? launch_t<true, true, PACKED>(a, pk, s) : launch_t<false, true, PACKED>(a, pk, s);
+  return bias ? launch_t<true, false, PACKED>(a, pk, s) : launch_t<false, false, PACKED>(a, pk, s);
 }
 }  // namespace
 
-int launch_pass_f32(const PolyPassArgs& a, cudaStream_t s) {
-  const bool bias = a.bias != nullptr, sc = a.softclamp > 0.f;
-  int rc;
-  if (sc) rc = bias ? launch_t<true, true>(a, s) : launch_t<false, true>(a, s);
-  else rc = bias ? launch_t<true, false>(a, s) : launch_t<false, false>(a, s);
-  if (rc) return rc;
-  note_launch(1);
-  return cuda_status(cudaGetLastError(), "pass_f32 launch");
+int launch_pass_f32(const PolyPassArgs& a, cudaStream_t s) { return launch_any<false>(a, nullptr, s); }
+
+// The slots are the grid's second axis, which holds 65535.
+bool packed_f32_eligible(const PolyPackedArgs& pa) {
+  const PolyPassArgs& a = pa.pass;
+  if (a.dtype != POLY_F32 || a.head_dim != D || a.seq_q / BM + pa.seqs > 65535) return false;
+  if (!al(a.k, 16) || !al(a.v, 16) || !al(a.out, 8)) return false;
+  return !((a.k_stride[1] | a.k_stride[2] | a.v_stride[1] | a.v_stride[2]) & 3) && !((a.out_stride[1] | a.out_stride[2]) & 1);
+}
+int launch_packed_fwd_f32(PolyPassArgs a, const PackedSeqs& q, cudaStream_t s) {
+  return launch_any<true>(a, &q, s);
 }
 
 }  // namespace poly

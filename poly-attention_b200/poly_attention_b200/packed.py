@@ -201,6 +201,18 @@ def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softcl
     return dq, dk, dv if dright is None else (dv, dright), dbias
 
 
+def packed_kernel_names(q, k, v, max_seqlen=None):
+    """(forward, backward) kernel family the library picks for these packed tensors."""
+    a, b = PolyPackedArgs(), PolyPackedBwdArgs()
+    for x, f in ((a, a.fwd), (b, b.bwd.fwd)):
+        _fill(f, q, k, v, None, False, None, None)
+        _set(f, "out", q)
+        x.cu_seqlens, x.seqs, x.max_len = 1, 1, int(max_seqlen or 0)
+    for name, t in (("dout", q), ("dq", q), ("dk", k), ("dv", v)):
+        _set(b.bwd, name, t)
+    return lib.poly_packed_pass_fwd_kernel_name(a).decode(), lib.poly_packed_pass_bwd_kernel_name(b).decode()
+
+
 class _PackedChain(torch.autograd.Function):
     """The order-n chain. Inputs: order queries ql, order keys qr and order - 1 values; shared[t] says
     that ql[t] is qr[t - 1], whose two gradients are then summed inside the kernel."""

@@ -98,3 +98,15 @@ def test_slot_numbering_covers_every_tile_once(block):
             t = locate(wild, total, s)
             if t:
                 assert 0 <= t[1] and t[1] + t[2] <= total and t[1] + t[3] * block < total
+
+
+@pytest.mark.parametrize("dtype,d,bound,want", [
+    (torch.bfloat16, 64, None, ("tc100", "tc100")), (torch.float16, 128, 129, ("tc100", "tc100")),
+    (torch.bfloat16, 64, 128, ("small", "small")), (torch.float16, 128, 1, ("small", "small")),
+    (torch.float32, 64, 128, ("tf32x3", "simt")), (torch.float32, 128, None, ("simt", "simt")),
+    (torch.bfloat16, 32, 16, ("simt", "simt"))])
+def test_kernel_choice(dtype, d, bound, want):
+    """The kernels that the GPU tests mean to reach (the choice looks at sizes and addresses only)."""
+    from poly_attention_b200.packed import packed_kernel_names
+    q, k = torch.empty(400, 4, d, dtype=dtype), torch.empty(400, 2, d, dtype=dtype)
+    assert packed_kernel_names(q, k, k, bound) == want
