@@ -339,6 +339,92 @@ typedef struct {
 POLY_API int poly_rotary(const PolyRotaryArgs* args, void* stream);
 
 /*
+ * Decoding steps over trees of drafted tokens. Every sequence b has its own
+ * number of cached tokens, lengths[b] (device int32), and a tree of `nodes` <= 64
+ * drafted tokens given by parents[b][node] (device int32): the parent's index
+ * (smaller than the node's own), -1 for a child of the cached tokens, or -2 for
+ * a node that is padding (as are nodes below a padding node, nodes whose parent
+ * index is not smaller than their own, and nodes past the capacity). A node sees
+ * the cached tokens, its ancestors and itself:
+ *
+ *   s_ij = scale q_i . k_j (softclamp) + bias_j ;  out_i = softmax_j(s_ij) (v_j * v_mul_j)
+ *
+ * over the cache's rows j < lengths[b] and the rows lengths[b] + node that the
+ * tree's own keys and values occupy (poly_tree_append writes them, a padding
+ * node's as zeros). Padding nodes, and nodes that see dead keys only (bias
+ * <= -FLT_MAX / 2), get out = 0 and lse = -FLT_MAX. Lengths are clamped to [0, capacity];
+ * nothing outside the caches is ever accessed.
+ *
+ * out / lse take the nodes' rows; cache_out / cache_lse take them at the cache
+ * rows lengths[b] + node (the next level's values and bias). Each may be NULL.
+ * Everything is stream-ordered and reads lengths and parents on the device, so a
+ * step can be captured in a graph and replayed.
+ */
+#define POLY_MAX_TREE_NODES 64
+typedef struct PolyTreePass {
+  int32_t batch, heads, kv_heads, nodes;
+  int32_t head_dim, dtype, capacity, reserved;
+  float scale, softclamp;
+  const void* q;      int64_t q_stride[3];       /* [batch, heads, nodes, d]       */
+  const void* k;      int64_t k_stride[3];       /* [batch, kv_heads, capacity, d] */
+  const void* v;      int64_t v_stride[3];       /* [batch, kv_heads, capacity, d] */
+  const void* v_mul;  int64_t v_mul_stride[3];   /* [batch, kv_heads, capacity, d] | NULL */
+  const float* bias;  int64_t bias_stride[2];    /* [batch, kv_heads, capacity] | NULL */
+  const int32_t* lengths;                        /* [batch] */
+  const int32_t* parents; int64_t parents_stride; /* [batch, nodes], row stride */
+  void* out;          int64_t out_stride[3];     /* [batch, heads, nodes, d] | NULL */
+  float* lse;         int64_t lse_stride[2];     /* [batch, heads, nodes] | NULL */
+  void* cache_out;    int64_t cache_out_stride[3]; /* [batch, heads, capacity, d] | NULL */
+  float* cache_lse;   int64_t cache_lse_stride[2]; /* [batch, heads, capacity] | NULL */
+  void* workspace;    /* >= poly_tree_workspace_size() bytes; passes of a chain may share it */
+  size_t workspace_bytes;
+} PolyTreePass;
+
+/* New rows of up to 16 caches of one shape: src [batch, kv_heads, nodes, d] to
+ * cache rows lengths[b] + node. d * element size must be a multiple of 2 bytes. */
+#define POLY_MAX_TREE_CACHES 16
+typedef struct PolyTreeAppend {
+  int32_t batch, kv_heads, nodes, row_bytes;
+  int32_t capacity, n;
+  const int32_t* lengths;
+  const int32_t* parents; int64_t parents_stride;
+  struct {
+    const void* src; int64_t src_stride[3];   /* bytes: batch, head, node */
+    void* cache;     int64_t cache_stride[3]; /* bytes: batch, head, row */
+  } t[POLY_MAX_TREE_CACHES];
+} PolyTreeAppend;
+
+/* Keeps the accepted nodes: cache rows lengths[b] + path[b][i] move to
+ * lengths[b] + i for i < count[b], then lengths[b] += count[b]. path[b] holds
+ * path_len entries and ascends (a root-to-leaf path does); an entry smaller than
+ * its place is taken as its place, one past the nodes as the last node; count is
+ * clamped to [0, min(path_len, nodes)] and to the capacity. */
+typedef struct PolyTreeCommit {
+  int32_t batch, kv_heads, nodes, capacity;
+  int32_t n, path_len;
+  int32_t* lengths;
+  const int32_t* path;  int64_t path_stride;   /* [batch, path_len], row stride */
+  const int32_t* count;                        /* [batch] */
+  struct {
+    void* cache; int64_t cache_stride[3];      /* bytes: batch, head, row */
+    int64_t row_bytes;
+  } t[POLY_MAX_TREE_CACHES];
+} PolyTreeCommit;
+
+/* The append (or NULL), then n passes in order, each launched so that its CTAs
+ * start while the previous kernel drains: a pass may read what an earlier one
+ * wrote only in rows lengths[b] and after of its v, v_mul and bias. */
+POLY_API int poly_tree_chain(const PolyTreeAppend* append, const PolyTreePass* passes, int n, void* stream);
+POLY_API size_t poly_tree_workspace_size(const PolyTreePass* pass);
+POLY_API int poly_tree_commit(const PolyTreeCommit* args, void* stream);
+/* positions[b][node] = lengths[b] + the node's ancestors in the tree (rotary
+ * positions of the drafted tokens); lengths[b] for padding. */
+POLY_API int poly_tree_positions(const int32_t* lengths, const int32_t* parents, int64_t parents_stride, int batch,
+                                 int nodes, int32_t* positions, int64_t positions_stride, void* stream);
+/* "tree" (mma.sync) or "simt", "invalid" if validation fails */
+POLY_API const char* poly_tree_kernel_name(const PolyTreePass* pass);
+
+/*
  * poly_pass_bwd without a caller workspace. No counterpart in the reference:
  * it exists for callers that cannot allocate device memory (FFI hosts that
  * only pass existing buffers, processes whose device memory another
@@ -390,6 +476,9 @@ POLY_API size_t poly_sizeof_pass_bwd_args(void);
 POLY_API size_t poly_sizeof_merge_args(void);
 POLY_API size_t poly_sizeof_rotary_args(void);
 POLY_API size_t poly_sizeof_packed_args(void);
+POLY_API size_t poly_sizeof_tree_pass(void);
+POLY_API size_t poly_sizeof_tree_append(void);
+POLY_API size_t poly_sizeof_tree_commit(void);
 POLY_API size_t poly_sizeof_packed_bwd_args(void);
 
 #ifdef __cplusplus

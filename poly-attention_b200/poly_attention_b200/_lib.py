@@ -92,6 +92,43 @@ class PolyPackedBwdArgs(ctypes.Structure):
                 ("dv_right", c_vp), ("dv_right_stride", I64x2)]
 
 
+MAX_TREE_NODES = 64
+MAX_TREE_CACHES = 16
+
+
+class PolyTreePass(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("heads", c_i32), ("kv_heads", c_i32), ("nodes", c_i32), ("head_dim", c_i32), ("dtype", c_i32),
+        ("capacity", c_i32), ("reserved", c_i32), ("scale", c_f32), ("softclamp", c_f32),
+        ("q", c_vp), ("q_stride", I64x3), ("k", c_vp), ("k_stride", I64x3), ("v", c_vp), ("v_stride", I64x3),
+        ("v_mul", c_vp), ("v_mul_stride", I64x3), ("bias", c_vp), ("bias_stride", I64x2),
+        ("lengths", c_vp), ("parents", c_vp), ("parents_stride", c_i64),
+        ("out", c_vp), ("out_stride", I64x3), ("lse", c_vp), ("lse_stride", I64x2),
+        ("cache_out", c_vp), ("cache_out_stride", I64x3), ("cache_lse", c_vp), ("cache_lse_stride", I64x2),
+        ("workspace", c_vp), ("workspace_bytes", c_sz),
+    ]
+
+
+class _TreeAppendRow(ctypes.Structure):
+    _fields_ = [("src", c_vp), ("src_stride", I64x3), ("cache", c_vp), ("cache_stride", I64x3)]
+
+
+class PolyTreeAppend(ctypes.Structure):
+    _fields_ = [("batch", c_i32), ("kv_heads", c_i32), ("nodes", c_i32), ("row_bytes", c_i32), ("capacity", c_i32),
+                ("n", c_i32), ("lengths", c_vp), ("parents", c_vp), ("parents_stride", c_i64),
+                ("t", _TreeAppendRow * MAX_TREE_CACHES)]
+
+
+class _TreeCommitRow(ctypes.Structure):
+    _fields_ = [("cache", c_vp), ("cache_stride", I64x3), ("row_bytes", c_i64)]
+
+
+class PolyTreeCommit(ctypes.Structure):
+    _fields_ = [("batch", c_i32), ("kv_heads", c_i32), ("nodes", c_i32), ("capacity", c_i32), ("n", c_i32),
+                ("path_len", c_i32), ("lengths", c_vp), ("path", c_vp), ("path_stride", c_i64), ("count", c_vp),
+                ("t", _TreeCommitRow * MAX_TREE_CACHES)]
+
+
 class PolyRotaryTensor(ctypes.Structure):
     _fields_ = [("src", c_vp), ("dst", c_vp), ("heads", c_i32), ("reserved", c_i32),
                 ("src_stride", I64x3), ("dst_stride", I64x3)]
@@ -125,6 +162,11 @@ EXPORTS = {
     "poly_packed_pass_bwd_workspace_size": (c_sz, [ctypes.POINTER(PolyPackedBwdArgs)]),
     "poly_packed_pass_fwd_kernel_name": (ctypes.c_char_p, [ctypes.POINTER(PolyPackedArgs)]),
     "poly_packed_pass_bwd_kernel_name": (ctypes.c_char_p, [ctypes.POINTER(PolyPackedBwdArgs)]),
+    "poly_tree_chain": (ctypes.c_int, [ctypes.POINTER(PolyTreeAppend), ctypes.POINTER(PolyTreePass), ctypes.c_int, c_vp]),
+    "poly_tree_workspace_size": (c_sz, [ctypes.POINTER(PolyTreePass)]),
+    "poly_tree_commit": (ctypes.c_int, [ctypes.POINTER(PolyTreeCommit), c_vp]),
+    "poly_tree_positions": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp]),
+    "poly_tree_kernel_name": (ctypes.c_char_p, [ctypes.POINTER(PolyTreePass)]),
     "poly_rotary": (ctypes.c_int, [ctypes.POINTER(PolyRotaryArgs), c_vp]),
     "poly_pass_bwd_noalloc": (ctypes.c_int, [ctypes.POINTER(PolyPassBwdArgs), c_vp]),
     "poly_noalloc_scratch_bytes": (c_sz, []),
@@ -141,6 +183,9 @@ EXPORTS = {
     "poly_sizeof_rotary_args": (c_sz, []),
     "poly_sizeof_packed_args": (c_sz, []),
     "poly_sizeof_packed_bwd_args": (c_sz, []),
+    "poly_sizeof_tree_pass": (c_sz, []),
+    "poly_sizeof_tree_append": (c_sz, []),
+    "poly_sizeof_tree_commit": (c_sz, []),
 }
 
 
@@ -157,7 +202,9 @@ def _load():
         raise ImportError("libpolyattn.so ABI version mismatch")
     for fn, st in (("poly_sizeof_pass_args", PolyPassArgs), ("poly_sizeof_pass_bwd_args", PolyPassBwdArgs),
                    ("poly_sizeof_merge_args", PolyMergeArgs), ("poly_sizeof_rotary_args", PolyRotaryArgs),
-                   ("poly_sizeof_packed_args", PolyPackedArgs), ("poly_sizeof_packed_bwd_args", PolyPackedBwdArgs)):
+                   ("poly_sizeof_packed_args", PolyPackedArgs), ("poly_sizeof_packed_bwd_args", PolyPackedBwdArgs),
+                   ("poly_sizeof_tree_pass", PolyTreePass), ("poly_sizeof_tree_append", PolyTreeAppend),
+                   ("poly_sizeof_tree_commit", PolyTreeCommit)):
         if getattr(lib, fn)() != ctypes.sizeof(st):
             raise ImportError(f"libpolyattn.so struct layout mismatch ({st.__name__})")
     return lib

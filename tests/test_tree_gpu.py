@@ -1,0 +1,342 @@
+"""Decoding over trees of drafted tokens: every level against 64 bits (tolerances:
+pass_reference.py, on the rows that the level read), the step against decoding
+token by token, commits, graphs, refusals."""
+import random
+
+import pytest
+import torch
+
+import pass_reference as R
+
+pytestmark = pytest.mark.gpu
+LOW = torch.finfo(torch.float32).min
+
+
+def tree(kind, n, rng):
+    if kind == "chain":
+        return [i - 1 for i in range(n)]
+    if kind == "star":
+        return [-1] * n
+    return [-1 if i == 0 else rng.randrange(-1, i) for i in range(n)]
+
+
+def visible(parents):
+    """Truth values [T, T] and which nodes are not padding."""
+    n = len(parents)
+    see = torch.zeros(n, n, dtype=torch.bool)
+    for i, p in enumerate(parents):
+        ok = -1 <= p < i and (p < 0 or bool(see[p, p]))
+        if ok:
+            see[i, i] = True
+            if p >= 0:
+                see[i] |= see[p]
+    return see.cuda()
+
+
+class Case:
+    def __init__(self, *, order, h, g, d, dtype, lens, parents, cap=None, seed=0, clamp=None, max_nodes=None, stale=None):
+        import poly_attention_b200 as P
+        b, t = len(lens), len(parents[0])
+        cap = cap or max(lens) + t
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda")   # noqa: E731
+        self.lens, self.parents, self.clamp, self.d, self.dtype, self.order = lens, parents, clamp, d, dtype, order
+        self.dec = P.TreeDecoder(batch=b, order=order, heads=h, kv_heads=g, dim_head=d, capacity=cap, max_nodes=max_nodes or t,
+                                 dtype=dtype, softclamp_value=clamp)
+        n = max(lens)
+        rows = [rnd(b, g, n, d).to(dtype) for _ in range(3 * order - 2)]
+        lses = [2 + rnd(b, g, n) for _ in range(order - 1)]
+        self.dec.load(rows[:order], rows[order:2 * order - 1], lses, rows[2 * order - 1:], lens)
+        if stale is not None:      # whatever lies behind the lengths
+            for c in self.dec.keys + self.dec.vals + self.dec.msgs + self.dec.lses:
+                for i, m in enumerate(lens):
+                    c[i, :, m:] = stale
+        self.q1 = rnd(b, h, t, d).to(dtype)
+        self.nk = [rnd(b, g, t, d).to(dtype) for _ in range(order)]
+        self.nv = [rnd(b, g, t, d).to(dtype) for _ in range(order - 1)]
+        self.par = torch.tensor(parents, dtype=torch.int32, device="cuda")
+
+    def step(self, **kw):
+        return self.dec.step(self.q1, self.nk, self.nv, self.par, **kw)
+
+    def check(self):
+        dec, order, t = self.dec, self.order, self.q1.shape[2]
+        out, msgs, lses = self.step(return_rows=True)
+        for i, n in enumerate(self.lens):
+            see = visible(self.parents[i])
+            live = see.diagonal()
+            end = n + t
+            keep = torch.cat((torch.ones(t, n, dtype=torch.bool, device="cuda"), see), 1)
+            for new, cache in zip(self.nk + self.nv, dec.keys + dec.vals):
+                assert torch.equal(cache[i, :, n:end][:, live], new[i][:, live]) and (cache[i, :, n:end][:, ~live] == 0).all()
+            for lvl in range(order - 1, -1, -1):
+                at = order - 1 - lvl
+                q = (self.q1 if lvl == 0 else self.nk[lvl - 1])[i].double()
+                k = dec.keys[lvl][i, :, :end].double()
+                if lvl == order - 1:
+                    v = dec.vals[-1][i, :, :end].double()
+                elif lvl:
+                    v = (dec.vals[lvl - 1][i, :, :end] * dec.msgs[order - 2 - lvl][i, :, :end]).double()
+                else:
+                    v = dec.msgs[order - 2][i, :, :end].double()
+                bias = None if lvl == order - 1 else dec.lses[order - 2 - lvl][i, :, :end].double()
+                seen = keep
+                if bias is not None:
+                    dead = bias <= LOW / 2
+                    assert torch.equal(dead, dead[:1].expand_as(dead))
+                    seen = keep & ~dead[:1]
+                    bias = bias.masked_fill(dead, 0.0)
+                some = live & seen.any(1)
+                (o, ot), (l, lt), _ = R.forward(q[:, some], k, v, bias, seen[some], self.d ** -0.5, self.clamp, self.dtype)
+                what = f"level {lvl} sequence {i}"
+                got = out[i] if lvl == 0 else msgs[at][i]
+                R.assert_within(got[:, some], o, ot, "rows " + what)
+                assert (got[:, ~some] == 0).all()
+                if lvl:
+                    R.assert_within(lses[at][i][:, some], l, lt, "lse " + what)
+                    assert (lses[at][i][:, ~some] == LOW).all()
+                    assert torch.equal(dec.msgs[at][i, :, n:end], msgs[at][i]) and torch.equal(dec.lses[at][i, :, n:end], lses[at][i])
+        return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("order", [2, 3])
+@pytest.mark.parametrize("h,g,d", [(4, 4, 64), (4, 1, 128), (6, 2, 64), (4, 2, 24), (32, 2, 128)])
+@pytest.mark.parametrize("lens,nodes", [([0], 1), ([1, 5], 3), ([63, 64, 65, 0], 7), ([300, 17], 16), ([130, 700], 33), ([1000], 64)])
+def test_step(lens, nodes, h, g, d, order, dtype):
+    rng = random.Random(nodes)
+    kinds = ["random", "chain", "star", "random"]
+    Case(order=order, h=h, g=g, d=d, dtype=dtype, lens=lens, parents=[tree(kinds[i], nodes, rng) for i in range(len(lens))]).check()
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float32, 32)])
+def test_order_four_and_softclamp(dtype, d):
+    rng = random.Random(1)
+    Case(order=4, h=4, g=2, d=d, dtype=dtype, lens=[100, 41], parents=[tree("random", 9, rng) for _ in range(2)]).check()
+    Case(order=3, h=4, g=2, d=d, dtype=dtype, lens=[100, 41], parents=[tree("random", 9, rng) for _ in range(2)], clamp=3.0).check()
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 64)])
+@pytest.mark.parametrize("order", [2, 3])
+def test_padding_nodes_and_stale_rows(dtype, d, order):
+    """Trees of different sizes in one call; NaN behind the lengths and in the padding's rows reaches nothing."""
+    rng = random.Random(2)
+    parents = [tree("random", 20, rng), tree("random", 20, rng), [-2] * 20, [-1, 0, -2, 1, 2, 4] + [-2] * 14, [3, 9] + [-2] * 18]
+    for i in range(7, 20):
+        parents[1][i] = -2
+    c = Case(order=order, h=4, g=2, d=d, dtype=dtype, lens=[90, 128, 33, 0, 5], parents=parents, cap=200, stale=float("nan"))
+    for i in range(5):
+        live = visible(parents[i]).diagonal()
+        for x in [c.q1] + c.nk + c.nv:
+            x[i][:, ~live] = float("nan")
+    out = c.check()
+    assert torch.isfinite(out).all()
+
+
+def test_dead_cached_keys():
+    for dtype, d in ((torch.bfloat16, 64), (torch.float32, 40)):
+        c = Case(order=3, h=4, g=2, d=d, dtype=dtype, lens=[70, 12], parents=[[-1, 0, 0], [-1, 0, -2]])
+        for x in c.dec.lses:
+            x[0, :, :33] = LOW
+            x[1, :, :12] = float("-inf")
+        c.check()
+
+
+def test_many_splits_and_groups():
+    """One sequence over many key ranges, and more groups than fit at once (no split)."""
+    rng = random.Random(3)
+    Case(order=2, h=8, g=2, d=128, dtype=torch.bfloat16, lens=[5003], parents=[tree("random", 5, rng)]).check()
+    Case(order=2, h=2, g=2, d=64, dtype=torch.float16, lens=[rng.randrange(200) for _ in range(170)],
+         parents=[tree("random", 4, rng) for _ in range(170)], cap=1000).check()
+
+
+def test_strides_and_shared_tree():
+    rng = random.Random(4)
+    shared = tree("random", 8, rng)
+    c = Case(order=2, h=4, g=2, d=64, dtype=torch.bfloat16, lens=[50, 77], parents=[shared, shared])
+    want = c.step().clone()
+    one = c.dec.step(c.q1, c.nk, c.nv, torch.tensor(shared, dtype=torch.int32, device="cuda"))
+    assert torch.equal(one, want)
+    token_major = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)   # noqa: E731
+    assert torch.equal(c.dec.step(token_major(c.q1), [token_major(t) for t in c.nk], [token_major(t) for t in c.nv], c.par), want)
+    spread = lambda t: torch.stack((t, t), -1).flatten(-2)[..., ::2]   # noqa: E731
+    assert torch.equal(c.dec.step(spread(c.q1), [spread(t) for t in c.nk], [spread(t) for t in c.nv], c.par), want)
+
+    def odd(t):     # an address that is a multiple of 2 bytes only
+        buf = torch.empty(t.numel() + 1, device="cuda", dtype=t.dtype)
+        buf[1:] = t.reshape(-1)
+        return buf[1:].view(t.shape)
+    got = c.dec.step(odd(c.q1), [odd(t) for t in c.nk], [odd(t) for t in c.nv], c.par)
+    # other kernels, the same roundings of 16-bit operands: two steps of the type
+    assert ((got - want).abs() <= 2 * torch.finfo(torch.bfloat16).eps * want.abs() + 4e-3).all()
+
+
+@pytest.mark.parametrize("order", [2, 3])
+@pytest.mark.parametrize("dtype,tol", [(torch.float32, 1e-4), (torch.bfloat16, 2e-2)])
+def test_a_path_of_the_tree_is_decoding_token_by_token(order, dtype, tol):
+    """Every node's output is that of ChainDecoder fed its path (the framework's bars: fp32 1e-4, bf16 2e-2 + 1e-2 |x|)."""
+    from poly_attention_b200.decode import ChainDecoder
+    n = 37
+    parents = [-1, 0, 0, 1, 3, 2]
+    c = Case(order=order, h=4, g=2, d=64, dtype=dtype, lens=[n], parents=[parents])
+    dec = c.dec
+    keep = [x[:, :, :n].clone() for x in dec.keys + dec.vals + dec.lses + dec.msgs]
+    out = c.step()
+    for leaf in (4, 5):
+        path, p = [], leaf
+        while p >= 0:
+            path.insert(0, p)
+            p = parents[p]
+        cd = ChainDecoder(batch=1, order=order, heads=4, kv_heads=2, dim_head=64, capacity=n + 8, dtype=dtype)
+        for dst, src in zip(cd.qs + cd.vs + cd.lses + cd.msgs, keep):
+            dst[:, :, :n] = src
+        cd.length = n
+        for node in path:
+            at = slice(node, node + 1)
+            cd.append_kv([t[:, :, at] for t in c.nk], [t[:, :, at] for t in c.nv])
+            y = cd.step(c.q1[:, :, at])
+            assert ((out[:, :, at] - y).abs() <= tol + (1e-2 if dtype != torch.float32 else 0) * y.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_commit(dtype):
+    rng = random.Random(5)
+    lens = [20, 0, 64, 9]
+    parents = [tree("random", 12, rng) for _ in lens]
+    c = Case(order=3, h=4, g=2, d=64, dtype=dtype, lens=lens, parents=parents, cap=100)
+    c.step()
+    caches = c.dec.keys + c.dec.vals + c.dec.msgs + c.dec.lses
+    before = [x.clone() for x in caches]
+    paths = []
+    for p in parents:
+        node, path = rng.randrange(12), []
+        while node >= 0:
+            path.insert(0, node)
+            node = p[node]
+        paths.append(path)
+    paths[3] = []
+    path = torch.full((4, 12), 99, dtype=torch.int32)
+    for i, p in enumerate(paths):
+        path[i, :len(p)] = torch.tensor(p, dtype=torch.int32)
+    c.dec.commit(path.cuda(), torch.tensor([len(p) for p in paths], dtype=torch.int32, device="cuda"))
+    assert c.dec.lengths.tolist() == [n + len(p) for n, p in zip(lens, paths)]
+    for x, old in zip(caches, before):
+        for i, (n, p) in enumerate(zip(lens, paths)):
+            assert torch.equal(x[i, :, :n], old[i, :, :n])
+            assert torch.equal(x[i, :, n:n + len(p)], old[i, :, [n + j for j in p]])
+    # the next step continues from the kept rows
+    c.lens = c.dec.lengths.tolist()
+    c.check()
+
+
+def test_commit_of_bad_paths_stays_inside():
+    c = Case(order=2, h=2, g=2, d=64, dtype=torch.bfloat16, lens=[5, 96], parents=[[-1, 0, 1]] * 2, cap=99)
+    c.step()
+    rest = [x[0, :, 8:].clone() for x in c.dec.keys]
+    c.dec.commit(torch.tensor([[2, 0, -7], [1 << 30, 2, 2]], dtype=torch.int32, device="cuda"),
+                 torch.tensor([1 << 30, 50], dtype=torch.int32, device="cuda"))
+    assert c.dec.lengths.tolist() == [8, 99]
+    for x, r in zip(c.dec.keys, rest):
+        assert torch.equal(x[0, :, 8:], r)
+    c.dec.lengths.fill_(5)
+    c.dec.commit(torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.tensor([-3, 3], dtype=torch.int32, device="cuda"))
+    assert c.dec.lengths.tolist() == [5, 6]
+
+
+def test_full_cache():
+    c = Case(order=2, h=2, g=2, d=64, dtype=torch.bfloat16, lens=[10, 4], parents=[[-1, 0, 1]] * 2, cap=13)
+    c.check()
+    one = torch.ones(2, dtype=torch.int32, device="cuda")
+    c.dec.commit(torch.zeros(2, 1, dtype=torch.int32, device="cuda"), one)
+    with pytest.raises(ValueError, match="capacity"):
+        c.step()
+    c.dec.lengths.fill_(3)
+    c.dec.refresh()
+    c.lens = [3, 3]
+    c.check()
+    # past the host's check (lengths changed on the device, as in a replayed graph): nodes without room are padding
+    guard = [x[1].clone() for x in c.dec.keys]
+    c.dec.lengths.copy_(torch.tensor([12, 1 << 30], dtype=torch.int32))
+    out = c.step()
+    assert (out[0, :, 1:] == 0).all() and (out[0, :, 0] != 0).any() and (out[1] == 0).all()
+    for x, old in zip(c.dec.keys, guard):
+        assert torch.equal(x[1], old)
+    c.dec.lengths.fill_(-5)
+    c.dec.refresh()
+    c.lens = [0, 0]
+    c.check()
+
+
+def test_positions():
+    c = Case(order=2, h=2, g=2, d=64, dtype=torch.bfloat16, lens=[10, 4], parents=[[-1, 0, 1, 0], [-1, -1, -2, 2]], cap=50)
+    assert c.dec.positions(c.par).tolist() == [[10, 11, 12, 11], [4, 4, 4, 4]]
+
+
+def test_graph_replays_follow_the_lengths():
+    rng = random.Random(6)
+    lens = [100, 30]
+    c = Case(order=3, h=4, g=2, d=64, dtype=torch.bfloat16, lens=lens, parents=[tree("random", 6, rng) for _ in lens], cap=400)
+    other = Case(order=3, h=4, g=2, d=64, dtype=torch.bfloat16, lens=lens, parents=c.parents, cap=400)
+    path = torch.tensor([[0, 3, 5, 0], [1, 2, 4, 0]], dtype=torch.int32, device="cuda")
+    count = torch.tensor([3, 2], dtype=torch.int32, device="cuda")
+    c.step()          # before capture: first-launch settings
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.step()
+        c.dec.commit(path, count)
+    assert c.dec.lengths.tolist() == lens
+    for it in range(5):
+        for x, y in zip([c.q1] + c.nk + c.nv, [other.q1] + other.nk + other.nv):
+            x.copy_(torch.randn(x.shape, device="cuda"))
+            y.copy_(x)
+        graph.replay()
+        want = other.step()
+        other.dec.commit(path, count)
+        assert torch.equal(out, want)
+    assert c.dec.lengths.tolist() == [115, 40]
+    for x, y in zip(c.dec.keys + c.dec.msgs + c.dec.lses, other.dec.keys + other.dec.msgs + other.dec.lses):
+        assert torch.equal(x[0, :, :115], y[0, :, :115]) and torch.equal(x[1, :, :40], y[1, :, :40])
+
+
+def test_two_decoders_on_two_streams():
+    rng = random.Random(7)
+    cases = [Case(order=3, h=8, g=2, d=128, dtype=torch.bfloat16, lens=[3000 + i, 500], parents=[tree("random", 10, rng)] * 2, seed=i)
+             for i in range(2)]
+    want = [c.step().clone() for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for _ in range(3):
+        got = []
+        for c, s in zip(cases, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(c.step())
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_refusals():
+    c = Case(order=2, h=4, g=2, d=64, dtype=torch.bfloat16, lens=[10, 4], parents=[[-1, 0, 1]] * 2, cap=50)
+    q, nk, nv, par = c.q1, c.nk, c.nv, c.par
+    wide = torch.randn(2, 4, 9, 64, device="cuda").bfloat16()
+    for err, args in ((ValueError, (q[0], nk, nv, par)), (ValueError, (wide, nk, nv, par)), (ValueError, (q, nk[:1], nv, par)),
+                      (ValueError, (q, nk, [nv[0][:, :1]], par)), (TypeError, (q.float(), nk, nv, par)), (TypeError, (q, [nk[0].half(), nk[1]], nv, par)),
+                      (TypeError, (q, nk, nv, par.long())), (ValueError, (q, nk, nv, par[:, :2])), (RuntimeError, (q, nk, nv, par.cpu())),
+                      (RuntimeError, (q.cpu(), nk, nv, par))):
+        with pytest.raises(err):
+            c.dec.step(*args)
+    with pytest.raises(ValueError):
+        c.dec.step(q, nk, nv, par, out=torch.empty(2, 4, 3, 32, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="no step"):
+        Case(order=2, h=2, g=2, d=64, dtype=torch.bfloat16, lens=[3], parents=[[-1]]).dec.commit(par[:1], torch.ones(1, dtype=torch.int32, device="cuda"))
+    c.step()
+    one = torch.ones(2, dtype=torch.int32, device="cuda")
+    for err, args in ((TypeError, (par.long(), one)), (ValueError, (par[:1], one)), (ValueError, (par, one[:1])), (RuntimeError, (par.cpu(), one))):
+        with pytest.raises(err):
+            c.dec.commit(*args)
+    rows = [torch.zeros(2, 2, 20, 64, device="cuda")] * 2
+    for lens in ([21, 0], [-1, 0], [3]):
+        with pytest.raises(ValueError):
+            c.dec.load(rows, rows[:1], [torch.zeros(2, 2, 20, device="cuda")], rows[:1], lens)
