@@ -11,7 +11,10 @@
 // natural-log units.
 //
 // PACKED: one CTA per (packed sequence, head) where the caller bounds the
-// lengths by 128; the CTA takes the rows of its sequence.
+// lengths by 128; the CTA takes the rows of its sequence. Sequences of up to 64
+// and of 65 to 128 rows have a launch each (NMAX): the warps and score registers
+// of 128 rows, idle in a short sequence, left one CTA per SM.
+#include <algorithm>
 #include <cfloat>
 #include <mutex>
 #include <type_traits>
@@ -49,17 +52,17 @@ __device__ __forceinline__ void store_packed(const PolyPassArgs& a, const Packed
   }
 }
 
-template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP, bool PACKED>
-__global__ void __launch_bounds__(256) pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
+template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP, bool PACKED, int NMAX>
+__global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
   constexpr int KS = D / 16, NB = D / 8, CH = D / 8;
-  constexpr int KNB = kMaxN / 8;   // key n-blocks
+  constexpr int KNB = NMAX / 8;   // key n-blocks
   const int bh = blockIdx.x;
   const int b = PACKED ? 0 : bh / a.heads, h = bh - (PACKED ? bh / a.heads : b) * a.heads;
   int nq = a.seq_q, nk = a.seq_k;
   if constexpr (PACKED) {
     const int first = packed_at(pk.cu, bh / a.heads, pk.total);
     nq = nk = min(packed_at(pk.cu, bh / a.heads + 1, pk.total) - first, pk.max_len);
-    if (nk <= 0) return;
+    if (nk <= 0 || (NMAX == 64 ? nk > 64 : nk <= 64)) return;
     const int64_t f = first;
     a.q = (const T*)a.q + f * a.q_stride[2];
     a.k = (const T*)a.k + f * a.k_stride[2];
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(256) pass_small_kernel(PolyPassArgs a, const P
 #pragma unroll
   for (int n = 0; n < NB; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 #pragma unroll
-  for (int kk = 0; kk < kMaxN / 16; ++kk) {
+  for (int kk = 0; kk < NMAX / 16; ++kk) {
     if (kk * 16 < kp) {
       const uint32_t pa0 = pk2<T>(s[2 * kk][0], s[2 * kk][1]), pa1 = pk2<T>(s[2 * kk][2], s[2 * kk][3]);
       const uint32_t pa2 = pk2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
@@ -239,23 +242,32 @@ __global__ void __launch_bounds__(256) pass_small_kernel(PolyPassArgs a, const P
   }
 }
 
-template <typename T, int D, bool B, bool C, bool PACKED>
-int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
-  constexpr int smem = 2 * kMaxN * D * 2 + kMaxN * 4;
+template <typename T, int D, bool B, bool C, bool PACKED, int NMAX>
+int launch_n(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
+  constexpr int smem = 2 * NMAX * D * 2 + NMAX * 4;
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
   std::call_once(once, [] {
-    err = cudaFuncSetAttribute(pass_small_kernel<T, D, B, C, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    err = cudaFuncSetAttribute(pass_small_kernel<T, D, B, C, PACKED, NMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(small)");
-  const int nq = PACKED ? pk->max_len : a.seq_q, nk = PACKED ? pk->max_len : a.seq_k;
+  const int nq = PACKED ? std::min(pk->max_len, NMAX) : a.seq_q, nk = PACKED ? nq : a.seq_k;
   const int threads = 32 * ((nq + 15) / 16);
   const int kp = (nk + 15) & ~15;
   const int bytes = 2 * kp * D * 2 + kp * 4;   // <= smem (the attribute's maximum)
   const unsigned grid = (unsigned)((PACKED ? pk->seqs : a.batch) * a.heads);
-  pass_small_kernel<T, D, B, C, PACKED><<<grid, threads, bytes, s>>>(a, PACKED ? *pk : PackedSeqs{});
+  pass_small_kernel<T, D, B, C, PACKED, NMAX><<<grid, threads, bytes, s>>>(a, PACKED ? *pk : PackedSeqs{});
   note_launch(1);
   return cuda_status(cudaGetLastError(), "pass_small launch");
+}
+
+template <typename T, int D, bool B, bool C, bool PACKED>
+int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
+  if (PACKED) {
+    const int rc = launch_n<T, D, B, C, true, 64>(a, pk, s);
+    if (rc || pk->max_len <= 64) return rc;
+  }
+  return launch_n<T, D, B, C, PACKED, kMaxN>(a, pk, s);
 }
 
 template <typename T, int D, bool PACKED>

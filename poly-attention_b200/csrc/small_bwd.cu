@@ -12,7 +12,10 @@
 // the log2-domain lse are formed here: one launch and no workspace.
 //
 // Bound by latency: per CTA a few microseconds of dependent loads, products and
-// stores, so several CTAs share an SM (96 KB of shared memory at d = 64).
+// stores, so several CTAs have to share an SM. Sequences of up to 64 and of 65 to
+// 128 rows therefore have a launch each (NMAX), the first with half the threads
+// and 40 KB of shared memory at d = 64.
+#include <algorithm>
 #include <cfloat>
 #include <mutex>
 
@@ -32,21 +35,22 @@ struct SmallBwd {
   int rows;   // shared-memory rows: the length bound, padded to 16
 };
 
-template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP>
-__global__ void __launch_bounds__(256) small_bwd_kernel(const __grid_constant__ SmallBwd P) {
+template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP, int NMAX>
+__global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_kernel(const __grid_constant__ SmallBwd P) {
   constexpr int KS = D / 16, NB = D / 8, CH = D / 8;
+  constexpr int SP = NMAX * 2;   // bytes of a dS row
   const PolyPassBwdArgs& a = P.a;
   const PolyPassArgs& f = a.fwd;
   const PackedSeqs& pk = P.pk;
   const int seq = blockIdx.x / f.kv_heads, g = blockIdx.x - seq * f.kv_heads;
   const int64_t first = packed_at(pk.cu, seq, pk.total);
   const int n = min(packed_at(pk.cu, seq + 1, pk.total) - (int)first, pk.max_len);
-  if (n <= 0) return;
+  if (n <= 0 || (NMAX == 64 ? n > 64 : n <= 64)) return;
   const int np = (n + 15) & ~15;
   extern __shared__ __align__(16) uint8_t sm[];
   const int tile = P.rows * D * 2;
-  uint8_t *pK = sm, *pV = sm + tile, *pQ = sm + 2 * tile, *pG = sm + 3 * tile, *pS = sm + 4 * tile;   // pS [rows][128]
-  float* sLse = reinterpret_cast<float*>(pS + P.rows * kMaxN * 2);   // -lse in the log2 domain
+  uint8_t *pK = sm, *pV = sm + tile, *pQ = sm + 2 * tile, *pG = sm + 3 * tile, *pS = sm + 4 * tile;   // pS [rows][NMAX]
+  float* sLse = reinterpret_cast<float*>(pS + P.rows * SP);   // -lse in the log2 domain
   float* sDel = sLse + P.rows;
   const uint32_t sK = tc::smem_u32(pK), sV = tc::smem_u32(pV), sQ = tc::smem_u32(pQ), sG = tc::smem_u32(pG), sS = tc::smem_u32(pS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
@@ -171,8 +175,8 @@ __global__ void __launch_bounds__(256) small_bwd_kernel(const __grid_constant__ 
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const int ch = c * 2 + hf;
-          *reinterpret_cast<uint32_t*>(pS + k0 * 256 + ((ch ^ (k0 & 7)) << 4) + 4 * tq) = da[2 * hf];
-          *reinterpret_cast<uint32_t*>(pS + k1 * 256 + ((ch ^ (k1 & 7)) << 4) + 4 * tq) = da[2 * hf + 1];
+          *reinterpret_cast<uint32_t*>(pS + k0 * SP + ((ch ^ (k0 & 7)) << 4) + 4 * tq) = da[2 * hf];
+          *reinterpret_cast<uint32_t*>(pS + k1 * SP + ((ch ^ (k1 & 7)) << 4) + 4 * tq) = da[2 * hf + 1];
         }
         const int brow = c * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, bch = lane >> 4;
 #pragma unroll
@@ -197,7 +201,7 @@ __global__ void __launch_bounds__(256) small_bwd_kernel(const __grid_constant__ 
       for (int kk = 0; kk < kend; ++kk) {
         uint32_t x[4], y[4];
         const int r = kk * 16 + (lane & 7) + (lane >> 4) * 8, ch = warp * 2 + ((lane >> 3) & 1);
-        ldsm4t(sS + r * 256 + ((ch ^ (r & 7)) << 4), x[0], x[1], x[2], x[3]);
+        ldsm4t(sS + r * SP + ((ch ^ (r & 7)) << 4), x[0], x[1], x[2], x[3]);
         const int brow = kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, bch = lane >> 4;
 #pragma unroll
         for (int n2 = 0; n2 < NB / 2; ++n2) {
@@ -262,18 +266,25 @@ __global__ void __launch_bounds__(256) small_bwd_kernel(const __grid_constant__ 
   }
 }
 
-template <typename T, int D, bool B, bool C>
-int launch_t(const SmallBwd& p, cudaStream_t s) {
-  constexpr int row = 4 * D * 2 + kMaxN * 2 + 8;   // K, V, Q, dO, dS, lse and delta of one row
+template <typename T, int D, bool B, bool C, int NMAX>
+int launch_n(SmallBwd p, cudaStream_t s) {
+  constexpr int row = 4 * D * 2 + NMAX * 2 + 8;   // K, V, Q, dO, dS, lse and delta of one row
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
   std::call_once(once, [] {
-    err = cudaFuncSetAttribute(small_bwd_kernel<T, D, B, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxN * row);
+    err = cudaFuncSetAttribute(small_bwd_kernel<T, D, B, C, NMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, NMAX * row);
   });
   if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(small bwd)");
-  small_bwd_kernel<T, D, B, C><<<(unsigned)(p.pk.seqs * p.a.fwd.kv_heads), 2 * p.rows, p.rows * row, s>>>(p);
+  p.rows = std::min(p.rows, NMAX);
+  small_bwd_kernel<T, D, B, C, NMAX><<<(unsigned)(p.pk.seqs * p.a.fwd.kv_heads), 2 * p.rows, p.rows * row, s>>>(p);
   note_launch(1);
   return cuda_status(cudaGetLastError(), "small_bwd launch");
+}
+
+template <typename T, int D, bool B, bool C>
+int launch_t(const SmallBwd& p, cudaStream_t s) {
+  const int rc = launch_n<T, D, B, C, 64>(p, s);
+  return rc || p.rows <= 64 ? rc : launch_n<T, D, B, C, kMaxN>(p, s);
 }
 
 template <typename T, int D>
