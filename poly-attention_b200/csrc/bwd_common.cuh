@@ -184,6 +184,11 @@ __global__ void bwd_dq_convert_kernel(const PolyPassBwdArgs a, const float* dq_a
 template <typename T, int D>
 __global__ void __launch_bounds__(256) packed_bwd_prep_kernel(const PolyPassBwdArgs a, const PackedSeqs q, float* dq_acc,
                                                               float* lse2, float* delta, int64_t nq_pad) {
+  const int own = (q.total / 128 + q.seqs) * 4;   // the CTAs behind these zero the rows outside the sequences
+  if ((int)blockIdx.x >= own) {
+    if (blockIdx.y == 0) packed_zero_rest(q, blockIdx.x - own);
+    return;
+  }
   PackedTile t;
   const int slot = blockIdx.x >> 2;
   if (!packed_tile<128>(q.cu, q.seqs, q.total, slot, t)) return;

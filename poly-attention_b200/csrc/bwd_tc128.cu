@@ -476,7 +476,7 @@ int launch_t(const PolyPassBwdArgs& a, const PackedSeqs* seqs, cudaStream_t s) {
   if (rc) return rc;
   const dim3 pgrid((unsigned)(pw.slots * 4), (unsigned)f.heads);
   if (PACKED) {
-    packed_bwd_prep_kernel<T, D><<<pgrid, 256, 0, s>>>(a, *seqs, w.dq_acc, w.lse2, w.delta, pw.nq_pad);
+    packed_bwd_prep_kernel<T, D><<<dim3(pgrid.x + zero_ctas(*seqs), pgrid.y), 256, 0, s>>>(a, *seqs, w.dq_acc, w.lse2, w.delta, pw.nq_pad);
   } else {
     rc = cuda_status(cudaMemsetAsync(w.dq_acc, 0, (size_t)f.batch * f.heads * f.seq_q * D * 4, s), "memset dq acc");
     if (rc) return rc;

@@ -89,6 +89,16 @@ int copy_rows(const PolyRowCopy* copies, int n, cudaStream_t s);
 int head_rmsnorm(const PolyHeadNorm* norms, int n, cudaStream_t s);
 int rotary(const PolyRotaryArgs* args, cudaStream_t s);
 
+// Outputs whose rows outside every packed sequence are written as zeros (packed.cuh).
+struct ZeroRest {
+  struct {
+    char* p;
+    int heads, row_bytes;
+    int64_t head_stride, row_stride;   // bytes
+  } t[5];
+  int n;
+};
+
 // Sequences packed end to end (packed.cuh): device offsets, their number, rows in all.
 struct PackedSeqs {
   const int* cu;
@@ -98,7 +108,10 @@ struct PackedSeqs {
   const void* v_left; int64_t v_left_stride[2];
   const void* v_right; int64_t v_right_stride[2];
   void* dv_right; int64_t dv_right_stride[2];
+  ZeroRest zero;        // the work of kZeroCtas extra CTAs of the pass's first kernel (none if zero.n is 0)
 };
+constexpr int kZeroCtas = 16;
+inline unsigned zero_ctas(const PackedSeqs& q) { return q.zero.n ? kZeroCtas : 0; }
 int launch_packed_fwd_simt(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s);
 int launch_packed_bwd_simt(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s);
 size_t packed_bwd_simt_workspace(const PolyPassBwdArgs& a);

@@ -162,6 +162,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   // group at one pair index before the next, so the dispatch is
   // longest-first while the CTAs in flight share few K / V streams
   int bh, yi;
+  if constexpr (PACKED) {
+    const int own = p.n_bh * p.m_tiles;   // the CTAs behind these zero the rows outside the sequences
+    if ((int)blockIdx.x >= own) {
+      packed_zero_rest(p.pk, blockIdx.x - own);
+      return;
+    }
+  }
   {
     const int lin = blockIdx.x;
     const int grp = lin / (p.grp_bh * p.m_tiles);
@@ -593,7 +600,7 @@ int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t st) {
   const int grp_kv = (int)std::max<size_t>(1, (32u << 20) / std::max<size_t>(kv_bytes, 1));
   p.n_bh = a.batch * a.heads;
   p.grp_bh = std::min(p.n_bh, grp_kv * rep_h);
-  dim3 grid((unsigned)(p.n_bh * p.m_tiles));
+  dim3 grid((unsigned)(p.n_bh * p.m_tiles) + (PACKED ? zero_ctas(*pk) : 0));
   pass_fwd_tc2_kernel<T, HAS_BIAS, D, PACKED, SOFTCLAMP><<<grid, kThreads, L2::kAlloc, st>>>(tq, tk, tv, tb, p);
   note_launch(1);
   return cuda_status(cudaGetLastError(), "pass_fwd_tc2 launch");

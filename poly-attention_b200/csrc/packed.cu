@@ -35,32 +35,6 @@ int check_packed(const PolyPassArgs& a, const int32_t* cu, int seqs, int max_len
   return POLY_OK;
 }
 
-// Rows before the first and behind the last sequence of up to 5 outputs, as
-// zeros. Usually there are none: the CTAs read two offsets and leave.
-struct ZeroRest {
-  struct {
-    char* p;
-    int heads, row_bytes;
-    int64_t head_stride, row_stride;   // bytes
-  } t[5];
-  int n;
-};
-
-__global__ void __launch_bounds__(128) packed_zero_rest_kernel(const ZeroRest z, const int* cu, int seqs, int total) {
-  const int lo = min(max(cu[0], 0), total), hi = min(max(cu[seqs], lo), total);
-  const int rest = lo + (total - hi);
-  for (int r = blockIdx.x; r < rest; r += gridDim.x) {
-    const int64_t row = r < lo ? r : hi + (r - lo);
-    for (int k = 0; k < z.n; ++k) {
-      const int words = z.t[k].row_bytes >> 1;   // 16-bit words: rows need no more than their type's alignment
-      for (int i = threadIdx.x; i < z.t[k].heads * words; i += blockDim.x) {
-        const int h = i / words, w = i - h * words;
-        *reinterpret_cast<uint16_t*>(z.t[k].p + h * z.t[k].head_stride + row * z.t[k].row_stride + 2 * w) = 0;
-      }
-    }
-  }
-}
-
 void zero_add(ZeroRest& z, void* p, int heads, int dim, int es, int64_t head_stride, int64_t row_stride) {
   if (!p) return;
   auto& t = z.t[z.n++];
@@ -69,12 +43,6 @@ void zero_add(ZeroRest& z, void* p, int heads, int dim, int es, int64_t head_str
   t.row_bytes = dim * es;
   t.head_stride = head_stride * es;
   t.row_stride = row_stride * es;
-}
-
-int zero_rest(const ZeroRest& z, const PackedSeqs& q, cudaStream_t s) {
-  packed_zero_rest_kernel<<<64, 128, 0, s>>>(z, q.cu, q.seqs, q.total);
-  note_launch(1);
-  return cuda_status(cudaGetLastError(), "packed_zero_rest launch");
 }
 
 int check_fwd(const PolyPackedArgs* a) {
@@ -146,13 +114,11 @@ int poly_packed_pass_fwd(const PolyPackedArgs* a, void* stream) {
   if (a->zero_rest) {
     const PolyPassArgs& f = a->pass;
     const int es = f.dtype == POLY_F32 ? 4 : 2;
-    ZeroRest z{};
+    ZeroRest& z = q.zero;
     zero_add(z, f.out, f.heads, f.head_dim, es, f.out_stride[1], f.out_stride[2]);
     zero_add(z, f.epi_out, f.heads, f.head_dim, es, f.epi_out_stride[1], f.epi_out_stride[2]);
     zero_add(z, f.lse, f.heads, 1, 4, f.lse_stride[1], 1);
     zero_add(z, a->out_lo, f.heads, f.head_dim, es, f.out_stride[1], f.out_stride[2]);
-    const int rz = zero_rest(z, q, (cudaStream_t)stream);
-    if (rz) return rz;
   }
   switch (choose_fwd(*a)) {
     case Kind::kTc: return launch_packed_fwd_tc(a->pass, q, (cudaStream_t)stream);
@@ -200,14 +166,12 @@ int poly_packed_pass_bwd(const PolyPackedBwdArgs* a, void* stream) {
   if (a->zero_rest) {
     const PolyPassArgs& f = b.fwd;
     const int es = f.dtype == POLY_F32 ? 4 : 2;
-    ZeroRest z{};
+    ZeroRest& z = q.zero;
     if (!b.dq_accumulate) zero_add(z, b.dq, f.heads, f.head_dim, es, b.dq_stride[1], b.dq_stride[2]);
     zero_add(z, b.dk, f.kv_heads, f.head_dim, es, b.dk_stride[1], b.dk_stride[2]);
     zero_add(z, b.dv, f.kv_heads, f.head_dim, es, b.dv_stride[1], b.dv_stride[2]);
     zero_add(z, b.dbias, f.kv_heads, 1, 4, b.dbias_stride[1], 1);
     zero_add(z, a->dv_right, f.kv_heads, f.head_dim, es, a->dv_right_stride[0], a->dv_right_stride[1]);
-    const int rz = zero_rest(z, q, (cudaStream_t)stream);
-    if (rz) return rz;
   }
   switch (choose_bwd(*a)) {
     case Kind::kTc: return launch_packed_bwd_tc(b, q, (cudaStream_t)stream);

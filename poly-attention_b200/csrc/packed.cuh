@@ -12,6 +12,8 @@
 
 #include <stdint.h>
 
+#include "common.cuh"
+
 namespace poly {
 
 __device__ __forceinline__ int packed_at(const int* cu, int s, int total) { return min(max(cu[s], 0), total); }
@@ -46,6 +48,25 @@ __device__ __forceinline__ bool packed_tile(const int* cu, int seqs, int total, 
   t.slot0 = t.start / B + lo;
   t.tile = slot - t.slot0;
   return t.tile >= 0 && t.tile * B < t.len;
+}
+
+// Rows before the first and behind the last sequence of a pass's outputs, as zeros:
+// CTA `part` of kZeroCtas that the pass's first kernel has for it beside its own.
+// Usually there are none, and the CTA reads two offsets and leaves.
+__device__ __forceinline__ void packed_zero_rest(const PackedSeqs& q, int part) {
+  const int lo = packed_at(q.cu, 0, q.total), hi = max(packed_at(q.cu, q.seqs, q.total), lo);
+  const int rest = lo + (q.total - hi);
+  for (int r = part; r < rest; r += kZeroCtas) {
+    const int64_t row = r < lo ? r : hi + (r - lo);
+    for (int k = 0; k < q.zero.n; ++k) {
+      const auto& t = q.zero.t[k];
+      const int words = t.row_bytes >> 1;   // 16-bit words: rows need no more than their type's alignment
+      for (int i = threadIdx.x; i < t.heads * words; i += blockDim.x) {
+        const int h = i / words, w = i - h * words;
+        *reinterpret_cast<uint16_t*>(t.p + h * t.head_stride + row * t.row_stride + 2 * w) = 0;
+      }
+    }
+  }
 }
 
 }  // namespace poly

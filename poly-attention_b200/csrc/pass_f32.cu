@@ -66,8 +66,13 @@ __global__ void __launch_bounds__(128) pass_f32_kernel(PolyPassArgs a, const Pac
   const int b = PACKED ? 0 : bh / a.heads, h = bh - b * a.heads, g = h / (a.heads / a.kv_heads);
   int tile = blockIdx.x;
   if constexpr (PACKED) {
+    const int own = pk.total / BM + pk.seqs;   // the CTAs behind these zero the rows outside the sequences
+    if ((int)blockIdx.y >= own) {
+      if (bh == 0) packed_zero_rest(pk, blockIdx.y - own);
+      return;
+    }
     PackedTile t;
-    if (!packed_tile<BM>(pk.cu, pk.seqs, pk.total, gridDim.y - 1 - blockIdx.y, t)) return;
+    if (!packed_tile<BM>(pk.cu, pk.seqs, pk.total, own - 1 - blockIdx.y, t)) return;
     tile = t.tile;
     a.seq_q = a.seq_k = t.len;
     const int64_t f = t.start;
@@ -307,7 +312,7 @@ int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
     err = cudaFuncSetAttribute(pass_f32_kernel<B, C, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(f32)");
-  const dim3 grid = PACKED ? dim3(a.heads, a.seq_q / BM + pk->seqs) : dim3((a.seq_q + BM - 1) / BM, a.batch * a.heads);
+  const dim3 grid = PACKED ? dim3(a.heads, a.seq_q / BM + pk->seqs + zero_ctas(*pk)) : dim3((a.seq_q + BM - 1) / BM, a.batch * a.heads);
   pass_f32_kernel<B, C, PACKED><<<grid, 128, kSmem, s>>>(a, PACKED ? *pk : PackedSeqs{});
   note_launch(1);
   return cuda_status(cudaGetLastError(), "pass_f32 launch");
@@ -326,7 +331,7 @@ int launch_pass_f32(const PolyPassArgs& a, cudaStream_t s) { return launch_any<f
 // The slots are the grid's second axis, which holds 65535.
 bool packed_f32_eligible(const PolyPackedArgs& pa) {
   const PolyPassArgs& a = pa.pass;
-  if (a.dtype != POLY_F32 || a.head_dim != D || a.seq_q / BM + pa.seqs > 65535) return false;
+  if (a.dtype != POLY_F32 || a.head_dim != D || a.seq_q / BM + pa.seqs > 65535 - kZeroCtas) return false;
   if (!al(a.k, 16) || !al(a.v, 16) || !al(a.out, 8)) return false;
   return !((a.k_stride[1] | a.k_stride[2] | a.v_stride[1] | a.v_stride[2]) & 3) && !((a.out_stride[1] | a.out_stride[2]) & 1);
 }

@@ -65,6 +65,11 @@ __global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(PolyPassArgs
   int row0 = blockIdx.x * kWarps;
   int64_t first = 0;   // the sequence's first row
   if constexpr (PACKED) {
+    const int own = pk.total / kWarps + pk.seqs;   // the slots; the CTAs behind them zero the rest
+    if ((int)blockIdx.x >= own) {
+      if (blockIdx.y == 0) packed_zero_rest(pk, blockIdx.x - own);
+      return;
+    }
     PackedTile t;
     if (!packed_tile<kWarps>(pk.cu, pk.seqs, pk.total, blockIdx.x, t)) return;
     row0 = t.tile * kWarps;
@@ -273,6 +278,11 @@ __global__ void __launch_bounds__(kWarps * 32) pass_bwd_dq_simt_kernel(PolyPassB
   const int d = a.head_dim;
   int64_t first = 0;
   if constexpr (PACKED) {
+    const int own = pk.total / kWarps + pk.seqs;
+    if ((int)blockIdx.x >= own) {
+      if (blockIdx.y == 0) packed_zero_rest(pk, blockIdx.x - own);
+      return;
+    }
     PackedTile t;
     if (!packed_tile<kWarps>(pk.cu, pk.seqs, pk.total, blockIdx.x, t)) return;
     row0 = t.tile * kWarps;
@@ -447,7 +457,7 @@ unsigned row_ctas(int rows, const PackedSeqs* pk) {
 
 template <typename T, int DMAX>
 int launch_fwd_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
-  dim3 grid(row_ctas(a.seq_q, pk), a.batch * a.heads);
+  dim3 grid(row_ctas(a.seq_q, pk) + (pk ? zero_ctas(*pk) : 0), a.batch * a.heads);
   if (pk)
     pass_fwd_simt_kernel<T, DMAX, true><<<grid, kWarps * 32, 0, s>>>(a, *pk);
   else
@@ -461,7 +471,7 @@ int launch_bwd_t(const PolyPassBwdArgs& a, const PackedSeqs* pk, cudaStream_t s)
   const int64_t rows = (int64_t)a.fwd.batch * a.fwd.heads * a.fwd.seq_q;
   float* delta = (float*)a.workspace;
   int* fb_count = (int*)(delta + rows);
-  dim3 gq(row_ctas(a.fwd.seq_q, pk), a.fwd.batch * a.fwd.heads);
+  dim3 gq(row_ctas(a.fwd.seq_q, pk) + (pk ? zero_ctas(*pk) : 0), a.fwd.batch * a.fwd.heads);
   dim3 gk(row_ctas(a.fwd.seq_k, pk), a.fwd.batch * a.fwd.kv_heads);
   const unsigned gd = (unsigned)((rows + 7) / 8);
   if (pk) {

@@ -60,6 +60,10 @@ __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, co
   const int b = PACKED ? 0 : bh / a.heads, h = bh - (PACKED ? bh / a.heads : b) * a.heads;
   int nq = a.seq_q, nk = a.seq_k;
   if constexpr (PACKED) {
+    if (bh >= pk.seqs * a.heads) {   // the CTAs behind the sequences' zero the rows outside them
+      packed_zero_rest(pk, bh - pk.seqs * a.heads);
+      return;
+    }
     const int first = packed_at(pk.cu, bh / a.heads, pk.total);
     nq = nk = min(packed_at(pk.cu, bh / a.heads + 1, pk.total) - first, pk.max_len);
     if (nk <= 0 || (NMAX == 64 ? nk > 64 : nk <= 64)) return;
@@ -255,8 +259,11 @@ int launch_n(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   const int threads = 32 * ((nq + 15) / 16);
   const int kp = (nk + 15) & ~15;
   const int bytes = 2 * kp * D * 2 + kp * 4;   // <= smem (the attribute's maximum)
-  const unsigned grid = (unsigned)((PACKED ? pk->seqs : a.batch) * a.heads);
-  pass_small_kernel<T, D, B, C, PACKED, NMAX><<<grid, threads, bytes, s>>>(a, PACKED ? *pk : PackedSeqs{});
+  PackedSeqs q{};
+  if (PACKED) q = *pk;
+  if (PACKED && NMAX != 64) q.zero.n = 0;   // done by the first launch
+  const unsigned grid = (unsigned)((PACKED ? pk->seqs : a.batch) * a.heads) + zero_ctas(q);
+  pass_small_kernel<T, D, B, C, PACKED, NMAX><<<grid, threads, bytes, s>>>(a, q);
   note_launch(1);
   return cuda_status(cudaGetLastError(), "pass_small launch");
 }

@@ -42,6 +42,10 @@ __global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_
   const PolyPassBwdArgs& a = P.a;
   const PolyPassArgs& f = a.fwd;
   const PackedSeqs& pk = P.pk;
+  if ((int)blockIdx.x >= pk.seqs * f.kv_heads) {   // the CTAs behind the sequences' zero the rows outside them
+    packed_zero_rest(pk, blockIdx.x - pk.seqs * f.kv_heads);
+    return;
+  }
   const int seq = blockIdx.x / f.kv_heads, g = blockIdx.x - seq * f.kv_heads;
   const int64_t first = packed_at(pk.cu, seq, pk.total);
   const int n = min(packed_at(pk.cu, seq + 1, pk.total) - (int)first, pk.max_len);
@@ -276,7 +280,8 @@ int launch_n(SmallBwd p, cudaStream_t s) {
   });
   if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(small bwd)");
   p.rows = std::min(p.rows, NMAX);
-  small_bwd_kernel<T, D, B, C, NMAX><<<(unsigned)(p.pk.seqs * p.a.fwd.kv_heads), 2 * p.rows, p.rows * row, s>>>(p);
+  if (NMAX != 64) p.pk.zero.n = 0;   // done by the first launch
+  small_bwd_kernel<T, D, B, C, NMAX><<<(unsigned)(p.pk.seqs * p.a.fwd.kv_heads) + zero_ctas(p.pk), 2 * p.rows, p.rows * row, s>>>(p);
   note_launch(1);
   return cuda_status(cudaGetLastError(), "small_bwd launch");
 }

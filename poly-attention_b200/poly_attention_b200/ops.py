@@ -5,6 +5,7 @@ projections' natural [b, n, h, d] memory layout is consumed without copies.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -51,6 +52,14 @@ def _mask(m, n):
 
 def _stream(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Context that makes ``device`` current for the launches in it (nothing to do where it already is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _ptr(t):

@@ -20,7 +20,7 @@ import torch
 
 from ._lib import PolyPackedArgs, PolyPackedBwdArgs, check, lib
 from .core import _autocast, _sc
-from .ops import _DTYPES, _require_cuda, _stream
+from .ops import _DTYPES, _on, _require_cuda, _stream
 
 
 def packed_offsets(lengths, device="cuda"):
@@ -61,13 +61,13 @@ def _rows(t):
 def _set(a, name, t):
     """A [total, heads, d] tensor (or [heads, total] fp32 vector) into its pointer and (batch, head, row) strides."""
     setattr(a, name, t.data_ptr())
-    st = getattr(a, name + "_stride")
-    if t.dim() == 3 and len(st) == 3:
-        st[0], st[1], st[2] = 0, t.stride(1), t.stride(0)
-    elif t.dim() == 3:
-        st[0], st[1] = t.stride(1), t.stride(0)
+    st, s = getattr(a, name + "_stride"), t.stride()
+    if len(s) == 3 and len(st) == 3:
+        st[1], st[2] = s[1], s[0]
+    elif len(s) == 3:
+        st[0], st[1] = s[1], s[0]
     else:
-        st[0], st[1] = 0, t.stride(0)
+        st[1] = s[0]
 
 
 def _vec(t, heads, total, what):
@@ -89,6 +89,35 @@ def _fill(a, q, k, v, bias, causal, softclamp, scale):
         _set(a, "bias", bias)
 
 
+def _forward(q, k, v, cu, bias, epi_mul, causal, softclamp, scale, max_seqlen, out_lo):
+    """pass_fwd_packed on checked tensors: (out, lse, epi or None, out_lo or None)."""
+    total, h, d = q.shape
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    a = PolyPackedArgs()
+    f = a.fwd
+    _fill(f, q, k, v, bias, causal, softclamp, scale)
+    out = q.new_empty(total, h, d)
+    lse = q.new_empty(h, total, dtype=torch.float32)
+    _set(f, "out", out)
+    _set(f, "lse", lse)
+    epi = lo = None
+    if epi_mul is not None:
+        epi_mul, epi = _rows(epi_mul), torch.empty_like(out)
+        _set(f, "epi_mul", epi_mul)
+        _set(f, "epi_out", epi)
+    if out_lo and q.dtype != torch.float32:
+        lo = torch.empty_like(out)
+        a.out_lo = lo.data_ptr()
+    a.cu_seqlens, a.seqs, a.max_len, a.zero_rest = cu.data_ptr(), cu.shape[0] - 1, int(max_seqlen or 0), 1
+    if a.seqs == 0 and total:
+        for t in (out, lse, epi, lo):
+            if t is not None:
+                t.zero_()
+    with _on(q.device):
+        check(lib.poly_packed_pass_fwd(a, _stream(q.device)), "poly_packed_pass_fwd")
+    return out, lse, epi, lo
+
+
 @torch.compiler.disable   # library calls through ctypes: dynamo runs them eagerly
 def pass_fwd_packed(q, k, v, cu_seqlens, *, causal=False, softclamp=None, scale=None, bias=None, epi_mul=None,
                     max_seqlen=None, out_lo=False):
@@ -101,81 +130,40 @@ def pass_fwd_packed(q, k, v, cu_seqlens, *, causal=False, softclamp=None, scale=
     """
     _tensors(q, k, v, bias, epi_mul)
     cu = _offsets(cu_seqlens, q)
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    total, h, d = q.shape
-    a = PolyPackedArgs()
     if bias is not None:
-        bias = _vec(bias, k.shape[1], total, "bias")
-    if h % max(k.shape[1], 1):
+        bias = _vec(bias, k.shape[1], q.shape[0], "bias")
+    if q.shape[1] % max(k.shape[1], 1):
         raise ValueError("heads must be divisible by kv_heads")
-    _fill(a.fwd, q, k, v, bias, causal, softclamp, scale)
-    out = q.new_empty(total, h, d)
-    lse = q.new_empty(h, total, dtype=torch.float32)
-    _set(a.fwd, "out", out)
-    _set(a.fwd, "lse", lse)
-    epi = None
-    if epi_mul is not None:
-        if epi_mul.shape != q.shape or epi_mul.dtype != q.dtype:
-            raise ValueError("epi_mul must have q's shape and dtype")
-        epi_mul, epi = _rows(epi_mul), torch.empty_like(out)
-        _set(a.fwd, "epi_mul", epi_mul)
-        _set(a.fwd, "epi_out", epi)
-    lo = torch.empty_like(out) if out_lo and q.dtype != torch.float32 else None
-    if lo is not None:
-        a.out_lo = lo.data_ptr()
-    a.cu_seqlens, a.seqs, a.max_len, a.zero_rest = cu.data_ptr(), cu.shape[0] - 1, int(max_seqlen or 0), 1
-    if a.seqs == 0 and total:
-        for t in (out, lse, epi, lo):
-            if t is not None:
-                t.zero_()
-    with torch.cuda.device(q.device):
-        check(lib.poly_packed_pass_fwd(a, _stream(q.device)), "poly_packed_pass_fwd")
+    if epi_mul is not None and (epi_mul.shape != q.shape or epi_mul.dtype != q.dtype):
+        raise ValueError("epi_mul must have q's shape and dtype")
+    out, lse, epi, lo = _forward(q, k, v, cu, bias, epi_mul, causal, softclamp, scale, max_seqlen, out_lo)
     return (out, lse) + ((epi,) if epi is not None else ()) + ((lo,) if out_lo else ())
 
 
-@torch.compiler.disable
-def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softclamp=None, scale=None, bias=None,
-                    dlse=None, dq=None, want_dbias=False, max_seqlen=None, out_lo=None, factors=None):
-    """Backward of ``pass_fwd_packed``. Returns (dq, dk, dv, dbias-or-None). With ``dq`` given the
-    query gradient is added to it in place. With ``factors`` = (left, right), whose product the
-    values were, dv is the pair of their gradients."""
-    _tensors(q, k, v, out, lse, dout, bias, dlse, dq, out_lo, *(factors or ()))
-    cu = _offsets(cu_seqlens, q)
-    q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout.to(q.dtype))
+def _backward(q, k, v, cu, out, lse, dout, bias, dlse, dq, want_dbias, out_lo, factors, causal, softclamp, scale, max_seqlen):
+    """pass_bwd_packed on checked tensors."""
+    q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
     total, h, d = q.shape
     g = k.shape[1]
-    if h % max(g, 1):
-        raise ValueError("heads must be divisible by kv_heads")
-    if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out and dout must have q's shape, out its dtype")
     if any(st <= 0 for st in dout.stride()):
         dout = dout.contiguous()        # broadcast gradients (out.sum().backward())
-    if dq is not None and (dq.shape != q.shape or dq.dtype != q.dtype or dq.stride(-1) != 1):
-        raise ValueError("dq must have q's shape and dtype and a contiguous last dim")
-    lse = _vec(lse, h, total, "lse")
     a = PolyPackedBwdArgs()
     b = a.bwd
-    if bias is not None:
-        bias = _vec(bias, g, total, "bias")
-    _fill(b.fwd, q, k, v, bias, causal, softclamp, scale)
-    _set(b.fwd, "out", out)
-    _set(b.fwd, "lse", lse)
+    f = b.fwd
+    _fill(f, q, k, v, bias, causal, softclamp, scale)
+    _set(f, "out", out)
+    _set(f, "lse", lse)
     _set(b, "dout", dout)
     if dlse is not None:
-        dlse = _vec(dlse, h, total, "dlse")
         _set(b, "dlse", dlse)
     if out_lo is not None:
-        if out_lo.shape != out.shape or out_lo.dtype != out.dtype or out_lo.stride() != out.stride():
-            raise ValueError("out_lo must have out's shape, dtype and strides")
         a.out_lo = out_lo.data_ptr()
     dright = None
     if factors is not None:
-        if any(t.shape != v.shape or t.dtype != v.dtype for t in factors):
-            raise ValueError("the values' factors must have their shape and dtype")
-        factors = tuple(_rows(t) for t in factors)
+        left, right = (_rows(t) for t in factors)
         dright = v.new_empty(total, g, d)
-        _set(a, "v_left", factors[0])
-        _set(a, "v_right", factors[1])
+        _set(a, "v_left", left)
+        _set(a, "v_right", right)
         _set(a, "dv_right", dright)
     b.dq_accumulate = int(dq is not None)
     if dq is None:
@@ -192,13 +180,42 @@ def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softcl
         for t in (dk, dv, dbias, dright, None if b.dq_accumulate else dq):
             if t is not None:
                 t.zero_()
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         need = lib.poly_packed_pass_bwd_workspace_size(a)
         ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
         if need:
             b.workspace, b.workspace_bytes = ws.data_ptr(), need
         check(lib.poly_packed_pass_bwd(a, _stream(q.device)), "poly_packed_pass_bwd")
     return dq, dk, dv if dright is None else (dv, dright), dbias
+
+
+@torch.compiler.disable
+def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softclamp=None, scale=None, bias=None,
+                    dlse=None, dq=None, want_dbias=False, max_seqlen=None, out_lo=None, factors=None):
+    """Backward of ``pass_fwd_packed``. Returns (dq, dk, dv, dbias-or-None). With ``dq`` given the
+    query gradient is added to it in place. With ``factors`` = (left, right), whose product the
+    values were, dv is the pair of their gradients."""
+    _tensors(q, k, v, out, lse, dout, bias, dlse, dq, out_lo, *(factors or ()))
+    cu = _offsets(cu_seqlens, q)
+    total, h = q.shape[:2]
+    g = k.shape[1]
+    if h % max(g, 1):
+        raise ValueError("heads must be divisible by kv_heads")
+    if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out and dout must have q's shape, out its dtype")
+    if dq is not None and (dq.shape != q.shape or dq.dtype != q.dtype or dq.stride(-1) != 1):
+        raise ValueError("dq must have q's shape and dtype and a contiguous last dim")
+    if out_lo is not None and (out_lo.shape != out.shape or out_lo.dtype != out.dtype or out_lo.stride() != out.stride()):
+        raise ValueError("out_lo must have out's shape, dtype and strides")
+    if out_lo is not None and out.stride(-1) != 1:
+        raise ValueError("out and out_lo must have a contiguous last dim")
+    if factors is not None and any(t.shape != v.shape or t.dtype != v.dtype for t in factors):
+        raise ValueError("the values' factors must have their shape and dtype")
+    lse = _vec(lse, h, total, "lse")
+    bias = None if bias is None else _vec(bias, g, total, "bias")
+    dlse = None if dlse is None else _vec(dlse, h, total, "dlse")
+    return _backward(q, k, v, cu, out, lse, dout.to(q.dtype), bias, dlse, dq, want_dbias, out_lo, factors, causal, softclamp,
+                     scale, max_seqlen)
 
 
 def packed_kernel_names(q, k, v, max_seqlen=None):
@@ -213,6 +230,18 @@ def packed_kernel_names(q, k, v, max_seqlen=None):
     return lib.poly_packed_pass_fwd_kernel_name(a).decode(), lib.poly_packed_pass_bwd_kernel_name(b).decode()
 
 
+def _chain_forward(order, cu, opts, ql, qr, vs, keep):
+    """Per level: values, biases, messages, log-sum-exps, rounding residues (if ``keep``)."""
+    vals, biases, msgs, lses, los = ([None] * order for _ in range(5))
+    val, bias = vs[-1], None
+    for t in range(order - 1, -1, -1):
+        vals[t], biases[t] = val, bias
+        # V' = v * msg is written by the pass that makes msg (n_poly_attention.py:287)
+        msgs[t], lses[t], epi, los[t] = _forward(ql[t], qr[t], val, cu, bias, vs[t - 2] if t >= 2 else None, *opts, keep)
+        val, bias = epi if t >= 2 else msgs[t], lses[t]
+    return vals, biases, msgs, lses, los
+
+
 class _PackedChain(torch.autograd.Function):
     """The order-n chain. Inputs: order queries ql, order keys qr and order - 1 values; shared[t] says
     that ql[t] is qr[t - 1], whose two gradients are then summed inside the kernel."""
@@ -220,22 +249,10 @@ class _PackedChain(torch.autograd.Function):
     @staticmethod
     def forward(ctx, order, shared, cu, opts, *tensors):
         ql, qr, vs = tensors[:order], tensors[order:2 * order], tensors[2 * order:]
-        vals, biases, msgs, lses, los = ([None] * order for _ in range(5))
-        val, bias = vs[-1], None
-        keep = any(ctx.needs_input_grad)
-        for t in range(order - 1, -1, -1):
-            vals[t], biases[t] = val, bias
-            # V' = v * msg is written by the pass that makes msg (n_poly_attention.py:287)
-            res = pass_fwd_packed(ql[t], qr[t], val, cu, bias=bias, epi_mul=vs[t - 2] if t >= 2 else None, out_lo=keep,
-                                  **opts)
-            msgs[t], lses[t] = res[:2]
-            if keep:
-                los[t] = res[-1]
-            val, bias = res[2] if t >= 2 else msgs[t], lses[t]
+        vals, biases, msgs, lses, los = _chain_forward(order, cu, opts, ql, qr, vs, True)
         ctx.order, ctx.shared, ctx.opts = order, shared, opts
-        if keep:
-            ctx.has = [[x is not None for x in xs] for xs in (biases, los)]
-            ctx.save_for_backward(cu, *tensors, *vals, *msgs, *lses, *(x for x in (*biases, *los) if x is not None))
+        ctx.has = [[x is not None for x in xs] for xs in (biases, los)]
+        ctx.save_for_backward(cu, *tensors, *vals, *msgs, *lses, *(x for x in (*biases, *los) if x is not None))
         extra = (*lses[:0:-1], *msgs[:0:-1])        # level order - 1 first, as in the caches
         ctx.mark_non_differentiable(*extra)
         return (msgs[0], *extra)
@@ -243,20 +260,21 @@ class _PackedChain(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, *_unused):
-        n, saved = ctx.order, list(ctx.saved_tensors)
-        take = lambda k: [saved.pop(0) for _ in range(k)]   # noqa: E731
+        n, saved = ctx.order, iter(ctx.saved_tensors)
+        take = lambda k: [next(saved) for _ in range(k)]   # noqa: E731
         cu, = take(1)
         ql, qr, vs, vals, msgs, lses = take(n), take(n), take(n - 1), take(n), take(n), take(n)
-        biases, los = ([saved.pop(0) if x else None for x in has] for has in ctx.has)
+        biases, los = ([next(saved) if x else None for x in has] for has in ctx.has)
+        causal, softclamp, scale, max_seqlen = ctx.opts
         dql, dqr, dvs = [None] * n, [None] * n, [None] * (n - 1)
-        g_out, g_lse = dout, None
+        g_out, g_lse = dout.to(ql[0].dtype), None
         for t in range(n):
             # a key tensor that is the next level's query keeps one gradient: the second part is added in the
             # kernel to the first, which was rounded once to the tensors' type
-            dq, dqr[t], dv, g_lse = pass_bwd_packed(ql[t], qr[t], vals[t], cu, msgs[t], lses[t], g_out, bias=biases[t],
-                                                    dlse=g_lse, dq=dqr[t - 1] if ctx.shared[t] else None,
-                                                    want_dbias=t < n - 1, out_lo=los[t],
-                                                    factors=(vs[t - 1], msgs[t + 1]) if 0 < t < n - 1 else None, **ctx.opts)
+            dq, dqr[t], dv, g_lse = _backward(ql[t], qr[t], vals[t], cu, msgs[t], lses[t], g_out, biases[t], g_lse,
+                                              dqr[t - 1] if ctx.shared[t] else None, t < n - 1, los[t],
+                                              (vs[t - 1], msgs[t + 1]) if 0 < t < n - 1 else None, causal, softclamp, scale,
+                                              max_seqlen)
             if not ctx.shared[t]:
                 dql[t] = dq
             if t == n - 1:
@@ -268,6 +286,27 @@ class _PackedChain(torch.autograd.Function):
         return (None, None, None, None, *dql, *dqr, *dvs)
 
 
+def _chain(q_left, q_right, vs, cu_seqlens, softclamp_value, causal, max_seqlen):
+    order = len(q_left)
+    if order < 2 or len(q_right) != order or len(vs) != order - 1:
+        raise ValueError("a chain of order n >= 2 takes n queries, n keys and n - 1 values")
+    shared = tuple(t >= 1 and q_left[t] is q_right[t - 1] for t in range(order))
+    ql, qr, vv = _autocast(*q_left), _autocast(*q_right), _autocast(*vs)
+    ql = [qr[t - 1] if shared[t] else ql[t] for t in range(order)]
+    _tensors(ql[0], qr[0], vv[0], *ql[1:], *qr[1:], *vv[1:])
+    if any(t.shape != qr[0].shape or t.dtype != qr[0].dtype for t in (*ql[1:], *qr[1:], *vv)):
+        raise ValueError("key, value and lower query tensors must share one shape and dtype")
+    if ql[0].shape[1] % max(qr[0].shape[1], 1):
+        raise ValueError("heads must be divisible by kv_heads")
+    cu = _offsets(cu_seqlens, ql[0])
+    opts = (bool(causal), softclamp_value, None, max_seqlen)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (*ql, *qr, *vv)):
+        res = _PackedChain.apply(order, shared, cu, opts, *ql, *qr, *vv)
+        return res[0], res[1:order], res[order:]
+    _, _, msgs, lses, _ = _chain_forward(order, cu, opts, ql, qr, vv, False)
+    return msgs[0], tuple(lses[:0:-1]), tuple(msgs[:0:-1])
+
+
 @torch.compiler.disable
 def poly_attention_chain_packed(q_left, q_right, vs, cu_seqlens, *, softclamp_value=None, causal=False, max_seqlen=None):
     """Order-n chain over packed sequences (n = len(q_left)), as ``poly_attention_chain``.
@@ -275,28 +314,16 @@ def poly_attention_chain_packed(q_left, q_right, vs, cu_seqlens, *, softclamp_va
     q_left[0] = q1 [total, h, d]; q_left[t >= 1], q_right[t] and vs[t] are [total, g, d]. Returns
     (out [total, h, d], lses [g, total], msgs [total, g, d]), lses / msgs in the caches' order.
     """
-    order = len(q_left)
-    if order < 2 or len(q_right) != order or len(vs) != order - 1:
-        raise ValueError("a chain of order n >= 2 takes n queries, n keys and n - 1 values")
-    shared = tuple(t >= 1 and q_left[t] is q_right[t - 1] for t in range(order))
-    ql, qr, vv = list(_autocast(*q_left)), list(_autocast(*q_right)), list(_autocast(*vs))
-    ql = [qr[t - 1] if shared[t] else ql[t] for t in range(order)]
-    for t in range(order):
-        _tensors(ql[t], qr[t], vv[t - 1 if t else 0])
-        if t and ql[t].shape != qr[t].shape:
-            raise ValueError("levels below the last have as many query as key heads")
-    cu = _offsets(cu_seqlens, ql[0])
-    opts = dict(causal=bool(causal), softclamp=softclamp_value, max_seqlen=max_seqlen)
-    res = _PackedChain.apply(order, shared, cu, opts, *ql, *qr, *vv)
-    return res[0], res[1:order], res[order:]
+    return _chain(q_left, q_right, vs, cu_seqlens, softclamp_value, causal, max_seqlen)
 
 
+@torch.compiler.disable
 def poly_attention_order2_packed(q1, q2, q3, v3, cu_seqlens, *, q2_pass1=None, softclamp_value=None, causal=False,
                                  max_seqlen=None):
     """Order-2 poly attention over packed sequences, as ``poly_attention_order2``: q1 [total, h, d];
     q2, q3, v3 [total, g, d]. Returns (out, lse23 [g, total], msg [total, g, d])."""
-    out, lses, msgs = poly_attention_chain_packed([q1, q2 if q2_pass1 is None else q2_pass1], [q2, q3], [v3], cu_seqlens,
-                                                  softclamp_value=softclamp_value, causal=causal, max_seqlen=max_seqlen)
+    out, lses, msgs = _chain((q1, q2 if q2_pass1 is None else q2_pass1), (q2, q3), (v3,), cu_seqlens, softclamp_value, causal,
+                             max_seqlen)
     return out, lses[0], msgs[0]
 
 

@@ -19,7 +19,7 @@ from torch import nn
 
 from . import _lib
 from ._lib import PolyRotaryArgs, check, lib
-from .ops import _DTYPES, _require_cuda, _stream
+from .ops import _DTYPES, _on, _require_cuda, _stream
 
 
 def rotary_frequencies(dim, *, theta=10000.0, scaling=None, factor=1.0, original_length=None, fast_turns=32.0,
@@ -78,7 +78,7 @@ def _launch(xs, outs, inv_freq, positions, start, cu_seqlens, angles, interleave
     elif positions is not None:
         a.positions, a.pos_wide = positions.data_ptr(), positions.dtype == torch.int64
         a.pos_stride[0], a.pos_stride[1] = positions.stride(0), positions.stride(1)
-    with torch.cuda.device(x0.device):
+    with _on(x0.device):
         stream = _stream(x0.device)
         for i0 in range(0, len(xs), _lib.MAX_ROTARY):
             part = range(i0, min(len(xs), i0 + _lib.MAX_ROTARY))

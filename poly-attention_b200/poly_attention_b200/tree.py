@@ -24,11 +24,12 @@ import torch
 
 from . import _lib
 from ._lib import PolyTreeAppend, PolyTreeCommit, PolyTreePass, check, lib
-from .ops import _DTYPES, _require_cuda, _stream
+from .ops import _DTYPES, _on, _require_cuda, _stream
 
 
 def _st3(dst, t, size=1):
-    dst[0], dst[1], dst[2] = t.stride(0) * size, t.stride(1) * size, t.stride(2) * size
+    s = t.stride()
+    dst[0], dst[1], dst[2] = s[0] * size, s[1] * size, s[2] * size
 
 
 class TreeDecoder:
@@ -102,7 +103,7 @@ class TreeDecoder:
         need = 0
         for a in self._passes:
             a.q = a.parents = a.k      # any address: only the sizes count
-            with torch.cuda.device(self.device):
+            with _on(self.device):
                 for n in range(1, max_nodes + 1):
                     a.nodes = n
                     need = max(need, lib.poly_tree_workspace_size(a))
@@ -165,7 +166,7 @@ class TreeDecoder:
         nodes = parents.shape[-1]
         parents = self._parents(parents, nodes)
         out = torch.empty(self.b, nodes, device=self.device, dtype=torch.int32)
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             check(lib.poly_tree_positions(self.lengths.data_ptr(), parents.data_ptr(), parents.stride(0), self.b, nodes,
                                           out.data_ptr(), out.stride(0), _stream(self.device)), "poly_tree_positions")
         return out
@@ -222,7 +223,7 @@ class TreeDecoder:
                 lses.append(s)
             else:
                 a.out = a.lse = None
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             check(lib.poly_tree_chain(ap, self._passes, order, _stream(self.device)), "poly_tree_chain")
         return (out, msgs, lses) if return_rows else out
 
@@ -240,7 +241,7 @@ class TreeDecoder:
         c = self._commit
         c.nodes, c.path_len = self._append.nodes, path.shape[1]
         c.path, c.path_stride, c.count = path.data_ptr(), path.stride(0), count.data_ptr()
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             check(lib.poly_tree_commit(c, _stream(self.device)), "poly_tree_commit")
         self._bound = min(self.cap, self._bound + min(c.nodes, c.path_len))
 
