@@ -421,7 +421,7 @@ POLY_API int poly_tree_commit(const PolyTreeCommit* args, void* stream);
  * positions of the drafted tokens); lengths[b] for padding. */
 POLY_API int poly_tree_positions(const int32_t* lengths, const int32_t* parents, int64_t parents_stride, int batch,
                                  int nodes, int32_t* positions, int64_t positions_stride, void* stream);
-/* "tree" (mma.sync) or "simt", "invalid" if validation fails */
+/* "tree" (mma.sync), "tc100" (tcgen05: more than 32 rows per key) or "simt"; "invalid" if validation fails */
 POLY_API const char* poly_tree_kernel_name(const PolyTreePass* pass);
 
 /*

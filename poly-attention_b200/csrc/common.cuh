@@ -72,6 +72,7 @@ int read_device_error_fwd2(int* out, bool reset);
 int read_device_error_dec(int* out, bool reset);
 int read_device_error_bwd128(int* out, bool reset);
 int read_device_error_tree(int* out, bool reset);
+int read_device_error_tree_tc(int* out, bool reset);
 size_t pass_bwd_tc128_workspace(const PolyPassBwdArgs& a);
 int launch_pass_bwd_tc128(const PolyPassBwdArgs& a, cudaStream_t s);
 int selftest_wait_timeout(uint64_t limit_ns, int* result, cudaStream_t s);

@@ -5,6 +5,9 @@
 // the cache is read once and everything else is small beside it: HBM-bound like
 // the single-token decode kernel, until M reaches some hundred rows.
 //
+// Up to 32 rows, and where values are a product, tree_kernel here; more rows go to
+// the tcgen05 kernel of tree_tc100.cu.
+//
 // tree_kernel (16-bit, d = 64 / 128): a CTA takes 16 WR rows (WR = 1, 2, 4) of one
 // (sequence, kv head) and one of `splits` key ranges. Warp 4 fills a ring of
 // 64-key stages with TMA (128-byte swizzle) and the bias by cp.async; warps 0-3
@@ -23,6 +26,7 @@
 //
 // tree_simt_kernel serves the other types and head sizes: one warp per row, 32-key
 // tiles in shared memory, fp32.
+#include <algorithm>
 #include <cfloat>
 #include <cstring>
 #include <mutex>
@@ -33,6 +37,7 @@
 #include "mma_sync.cuh"
 #include "tc_host.cuh"
 #include "tc_ptx.cuh"
+#include "tree_common.cuh"
 
 namespace poly {
 
@@ -48,70 +53,11 @@ int read_device_error_tree(int* out, bool reset) {
 }
 
 namespace {
+using namespace treec;
 
 constexpr int kKeys = 64;                     // keys per stage
 constexpr int kWarps = 4;                     // consumer warps
 constexpr int kThreads = (kWarps + 1) * 32;
-constexpr int kMaxSplits = 64;
-constexpr int kNodes = POLY_MAX_TREE_NODES;
-
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-// Visible tree nodes of every node as bits (0: padding), by pointer jumping: after
-// round r a node knows its nearest 2^r ancestors. Callers with at least 64 threads.
-__device__ __forceinline__ void ancestors(const int32_t* parents, int nodes, int room, uint64_t* mask, int* up) {
-  const int i = threadIdx.x;
-  if (i < kNodes) {
-    int p = -2;
-    if (i < nodes && i < room) {
-      p = parents[i];
-      if (p >= i || p < -1) p = -2;
-    }
-    mask[i] = p == -2 ? 0ull : 1ull << i;
-    up[i] = p;
-  }
-  __syncthreads();
-  for (int round = 0; round < 6; ++round) {
-    uint64_t m = 0;
-    int p = -2;
-    if (i < kNodes) {
-      m = mask[i];
-      p = up[i];
-      if (p >= 0) {
-        // below a padding node: padding too
-        m = mask[p] ? m | mask[p] : 0ull;
-        p = mask[p] ? up[p] : -2;
-      }
-    }
-    __syncthreads();
-    if (i < kNodes) {
-      mask[i] = m;
-      up[i] = p;
-    }
-    __syncthreads();
-  }
-}
-
-__device__ __forceinline__ int seq_length(const int32_t* lengths, int b, int capacity) {
-  return min(max(lengths[b], 0), capacity);
-}
-
-// Row `m` of a group: query head g * R + m % R, node m / R.
-template <typename T>
-__device__ __forceinline__ void write_row(const PolyTreePass& a, int b, int h, int node, int len, int c, float x, float y) {
-  const uint32_t w = ms::pk2<T>(x, y);
-  if (a.out)
-    *reinterpret_cast<uint32_t*>((T*)a.out + b * a.out_stride[0] + h * a.out_stride[1] + node * a.out_stride[2] + c) = w;
-  if (a.cache_out && len + node < a.capacity)
-    *reinterpret_cast<uint32_t*>((T*)a.cache_out + b * a.cache_out_stride[0] + h * a.cache_out_stride[1] +
-                                 (int64_t)(len + node) * a.cache_out_stride[2] + c) = w;
-}
-__device__ __forceinline__ void write_lse(const PolyTreePass& a, int b, int h, int node, int len, float v) {
-  if (a.lse) a.lse[b * a.lse_stride[0] + h * a.lse_stride[1] + node] = v;
-  if (a.cache_lse && len + node < a.capacity)
-    a.cache_lse[b * a.cache_lse_stride[0] + h * a.cache_lse_stride[1] + len + node] = v;
-}
 
 template <int D, int NARR>
 struct Ring {
@@ -153,11 +99,6 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {   // one roun
 __device__ __forceinline__ uint32_t swz(int key, int ch) {
   return (uint32_t)((ch >> 3) * (kKeys * 128) + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
 }
-
-struct TreeGeom {
-  int splits, row_blocks;
-  float* part;   // [group][row of the group][split][D + 2]
-};
 
 template <typename T, int D, int WR, bool VMUL>
 __global__ void __launch_bounds__(kThreads, 2) tree_kernel(const __grid_constant__ CUtensorMap tm_k,
@@ -446,6 +387,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
     const float* r = p + s * (D + 2);
     const float f = r[0] == -INFINITY ? 0.f : exp2f(r[0] - M);
     L = fmaf(r[1], f, L);
+    if (f == 0.f) continue;   // an empty range's record holds no sums
 #pragma unroll
     for (int t = 0; t < D / 64; ++t) {
       const float2 v = *reinterpret_cast<const float2*>(r + 2 + t * 64 + 2 * lane);
@@ -636,15 +578,19 @@ int warp_rows(const PolyTreePass& a) {
   return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
 }
 
-// Key ranges per (sequence, kv head): as many as fill two CTAs per SM, at least
-// one stage of the capacity each.
-TreeGeom geometry(const PolyTreePass& a) {
+// Key ranges per (sequence, kv head): as many as fill the CTAs that fit at once (two
+// of tree_kernel per SM, one of the tcgen05 kernel), at least one key tile of the
+// capacity each.
+TreeGeom geometry(const PolyTreePass& a, bool may_tc = true) {
   TreeGeom geo{};
   const int rows = a.nodes * (a.heads / a.kv_heads), wr = warp_rows(a);
-  geo.row_blocks = (rows + 16 * wr - 1) / (16 * wr);
+  geo.row_blocks = may_tc ? tree_tc_row_blocks(a) : 0;
+  geo.tcgen05 = geo.row_blocks > 0;
+  if (!geo.tcgen05) geo.row_blocks = (rows + 16 * wr - 1) / (16 * wr);
   const int64_t ctas = (int64_t)a.batch * a.kv_heads * geo.row_blocks;
-  const int tiles = (a.capacity + kKeys - 1) / kKeys;
-  geo.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxSplits, tiles), 2 * sm_count() / ctas));
+  const int keys = geo.tcgen05 ? 128 : kKeys, tiles = (a.capacity + keys - 1) / keys;
+  const int slots = (geo.tcgen05 ? 1 : 2) * sm_count();
+  geo.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxSplits, tiles), slots / ctas));
   return geo;
 }
 
@@ -679,6 +625,12 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cu
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+template <typename T, int D>
+int launch_combine(const PolyTreePass& a, const TreeGeom& geo, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.batch * a.heads * a.nodes;
+  return cuda_status(launch(tree_combine_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, s, true, a, geo), "tree launch");
+}
+
 template <typename T, int D, int WR, bool VMUL>
 int launch_tree(const PolyTreePass& a, cudaStream_t s, bool dep) {
   using R_ = Ring<D, VMUL ? 3 : 2>;
@@ -699,15 +651,18 @@ int launch_tree(const PolyTreePass& a, cudaStream_t s, bool dep) {
   const int groups = a.batch * a.kv_heads;
   cudaError_t e = launch(tree_kernel<T, D, WR, VMUL>, dim3(geo.splits * geo.row_blocks, groups), kThreads, R_::kAlloc, s, dep,
                          tk, tv, tm, a, geo);
-  if (e == cudaSuccess && geo.splits > 1) {
-    const int64_t rows = (int64_t)groups * a.nodes * (a.heads / a.kv_heads);
-    e = launch(tree_combine_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, s, true, a, geo);
-  }
-  return cuda_status(e, "tree launch");
+  rc = cuda_status(e, "tree launch");
+  return rc || geo.splits <= 1 ? rc : launch_combine<T, D>(a, geo, s);
 }
 
 template <typename T, int D>
 int launch_rows(const PolyTreePass& a, cudaStream_t s, bool dep) {
+  TreeGeom geo = geometry(a);
+  if (geo.tcgen05) {
+    geo.part = (float*)a.workspace;
+    const int rc = launch_tree_tc(a, geo, s, dep);
+    return rc || geo.splits <= 1 ? rc : launch_combine<T, D>(a, geo, s);
+  }
   const bool vm = a.v_mul != nullptr;
   switch (warp_rows(a)) {
     case 1: return vm ? launch_tree<T, D, 1, true>(a, s, dep) : launch_tree<T, D, 1, false>(a, s, dep);
@@ -773,14 +728,19 @@ size_t poly_sizeof_tree_commit(void) { return sizeof(PolyTreeCommit); }
 
 const char* poly_tree_kernel_name(const PolyTreePass* a) {
   if (check_pass(a) != POLY_OK) return "invalid";
-  return on_tensor_cores(*a) ? "tree" : "simt";
+  if (!on_tensor_cores(*a)) return "simt";
+  return a->nodes > 0 && tree_tc_row_blocks(*a) ? "tc100" : "tree";
 }
 
 size_t poly_tree_workspace_size(const PolyTreePass* a) {
   if (check_pass(a) != POLY_OK || !on_tensor_cores(*a) || a->batch == 0 || a->nodes == 0 || a->capacity == 0) return 0;
-  const TreeGeom geo = geometry(*a);
-  if (geo.splits <= 1) return 0;
-  return (size_t)a->batch * a->heads * a->nodes * geo.splits * (a->head_dim + 2) * sizeof(float);
+  // enough for either kernel: which one runs depends on q's address and strides, which may change from step to step
+  PolyTreePass any = *a;
+  any.q = nullptr;
+  any.q_stride[0] = any.q_stride[1] = any.q_stride[2] = 8;
+  const int splits = std::max(geometry(any, false).splits, geometry(any, true).splits);
+  if (splits <= 1) return 0;
+  return (size_t)a->batch * a->heads * a->nodes * splits * (a->head_dim + 2) * sizeof(float);
 }
 
 int poly_tree_chain(const PolyTreeAppend* append, const PolyTreePass* passes, int n, void* stream) {

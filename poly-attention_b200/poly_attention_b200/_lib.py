@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpolyattn.so")
@@ -146,6 +147,23 @@ class PolyRotaryArgs(ctypes.Structure):
         ("cu_seqlens", c_vp), ("seqs", c_i32), ("reserved", c_i32),
         ("t", PolyRotaryTensor * MAX_ROTARY),
     ]
+
+
+def packer(cls):
+    """struct.Struct of a ctypes Structure without nested arrays of structures: argument blocks of calls whose
+    latency counts are packed in one go (some 60 attribute writes cost more than the launch)."""
+    codes = {c_i32: "i", c_i64: "q", c_f32: "f", c_vp: "Q", c_sz: "Q"}
+
+    def flat(t):
+        if issubclass(t, ctypes.Structure):
+            return "".join(flat(f[1]) for f in t._fields_)
+        if issubclass(t, ctypes.Array):
+            return flat(t._type_) * t._length_
+        return codes[t]
+    st = struct.Struct("@" + flat(cls))
+    if st.size > ctypes.sizeof(cls):
+        raise ImportError(f"cannot pack {cls.__name__}")
+    return st
 
 
 EXPORTS = {

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _lib
 from ._lib import PolyPackedArgs, PolyPackedBwdArgs, check, lib
 from .core import _autocast, _sc
 from .ops import _DTYPES, _on, _require_cuda, _stream
@@ -39,18 +40,24 @@ def _offsets(cu_seqlens, like):
     if (cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64)
             or cu_seqlens.device != like.device):
         raise ValueError("cu_seqlens must be an int32 / int64 tensor [s + 1] on the tensors' device")
+    if cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous():
+        return cu_seqlens
     return cu_seqlens.to(torch.int32).contiguous()
 
 
 def _tensors(q, k, v, *same):
-    _require_cuda(q, k, v, *same)
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"q, k, v must share one of {list(_DTYPES)}; got {q.dtype}, {k.dtype}, {v.dtype}")
+    dtype, device = q.dtype, q.device
+    if dtype not in _DTYPES or k.dtype != dtype or v.dtype != dtype:
+        _require_cuda(q, k, v)
+        raise TypeError(f"q, k, v must share one of {list(_DTYPES)}; got {dtype}, {k.dtype}, {v.dtype}")
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[::2] != k.shape[::2]:
         raise ValueError(f"packed tensors are q [total, h, d] and k, v [total, g, d]; got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if device.type != "cuda":
+        _require_cuda(q)
     for t in (k, v, *same):
-        if t is not None and t.device != q.device:
+        if t is not None and t.device != device:
+            _require_cuda(t)
             raise ValueError("packed tensors must be on one device")
 
 
@@ -89,30 +96,35 @@ def _fill(a, q, k, v, bias, causal, softclamp, scale):
         _set(a, "bias", bias)
 
 
+_FWD = _lib.packer(PolyPackedArgs)
+
+
 def _forward(q, k, v, cu, bias, epi_mul, causal, softclamp, scale, max_seqlen, out_lo):
     """pass_fwd_packed on checked tensors: (out, lse, epi or None, out_lo or None)."""
     total, h, d = q.shape
     q, k, v = _rows(q), _rows(k), _rows(v)
-    a = PolyPackedArgs()
-    f = a.fwd
-    _fill(f, q, k, v, bias, causal, softclamp, scale)
     out = q.new_empty(total, h, d)
     lse = q.new_empty(h, total, dtype=torch.float32)
-    _set(f, "out", out)
-    _set(f, "lse", lse)
     epi = lo = None
     if epi_mul is not None:
         epi_mul, epi = _rows(epi_mul), torch.empty_like(out)
-        _set(f, "epi_mul", epi_mul)
-        _set(f, "epi_out", epi)
     if out_lo and q.dtype != torch.float32:
         lo = torch.empty_like(out)
-        a.out_lo = lo.data_ptr()
-    a.cu_seqlens, a.seqs, a.max_len, a.zero_rest = cu.data_ptr(), cu.shape[0] - 1, int(max_seqlen or 0), 1
-    if a.seqs == 0 and total:
+    seqs = cu.shape[0] - 1
+    if seqs == 0 and total:
         for t in (out, lse, epi, lo):
             if t is not None:
                 t.zero_()
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    ms = epi_mul.stride() if epi is not None else (0, 0)
+    # PolyPackedArgs in its order; tensors as pointer and (batch, head, row) strides
+    a = PolyPackedArgs.from_buffer_copy(_FWD.pack(
+        1, h, k.shape[1], total, total, d, _DTYPES[q.dtype], bool(causal), d ** -0.5 if scale is None else scale, _sc(softclamp),
+        q.data_ptr(), 0, qs[1], qs[0], k.data_ptr(), 0, ks[1], ks[0], v.data_ptr(), 0, vs[1], vs[0], 0, 0, 0, 0,
+        0 if bias is None else bias.data_ptr(), 0, 0 if bias is None else bias.stride(0), 0, 0, 0, 0,
+        out.data_ptr(), 0, d, h * d, lse.data_ptr(), 0, total,
+        0 if epi is None else epi_mul.data_ptr(), 0, ms[1], ms[0], 0 if epi is None else epi.data_ptr(), 0, d, h * d, 0, 0, 0, 0,
+        cu.data_ptr(), seqs, max_seqlen or 0, 1, 0, 0 if lo is None else lo.data_ptr()))
     with _on(q.device):
         check(lib.poly_packed_pass_fwd(a, _stream(q.device)), "poly_packed_pass_fwd")
     return out, lse, epi, lo
@@ -294,8 +306,10 @@ def _chain(q_left, q_right, vs, cu_seqlens, softclamp_value, causal, max_seqlen)
     ql, qr, vv = _autocast(*q_left), _autocast(*q_right), _autocast(*vs)
     ql = [qr[t - 1] if shared[t] else ql[t] for t in range(order)]
     _tensors(ql[0], qr[0], vv[0], *ql[1:], *qr[1:], *vv[1:])
-    if any(t.shape != qr[0].shape or t.dtype != qr[0].dtype for t in (*ql[1:], *qr[1:], *vv)):
-        raise ValueError("key, value and lower query tensors must share one shape and dtype")
+    shape, dtype = qr[0].shape, qr[0].dtype
+    for t in (*ql[1:], *qr[1:], *vv):
+        if t.shape != shape or t.dtype != dtype:
+            raise ValueError("key, value and lower query tensors must share one shape and dtype")
     if ql[0].shape[1] % max(qr[0].shape[1], 1):
         raise ValueError("heads must be divisible by kv_heads")
     cu = _offsets(cu_seqlens, ql[0])

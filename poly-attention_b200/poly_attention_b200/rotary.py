@@ -11,7 +11,9 @@ There is no CPU implementation: CPU tensors raise.
 """
 from __future__ import annotations
 
+import ctypes
 import math
+import struct
 from typing import List, Optional
 
 import torch
@@ -57,45 +59,42 @@ def rotary_frequencies(dim, *, theta=10000.0, scaling=None, factor=1.0, original
 def _empty_like(x):
     """Output with x's axis order in memory (token-major views stay token-major), dense."""
     b, h, n, d = x.shape
-    if x.stride(1) <= x.stride(2):
-        return x.new_empty((b, n, h, d)).permute(0, 2, 1, 3)
-    return x.new_empty((b, h, n, d))
+    s = x.stride()
+    token_major = s[1] <= s[2]
+    return torch.empty_strided((b, h, n, d), (h * n * d, d, h * d, 1) if token_major else (h * n * d, n * d, d, 1),
+                               dtype=x.dtype, device=x.device)
 
 
-def _launch(xs, outs, inv_freq, positions, start, cu_seqlens, angles, interleaved, factor, inverse):
-    x0 = xs[0]
-    a = PolyRotaryArgs()
-    a.batch, _, a.rows, a.dim = x0.shape
-    a.dtype, a.interleaved, a.inverse, a.factor = _DTYPES[x0.dtype], interleaved, inverse, factor
-    a.pos_start = start
-    if angles is not None:
-        a.rot, a.angles = 2 * angles.shape[-1], angles.data_ptr()
-        a.angle_stride[0], a.angle_stride[1] = angles.stride(0), angles.stride(1)
-    else:
-        a.rot, a.inv_freq = 2 * inv_freq.shape[0], inv_freq.data_ptr()
-    if cu_seqlens is not None:
-        a.cu_seqlens, a.seqs = cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1
-    elif positions is not None:
-        a.positions, a.pos_wide = positions.data_ptr(), positions.dtype == torch.int64
-        a.pos_stride[0], a.pos_stride[1] = positions.stride(0), positions.stride(1)
-    with _on(x0.device):
-        stream = _stream(x0.device)
-        for i0 in range(0, len(xs), _lib.MAX_ROTARY):
-            part = range(i0, min(len(xs), i0 + _lib.MAX_ROTARY))
-            a.n = len(part)
-            for t, i in zip(a.t, part):
-                x, y = xs[i], outs[i]
-                t.src, t.dst, t.heads = x.data_ptr(), y.data_ptr(), x.shape[1]
-                s, d = x.stride(), y.stride()
-                t.src_stride[0], t.src_stride[1], t.src_stride[2] = s[0], s[1], s[2]
-                t.dst_stride[0], t.dst_stride[1], t.dst_stride[2] = d[0], d[1], d[2]
-            check(lib.poly_rotary(a, stream), "poly_rotary")
+_HEAD = struct.Struct("@8if i Qqqq QQqq Qii")    # PolyRotaryArgs before its tensors
+_TENSOR = struct.Struct("@QQii6q")
+assert _HEAD.size + _lib.MAX_ROTARY * _TENSOR.size == ctypes.sizeof(PolyRotaryArgs)
 
 
 def _rotate(xs, inv_freq, positions, start, cu_seqlens, angles, interleaved, factor, inverse):
     xs = [x if x.stride(-1) == 1 else x.contiguous() for x in xs]
     outs = [_empty_like(x) for x in xs]
-    _launch(xs, outs, inv_freq, positions, start, cu_seqlens, angles, interleaved, factor, inverse)
+    x0 = xs[0]
+    b, _, n, d = x0.shape
+    rot = 2 * (inv_freq if angles is None else angles).shape[-1]
+    ps = positions.stride() if positions is not None else (0, 0)
+    an = angles.stride() if angles is not None else (0, 0)
+    with _on(x0.device):
+        stream = _stream(x0.device)
+        for i0 in range(0, len(xs), _lib.MAX_ROTARY):
+            part = xs[i0:i0 + _lib.MAX_ROTARY]
+            buf = bytearray(ctypes.sizeof(PolyRotaryArgs))
+            _HEAD.pack_into(buf, 0, b, n, d, rot, _DTYPES[x0.dtype], interleaved, inverse, len(part), factor,
+                            positions is not None and positions.dtype == torch.int64,
+                            positions.data_ptr() if positions is not None else 0, ps[0], ps[1], start,
+                            inv_freq.data_ptr() if angles is None else 0, 0 if angles is None else angles.data_ptr(), an[0], an[1],
+                            cu_seqlens.data_ptr() if cu_seqlens is not None else 0,
+                            cu_seqlens.shape[0] - 1 if cu_seqlens is not None else 0, 0)
+            at = _HEAD.size
+            for x, y in zip(part, outs[i0:]):
+                s, t = x.stride(), y.stride()
+                _TENSOR.pack_into(buf, at, x.data_ptr(), y.data_ptr(), x.shape[1], 0, s[0], s[1], s[2], t[0], t[1], t[2])
+                at += _TENSOR.size
+            check(lib.poly_rotary(PolyRotaryArgs.from_buffer(buf), stream), "poly_rotary")
     return outs
 
 
@@ -178,14 +177,24 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
     if packed:
         xs = [x.transpose(0, 1).unsqueeze(0) if x.dim() == 3 else x for x in xs]
         x0 = xs[0]
-    if any(x.dim() != 4 for x in xs):
+    if x0.dim() != 4:
         raise ValueError("apply_rotary takes tensors [b, h, n, d] or [total, h, d]")
     b, _, n, d = x0.shape
-    _require_cuda(*xs, inv_freq, angles, cu_seqlens)
-    if x0.dtype not in _DTYPES or any(x.dtype != x0.dtype for x in xs):
-        raise TypeError(f"rotary tensors must share one of {list(_DTYPES)}; got {[x.dtype for x in xs]}")
-    if any((x.shape[0], x.shape[2], x.shape[3]) != (b, n, d) or x.device != x0.device for x in xs):
-        raise ValueError("rotary tensors must share batch, length, features and device")
+    dtype, device = x0.dtype, x0.device
+    if device.type != "cuda":
+        _require_cuda(x0)
+    if dtype not in _DTYPES:
+        raise TypeError(f"rotary tensors must be one of {list(_DTYPES)}; got {dtype}")
+    grad = False
+    for x in xs:
+        if x.dtype != dtype:
+            raise TypeError(f"rotary tensors must share one dtype; got {[x.dtype for x in xs]}")
+        s = x.shape
+        if len(s) != 4 or s[0] != b or s[2] != n or s[3] != d or x.device != device:
+            _require_cuda(x)
+            raise ValueError("rotary tensors must share batch, length, features and device")
+        grad = grad or x.requires_grad
+    _require_cuda(inv_freq, angles, cu_seqlens)
     if (inv_freq is None) == (angles is None):
         raise ValueError("give either inv_freq or angles")
     table = inv_freq if angles is None else angles
@@ -194,7 +203,7 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
     rot = 2 * table.shape[-1]
     if rot == 0 or rot > d or d > 256:
         raise ValueError(f"rotary features ({rot}) must be in [2, {d}] and the head at most 256")
-    if table.device != x0.device:
+    if table.device != device:
         raise ValueError("rotary frequencies must be on the tensors' device")
     start = 0
     if angles is not None:
@@ -212,7 +221,8 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
     else:
         if inv_freq.dim() != 1:
             raise ValueError("inv_freq must be [rot / 2]")
-        inv_freq = inv_freq.float().contiguous()
+        if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+            inv_freq = inv_freq.float().contiguous()
         if cu_seqlens is not None:
             if torch.is_tensor(positions) or positions != 0:
                 raise ValueError("positions and cu_seqlens exclude one another")
@@ -232,11 +242,11 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
         else:
             start, positions = int(positions), None
     args = (inv_freq, positions, start, cu_seqlens, angles, bool(interleaved), float(attention_factor))
-    if x0.numel() == 0 and all(x.numel() == 0 for x in xs):
+    if b == 0 or n == 0:
         ys = [x.clone() for x in xs]
     elif torch.compiler.is_compiling():
         ys = _rotary_op(xs, *args, False)
-    elif torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+    elif grad and torch.is_grad_enabled():
         ys = _Rotary.apply(args, *xs)
     else:
         ys = _rotate(xs, *args, False)

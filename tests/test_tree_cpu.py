@@ -36,6 +36,9 @@ def test_struct_sizes_and_checks():
     assert lib.poly_tree_kernel_name(args(dtype=_lib.POLY_F32)) == b"simt"
     assert lib.poly_tree_kernel_name(args(head_dim=96)) == b"simt"
     assert lib.poly_tree_kernel_name(args(k=258)) == b"simt"
+    assert lib.poly_tree_kernel_name(args(nodes=17)) == b"tc100" and lib.poly_tree_kernel_name(args(nodes=17, q=264)) == b"tree"
+    # the workspace does not depend on where q is
+    assert lib.poly_tree_workspace_size(args(nodes=17)) == lib.poly_tree_workspace_size(args(nodes=17, q=264)) > 0
     need = lib.poly_tree_workspace_size(args())
     assert need > 0
     assert lib.poly_tree_chain(None, args(workspace=256, workspace_bytes=need - 1), 1, None) == _lib.POLY_EINVAL

@@ -146,6 +146,8 @@ def test_many_splits_and_groups():
     """One sequence over many key ranges, and more groups than fit at once (no split)."""
     rng = random.Random(3)
     Case(order=2, h=8, g=2, d=128, dtype=torch.bfloat16, lens=[5003], parents=[tree("random", 5, rng)]).check()
+    Case(order=2, h=8, g=2, d=128, dtype=torch.bfloat16, lens=[5003, 4000], parents=[tree("random", 60, rng) for _ in range(2)]).check()
+    Case(order=3, h=4, g=4, d=64, dtype=torch.float16, lens=[2100], parents=[tree("random", 50, rng)], max_nodes=64).check()
     Case(order=2, h=2, g=2, d=64, dtype=torch.float16, lens=[rng.randrange(200) for _ in range(170)],
          parents=[tree("random", 4, rng) for _ in range(170)], cap=1000).check()
 
