@@ -44,13 +44,6 @@ __device__ __forceinline__ void mma8(float* c, uint32_t a0, uint32_t a1, uint32_
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// c += a.b in 3xTF32
-__device__ __forceinline__ void mma3(float* c, const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t bh0,
-                                     uint32_t bh1, uint32_t bl0, uint32_t bl1) {
-  mma8(c, al[0], al[1], al[2], al[3], bh0, bh1);
-  mma8(c, ah[0], ah[1], ah[2], ah[3], bl0, bl1);
-  mma8(c, ah[0], ah[1], ah[2], ah[3], bh0, bh1);
-}
 __device__ __forceinline__ void cp16(uint32_t sa, const void* g, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sa), "l"(g), "r"(ok ? 16 : 0) : "memory");
 }
@@ -150,19 +143,27 @@ __global__ void __launch_bounds__(128) pass_f32_kernel(PolyPassArgs a, const Pac
     const int st = t & 1, j0 = t * BN;
     const float* K = sK[st];
     const float* V = sV[st];
-    // S = Q K^T: n-block nb = keys j0 + 8 nb .. + 7
+    // S = Q K^T: n-block nb = keys j0 + 8 nb .. + 7. The three products of a step go
+    // round all n-blocks in turn: MMAs on one accumulator wait for one another (about
+    // 33 cycles), eight accumulators hide that. Each accumulator's order of sums is kept.
     float s[BN / 8][4];
 #pragma unroll
-    for (int nb = 0; nb < BN / 8; ++nb) {
-      s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
-      const float* kr = K + (nb * 8 + gq) * LD;
+    for (int nb = 0; nb < BN / 8; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < D / 8; ++ks) {
-        uint32_t bh0, bl0, bh1, bl1;
-        split(kr[ks * 8 + tq], bh0, bl0);
-        split(kr[ks * 8 + tq + 4], bh1, bl1);
-        mma3(s[nb], qh[ks], ql[ks], bh0, bh1, bl0, bl1);
+    for (int ks = 0; ks < D / 8; ++ks) {
+      uint32_t bh[BN / 8][2], bl[BN / 8][2];
+#pragma unroll
+      for (int nb = 0; nb < BN / 8; ++nb) {
+        const float* kr = K + (nb * 8 + gq) * LD + ks * 8 + tq;
+        split(kr[0], bh[nb][0], bl[nb][0]);
+        split(kr[4], bh[nb][1], bl[nb][1]);
       }
+#pragma unroll
+      for (int nb = 0; nb < BN / 8; ++nb) mma8(s[nb], ql[ks][0], ql[ks][1], ql[ks][2], ql[ks][3], bh[nb][0], bh[nb][1]);
+#pragma unroll
+      for (int nb = 0; nb < BN / 8; ++nb) mma8(s[nb], qh[ks][0], qh[ks][1], qh[ks][2], qh[ks][3], bl[nb][0], bl[nb][1]);
+#pragma unroll
+      for (int nb = 0; nb < BN / 8; ++nb) mma8(s[nb], qh[ks][0], qh[ks][1], qh[ks][2], qh[ks][3], bh[nb][0], bh[nb][1]);
     }
     float mx0 = m0, mx1 = m1;
 #pragma unroll
@@ -213,13 +214,18 @@ __global__ void __launch_bounds__(128) pass_f32_kernel(PolyPassArgs a, const Pac
       split(s[nb][3], ph[3], pl[3]);
       const float* v0 = V + (nb * 8 + 2 * tq) * LD;
       const float* v1 = v0 + LD;
+      uint32_t bh[D / 8][2], bl[D / 8][2];
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
-        uint32_t bh0, bl0, bh1, bl1;
-        split(v0[n * 8 + gq], bh0, bl0);
-        split(v1[n * 8 + gq], bh1, bl1);
-        mma3(o[n], ph, pl, bh0, bh1, bl0, bl1);
+        split(v0[n * 8 + gq], bh[n][0], bl[n][0]);
+        split(v1[n * 8 + gq], bh[n][1], bl[n][1]);
       }
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) mma8(o[n], pl[0], pl[1], pl[2], pl[3], bh[n][0], bh[n][1]);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) mma8(o[n], ph[0], ph[1], ph[2], ph[3], bl[n][0], bl[n][1]);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) mma8(o[n], ph[0], ph[1], ph[2], ph[3], bh[n][0], bh[n][1]);
     }
     __syncthreads();   // the stage is refilled next iteration
   }
