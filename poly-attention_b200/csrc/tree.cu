@@ -15,9 +15,10 @@
 // O += P V' on mma.sync m16n8k16, online softmax in the log2 domain with a lazy
 // maximum. Few rows are spread over the keys, many rows over the warps, so no
 // product is spent on padding while there are 64 rows to fill. The warps' states
-// merge in shared memory; with more than one split the CTA's records go to the
-// workspace and tree_combine_kernel joins them. Key ranges follow the lengths on
-// the device, so the grid needs the capacity only.
+// merge in shared memory; up to 8 splits are a cluster and join through distributed
+// shared memory, more (few groups, a long cache) go through the workspace and
+// tree_combine_kernel. Key ranges follow the lengths on the device, so the grid
+// needs the capacity only.
 //
 // The kernels of a step are programmatic dependents of one another: a pass
 // streams the cached rows while its predecessor drains, and waits for it
@@ -26,6 +27,8 @@
 //
 // tree_simt_kernel serves the other types and head sizes: one warp per row, 32-key
 // tiles in shared memory, fp32.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cfloat>
 #include <cstring>
@@ -38,6 +41,8 @@
 #include "tc_host.cuh"
 #include "tc_ptx.cuh"
 #include "tree_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace poly {
 
@@ -65,7 +70,7 @@ struct Ring {
   static constexpr int kStage = NARR * kArr;
   // ~100 KB a CTA: two CTAs per SM
   static constexpr int kStages = 100 * 1024 / kStage > 4 ? 4 : 100 * 1024 / kStage;
-  static constexpr int kRecords = kWarps * 16 * (D + 4) * 4;   // the warps' records reuse the ring
+  static constexpr int kRecords = 2 * kWarps * 16 * kRecord<D> * 4;   // the warps' and the CTA's records reuse the ring
   static constexpr int kBias = kStages * kStage > kRecords ? kStages * kStage : kRecords;
   static constexpr int kMask = kBias + kStages * kKeys * 4;
   static constexpr int kUp = kMask + kNodes * 8;
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_kernel(const __grid_constant
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
   }
   __syncthreads();   // the ring is idle (every issued stage consumed or drained): it takes the warps' records
-  constexpr int RS = D + 4;   // record: acc[D], m, l (padded)
+  constexpr int RS = kRecord<D>;
   float* rec = reinterpret_cast<float*>(dsm);
   if (warp < kWarps) {
 #pragma unroll
@@ -331,36 +336,57 @@ __global__ void __launch_bounds__(kThreads, 2) tree_kernel(const __grid_constant
   }
   __syncthreads();
   pdl_wait();   // nothing is written before the previous kernel of the step is done (a shared workspace, the caches)
-  for (int idx = threadIdx.x; idx < 16 * WR * (D / 2); idx += kThreads) {
-    const int rr = idx / (D / 2), c = (idx - rr * (D / 2)) * 2;
-    const int m = rb * 16 * WR + rr;
-    if (m >= rows) break;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WK; ++w) M = fmaxf(M, rec[(w * WR * 16 + rr) * RS + D]);
-    float x = 0.f, y = 0.f, L = 0.f;
-#pragma unroll
-    for (int w = 0; w < WK; ++w) {
-      const float* r = rec + (w * WR * 16 + rr) * RS;
+  // rows' states over the WK warps that share them; with several splits a record of them
+  auto merge = [&](int rr, int c, auto at, int count, float& M, float& x, float& y, float& L) {
+    M = -INFINITY;
+    for (int w = 0; w < count; ++w) M = fmaxf(M, at(w)[rr * RS + D]);
+    x = y = L = 0.f;
+    for (int w = 0; w < count; ++w) {
+      const float* r = at(w) + rr * RS;
       const float f = r[D] == -INFINITY ? 0.f : exp2f(r[D] - M);
       x = fmaf(r[c], f, x);
       y = fmaf(r[c + 1], f, y);
       L = fmaf(r[D + 1], f, L);
     }
-    if (geo.splits > 1) {
-      float* p = geo.part + (((int64_t)blockIdx.y * rows + m) * geo.splits + split) * (D + 2);
-      p[2 + c] = x;
-      p[2 + c + 1] = y;
-      if (c == 0) {
-        p[0] = M;
-        p[1] = L;
-      }
-    } else {
-      const int h = g * R + m % R, node = m / R;
-      const float inv = L > 0.f ? 1.f / L : 0.f;
-      write_row<T>(a, b, h, node, len, c, x * inv, y * inv);
-      if (c == 0) write_lse(a, b, h, node, len, L > 0.f ? (M + __log2f(L)) * kLn2 : -FLT_MAX);
+  };
+  auto put = [&](int rr, int c, float M, float x, float y, float L) {
+    const int m = rb * 16 * WR + rr;
+    if (m >= rows) return;
+    const int h = g * R + m % R, node = m / R;
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    write_row<T>(a, b, h, node, len, c, x * inv, y * inv);
+    if (c == 0) write_lse(a, b, h, node, len, L > 0.f ? (M + __log2f(L)) * kLn2 : -FLT_MAX);
+  };
+  float* crec = rec + kWarps * 16 * RS;   // this CTA's
+  const bool local = geo.splits == 1 || geo.cluster;
+  for (int idx = threadIdx.x; idx < 16 * WR * (D / 2); idx += kThreads) {
+    const int rr = idx / (D / 2), c = (idx - rr * (D / 2)) * 2;
+    float M, x, y, L;
+    merge(rr, c, [&](int w) { return rec + w * WR * 16 * RS; }, WK, M, x, y, L);
+    if (geo.splits == 1) {
+      put(rr, c, M, x, y, L);
+      continue;
     }
+    const int m = rb * 16 * WR + rr;
+    if (!local && m >= rows) break;
+    float* p = local ? crec + rr * RS : geo.part + (((int64_t)blockIdx.y * rows + m) * geo.splits + split) * RS;
+    *reinterpret_cast<float2*>(p + c) = make_float2(x, y);
+    if (c == 0) {
+      p[D] = M;
+      p[D + 1] = L;
+    }
+  }
+  if (geo.cluster) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();   // every CTA's records are visible to the cluster
+    // CTA `split` joins and writes its share of the rows
+    for (int idx = split * kThreads + threadIdx.x; idx < 16 * WR * (D / 2); idx += geo.splits * kThreads) {
+      const int rr = idx / (D / 2), c = (idx - rr * (D / 2)) * 2;
+      float M, x, y, L;
+      merge(rr, c, [&](int w) { return (const float*)cluster.map_shared_rank(crec, w); }, geo.splits, M, x, y, L);
+      put(rr, c, M, x, y, L);
+    }
+    cluster.sync();   // no CTA leaves while its records may still be read
   }
 }
 
@@ -375,22 +401,21 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   if (row >= (int64_t)a.batch * a.kv_heads * rows) return;
   const int group = (int)(row / rows), m = (int)(row - (int64_t)group * rows);
   const int b = group / a.kv_heads, g = group - b * a.kv_heads;
-  const float* p = geo.part + row * geo.splits * (D + 2);
+  const float* p = geo.part + row * geo.splits * kRecord<D>;
   float M = -INFINITY;
-  for (int s = lane; s < geo.splits; s += 32) M = fmaxf(M, p[s * (D + 2)]);
+  for (int s = lane; s < geo.splits; s += 32) M = fmaxf(M, p[s * kRecord<D> + D]);
   M = warp_max(M);
   float L = 0.f, acc[D / 32];
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) acc[t] = 0.f;
 #pragma unroll 4
   for (int s = 0; s < geo.splits; ++s) {
-    const float* r = p + s * (D + 2);
-    const float f = r[0] == -INFINITY ? 0.f : exp2f(r[0] - M);
-    L = fmaf(r[1], f, L);
-    if (f == 0.f) continue;   // an empty range's record holds no sums
+    const float* r = p + s * kRecord<D>;
+    const float f = r[D] == -INFINITY ? 0.f : exp2f(r[D] - M);
+    L = fmaf(r[D + 1], f, L);
 #pragma unroll
     for (int t = 0; t < D / 64; ++t) {
-      const float2 v = *reinterpret_cast<const float2*>(r + 2 + t * 64 + 2 * lane);
+      const float2 v = *reinterpret_cast<const float2*>(r + t * 64 + 2 * lane);
       acc[2 * t] = fmaf(v.x, f, acc[2 * t]);
       acc[2 * t + 1] = fmaf(v.y, f, acc[2 * t + 1]);
     }
@@ -590,7 +615,16 @@ TreeGeom geometry(const PolyTreePass& a, bool may_tc = true) {
   const int64_t ctas = (int64_t)a.batch * a.kv_heads * geo.row_blocks;
   const int keys = geo.tcgen05 ? 128 : kKeys, tiles = (a.capacity + keys - 1) / keys;
   const int slots = (geo.tcgen05 ? 1 : 2) * sm_count();
-  geo.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxSplits, tiles), slots / ctas));
+  const int want = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxSplits, tiles), slots / ctas));
+  if (geo.tcgen05) {
+    geo.splits = want;
+  } else {
+    // a cluster's 8 splits, or more of at least 16 tiles each (a second launch and the records' way through
+    // L2 cost about 5 us)
+    const int long_splits = std::min(want, tiles / 16);
+    geo.splits = long_splits > 8 ? long_splits : std::min(want, 8);
+    geo.cluster = geo.splits > 1 && geo.splits <= 8;
+  }
   return geo;
 }
 
@@ -610,17 +644,27 @@ int check_pass(const PolyTreePass* a) {
 
 // A kernel of a step: a programmatic dependent of the one before it.
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, bool dependent, A... args) {
+cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, bool dependent, int cluster,
+                   A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (dependent) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 1 : 0;
+  cfg.numAttrs = n;
   note_launch(1);
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
@@ -628,7 +672,7 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cu
 template <typename T, int D>
 int launch_combine(const PolyTreePass& a, const TreeGeom& geo, cudaStream_t s) {
   const int64_t rows = (int64_t)a.batch * a.heads * a.nodes;
-  return cuda_status(launch(tree_combine_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, s, true, a, geo), "tree launch");
+  return cuda_status(launch(tree_combine_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, s, true, 0, a, geo), "tree launch");
 }
 
 template <typename T, int D, int WR, bool VMUL>
@@ -650,9 +694,9 @@ int launch_tree(const PolyTreePass& a, cudaStream_t s, bool dep) {
   if (rc) return rc;
   const int groups = a.batch * a.kv_heads;
   cudaError_t e = launch(tree_kernel<T, D, WR, VMUL>, dim3(geo.splits * geo.row_blocks, groups), kThreads, R_::kAlloc, s, dep,
-                         tk, tv, tm, a, geo);
+                         geo.cluster ? geo.splits : 0, tk, tv, tm, a, geo);
   rc = cuda_status(e, "tree launch");
-  return rc || geo.splits <= 1 ? rc : launch_combine<T, D>(a, geo, s);
+  return rc || geo.splits <= 1 || geo.cluster ? rc : launch_combine<T, D>(a, geo, s);
 }
 
 template <typename T, int D>
@@ -675,7 +719,7 @@ template <typename T, int DMAX>
 int launch_simt(const PolyTreePass& a, cudaStream_t s, bool dep) {
   const int rows = a.nodes * (a.heads / a.kv_heads);
   return cuda_status(launch(tree_simt_kernel<T, DMAX>, dim3((rows + kSimtWarps - 1) / kSimtWarps, a.batch * a.kv_heads),
-                            kSimtWarps * 32, 0, s, dep, a), "tree launch");
+                            kSimtWarps * 32, 0, s, dep, 0, a), "tree launch");
 }
 
 template <typename T>
@@ -710,8 +754,8 @@ int launch_append(const PolyTreeAppend& a, cudaStream_t s) {
     for (int x = 0; x < 3; ++x) bits |= (uint64_t)a.t[i].src_stride[x] | (uint64_t)a.t[i].cache_stride[x];
   }
   const dim3 grid(a.batch * a.kv_heads, a.n);
-  const cudaError_t e = bits & 15 ? launch(tree_append_kernel<uint16_t>, grid, 128, 0, s, false, a)
-                                  : launch(tree_append_kernel<uint4>, grid, 128, 0, s, false, a);
+  const cudaError_t e = bits & 15 ? launch(tree_append_kernel<uint16_t>, grid, 128, 0, s, false, 0, a)
+                                  : launch(tree_append_kernel<uint4>, grid, 128, 0, s, false, 0, a);
   return cuda_status(e, "tree append launch");
 }
 
@@ -738,9 +782,14 @@ size_t poly_tree_workspace_size(const PolyTreePass* a) {
   PolyTreePass any = *a;
   any.q = nullptr;
   any.q_stride[0] = any.q_stride[1] = any.q_stride[2] = 8;
-  const int splits = std::max(geometry(any, false).splits, geometry(any, true).splits);
-  if (splits <= 1) return 0;
-  return (size_t)a->batch * a->heads * a->nodes * splits * (a->head_dim + 2) * sizeof(float);
+  any.out = any.cache_out = nullptr;
+  size_t need = 0;
+  for (const bool tc : {false, true}) {
+    const TreeGeom geo = geometry(any, tc);
+    if (geo.splits > 1 && !geo.cluster)
+      need = std::max(need, (size_t)a->batch * a->heads * a->nodes * geo.splits * (a->head_dim + 4) * sizeof(float));
+  }
+  return need;
 }
 
 int poly_tree_chain(const PolyTreeAppend* append, const PolyTreePass* passes, int n, void* stream) {

@@ -28,7 +28,7 @@ __device__ __forceinline__ void ancestors(const int32_t* parents, int nodes, int
     up[i] = p;
   }
   __syncthreads();
-  for (int round = 0; round < 6; ++round) {
+  for (;;) {   // at most 6 rounds: each doubles the distance
     uint64_t m = 0;
     int p = -2;
     if (i < kNodes) {
@@ -45,7 +45,7 @@ __device__ __forceinline__ void ancestors(const int32_t* parents, int nodes, int
       mask[i] = m;
       up[i] = p;
     }
-    __syncthreads();
+    if (!__syncthreads_or(p >= 0)) break;
   }
 }
 
@@ -63,6 +63,16 @@ __device__ __forceinline__ void write_row(const PolyTreePass& a, int b, int h, i
     *reinterpret_cast<uint32_t*>((T*)a.cache_out + b * a.cache_out_stride[0] + h * a.cache_out_stride[1] +
                                  (int64_t)(len + node) * a.cache_out_stride[2] + c) = w;
 }
+// Eight features at once, where the outputs allow 16-byte stores.
+template <typename T>
+__device__ __forceinline__ void write_row8(const PolyTreePass& a, int b, int h, int node, int len, int c, const float (&x)[8]) {
+  const uint4 w = make_uint4(ms::pk2<T>(x[0], x[1]), ms::pk2<T>(x[2], x[3]), ms::pk2<T>(x[4], x[5]), ms::pk2<T>(x[6], x[7]));
+  if (a.out)
+    *reinterpret_cast<uint4*>((T*)a.out + b * a.out_stride[0] + h * a.out_stride[1] + node * a.out_stride[2] + c) = w;
+  if (a.cache_out && len + node < a.capacity)
+    *reinterpret_cast<uint4*>((T*)a.cache_out + b * a.cache_out_stride[0] + h * a.cache_out_stride[1] +
+                              (int64_t)(len + node) * a.cache_out_stride[2] + c) = w;
+}
 __device__ __forceinline__ void write_lse(const PolyTreePass& a, int b, int h, int node, int len, float v) {
   if (a.lse) a.lse[b * a.lse_stride[0] + h * a.lse_stride[1] + node] = v;
   if (a.cache_lse && len + node < a.capacity)
@@ -73,8 +83,12 @@ __device__ __forceinline__ void write_lse(const PolyTreePass& a, int b, int h, i
 struct TreeGeom {
   int splits, row_blocks;
   bool tcgen05;  // the kernel of tree_tc100.cu
-  float* part;   // [group][row of the group][split][D + 2]
+  bool cluster;  // tree_kernel: the splits are a cluster's CTAs and join through its shared memory
+  float* part;   // records acc[D], m, l, 2 unused: [group][row of the group][split]
 };
+// floats of a record (16-byte aligned: a thread writes its row's in float4)
+template <int D>
+constexpr int kRecord = D + 4;
 
 }  // namespace treec
 

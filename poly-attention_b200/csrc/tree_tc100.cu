@@ -398,8 +398,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (ROWS2 || x == 0) {
       const int rows = R * a.nodes, m = node * R + head;
-      float* rec = P.geo.splits > 1 ? P.geo.part + (((int64_t)blockIdx.y * rows + m) * P.geo.splits + split) * (D + 2) : nullptr;
+      float* rec = P.geo.splits > 1 ? P.geo.part + (((int64_t)blockIdx.y * rows + m) * P.geo.splits + split) * kRecord<D> : nullptr;
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      const bool keep0 = have && f0 != 0.f && l_run != 0.f, keep1 = !ROWS2 && f1 != 0.f && l_run != 0.f;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -408,24 +409,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_ld();
         }
 #pragma unroll
-        for (int t = 0; t < 32; t += 2) {
-          float y0 = have && f0 != 0.f ? __uint_as_float(o[t]) * f0 : 0.f, y1 = have && f0 != 0.f ? __uint_as_float(o[t + 1]) * f0 : 0.f;
-          if (!ROWS2 && f1 != 0.f) {
-            const float2 z = *reinterpret_cast<const float2*>(side + c * 32 + t);
-            y0 = fmaf(z.x, f1, y0);
-            y1 = fmaf(z.y, f1, y1);
+        for (int t = 0; t < 32; t += 8) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = keep0 ? __uint_as_float(o[t + e]) * f0 : 0.f;
+          if (keep1) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+              const float4 z = *reinterpret_cast<const float4*>(side + c * 32 + t + e);
+              y[e] = fmaf(z.x, f1, y[e]);
+              y[e + 1] = fmaf(z.y, f1, y[e + 1]);
+              y[e + 2] = fmaf(z.z, f1, y[e + 2]);
+              y[e + 3] = fmaf(z.w, f1, y[e + 3]);
+            }
           }
-          if (l_run == 0.f) y0 = y1 = 0.f;
-          if (row_ok) {
-            if (rec) *reinterpret_cast<float2*>(rec + 2 + c * 32 + t) = make_float2(y0, y1);
-            else write_row<T>(a, b, g * R + head, node, len, c * 32 + t, y0 * inv, y1 * inv);
+          if (!row_ok) continue;
+          if (rec) {
+            *reinterpret_cast<float4*>(rec + c * 32 + t) = make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<float4*>(rec + c * 32 + t + 4) = make_float4(y[4], y[5], y[6], y[7]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] *= inv;
+            write_row8<T>(a, b, g * R + head, node, len, c * 32 + t, y);
           }
         }
       }
       if (row_ok) {
         if (rec) {
-          rec[0] = m_run;
-          rec[1] = l_run;
+          rec[D] = m_run;
+          rec[D + 1] = l_run;
         } else {
           write_lse(a, b, g * R + head, node, len, l_run > 0.f ? (m_run + __log2f(l_run)) * kLn2 : -FLT_MAX);
         }
@@ -483,11 +495,14 @@ int launch_d(const PolyTreePass& a, const TreeGeom& geo, cudaStream_t s, bool de
 }  // namespace
 
 // Row blocks of the tcgen05 pass, or 0 where the mma.sync kernel serves: its 16-row
-// tiles keep up with the cache to about 32 rows; q has to suit a TMA box per head.
+// tiles keep up with the cache to about 32 rows; q has to suit a
+// TMA box per head and the outputs 16-byte stores.
 int tree_tc_row_blocks(const PolyTreePass& a) {
   const int R = a.heads / a.kv_heads;
   if (a.v_mul || a.nodes * R <= 32 || a.scale < 0.f) return 0;
   if (!aligned16(a.q) || !strides_ok(a.q_stride, 3)) return 0;
+  if (a.out && (!aligned16(a.out) || !strides_ok(a.out_stride, 3))) return 0;
+  if (a.cache_out && (!aligned16(a.cache_out) || !strides_ok(a.cache_out_stride, 3))) return 0;
   const int per_tile = BM / padded_nodes(a), per_block = R > per_tile ? 2 * per_tile : per_tile;
   return (R + per_block - 1) / per_block;
 }

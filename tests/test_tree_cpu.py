@@ -15,7 +15,7 @@ def test_struct_sizes_and_checks():
 
     def args(**kw):
         a = _lib.PolyTreePass()
-        a.batch, a.heads, a.kv_heads, a.nodes, a.head_dim, a.dtype, a.capacity, a.scale = 2, 4, 2, 8, 64, _lib.POLY_BF16, 100, 0.1
+        a.batch, a.heads, a.kv_heads, a.nodes, a.head_dim, a.dtype, a.capacity, a.scale = 2, 4, 2, 8, 64, _lib.POLY_BF16, 20000, 0.1
         a.q = a.k = a.v = a.lengths = a.parents = 256
         for n in ("q", "k", "v"):
             st = getattr(a, n + "_stride")
