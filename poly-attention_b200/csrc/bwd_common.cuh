@@ -23,6 +23,7 @@ struct BwdParams {
   void* dv; int64_t dv_stride[3];
   float* dbias; int64_t dbias_stride[2];
   PackedSeqs pk;                 // packed sequences: rows of slots of 128 in dq_acc, lse2 and delta
+  const int* order;              // and the slots, longest walk first (NULL: as they are)
 };
 
 template <typename T>
@@ -183,17 +184,24 @@ __global__ void bwd_dq_convert_kernel(const PolyPassBwdArgs a, const float* dq_a
 // the accumulator's rows as zeros. A row that saw no live key gets p = 0.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) packed_bwd_prep_kernel(const PolyPassBwdArgs a, const PackedSeqs q, float* dq_acc,
-                                                              float* lse2, float* delta, int64_t nq_pad) {
+                                                              float* lse2, float* delta, int64_t nq_pad, int* order) {
+  if (order) {   // CTA 0 of every head is extra: the first sorts the slots
+    if (blockIdx.x == 0) {
+      if (blockIdx.y == 0) packed_order<128>(q, q.total / 128 + q.seqs, a.fwd.causal != 0, order);
+      return;
+    }
+  }
+  const int bx = blockIdx.x - (order ? 1 : 0);
   const int own = (q.total / 128 + q.seqs) * 4;   // the CTAs behind these zero the rows outside the sequences
-  if ((int)blockIdx.x >= own) {
-    if (blockIdx.y == 0) packed_zero_rest(q, blockIdx.x - own);
+  if (bx >= own) {
+    if (blockIdx.y == 0) packed_zero_rest(q, bx - own);
     return;
   }
   PackedTile t;
-  const int slot = blockIdx.x >> 2;
+  const int slot = bx >> 2;
   if (!packed_tile<128>(q.cu, q.seqs, q.total, slot, t)) return;
   const int h = blockIdx.y, sub = threadIdx.x & 7;
-  const int r = (blockIdx.x & 3) * 32 + (threadIdx.x >> 3);   // row of the slot
+  const int r = (bx & 3) * 32 + (threadIdx.x >> 3);   // row of the slot
   const int i = t.tile * 128 + r;                              // row of the sequence
   const int64_t w = h * nq_pad + (int64_t)slot * 128 + r;
   const bool live = i < t.len;
@@ -326,6 +334,7 @@ struct PackedBwdWs {
   float* dq_acc;
   float* lse2;
   float* delta;
+  int* order;
   int slots;
   int64_t nq_pad;
   size_t bytes;
@@ -336,10 +345,12 @@ inline PackedBwdWs packed_bwd_ws(const PolyPassBwdArgs& a, int seqs) {
   w.slots = a.fwd.seq_q / 128 + seqs;
   w.nq_pad = (int64_t)w.slots * 128;
   const size_t rows = (size_t)a.fwd.heads * w.nq_pad;
-  w.bytes = rows * (a.fwd.head_dim + 2) * 4;
+  const bool sorted = w.slots <= kOrderSlots;
+  w.bytes = rows * (a.fwd.head_dim + 2) * 4 + (sorted ? (size_t)w.slots * 4 : 0);
   w.dq_acc = (float*)a.workspace;
   w.lse2 = w.dq_acc + rows * a.fwd.head_dim;
   w.delta = w.lse2 + rows;
+  w.order = sorted ? (int*)(w.delta + rows) : nullptr;
   return w;
 }
 

@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int seq_k = p.seq_k, q_tiles = p.q_tiles;
   if constexpr (PACKED) {
     PackedTile t;
-    if (!packed_tile<BK>(p.pk.cu, p.pk.seqs, p.pk.total, kt, t)) return;
+    if (!packed_tile<BK>(p.pk.cu, p.pk.seqs, p.pk.total, p.order ? p.order[kt] : kt, t)) return;
     kt = t.tile;
     first = t.start;
     slot_row = t.slot0 * BK;
@@ -476,7 +476,8 @@ int launch_t(const PolyPassBwdArgs& a, const PackedSeqs* seqs, cudaStream_t s) {
   if (rc) return rc;
   const dim3 pgrid((unsigned)(pw.slots * 4), (unsigned)f.heads);
   if (PACKED) {
-    packed_bwd_prep_kernel<T, D><<<dim3(pgrid.x + zero_ctas(*seqs), pgrid.y), 256, 0, s>>>(a, *seqs, w.dq_acc, w.lse2, w.delta, pw.nq_pad);
+    packed_bwd_prep_kernel<T, D><<<dim3(pgrid.x + (pw.order ? 1 : 0) + zero_ctas(*seqs), pgrid.y), 256, 0, s>>>(
+        a, *seqs, w.dq_acc, w.lse2, w.delta, pw.nq_pad, pw.order);
   } else {
     rc = cuda_status(cudaMemsetAsync(w.dq_acc, 0, (size_t)f.batch * f.heads * f.seq_q * D * 4, s), "memset dq acc");
     if (rc) return rc;
@@ -512,6 +513,7 @@ int launch_t(const PolyPassBwdArgs& a, const PackedSeqs* seqs, cudaStream_t s) {
   p.dbias_stride[1] = a.dbias_stride[1];
   p.k_tiles = PACKED ? pw.slots : (f.seq_k + BK - 1) / BK;
   if (PACKED) p.pk = *seqs;
+  p.order = pw.order;
   dim3 grid(p.k_tiles * f.batch * f.kv_heads);
   pass_bwd_tc128_kernel<T, SOFTCLAMP, HAS_BIAS, DB, PACKED><<<grid, kThreads, L::kAlloc, s>>>(tq, tdo, tk, tv, tdq, p);
   if (PACKED) {

@@ -54,12 +54,12 @@ enum class Kind { kSimt, kTc, kSmall, kF32 };
 
 bool short_sequences(int max_len) { return max_len > 0 && max_len <= 128; }
 
-// The tcgen05 kernels take the row maximum on unscaled scores: no negative scale.
+// The 16-bit tensor-core kernels take the row maximum on unscaled scores: the scale
+// has to be positive.
 Kind choose_fwd(const PolyPackedArgs& a) {
   if (packed_f32_eligible(a)) return Kind::kF32;
-  if (!packed_fwd_tc_eligible(a.pass, a.out_lo)) return Kind::kSimt;   // the short kernel takes the same tensors
-  if (short_sequences(a.max_len)) return Kind::kSmall;
-  return a.pass.scale >= 0.f ? Kind::kTc : Kind::kSimt;
+  if (!packed_fwd_tc_eligible(a.pass, a.out_lo) || !(a.pass.scale > 0.f)) return Kind::kSimt;
+  return short_sequences(a.max_len) ? Kind::kSmall : Kind::kTc;   // both take the same tensors
 }
 
 Kind choose_bwd(const PolyPackedBwdArgs& a) {

@@ -69,4 +69,34 @@ __device__ __forceinline__ void packed_zero_rest(const PackedSeqs& q, int part) 
   }
 }
 
+// The slots of a launch by descending number of tiles to walk, `order`[slots], by one CTA:
+// a launch that starts its longest CTAs first ends even. Empty slots go last. Equal
+// ones come in any order (it decides when a CTA runs, not what it computes).
+constexpr int kOrderSlots = 8192;   // more slots are left in their own order
+template <int B>
+__device__ __forceinline__ void packed_order(const PackedSeqs& q, int slots, bool causal, int* order) {
+  constexpr int kBins = 512;
+  __shared__ int at[kBins];
+  auto bin = [&](int s) {
+    PackedTile t;
+    if (!packed_tile<B>(q.cu, q.seqs, q.total, s, t)) return kBins - 1;
+    const int tiles = (t.len + B - 1) / B;
+    return kBins - 1 - min(causal ? tiles - t.tile : tiles, kBins - 1);
+  };
+  for (int i = threadIdx.x; i < kBins; i += blockDim.x) at[i] = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < slots; s += blockDim.x) atomicAdd(&at[bin(s)], 1);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int sum = 0;
+    for (int i = 0; i < kBins; ++i) {
+      const int c = at[i];
+      at[i] = sum;
+      sum += c;
+    }
+  }
+  __syncthreads();
+  for (int s = threadIdx.x; s < slots; s += blockDim.x) order[atomicAdd(&at[bin(s)], 1)] = s;
+}
+
 }  // namespace poly

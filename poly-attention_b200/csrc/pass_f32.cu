@@ -15,7 +15,11 @@
 //
 // PACKED: sequences laid end to end, one CTA per 64-row slot (packed.cuh) and
 // head; slots are taken from the last to the first, so that of a causal sequence
-// the rows with the most keys start first.
+// the rows with the most keys start first. Two groups of 4 warps share the CTA's
+// rows, one taking the even key tiles, one the odd, and join at the end: sequences of
+// unequal lengths leave few CTAs for the longest one's last rows, and their walk over
+// the keys (some 5 us a tile) was what the launch waited for (270 -> 231 us an order-2
+// forward of 4099 tokens in 7 sequences, h8 d64).
 #include <cfloat>
 #include <mutex>
 
@@ -26,6 +30,7 @@ namespace poly {
 namespace {
 
 constexpr int D = 64, BM = 64, BN = 64, LD = D + 4;   // padded row pitch (floats)
+constexpr int kSmem = (4 * BN * LD + 2 * BN) * 4;      // a two-stage ring: K, V, bias
 
 __device__ __forceinline__ uint32_t tf32(float x) {
   uint32_t r;
@@ -49,11 +54,18 @@ __device__ __forceinline__ void cp16(uint32_t sa, const void* g, bool ok) {
 }
 
 template <bool HAS_BIAS, bool SOFTCLAMP, bool PACKED>
-__global__ void __launch_bounds__(128) pass_f32_kernel(PolyPassArgs a, const PackedSeqs pk) {
+__global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassArgs a, const PackedSeqs pk) {
+  constexpr int KG = PACKED ? 2 : 1;   // groups of 4 warps over the key tiles
   extern __shared__ __align__(16) float smf[];
-  float(*sK)[BN * LD] = reinterpret_cast<float(*)[BN * LD]>(smf);
-  float(*sV)[BN * LD] = reinterpret_cast<float(*)[BN * LD]>(smf + 2 * BN * LD);
-  float(*sB)[BN] = reinterpret_cast<float(*)[BN]>(smf + 4 * BN * LD);
+  const int kg = PACKED ? threadIdx.x >> 7 : 0, tid = threadIdx.x & 127;
+  float* ring = smf + kg * (kSmem / 4);
+  float(*sK)[BN * LD] = reinterpret_cast<float(*)[BN * LD]>(ring);
+  float(*sV)[BN * LD] = reinterpret_cast<float(*)[BN * LD]>(ring + 2 * BN * LD);
+  float(*sB)[BN] = reinterpret_cast<float(*)[BN]>(ring + 4 * BN * LD);
+  auto sync = [&] {   // the group's warps
+    if constexpr (PACKED) asm volatile("bar.sync %0, 128;" ::"r"(1 + kg) : "memory");
+    else __syncthreads();
+  };
   // packed: heads fastest, so that CTAs running together share a sequence's keys
   const int bh = PACKED ? blockIdx.x : blockIdx.y;
   const int b = PACKED ? 0 : bh / a.heads, h = bh - b * a.heads, g = h / (a.heads / a.kv_heads);
@@ -80,32 +92,32 @@ __global__ void __launch_bounds__(128) pass_f32_kernel(PolyPassArgs a, const Pac
       a.epi_out = (float*)a.epi_out + f * a.epi_out_stride[2];
     }
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+  const int warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
   const int i0 = tile * BM + warp * 16 + gq, i1 = i0 + 8;   // this thread's two rows
   const int nq = a.seq_q, nk = a.seq_k;
-  const float* kg = (const float*)a.k + b * a.k_stride[0] + g * a.k_stride[1];
+  const float* kp = (const float*)a.k + b * a.k_stride[0] + g * a.k_stride[1];
   const float* vg = (const float*)a.v + b * a.v_stride[0] + g * a.v_stride[1];
   const float* bg = HAS_BIAS ? a.bias + b * a.bias_stride[0] + g * a.bias_stride[1] : nullptr;
   const int kend = a.causal ? min(nk, tile * BM + BM) : nk;
   const int ntile = (kend + BN - 1) / BN;
 
   auto issue = [&](int t) {
-    const int st = t & 1, j0 = t * BN;
-    for (int c = threadIdx.x; c < BN * (D / 4); c += 128) {
+    const int st = (t / KG) & 1, j0 = t * BN;
+    for (int c = tid; c < BN * (D / 4); c += 128) {
       const int r = c / (D / 4), ch = c - r * (D / 4);
       const bool ok = j0 + r < nk;
       const int rr = ok ? j0 + r : 0;
-      cp16((uint32_t)__cvta_generic_to_shared(&sK[st][r * LD + ch * 4]), kg + (int64_t)rr * a.k_stride[2] + ch * 4, ok);
+      cp16((uint32_t)__cvta_generic_to_shared(&sK[st][r * LD + ch * 4]), kp + (int64_t)rr * a.k_stride[2] + ch * 4, ok);
       cp16((uint32_t)__cvta_generic_to_shared(&sV[st][r * LD + ch * 4]), vg + (int64_t)rr * a.v_stride[2] + ch * 4, ok);
     }
-    if (threadIdx.x < BN) {
-      const int j = j0 + threadIdx.x;
+    if (tid < BN) {
+      const int j = j0 + tid;
       float x = 0.f;
       if (HAS_BIAS && j < nk) {
         const float raw = bg[j];
         x = raw <= kDeadBias ? -INFINITY : raw * kLog2e;
       }
-      sB[st][threadIdx.x] = x;
+      sB[st][tid] = x;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -131,16 +143,16 @@ __global__ void __launch_bounds__(128) pass_f32_kernel(PolyPassArgs a, const Pac
   for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-  if (ntile > 0) issue(0);
-  for (int t = 0; t < ntile; ++t) {
-    if (t + 1 < ntile) {
-      issue(t + 1);
+  if (kg < ntile) issue(kg);
+  for (int t = kg; t < ntile; t += KG) {
+    if (t + KG < ntile) {
+      issue(t + KG);
       asm volatile("cp.async.wait_group 1;" ::: "memory");
     } else {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    __syncthreads();
-    const int st = t & 1, j0 = t * BN;
+    sync();
+    const int st = (t / KG) & 1, j0 = t * BN;
     const float* K = sK[st];
     const float* V = sV[st];
     // S = Q K^T: n-block nb = keys j0 + 8 nb .. + 7. The three products of a step go
@@ -227,12 +239,41 @@ __global__ void __launch_bounds__(128) pass_f32_kernel(PolyPassArgs a, const Pac
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) mma8(o[n], ph[0], ph[1], ph[2], ph[3], bh[n][0], bh[n][1]);
     }
-    __syncthreads();   // the stage is refilled next iteration
+    sync();   // the stage is refilled next iteration
   }
   l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
   l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
   l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
   l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+  if constexpr (PACKED) {
+    // the odd tiles' sums, thread by thread, through shared memory (the rings are idle)
+    float* side = smf + tid;   // [4 D / 8 + 4][128 threads]
+    __syncthreads();
+    if (kg == 1) {
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) side[(n * 4 + e) * 128] = o[n][e];
+      side[D / 2 * 128] = m0;
+      side[(D / 2 + 1) * 128] = m1;
+      side[(D / 2 + 2) * 128] = l0;
+      side[(D / 2 + 3) * 128] = l1;
+    }
+    __syncthreads();
+    if (kg == 1) return;
+    const float y0 = side[D / 2 * 128], y1 = side[(D / 2 + 1) * 128];
+    const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
+    const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
+    const float g0 = y0 == -INFINITY ? 0.f : exp2f(y0 - n0), g1 = y1 == -INFINITY ? 0.f : exp2f(y1 - n1);
+    m0 = n0;
+    m1 = n1;
+    l0 = l0 * f0 + side[(D / 2 + 2) * 128] * g0;
+    l1 = l1 * f1 + side[(D / 2 + 3) * 128] * g1;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = o[n][e] * (e < 2 ? f0 : f1) + side[(n * 4 + e) * 128] * (e < 2 ? g0 : g1);
+  }
 
   float* ob = (float*)a.out + b * a.out_stride[0] + h * a.out_stride[1];
 #pragma unroll
@@ -308,18 +349,17 @@ bool pass_f32_eligible(const PolyPassArgs& a) {
 }
 
 namespace {
-constexpr int kSmem = (4 * BN * LD + 2 * BN) * 4;
-
 template <bool B, bool C, bool PACKED>
 int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
   std::call_once(once, [] {
-    err = cudaFuncSetAttribute(pass_f32_kernel<B, C, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    err = cudaFuncSetAttribute(pass_f32_kernel<B, C, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (PACKED ? 2 : 1) * kSmem);
   });
   if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(f32)");
   const dim3 grid = PACKED ? dim3(a.heads, a.seq_q / BM + pk->seqs + zero_ctas(*pk)) : dim3((a.seq_q + BM - 1) / BM, a.batch * a.heads);
-  pass_f32_kernel<B, C, PACKED><<<grid, 128, kSmem, s>>>(a, PACKED ? *pk : PackedSeqs{});
+  pass_f32_kernel<B, C, PACKED><<<grid, PACKED ? 256 : 128, (PACKED ? 2 : 1) * kSmem, s>>>(a, PACKED ? *pk : PackedSeqs{});
   note_launch(1);
   return cuda_status(cudaGetLastError(), "pass_f32 launch");
 }

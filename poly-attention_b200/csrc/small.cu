@@ -30,27 +30,32 @@ using namespace ms;
 
 constexpr int kMaxN = 128;
 
-// Two neighbouring features of a packed sequence's output row (a's pointers are
-// at the sequence): out, its rounding residue, the epilogue's product.
+// A packed sequence's output row: out, its rounding residue, the epilogue's product.
 template <typename T>
-__device__ __forceinline__ void store_packed(const PolyPassArgs& a, const PackedSeqs& pk, int h, int row, int c, float x,
-                                             float y) {
-  const int64_t at = h * a.out_stride[1] + (int64_t)row * a.out_stride[2] + c;
-  const uint32_t w = pk2<T>(x, y);
-  *reinterpret_cast<uint32_t*>((T*)a.out + at) = w;
-  if (pk.out_lo) {
-    const T* e = reinterpret_cast<const T*>(&w);
-    const int64_t first = (int64_t)packed_at(pk.cu, blockIdx.x / a.heads, pk.total) * a.out_stride[2];
-    *reinterpret_cast<uint32_t*>((T*)pk.out_lo + first + at) = pk2<T>(x - to_f32(e[0]), y - to_f32(e[1]));
+struct PackedRow {
+  T *out, *lo, *eo;
+  const T* em;
+  __device__ __forceinline__ PackedRow(const PolyPassArgs& a, const PackedSeqs& pk, int h, int64_t first, int row) {
+    const int64_t at = h * a.out_stride[1] + row * a.out_stride[2];   // a's pointers are at the sequence
+    out = (T*)a.out + at;
+    lo = pk.out_lo ? (T*)pk.out_lo + first * a.out_stride[2] + at : nullptr;
+    eo = a.epi_out ? (T*)a.epi_out + h * a.epi_out_stride[1] + row * a.epi_out_stride[2] : nullptr;
+    em = a.epi_out ? (const T*)a.epi_mul + h * a.epi_mul_stride[1] + row * a.epi_mul_stride[2] : nullptr;
   }
-  if (a.epi_out) {
-    const uint32_t mw = *reinterpret_cast<const uint32_t*>((const T*)a.epi_mul + h * a.epi_mul_stride[1] +
-                                                           (int64_t)row * a.epi_mul_stride[2] + c);
-    const T* m = reinterpret_cast<const T*>(&mw);
-    *reinterpret_cast<uint32_t*>((T*)a.epi_out + h * a.epi_out_stride[1] + (int64_t)row * a.epi_out_stride[2] + c) =
-        pk2<T>(x * to_f32(m[0]), y * to_f32(m[1]));
+  __device__ __forceinline__ void put(int c, float x, float y) const {   // features c, c + 1
+    const uint32_t w = pk2<T>(x, y);
+    *reinterpret_cast<uint32_t*>(out + c) = w;
+    if (lo) {
+      const T* e = reinterpret_cast<const T*>(&w);
+      *reinterpret_cast<uint32_t*>(lo + c) = pk2<T>(x - to_f32(e[0]), y - to_f32(e[1]));
+    }
+    if (eo) {
+      const uint32_t mw = *reinterpret_cast<const uint32_t*>(em + c);
+      const T* m = reinterpret_cast<const T*>(&mw);
+      *reinterpret_cast<uint32_t*>(eo + c) = pk2<T>(x * to_f32(m[0]), y * to_f32(m[1]));
+    }
   }
-}
+};
 
 template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP, bool PACKED, int NMAX>
 __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
@@ -59,6 +64,7 @@ __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, co
   const int bh = blockIdx.x;
   const int b = PACKED ? 0 : bh / a.heads, h = bh - (PACKED ? bh / a.heads : b) * a.heads;
   int nq = a.seq_q, nk = a.seq_k;
+  int64_t first_row = 0;
   if constexpr (PACKED) {
     if (bh >= pk.seqs * a.heads) {   // the CTAs behind the sequences' zero the rows outside them
       packed_zero_rest(pk, bh - pk.seqs * a.heads);
@@ -67,7 +73,7 @@ __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, co
     const int first = packed_at(pk.cu, bh / a.heads, pk.total);
     nq = nk = min(packed_at(pk.cu, bh / a.heads + 1, pk.total) - first, pk.max_len);
     if (nk <= 0 || (NMAX == 64 ? nk > 64 : nk <= 64)) return;
-    const int64_t f = first;
+    const int64_t f = first_row = first;
     a.q = (const T*)a.q + f * a.q_stride[2];
     a.k = (const T*)a.k + f * a.k_stride[2];
     a.v = (const T*)a.v + f * a.v_stride[2];
@@ -144,10 +150,21 @@ __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, co
         mma<T>(s[nb], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b0, b1);
         mma<T>(s[nb], qa[ks + 1][0], qa[ks + 1][1], qa[ks + 1][2], qa[ks + 1][3], b2, b3);
       }
+      // packed: scores stay raw without a bias or clamp (the scale, positive here, goes into the
+      // exponent's FFMA), and only blocks on the diagonal or at the end test their entries
+      const bool plain = PACKED && nb * 8 + 8 <= nk && !(a.causal && nb * 8 + 7 > warp * 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = nb * 8 + 2 * tq + (e & 1);
         const int row = e < 2 ? r0 : r1;
+        if constexpr (PACKED) {
+          float x = s[nb][e];
+          if (SOFTCLAMP) x = HAS_BIAS ? fmaf(tanhf(x * qk), sc_out, sB[j]) : tanhf(x * qk) * sc_out;
+          else if (HAS_BIAS) x = fmaf(x, qk, sB[j]);
+          if (!plain && (j >= nk || (a.causal && j > row))) x = -INFINITY;
+          s[nb][e] = x;
+          continue;
+        }
         float x = s[nb][e] * qk;
         if (SOFTCLAMP) x = tanhf(x) * sc_out;
         if (HAS_BIAS) x += sB[j];
@@ -163,11 +180,23 @@ __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, co
   m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
   m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
   float l0 = 0.f, l1 = 0.f;
+  const float mul = PACKED && !HAS_BIAS && !SOFTCLAMP ? qk : 1.f;
+  if (PACKED) {
+    m0 *= mul;
+    m1 *= mul;
+  }
+  const float s0 = m0 == -INFINITY ? 0.f : m0, s1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
   for (int nb = 0; nb < KNB; ++nb) {
     if (nb * 8 < kp) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
+        if constexpr (PACKED) {
+          const float p = tc::ex2(fmaf(s[nb][e], mul, e < 2 ? -s0 : -s1));
+          s[nb][e] = p;
+          if (e < 2) l0 += p; else l1 += p;
+          continue;
+        }
         const float m = e < 2 ? m0 : m1;
         const float p = s[nb][e] == -INFINITY ? 0.f : exp2f(s[nb][e] - m);
         s[nb][e] = p;
@@ -227,17 +256,23 @@ __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, co
     }
   }
   const float j0 = l0 > 0.f ? 1.f / l0 : 0.f, j1 = l1 > 0.f ? 1.f / l1 : 0.f;
+  if constexpr (PACKED) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int row = hf ? r1 : r0;
+      if (row >= nq) continue;
+      const PackedRow<T> out(a, pk, h, first_row, row);
+      const float inv = hf ? j1 : j0;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) out.put(n * 8 + 2 * tq, o[n][2 * hf] * inv, o[n][2 * hf + 1] * inv);
+    }
+  }
   T* ob = (T*)a.out + b * a.out_stride[0] + h * a.out_stride[1];
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
+  for (int n = 0; n < (PACKED ? 0 : NB); ++n) {
     const int c = n * 8 + 2 * tq;
-    if constexpr (PACKED) {
-      if (r0 < nq) store_packed<T>(a, pk, h, r0, c, o[n][0] * j0, o[n][1] * j0);
-      if (r1 < nq) store_packed<T>(a, pk, h, r1, c, o[n][2] * j1, o[n][3] * j1);
-    } else {
-      if (r0 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r0 * a.out_stride[2] + c) = pk2<T>(o[n][0] * j0, o[n][1] * j0);
-      if (r1 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r1 * a.out_stride[2] + c) = pk2<T>(o[n][2] * j1, o[n][3] * j1);
-    }
+    if (r0 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r0 * a.out_stride[2] + c) = pk2<T>(o[n][0] * j0, o[n][1] * j0);
+    if (r1 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r1 * a.out_stride[2] + c) = pk2<T>(o[n][2] * j1, o[n][3] * j1);
   }
   if (a.lse && tq == 0) {
     float* lb = a.lse + b * a.lse_stride[0] + h * a.lse_stride[1];

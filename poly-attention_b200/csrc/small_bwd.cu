@@ -72,16 +72,12 @@ __global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_
 
   const int k0 = warp * 16 + gq, k1 = k0 + 8;   // this thread's two keys
   const bool active = warp * 16 < n;
-  float b0 = 0.f, b1 = 0.f;
-  bool live0 = k0 < n, live1 = k1 < n;
+  // the keys' term of the exponent; -inf (p = 0) for keys past the end and dead ones
+  float b0 = k0 < n ? 0.f : -INFINITY, b1 = k1 < n ? 0.f : -INFINITY;
   if (HAS_BIAS) {
     const float* bias = f.bias + g * f.bias_stride[1] + first;
-    if (live0) b0 = bias[k0];
-    if (live1) b1 = bias[k1];
-    live0 = live0 && !(b0 <= kDeadBias);
-    live1 = live1 && !(b1 <= kDeadBias);
-    b0 *= kLog2e;
-    b1 *= kLog2e;
+    if (k0 < n) b0 = bias[k0] <= kDeadBias ? -INFINITY : bias[k0] * kLog2e;
+    if (k1 < n) b1 = bias[k1] <= kDeadBias ? -INFINITY : bias[k1] * kLog2e;
   }
   const float qk = SOFTCLAMP ? f.scale / f.softclamp : f.scale * kLog2e;
   const float sc_out = SOFTCLAMP ? f.softclamp * kLog2e : 0.f;
@@ -148,12 +144,13 @@ __global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_
           mma<T>(dp[1], va[0], va[1], va[2], va[3], x[2], x[3]);
         }
         float ds[2][4];
+        const bool diag = f.causal && c == warp;
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int i = c * 16 + nb * 8 + 2 * tq + (e & 1), j = e < 2 ? k0 : k1;
-            const float off = sLse[i] + (HAS_BIAS ? (e < 2 ? b0 : b1) : 0.f);
+            const float off = sLse[i] + (e < 2 ? b0 : b1);
             float x, slope = 1.f;
             if (SOFTCLAMP) {
               const float th = tanhf(s[nb][e] * qk);
@@ -162,9 +159,9 @@ __global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_
             } else {
               x = fmaf(s[nb][e], qk, off);
             }
-            const bool keep = (e < 2 ? live0 : live1) && !(f.causal && j > i) && sLse[i] != -INFINITY;
-            const float p = keep ? exp2f(x) : 0.f;
-            const float d = keep ? p * (dp[nb][e] - sDel[i]) : 0.f;
+            if (diag && j > i) x = -INFINITY;
+            const float p = tc::ex2(x);
+            const float d = p * (dp[nb][e] - sDel[i]);
             if (e < 2) db0 += d; else db1 += d;
             s[nb][e] = p;
             ds[nb][e] = SOFTCLAMP ? d * slope : d;

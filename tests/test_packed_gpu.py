@@ -167,6 +167,25 @@ def test_dead_keys(dtype, d, bound):
             R.assert_within(got[sl].transpose(0, 1), want, t, name)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.2, 0.7])
+@pytest.mark.parametrize("dtype,bound", [(torch.bfloat16, None), (torch.bfloat16, 100), (torch.float32, None)])
+def test_scales(scale, dtype, bound):
+    import poly_attention_b200 as P
+    lens = [70, 100]
+    q, k, v, do, b, dl = make(lens, 2, 1, 64, dtype, bias=True)
+    cu, _ = P.packed_offsets(lens)
+    kw = dict(causal=True, scale=scale, bias=b, max_seqlen=bound)
+    out, lse = P.pass_fwd_packed(q, k, v, cu, **kw)
+    dq, dk, dv, _ = P.pass_bwd_packed(q, k, v, cu, out, lse, do, **kw)
+    for sl in seqs(lens):
+        ref = [t64(x, sl) for x in (q, k, v)]
+        (o, ot), (l, lt), st = R.forward(*ref, b[:, sl].double(), causal_keep(sl.stop - sl.start, True), scale, None, dtype)
+        R.assert_within(out[sl].transpose(0, 1), o, ot, "out")
+        R.assert_within(lse[:, sl], l, lt, "lse")
+        for name, got, (want, t) in zip(("dq", "dk", "dv"), (dq, dk, dv), R.backward(*ref, o, t64(do, sl), None, st, scale, None, dtype)):
+            R.assert_within(got[sl].transpose(0, 1), want, t.abs() + 1e-30, name)
+
+
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 128)])
 def test_strides_and_alignment(dtype, d):
     """Head-split views of one projection, head-major tensors, odd offsets, features not contiguous."""
