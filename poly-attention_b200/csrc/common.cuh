@@ -41,11 +41,33 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// Programmatic dependence between consecutive kernels: let the next one start, wait for the previous one.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// A kernel that shares nothing with its predecessor may start early without waiting; held as a
+// local of the kernel, this still makes it end after that one, so that what follows it in the
+// stream follows both.
+template <bool ON>
+struct EndAfterPrevious {
+  __device__ __forceinline__ ~EndAfterPrevious() {
+    if (ON) pdl_wait();
+  }
+};
+
 // Thread-local error message for poly_last_error().
 void set_error(const std::string& msg);
 
 // Counts kernel launches made by this library (poly_launch_count()).
 void note_launch(int n = 1);
+
+// Launch attribute of a programmatic dependent.
+inline cudaLaunchAttribute dependent_launch() {
+  cudaLaunchAttribute a;
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
 
 inline int cuda_status(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return POLY_OK;

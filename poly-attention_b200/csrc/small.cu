@@ -65,6 +65,10 @@ __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, co
   const int b = PACKED ? 0 : bh / a.heads, h = bh - (PACKED ? bh / a.heads : b) * a.heads;
   int nq = a.seq_q, nk = a.seq_k;
   int64_t first_row = 0;
+  // packed: the launch for 65 to 128 rows starts while the one for up to 64 drains (their
+  // sequences differ) and ends after it
+  if (PACKED && NMAX == 64) pdl_launch();
+  const EndAfterPrevious<PACKED && NMAX != 64> order;
   if constexpr (PACKED) {
     if (bh >= pk.seqs * a.heads) {   // the CTAs behind the sequences' zero the rows outside them
       packed_zero_rest(pk, bh - pk.seqs * a.heads);
@@ -298,9 +302,17 @@ int launch_n(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   if (PACKED) q = *pk;
   if (PACKED && NMAX != 64) q.zero.n = 0;   // done by the first launch
   const unsigned grid = (unsigned)((PACKED ? pk->seqs : a.batch) * a.heads) + zero_ctas(q);
-  pass_small_kernel<T, D, B, C, PACKED, NMAX><<<grid, threads, bytes, s>>>(a, q);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute dep = dependent_launch();
+  cfg.attrs = &dep;
+  cfg.numAttrs = PACKED && NMAX != 64 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, pass_small_kernel<T, D, B, C, PACKED, NMAX>, a, q);
   note_launch(1);
-  return cuda_status(cudaGetLastError(), "pass_small launch");
+  return cuda_status(e, "pass_small launch");
 }
 
 template <typename T, int D, bool B, bool C, bool PACKED>

@@ -42,6 +42,10 @@ __global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_
   const PolyPassBwdArgs& a = P.a;
   const PolyPassArgs& f = a.fwd;
   const PackedSeqs& pk = P.pk;
+  // the launch for 65 to 128 rows starts while the one for up to 64 drains (their sequences differ)
+  // and ends after it
+  if (NMAX == 64) pdl_launch();
+  const EndAfterPrevious<NMAX != 64> order;
   if ((int)blockIdx.x >= pk.seqs * f.kv_heads) {   // the CTAs behind the sequences' zero the rows outside them
     packed_zero_rest(pk, blockIdx.x - pk.seqs * f.kv_heads);
     return;
@@ -278,9 +282,17 @@ int launch_n(SmallBwd p, cudaStream_t s) {
   if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(small bwd)");
   p.rows = std::min(p.rows, NMAX);
   if (NMAX != 64) p.pk.zero.n = 0;   // done by the first launch
-  small_bwd_kernel<T, D, B, C, NMAX><<<(unsigned)(p.pk.seqs * p.a.fwd.kv_heads) + zero_ctas(p.pk), 2 * p.rows, p.rows * row, s>>>(p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.pk.seqs * p.a.fwd.kv_heads) + zero_ctas(p.pk));
+  cfg.blockDim = dim3(2 * p.rows);
+  cfg.dynamicSmemBytes = p.rows * row;
+  cfg.stream = s;
+  cudaLaunchAttribute dep = dependent_launch();
+  cfg.attrs = &dep;
+  cfg.numAttrs = NMAX != 64 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, small_bwd_kernel<T, D, B, C, NMAX>, p);
   note_launch(1);
-  return cuda_status(cudaGetLastError(), "small_bwd launch");
+  return cuda_status(e, "small_bwd launch");
 }
 
 template <typename T, int D, bool B, bool C>

@@ -653,10 +653,7 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cu
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (dependent) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
+  if (dependent) attr[n++] = dependent_launch();
   if (cluster > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
     attr[n].val.clusterDim.x = cluster;

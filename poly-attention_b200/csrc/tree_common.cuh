@@ -11,9 +11,6 @@ namespace treec {
 constexpr int kNodes = POLY_MAX_TREE_NODES;
 constexpr int kMaxSplits = 64;
 
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // Visible tree nodes of every node as bits (0: padding), by pointer jumping: after
 // round r a node knows its nearest 2^r ancestors. Callers with at least 64 threads.
 __device__ __forceinline__ void ancestors(const int32_t* parents, int nodes, int room, uint64_t* mask, int* up) {

@@ -476,10 +476,8 @@ int launch_t(const PolyTreePass& a, const TreeGeom& geo, cudaStream_t s, bool de
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = L::kAlloc;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
+  cudaLaunchAttribute attr = dependent_launch();
+  cfg.attrs = &attr;
   cfg.numAttrs = dependent ? 1 : 0;
   note_launch(1);
   return cuda_status(cudaLaunchKernelEx(&cfg, tree_tc_kernel<T, D, ROWS2, SC>, tq, tk, tv, p), "tree tc launch");
