@@ -14,15 +14,15 @@ from torch.nn import Module, RMSNorm
 from .core import poly_attention_chain, poly_attention_chain_cached
 from .head_norm import head_rmsnorm
 from .kv_cache import ModuleKVCache, usable as _inplace_usable
-from .packed import poly_attention_chain_packed
-from .poly_attention import (cast_tuple, check_packed, default, exists, merge_heads, rotate_by_angles, split_heads,
-                             token_rows)
+from .packed import check_packed, poly_attention_chain_packed, split_heads, token_rows
+from .poly_attention import cast_tuple, default, exists, merge_heads, rotate_by_angles
 from .rotary import RotaryEmbedding
+from .tree import TreeDecoding
 
 LinearNoBias = partial(nn.Linear, bias=False)
 
 
-class NPolyAttention(Module):
+class NPolyAttention(TreeDecoding, Module):
     def __init__(self, dim, order=3, heads=8, kv_heads=None, dim_head=64, causal=False, shared_kv=False,
                  softclamp_value=None, use_rotary_embed=False, prenorm=False, separate_context_norms=False,
                  multiply_root_value=False, use_root_value_as_attn_gate=False, attn_gate=False):

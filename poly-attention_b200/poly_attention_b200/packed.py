@@ -24,6 +24,26 @@ from .core import _autocast, _sc
 from .ops import _DTYPES, _on, _require_cuda, _stream
 
 
+def split_heads(t, split, heads):
+    """'b n (split h d) -> split b h n d' as strided views (no copy)."""
+    b, n, f = t.shape
+    d = f // (split * heads)
+    return t.view(b, n, split, heads, d).permute(2, 0, 3, 1, 4)
+
+
+def token_rows(t):
+    """[1, heads, total, d] -> [total, heads, d] (a view)."""
+    return t.squeeze(0).transpose(0, 1)
+
+
+def check_packed(x, context=None, mask=None, context_mask=None, cache=None, return_cache=False):
+    """A module's arguments with cu_seqlens."""
+    if x.dim() != 3 or x.shape[0] != 1:
+        raise ValueError("packed sequences (cu_seqlens) come as one row: x [1, total, dim]")
+    if any(t is not None for t in (context, mask, context_mask, cache)) or return_cache:
+        raise ValueError("packed sequences (cu_seqlens) take no context, masks or cache")
+
+
 def packed_offsets(lengths, device="cuda"):
     """(cu_seqlens, max_seqlen) of a list of sequence lengths."""
     lengths = [int(n) for n in lengths]
@@ -65,35 +85,10 @@ def _rows(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def _set(a, name, t):
-    """A [total, heads, d] tensor (or [heads, total] fp32 vector) into its pointer and (batch, head, row) strides."""
-    setattr(a, name, t.data_ptr())
-    st, s = getattr(a, name + "_stride"), t.stride()
-    if len(s) == 3 and len(st) == 3:
-        st[1], st[2] = s[1], s[0]
-    elif len(s) == 3:
-        st[0], st[1] = s[1], s[0]
-    else:
-        st[1] = s[0]
-
-
 def _vec(t, heads, total, what):
     if t.shape != (heads, total):
         raise ValueError(f"{what} must be [{heads}, {total}], got {tuple(t.shape)}")
     return _rows(t.float())
-
-
-def _fill(a, q, k, v, bias, causal, softclamp, scale):
-    a.batch, a.heads, a.kv_heads, a.head_dim = 1, q.shape[1], k.shape[1], q.shape[2]
-    a.seq_q = a.seq_k = q.shape[0]
-    a.dtype, a.causal = _DTYPES[q.dtype], int(bool(causal))
-    a.scale = float(q.shape[2] ** -0.5 if scale is None else scale)
-    a.softclamp = _sc(softclamp)
-    _set(a, "q", q)
-    _set(a, "k", k)
-    _set(a, "v", v)
-    if bias is not None:
-        _set(a, "bias", bias)
 
 
 _FWD = _lib.packer(PolyPackedArgs)
@@ -152,6 +147,9 @@ def pass_fwd_packed(q, k, v, cu_seqlens, *, causal=False, softclamp=None, scale=
     return (out, lse) + ((epi,) if epi is not None else ()) + ((lo,) if out_lo else ())
 
 
+_BWD = _lib.packer(PolyPackedBwdArgs)
+
+
 def _backward(q, k, v, cu, out, lse, dout, bias, dlse, dq, want_dbias, out_lo, factors, causal, softclamp, scale, max_seqlen):
     """pass_bwd_packed on checked tensors."""
     q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
@@ -159,39 +157,34 @@ def _backward(q, k, v, cu, out, lse, dout, bias, dlse, dq, want_dbias, out_lo, f
     g = k.shape[1]
     if any(st <= 0 for st in dout.stride()):
         dout = dout.contiguous()        # broadcast gradients (out.sum().backward())
-    a = PolyPackedBwdArgs()
-    b = a.bwd
-    f = b.fwd
-    _fill(f, q, k, v, bias, causal, softclamp, scale)
-    _set(f, "out", out)
-    _set(f, "lse", lse)
-    _set(b, "dout", dout)
-    if dlse is not None:
-        _set(b, "dlse", dlse)
-    if out_lo is not None:
-        a.out_lo = out_lo.data_ptr()
-    dright = None
+    left = right = dright = None
     if factors is not None:
         left, right = (_rows(t) for t in factors)
         dright = v.new_empty(total, g, d)
-        _set(a, "v_left", left)
-        _set(a, "v_right", right)
-        _set(a, "dv_right", dright)
-    b.dq_accumulate = int(dq is not None)
+    accumulate = dq is not None
     if dq is None:
         dq = q.new_empty(total, h, d)
     dk, dv = k.new_empty(total, g, d), v.new_empty(total, g, d)
     dbias = q.new_empty(g, total, dtype=torch.float32) if want_dbias else None
-    _set(b, "dq", dq)
-    _set(b, "dk", dk)
-    _set(b, "dv", dv)
-    if want_dbias:
-        _set(b, "dbias", dbias)
-    a.cu_seqlens, a.seqs, a.max_len, a.zero_rest = cu.data_ptr(), cu.shape[0] - 1, int(max_seqlen or 0), 1
-    if a.seqs == 0 and total:
-        for t in (dk, dv, dbias, dright, None if b.dq_accumulate else dq):
+    seqs = cu.shape[0] - 1
+    if seqs == 0 and total:
+        for t in (dk, dv, dbias, dright, None if accumulate else dq):
             if t is not None:
                 t.zero_()
+    qs, ks, vs, os, gs, dqs = q.stride(), k.stride(), v.stride(), out.stride(), dout.stride(), dq.stride()
+    ls, rs = (left.stride(), right.stride()) if left is not None else ((0, 0), (0, 0))
+    ptr = lambda t: 0 if t is None else t.data_ptr()   # noqa: E731
+    # PolyPackedBwdArgs in its order
+    a = PolyPackedBwdArgs.from_buffer_copy(_BWD.pack(
+        1, h, g, total, total, d, _DTYPES[q.dtype], bool(causal), d ** -0.5 if scale is None else scale, _sc(softclamp),
+        q.data_ptr(), 0, qs[1], qs[0], k.data_ptr(), 0, ks[1], ks[0], v.data_ptr(), 0, vs[1], vs[0], 0, 0, 0, 0,
+        ptr(bias), 0, 0 if bias is None else bias.stride(0), 0, 0, 0, 0,
+        out.data_ptr(), 0, os[1], os[0], lse.data_ptr(), 0, lse.stride(0), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+        dout.data_ptr(), 0, gs[1], gs[0], ptr(dlse), 0, 0 if dlse is None else dlse.stride(0),
+        dq.data_ptr(), 0, dqs[1], dqs[0], dk.data_ptr(), 0, d, g * d, dv.data_ptr(), 0, d, g * d, ptr(dbias), 0, total,
+        accumulate, 0, 0, 0, cu.data_ptr(), seqs, max_seqlen or 0, 1, 0, ptr(out_lo),
+        ptr(left), ls[1], ls[0], ptr(right), rs[1], rs[0], ptr(dright), d, g * d))
+    b = a.bwd
     with _on(q.device):
         need = lib.poly_packed_pass_bwd_workspace_size(a)
         ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
@@ -233,12 +226,21 @@ def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softcl
 def packed_kernel_names(q, k, v, max_seqlen=None):
     """(forward, backward) kernel family the library picks for these packed tensors."""
     a, b = PolyPackedArgs(), PolyPackedBwdArgs()
+
+    def put(x, name, t):
+        setattr(x, name, t.data_ptr())
+        st = getattr(x, name + "_stride")
+        st[1], st[2] = t.stride(1), t.stride(0)
+
     for x, f in ((a, a.fwd), (b, b.bwd.fwd)):
-        _fill(f, q, k, v, None, False, None, None)
-        _set(f, "out", q)
+        f.batch, f.heads, f.kv_heads, f.head_dim, f.dtype = 1, q.shape[1], k.shape[1], q.shape[2], _DTYPES[q.dtype]
+        f.seq_q = f.seq_k = q.shape[0]
+        f.scale = q.shape[2] ** -0.5
+        for name, t in (("q", q), ("k", k), ("v", v), ("out", q)):
+            put(f, name, t)
         x.cu_seqlens, x.seqs, x.max_len = 1, 1, int(max_seqlen or 0)
     for name, t in (("dout", q), ("dq", q), ("dk", k), ("dv", v)):
-        _set(b.bwd, name, t)
+        put(b.bwd, name, t)
     return lib.poly_packed_pass_fwd_kernel_name(a).decode(), lib.poly_packed_pass_bwd_kernel_name(b).decode()
 
 

@@ -15,8 +15,9 @@ from torch.nn import Module, RMSNorm
 from .core import poly_attention_order2, poly_attention_order2_cached
 from .head_norm import head_rmsnorm
 from .kv_cache import ModuleKVCache, usable as _inplace_usable
-from .packed import poly_attention_order2_packed
+from .packed import check_packed, poly_attention_order2_packed, split_heads, token_rows
 from .rotary import RotaryEmbedding, apply_rotary
+from .tree import TreeDecoding
 
 LinearNoBias = partial(nn.Linear, bias=False)
 
@@ -33,13 +34,6 @@ def cast_tuple(t, length=1):
     return (t,) * length if torch.is_tensor(t) or not isinstance(t, tuple) else t
 
 
-def split_heads(t, split, heads):
-    """'b n (split h d) -> split b h n d' as strided views (no copy)."""
-    b, n, f = t.shape
-    d = f // (split * heads)
-    return t.view(b, n, split, heads, d).permute(2, 0, 3, 1, 4)
-
-
 def merge_heads(t):
     """'b h n d -> b n (h d)'."""
     b, h, n, d = t.shape
@@ -53,19 +47,7 @@ def rotate_by_angles(rotary_pos_emb, qs):
     return apply_rotary(qs, angles=rotary_pos_emb[..., ::2])
 
 
-def check_packed(x, context, mask, context_mask, cache, return_cache):
-    if x.dim() != 3 or x.shape[0] != 1:
-        raise ValueError("packed sequences (cu_seqlens) come as one row: x [1, total, dim]")
-    if any(exists(t) for t in (context, mask, context_mask, cache)) or return_cache:
-        raise ValueError("packed sequences (cu_seqlens) take no context, masks or cache")
-
-
-def token_rows(t):
-    """[1, heads, total, d] -> [total, heads, d] (a view)."""
-    return t.squeeze(0).transpose(0, 1)
-
-
-class Order2PolyAttention(Module):
+class Order2PolyAttention(TreeDecoding, Module):
     def __init__(self, dim, heads=8, kv_heads=None, dim_head=64, causal=False, shared_kv=False, softclamp_value=None,
                  use_rotary_embed=False, prenorm=False, separate_context_norms=False, multiply_root_value=False,
                  use_root_value_as_attn_gate=False, attn_gate=False, use_flash_kernel=None):

@@ -24,7 +24,9 @@ import torch
 
 from . import _lib
 from ._lib import PolyTreeAppend, PolyTreeCommit, PolyTreePass, check, lib
+from .head_norm import head_rmsnorm
 from .ops import _DTYPES, _on, _require_cuda, _stream
+from .packed import check_packed, poly_attention_chain_packed, split_heads, token_rows
 
 
 def _st3(dst, t, size=1):
@@ -122,6 +124,7 @@ class TreeDecoder:
         if any(len(x) != n for x, n in ((keys, self.order), (vals, self.order - 1), (lses, self.order - 1), (msgs, self.order - 1))):
             raise ValueError("an order-n decoder holds n key caches and n - 1 of values, lses and messages")
         for c, t in zip(self.keys + self.vals + self.msgs + self.lses, (*keys, *vals, *msgs, *lses)):
+            t = t.detach()
             n = t.shape[2]
             if longest > n or n > self.cap or t.shape[:2] != c.shape[:2] or t.shape[3:] != c.shape[3:]:
                 raise ValueError(f"cache rows {tuple(t.shape)} do not fit {tuple(c.shape)} and lengths up to {longest}")
@@ -246,4 +249,51 @@ class TreeDecoder:
         self._bound = min(self.cap, self._bound + min(c.nodes, c.path_len))
 
 
-__all__ = ["TreeDecoder"]
+class TreeDecoding:
+    """Drafted-token decoding of the attention modules (``PolyAttention``, ``NPolyAttention``; causal ones): a packed
+    prompt batch fills a ``TreeDecoder``, then each step runs a tree of tokens per sequence through the module. With
+    ``use_rotary_embed`` the decoder holds rotated keys, every token at its position in its sequence."""
+
+    def _tree_project(self, x):
+        order = len(self.to_kvs)
+        normed = self.norm(x)
+        contexts = [norm(x) for norm in self.context_norms] if self.context_norms is not None else [normed] * order
+        qg = split_heads(self.to_q(normed), self.q_split, self.heads)
+        kvs = [split_heads(to_kv(c), self.kv1_split if i == 0 else self.kv_split, self.kv_heads)
+               for i, (to_kv, c) in enumerate(zip(self.to_kvs, contexts))]
+        if self.shared_kv:
+            root, vs = kvs[0][0], [kv[0] for kv in kvs[1:]]
+        else:
+            root, vs = kvs[0][1] if self.has_root_v else None, [kv[1] for kv in kvs[1:]]
+        qs = head_rmsnorm(self.q_norms, (qg[0], *(kv[0] for kv in kvs)))
+        return list(qs), vs, root, qg[1] if self.attn_gate else None
+
+    @torch.no_grad()
+    def tree_prefill(self, x, cu_seqlens, *, max_seqlen, capacity, max_nodes):
+        """Prompts x [1, total, dim] packed by cu_seqlens -> (y [1, total, dim], TreeDecoder of the sequences)."""
+        if not self.causal:
+            raise ValueError("decoding needs a causal module")
+        check_packed(x)
+        qs, vs, root, gates = self._tree_project(x)
+        if self.rotary_emb is not None:
+            qs = self.rotary_emb(qs, cu_seqlens=cu_seqlens)
+        qs, vals = [token_rows(q) for q in qs], [token_rows(v) for v in vs]
+        out, lses, msgs = poly_attention_chain_packed([qs[0], *qs[1:-1]], qs[1:], vals, cu_seqlens,
+                                                      softclamp_value=self.softclamp_value, causal=True, max_seqlen=max_seqlen)
+        dec = TreeDecoder(batch=cu_seqlens.shape[0] - 1, order=len(vs) + 1, heads=self.heads, kv_heads=self.kv_heads,
+                          dim_head=self.dim_head, capacity=capacity, max_nodes=max_nodes, dtype=out.dtype, device=out.device,
+                          softclamp_value=self.softclamp_value)
+        dec.load_packed(qs[1:], vals, lses, msgs, cu_seqlens, max_seqlen)
+        return self._finish(out.transpose(0, 1).unsqueeze(0), root, gates), dec
+
+    @torch.no_grad()
+    def tree_step(self, x, decoder, parents):
+        """Drafted tokens x [b, T, dim] with their trees (``TreeDecoder.step``) -> y [b, T, dim]. ``decoder.commit`` then
+        keeps the accepted ones."""
+        qs, vs, root, gates = self._tree_project(x)
+        if self.rotary_emb is not None:
+            qs = self.rotary_emb(qs, positions=decoder.positions(parents))
+        return self._finish(decoder.step(qs[0], qs[1:], vs, parents), root, gates)
+
+
+__all__ = ["TreeDecoder", "TreeDecoding"]
