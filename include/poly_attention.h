@@ -245,9 +245,9 @@ POLY_API int poly_head_rmsnorm(const PolyHeadNorm* norms, int n, void* stream);
  * [seqs + 1], not decreasing, within [0, seq_q]; lengths may be 0, and rows
  * outside every sequence are neither read into a result nor written. Offsets
  * that break this give wrong rows, never an access outside the tensors.
- * max_len: an upper bound of the lengths if the caller has one, else 0; rows
- * of a longer sequence are then undefined. Up to 128 it selects kernels that hold a
- * whole sequence per CTA. Bias, softclamp, grouped heads and the epilogue
+ * max_len: an upper bound of the lengths if the caller has one, else 0. Up to
+ * 128 it selects kernels that hold a whole sequence per CTA; all results of a
+ * longer sequence are then NaN (it is not looked at otherwise). Bias, softclamp, grouped heads and the epilogue
  * product as in poly_pass_fwd; masks, v_mul and causal_offset are
  * POLY_EUNSUPPORTED. A row whose every key is dead (bias <= -FLT_MAX / 2) gets
  * out = 0 and lse = -FLT_MAX, and no gradient. epi_out is epi_mul times the
@@ -285,6 +285,7 @@ typedef struct PolyPackedBwdArgs {
   void* dv_right;       int64_t dv_right_stride[2];
 } PolyPackedBwdArgs;
 
+/* The workspace of the backward is 16-byte aligned. */
 POLY_API int poly_packed_pass_fwd(const PolyPackedArgs* args, void* stream);
 POLY_API int poly_packed_pass_bwd(const PolyPackedBwdArgs* args, void* stream);
 POLY_API size_t poly_packed_pass_bwd_workspace_size(const PolyPackedBwdArgs* args);
@@ -376,7 +377,7 @@ typedef struct PolyTreePass {
   float* lse;         int64_t lse_stride[2];     /* [batch, heads, nodes] | NULL */
   void* cache_out;    int64_t cache_out_stride[3]; /* [batch, heads, capacity, d] | NULL */
   float* cache_lse;   int64_t cache_lse_stride[2]; /* [batch, heads, capacity] | NULL */
-  void* workspace;    /* >= poly_tree_workspace_size() bytes; passes of a chain may share it */
+  void* workspace;    /* >= poly_tree_workspace_size() bytes, 16-byte aligned; passes of a chain may share it */
   size_t workspace_bytes;
 } PolyTreePass;
 

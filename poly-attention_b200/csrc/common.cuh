@@ -118,6 +118,7 @@ struct ZeroRest {
     char* p;
     int heads, row_bytes;
     int64_t head_stride, row_stride;   // bytes
+    bool wide;                          // 16-byte stores
   } t[5];
   int n;
 };
@@ -133,7 +134,7 @@ struct PackedSeqs {
   void* dv_right; int64_t dv_right_stride[2];
   ZeroRest zero;        // the work of kZeroCtas extra CTAs of the pass's first kernel (none if zero.n is 0)
 };
-constexpr int kZeroCtas = 16;
+constexpr int kZeroCtas = 32;
 inline unsigned zero_ctas(const PackedSeqs& q) { return q.zero.n ? kZeroCtas : 0; }
 int launch_packed_fwd_simt(const PolyPassArgs& a, const PackedSeqs& q, cudaStream_t s);
 int launch_packed_bwd_simt(const PolyPassBwdArgs& a, const PackedSeqs& q, cudaStream_t s);

@@ -600,6 +600,13 @@ int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t st) {
   const int grp_kv = (int)std::max<size_t>(1, (32u << 20) / std::max<size_t>(kv_bytes, 1));
   p.n_bh = a.batch * a.heads;
   p.grp_bh = std::min(p.n_bh, grp_kv * rep_h);
+  if (PACKED) {
+    // groups of one size: a last group of one head would start its longest rows when
+    // the others are done (32768 tokens, 16 heads, order 2: 1916 us in groups of 15,
+    // 1757 us in groups of 8 or one of 16)
+    const int groups = (p.n_bh + p.grp_bh - 1) / p.grp_bh;
+    p.grp_bh = ((a.kv_heads + groups - 1) / groups) * rep_h;
+  }
   dim3 grid((unsigned)(p.n_bh * p.m_tiles) + (PACKED ? zero_ctas(*pk) : 0));
   pass_fwd_tc2_kernel<T, HAS_BIAS, D, PACKED, SOFTCLAMP><<<grid, kThreads, L2::kAlloc, st>>>(tq, tk, tv, tb, p);
   note_launch(1);

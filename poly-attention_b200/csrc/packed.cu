@@ -16,6 +16,7 @@ int fail(int code, const std::string& m) {
 // The checks of poly_pass_fwd that apply, then those of the packed layout.
 int check_packed(const PolyPassArgs& a, const int32_t* cu, int seqs, int max_len) {
   if (a.batch != 1) return fail(POLY_EINVAL, "packed passes have batch 1");
+  if (a.heads > 65535) return fail(POLY_EUNSUPPORTED, "more than 65535 heads");
   if (a.heads <= 0 || a.kv_heads <= 0 || a.seq_q < 0 || a.head_dim <= 0)
     return fail(POLY_EINVAL, "heads, kv_heads and head_dim must be positive, seq_q non-negative");
   if (a.seq_q != a.seq_k) return fail(POLY_EINVAL, "packed passes have seq_q == seq_k (the rows of all sequences)");
@@ -43,6 +44,7 @@ void zero_add(ZeroRest& z, void* p, int heads, int dim, int es, int64_t head_str
   t.row_bytes = dim * es;
   t.head_stride = head_stride * es;
   t.row_stride = row_stride * es;
+  t.wide = !(((uintptr_t)p | (uintptr_t)t.row_bytes | (uintptr_t)t.head_stride | (uintptr_t)t.row_stride) & 15);
 }
 
 int check_fwd(const PolyPackedArgs* a) {
@@ -163,6 +165,7 @@ int poly_packed_pass_bwd(const PolyPackedBwdArgs* a, void* stream) {
   const size_t need = poly_packed_pass_bwd_workspace_size(a);
   if (need && (!b.workspace || b.workspace_bytes < need))
     return fail(POLY_EINVAL, "workspace too small: need " + std::to_string(need) + " bytes");
+  if ((uintptr_t)b.workspace & 15) return fail(POLY_EINVAL, "workspace must be 16-byte aligned");
   if (a->zero_rest) {
     const PolyPassArgs& f = b.fwd;
     const int es = f.dtype == POLY_F32 ? 4 : 2;

@@ -60,13 +60,26 @@ __device__ __forceinline__ void packed_zero_rest(const PackedSeqs& q, int part) 
     const int64_t row = r < lo ? r : hi + (r - lo);
     for (int k = 0; k < q.zero.n; ++k) {
       const auto& t = q.zero.t[k];
-      const int words = t.row_bytes >> 1;   // 16-bit words: rows need no more than their type's alignment
-      for (int i = threadIdx.x; i < t.heads * words; i += blockDim.x) {
-        const int h = i / words, w = i - h * words;
-        *reinterpret_cast<uint16_t*>(t.p + h * t.head_stride + row * t.row_stride + 2 * w) = 0;
+      char* base = t.p + row * t.row_stride;
+      if (t.wide) {
+        const int words = t.row_bytes >> 4;
+        for (int i = threadIdx.x; i < t.heads * words; i += blockDim.x)
+          *reinterpret_cast<uint4*>(base + (i / words) * t.head_stride + (i % words) * 16) = make_uint4(0u, 0u, 0u, 0u);
+      } else {   // rows need no more than their type's alignment
+        const int words = t.row_bytes >> 1;
+        for (int i = threadIdx.x; i < t.heads * words; i += blockDim.x)
+          *reinterpret_cast<uint16_t*>(base + (i / words) * t.head_stride + (i % words) * 2) = 0;
       }
     }
   }
+}
+
+// Rows of one head as NaN (0x7fff is one in fp16 and in bf16): a sequence that is
+// longer than the caller's bound said.
+__device__ __forceinline__ void packed_nan_rows(void* p, int64_t head, int64_t row_stride, int64_t first, int rows, int dim) {
+  if (!p) return;
+  for (int i = threadIdx.x; i < rows * dim; i += blockDim.x)
+    ((uint16_t*)p)[head + (first + i / dim) * row_stride + i % dim] = 0x7fff;
 }
 
 // The slots of a launch by descending number of tiles to walk, `order`[slots], by one CTA:

@@ -75,7 +75,15 @@ __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, co
       return;
     }
     const int first = packed_at(pk.cu, bh / a.heads, pk.total);
-    nq = nk = min(packed_at(pk.cu, bh / a.heads + 1, pk.total) - first, pk.max_len);
+    nq = nk = packed_at(pk.cu, bh / a.heads + 1, pk.total) - first;
+    if (nk > pk.max_len) {   // the caller's bound is wrong: NaN, once
+      if (NMAX != 64) return;
+      packed_nan_rows(a.out, h * a.out_stride[1], a.out_stride[2], first, nk, D);
+      packed_nan_rows(pk.out_lo, h * a.out_stride[1], a.out_stride[2], first, nk, D);
+      packed_nan_rows(a.epi_out, h * a.epi_out_stride[1], a.epi_out_stride[2], first, nk, D);
+      for (int i = threadIdx.x; a.lse && i < nk; i += blockDim.x) a.lse[h * a.lse_stride[1] + first + i] = NAN;
+      return;
+    }
     if (nk <= 0 || (NMAX == 64 ? nk > 64 : nk <= 64)) return;
     const int64_t f = first_row = first;
     a.q = (const T*)a.q + f * a.q_stride[2];

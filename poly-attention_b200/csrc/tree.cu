@@ -798,6 +798,7 @@ int poly_tree_chain(const PolyTreeAppend* append, const PolyTreePass* passes, in
     const size_t need = poly_tree_workspace_size(&passes[i]);
     if (need && (!passes[i].workspace || passes[i].workspace_bytes < need))
       return fail(POLY_EINVAL, "tree pass " + std::to_string(i) + " needs a workspace of " + std::to_string(need) + " bytes");
+    if ((uintptr_t)passes[i].workspace & 15) return fail(POLY_EINVAL, "tree pass: workspace must be 16-byte aligned");
   }
   cudaStream_t s = (cudaStream_t)stream;
   bool dep = false;

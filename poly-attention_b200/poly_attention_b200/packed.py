@@ -12,9 +12,16 @@ zero gradients.
 The offsets stay on the device and are not checked there: they must not
 decrease and must lie in [0, total] (others give wrong rows, never an access
 outside the tensors). ``max_seqlen`` is an upper bound of the lengths, if the
-caller has one: up to 128 it selects kernels that hold a whole sequence per CTA.
+caller has one: up to 128 it selects kernels that hold a whole sequence per CTA, and
+a longer sequence then comes out as NaN.
+
+Gradients of queries over several key tiles are summed in 32 bits in no fixed order
+(16-bit tensors with heads of 64 or 128 features and no bound of 128): equal calls may
+differ in their last bit. Everything else is the same from call to call.
 """
 from __future__ import annotations
+
+import operator
 
 import torch
 
@@ -81,6 +88,15 @@ def _tensors(q, k, v, *same):
             raise ValueError("packed tensors must be on one device")
 
 
+def _bound(max_seqlen):
+    if max_seqlen is None:
+        return 0
+    max_seqlen = operator.index(max_seqlen)
+    if max_seqlen < 0:
+        raise ValueError("max_seqlen must be non-negative")
+    return min(max_seqlen, 1 << 30)
+
+
 def _rows(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
@@ -119,7 +135,7 @@ def _forward(q, k, v, cu, bias, epi_mul, causal, softclamp, scale, max_seqlen, o
         0 if bias is None else bias.data_ptr(), 0, 0 if bias is None else bias.stride(0), 0, 0, 0, 0,
         out.data_ptr(), 0, d, h * d, lse.data_ptr(), 0, total,
         0 if epi is None else epi_mul.data_ptr(), 0, ms[1], ms[0], 0 if epi is None else epi.data_ptr(), 0, d, h * d, 0, 0, 0, 0,
-        cu.data_ptr(), seqs, max_seqlen or 0, 1, 0, 0 if lo is None else lo.data_ptr()))
+        cu.data_ptr(), seqs, max_seqlen, 1, 0, 0 if lo is None else lo.data_ptr()))
     with _on(q.device):
         check(lib.poly_packed_pass_fwd(a, _stream(q.device)), "poly_packed_pass_fwd")
     return out, lse, epi, lo
@@ -143,7 +159,7 @@ def pass_fwd_packed(q, k, v, cu_seqlens, *, causal=False, softclamp=None, scale=
         raise ValueError("heads must be divisible by kv_heads")
     if epi_mul is not None and (epi_mul.shape != q.shape or epi_mul.dtype != q.dtype):
         raise ValueError("epi_mul must have q's shape and dtype")
-    out, lse, epi, lo = _forward(q, k, v, cu, bias, epi_mul, causal, softclamp, scale, max_seqlen, out_lo)
+    out, lse, epi, lo = _forward(q, k, v, cu, bias, epi_mul, causal, softclamp, scale, _bound(max_seqlen), out_lo)
     return (out, lse) + ((epi,) if epi is not None else ()) + ((lo,) if out_lo else ())
 
 
@@ -182,7 +198,7 @@ def _backward(q, k, v, cu, out, lse, dout, bias, dlse, dq, want_dbias, out_lo, f
         out.data_ptr(), 0, os[1], os[0], lse.data_ptr(), 0, lse.stride(0), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
         dout.data_ptr(), 0, gs[1], gs[0], ptr(dlse), 0, 0 if dlse is None else dlse.stride(0),
         dq.data_ptr(), 0, dqs[1], dqs[0], dk.data_ptr(), 0, d, g * d, dv.data_ptr(), 0, d, g * d, ptr(dbias), 0, total,
-        accumulate, 0, 0, 0, cu.data_ptr(), seqs, max_seqlen or 0, 1, 0, ptr(out_lo),
+        accumulate, 0, 0, 0, cu.data_ptr(), seqs, max_seqlen, 1, 0, ptr(out_lo),
         ptr(left), ls[1], ls[0], ptr(right), rs[1], rs[0], ptr(dright), d, g * d))
     b = a.bwd
     with _on(q.device):
@@ -220,7 +236,7 @@ def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softcl
     bias = None if bias is None else _vec(bias, g, total, "bias")
     dlse = None if dlse is None else _vec(dlse, h, total, "dlse")
     return _backward(q, k, v, cu, out, lse, dout.to(q.dtype), bias, dlse, dq, want_dbias, out_lo, factors, causal, softclamp,
-                     scale, max_seqlen)
+                     scale, _bound(max_seqlen))
 
 
 def packed_kernel_names(q, k, v, max_seqlen=None):
@@ -315,7 +331,7 @@ def _chain(q_left, q_right, vs, cu_seqlens, softclamp_value, causal, max_seqlen)
     if ql[0].shape[1] % max(qr[0].shape[1], 1):
         raise ValueError("heads must be divisible by kv_heads")
     cu = _offsets(cu_seqlens, ql[0])
-    opts = (bool(causal), softclamp_value, None, max_seqlen)
+    opts = (bool(causal), softclamp_value, None, _bound(max_seqlen))
     if torch.is_grad_enabled() and any(t.requires_grad for t in (*ql, *qr, *vv)):
         res = _PackedChain.apply(order, shared, cu, opts, *ql, *qr, *vv)
         return res[0], res[1:order], res[order:]

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import struct
 from typing import List, Optional
 
@@ -101,8 +102,10 @@ def _rotate(xs, inv_freq, positions, start, cu_seqlens, angles, interleaved, fac
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, args, *xs):
-        ctx.args = args
-        ctx.like = [(x.shape, x.dtype) for x in xs]
+        inv_freq, positions, ctx.start, cu_seqlens, angles, ctx.interleaved, ctx.factor = args
+        # saved, not kept: changing them in place before the backward is an error then, not another gradient
+        ctx.save_for_backward(inv_freq, positions, cu_seqlens, angles)
+        ctx.dtype = xs[0].dtype
         ctx.set_materialize_grads(False)
         return tuple(_rotate(xs, *args, False))
 
@@ -113,7 +116,9 @@ class _Rotary(torch.autograd.Function):
         live = [i for i, g in enumerate(dys) if g is not None]
         out = [None] * len(dys)
         if live:
-            for i, g in zip(live, _rotate([dys[i].to(ctx.like[i][1]) for i in live], *ctx.args, True)):
+            inv_freq, positions, cu_seqlens, angles = ctx.saved_tensors
+            for i, g in zip(live, _rotate([dys[i].to(ctx.dtype) for i in live], inv_freq, positions, ctx.start, cu_seqlens, angles,
+                                          ctx.interleaved, ctx.factor, True)):
                 out[i] = g
         return (None, *out)
 
@@ -240,7 +245,7 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
                 raise ValueError(f"positions must be [{n}] or [{b}, {n}], got {tuple(positions.shape)}")
             positions = positions.expand(b, -1)
         else:
-            start, positions = int(positions), None
+            start, positions = operator.index(positions), None
     args = (inv_freq, positions, start, cu_seqlens, angles, bool(interleaved), float(attention_factor))
     if b == 0 or n == 0:
         ys = [x.clone() for x in xs]

@@ -11,7 +11,14 @@ accepted path (its rows move together, the length grows) and the next step
 overwrites the rest.
 
 Lengths live on the device and every kernel reads them there, so a step or a
-commit can be captured in a CUDA graph and replayed as the sequences grow.
+commit can be captured in a CUDA graph and replayed as the sequences grow. A full
+cache raises ValueError in eager calls; a replay cannot, there the nodes that have
+no room are padding. A decoder's steps and commits belong on one stream (or
+ordered streams): its rows, lengths and workspace are one state.
+
+16-bit caches with heads of 64 or 128 features run on the tensor cores and split a
+long cache over the GPU; other types and sizes run on CUDA cores, one walk over the
+cache per 8 rows.
 
 Cache layout as ``ChainDecoder``'s (kv-head width):
   keys[t]  [b, g, cap, d]  t = 0 .. order - 1   (q2 .. q_{order + 1})
@@ -56,7 +63,9 @@ class TreeDecoder:
         self.lses = [torch.zeros(batch, kv_heads, capacity, device=device, dtype=torch.float32) for _ in range(order - 1)]
         self.lengths = torch.zeros(batch, device=device, dtype=torch.int32)
         self.device = self.lengths.device
-        self._bound = 0      # no sequence is longer than this
+        self._bound = 0          # no sequence is longer than this ...
+        self._replayed = False   # ... unless a captured commit is replayed
+        self._stepped = False    # rows of a step wait for a commit
         esz = self.keys[0].element_size()
 
         # one argument block per level, in launch order (element order - 1 - t is level t: queries q_{t+1}, keys q_{t+2})
@@ -130,7 +139,7 @@ class TreeDecoder:
                 raise ValueError(f"cache rows {tuple(t.shape)} do not fit {tuple(c.shape)} and lengths up to {longest}")
             c[:, :, :n].copy_(t)
         self.lengths.copy_(lengths)
-        self._bound = longest
+        self._bound, self._stepped = longest, False
 
     def load_packed(self, keys, vals, lses, msgs, cu_seqlens, max_seqlen):
         """The same from a packed prompt batch: keys / vals / msgs [total, g, d], lses [g, total] (what
@@ -150,8 +159,9 @@ class TreeDecoder:
         return self._bound
 
     def _room(self, nodes):
-        if self._bound + nodes > self.cap and not torch.cuda.is_current_stream_capturing() and self.refresh() + nodes > self.cap:
-            raise ValueError("KV cache capacity exceeded")
+        if self._replayed or self._bound + nodes > self.cap:
+            if not torch.cuda.is_current_stream_capturing() and self.refresh() + nodes > self.cap:
+                raise ValueError("KV cache capacity exceeded")
 
     def _parents(self, parents, nodes):
         _require_cuda(parents)
@@ -228,6 +238,7 @@ class TreeDecoder:
                 a.out = a.lse = None
         with _on(self.device):
             check(lib.poly_tree_chain(ap, self._passes, order, _stream(self.device)), "poly_tree_chain")
+        self._stepped = True
         return (out, msgs, lses) if return_rows else out
 
     def commit(self, path, count):
@@ -238,14 +249,16 @@ class TreeDecoder:
             raise TypeError("path and count must be int32 tensors on the decoder's device")
         if path.dim() != 2 or path.shape[0] != self.b or path.shape[1] < 1 or count.shape != (self.b,):
             raise ValueError(f"path must be [{self.b}, n] and count [{self.b}]")
-        if not self._append.nodes:
-            raise ValueError("nothing to commit: no step has been made")
+        if not self._stepped:
+            raise ValueError("nothing to commit: no step since the last commit")
         path, count = path if path.stride(1) == 1 else path.contiguous(), count.contiguous()
         c = self._commit
         c.nodes, c.path_len = self._append.nodes, path.shape[1]
         c.path, c.path_stride, c.count = path.data_ptr(), path.stride(0), count.data_ptr()
         with _on(self.device):
             check(lib.poly_tree_commit(c, _stream(self.device)), "poly_tree_commit")
+        self._stepped = False
+        self._replayed = self._replayed or torch.cuda.is_current_stream_capturing()
         self._bound = min(self.cap, self._bound + min(c.nodes, c.path_len))
 
 

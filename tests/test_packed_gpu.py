@@ -429,6 +429,27 @@ def test_offsets_that_break_the_contract_stay_inside():
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("bound", [60, 100])
+def test_a_wrong_length_bound_gives_nan(bound):
+    import poly_attention_b200 as P
+    lens = [50, 130, 7]
+    q, k, v, do, b, dl = make(lens, 4, 2, 64, torch.bfloat16, bias=True)
+    cu, _ = P.packed_offsets(lens)
+    kw = dict(causal=True, bias=b, max_seqlen=bound)
+    out, lse, epi, lo = P.pass_fwd_packed(q, k, v, cu, epi_mul=q, out_lo=True, **kw)
+    dq, (dv, dr), dk, db = [P.pass_bwd_packed(q, k, v, cu, q, lse, do, want_dbias=True, factors=(k, v), **kw)[i] for i in (0, 2, 1, 3)]
+    for x in (out, lse.T, epi, lo, dq, dk, dv, dr, db.T):
+        assert torch.isnan(x[50:180]).all() and torch.isfinite(x[:50]).all() and torch.isfinite(x[180:]).all()
+
+
+def test_long_rest_and_odd_rows():
+    import poly_attention_b200 as P
+    for dtype, d in ((torch.bfloat16, 64), (torch.float32, 64), (torch.float16, 20)):
+        lens = [40]
+        data = make(lens, 2, 1, d, dtype, rest=3000, bias=True)
+        check_pass(lens, 2, 1, d, dtype, True, rest=3000, data=data)
+
+
 def test_empty():
     import poly_attention_b200 as P
     for dtype in (torch.bfloat16, torch.float32):

@@ -145,6 +145,19 @@ def test_gradient_against_differences():
             assert abs(diff - float(g.reshape(-1)[i])) < 20 * 4 * 2 * 6e-7
 
 
+def test_positions_changed_before_the_backward_are_refused():
+    import poly_attention_b200 as P
+    inv = P.rotary_frequencies(16)[0].cuda()
+    x = torch.randn(1, 2, 5, 16, device="cuda", requires_grad=True)
+    pos = torch.arange(5, device="cuda")
+    y = P.apply_rotary(x, inv, positions=pos)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
+    with pytest.raises(TypeError):
+        P.apply_rotary(x, inv, positions=1.5)
+
+
 def test_strides_alignment_and_empty():
     import poly_attention_b200 as P
     inv = P.rotary_frequencies(16)[0].cuda()

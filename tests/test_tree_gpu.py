@@ -240,7 +240,11 @@ def test_commit_of_bad_paths_stays_inside():
     assert c.dec.lengths.tolist() == [8, 99]
     for x, r in zip(c.dec.keys, rest):
         assert torch.equal(x[0, :, 8:], r)
+    with pytest.raises(ValueError, match="since the last commit"):
+        c.dec.commit(torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.tensor([1, 1], dtype=torch.int32, device="cuda"))
     c.dec.lengths.fill_(5)
+    c.dec.refresh()
+    c.step()
     c.dec.commit(torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.tensor([-3, 3], dtype=torch.int32, device="cuda"))
     assert c.dec.lengths.tolist() == [5, 6]
 
@@ -296,6 +300,11 @@ def test_graph_replays_follow_the_lengths():
         other.dec.commit(path, count)
         assert torch.equal(out, want)
     assert c.dec.lengths.tolist() == [115, 40]
+    # after replays the host looks the lengths up again before an eager step
+    c.dec.lengths.fill_(396)
+    with pytest.raises(ValueError, match="capacity"):
+        c.step()
+    c.dec.lengths.copy_(torch.tensor([115, 40], dtype=torch.int32))
     for x, y in zip(c.dec.keys + c.dec.msgs + c.dec.lses, other.dec.keys + other.dec.msgs + other.dec.lses):
         assert torch.equal(x[0, :, :115], y[0, :, :115]) and torch.equal(x[1, :, :40], y[1, :, :40])
 
@@ -331,7 +340,7 @@ def test_refusals():
             c.dec.step(*args)
     with pytest.raises(ValueError):
         c.dec.step(q, nk, nv, par, out=torch.empty(2, 4, 3, 32, device="cuda", dtype=torch.bfloat16))
-    with pytest.raises(ValueError, match="no step"):
+    with pytest.raises(ValueError, match="nothing to commit"):
         Case(order=2, h=2, g=2, d=64, dtype=torch.bfloat16, lens=[3], parents=[[-1]]).dec.commit(par[:1], torch.ones(1, dtype=torch.int32, device="cuda"))
     c.step()
     one = torch.ones(2, dtype=torch.int32, device="cuda")
