@@ -54,13 +54,14 @@ __global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_
   const int64_t first = packed_at(pk.cu, seq, pk.total);
   const int n = packed_at(pk.cu, seq + 1, pk.total) - (int)first;
   if (n > pk.max_len) {   // the caller's bound is wrong: NaN, once
-    if (NMAX != 64) return;
-    for (int r = 0; r < f.heads / f.kv_heads; ++r)
-      packed_nan_rows(a.dq, (g * (f.heads / f.kv_heads) + r) * a.dq_stride[1], a.dq_stride[2], first, n, D);
-    packed_nan_rows(a.dk, g * a.dk_stride[1], a.dk_stride[2], first, n, D);
-    packed_nan_rows(a.dv, g * a.dv_stride[1], a.dv_stride[2], first, n, D);
-    if (pk.v_left) packed_nan_rows(pk.dv_right, g * pk.dv_right_stride[0], pk.dv_right_stride[1], first, n, D);
-    for (int i = threadIdx.x; a.dbias && i < n; i += blockDim.x) a.dbias[g * a.dbias_stride[1] + first + i] = NAN;
+    if constexpr (NMAX == 64) {
+      for (int r = 0; r < f.heads / f.kv_heads; ++r)
+        packed_nan_rows(a.dq, (g * (f.heads / f.kv_heads) + r) * a.dq_stride[1], a.dq_stride[2], first, n, D);
+      packed_nan_rows(a.dk, g * a.dk_stride[1], a.dk_stride[2], first, n, D);
+      packed_nan_rows(a.dv, g * a.dv_stride[1], a.dv_stride[2], first, n, D);
+      if (pk.v_left) packed_nan_rows(pk.dv_right, g * pk.dv_right_stride[0], pk.dv_right_stride[1], first, n, D);
+      for (int i = threadIdx.x; a.dbias && i < n; i += blockDim.x) a.dbias[g * a.dbias_stride[1] + first + i] = NAN;
+    }
     return;
   }
   if (n <= 0 || (NMAX == 64 ? n > 64 : n <= 64)) return;

@@ -614,7 +614,7 @@ TreeGeom geometry(const PolyTreePass& a, bool may_tc = true) {
   if (!geo.tcgen05) geo.row_blocks = (rows + 16 * wr - 1) / (16 * wr);
   const int64_t ctas = (int64_t)a.batch * a.kv_heads * geo.row_blocks;
   const int keys = geo.tcgen05 ? 128 : kKeys, tiles = (a.capacity + keys - 1) / keys;
-  const int slots = (geo.tcgen05 ? 1 : 2) * sm_count();
+  const int slots = geo.tcgen05 ? sm_count() : sm_count() * 3 / 2;
   const int want = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxSplits, tiles), slots / ctas));
   if (geo.tcgen05) {
     geo.splits = want;

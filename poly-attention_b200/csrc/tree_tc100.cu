@@ -61,7 +61,7 @@ struct Lay {
   static constexpr int kB = kV + S * kTile;              // bias [S][128]; before it, the nodes' ancestors
   static constexpr int kUp = kB + kNodes * 8;
   static constexpr int kBar = kB + S * BN * 4;
-  static constexpr int kNumBars = 1 + 3 * S + 2 + 2 + 2 + 3;
+  static constexpr int kNumBars = 1 + 4 * S + 2 + 2 + 2 + 3;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kAlloc = kMisc + 16 + 1024;
   static_assert(S * BN * 4 >= kNodes * 12 && kAlloc <= 227 * 1024, "shared memory");
@@ -112,13 +112,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = bars;
   uint64_t* k_full = bars + 1;
   uint64_t* v_full = bars + 1 + S;
-  uint64_t* kv_empty = bars + 1 + 2 * S;
-  uint64_t* s_full = bars + 1 + 3 * S;    // [2]
-  uint64_t* p_full = bars + 3 + 3 * S;    // [2]
-  uint64_t* o_done = bars + 5 + 3 * S;    // [2]
-  uint64_t* v_cut = bars + 7 + 3 * S;     // the last value tile arrives here if it has rows behind the tree ...
-  uint64_t* v_clean = bars + 8 + 3 * S;   // ... and is without them here
-  uint64_t* drain = bars + 9 + 3 * S;
+  uint64_t* k_empty = bars + 1 + 2 * S;   // keys: free once their scores are formed
+  uint64_t* v_empty = bars + 1 + 3 * S;   // values and bias: once multiplied
+  uint64_t* s_full = bars + 1 + 4 * S;    // [2]
+  uint64_t* p_full = bars + 3 + 4 * S;    // [2]
+  uint64_t* o_done = bars + 5 + 4 * S;    // [2]
+  uint64_t* v_cut = bars + 7 + 4 * S;     // the last value tile arrives here if it has rows behind the tree ...
+  uint64_t* v_clean = bars + 8 + 4 * S;   // ... and is without them here
+  uint64_t* drain = bars + 9 + 4 * S;
   uint32_t* tmem_slot = (uint32_t*)(smem + L::kMisc);
   volatile int* abort_flag = (volatile int*)(smem + L::kMisc + 4);
   int* err = g_tree_tc_error;
@@ -141,7 +142,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < S; ++s) {
       mbar_init(&k_full[s], 33);
       mbar_init(&v_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[x], 1);
@@ -183,21 +185,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int hf = 0; hf < D / 64; ++hf)
             tma_load_4d(smem + L::kQ + x * L::kTile + hf * kAtom + r * P.tp * 128, &tm_q, q_full, hf * 64, 0,
                         g * R + head0 + x * P.heads_tile + r, b);
-      int issued = 0;
+      int k_issued = 0, issued = 0;
       bool waited = false;
       for (int j = 0; j < n; ++j) {
         const int s = j % S, kb = (t0 + j) * BN;
-        if (j >= S && !mbar_wait(&kv_empty[s], ((j / S) - 1) & 1, abort_flag, err, 81)) break;
+        if (j >= S && !mbar_wait(&k_empty[s], ((j / S) - 1) & 1, abort_flag, err, 81)) break;
         if (!waited && kb + BN > len) {   // rows that the previous kernels of the step write
           pdl_wait();
           waited = true;
         }
         mbar_arrive_expect_tx(&k_full[s], L::kTile);
-        uint64_t* v_bar = j == cut_tile ? v_cut : &v_full[s];
-        mbar_arrive_expect_tx(v_bar, L::kTile);
 #pragma unroll
         for (int hf = 0; hf < D / 64; ++hf)
           tma_load_4d(sK + s * L::kTile + hf * kAtom, &tm_k, &k_full[s], hf * 64, kb, g, b);
+        k_issued = j + 1;
+        if (j >= S && !mbar_wait(&v_empty[s], ((j / S) - 1) & 1, abort_flag, err, 92)) break;
+        uint64_t* v_bar = j == cut_tile ? v_cut : &v_full[s];
+        mbar_arrive_expect_tx(v_bar, L::kTile);
 #pragma unroll
         for (int hf = 0; hf < D / 64; ++hf)
           tma_load_4d(sV + s * L::kTile + hf * kAtom, &tm_v, v_bar, hf * 64, kb, g, b);
@@ -205,8 +209,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (*abort_flag) {
         drain_wait(q_full, 0);
+        for (int j = max(0, k_issued - S); j < k_issued; ++j) drain_wait(&k_full[j % S], (j / S) & 1);
         for (int j = max(0, issued - S); j < issued; ++j) {
-          drain_wait(&k_full[j % S], (j / S) & 1);
           if (j == cut_tile) drain_wait(v_cut, 0);
           else drain_wait(&v_full[j % S], (j / S) & 1);
         }
@@ -230,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      idS, kk > 0);
         }
         mma_commit(&s_full[x]);
+        if (!ROWS2 || x == 1) mma_commit(&k_empty[s]);
         return true;
       };
       bool ok = mbar_wait(q_full, 0, abort_flag, err, 83) && issue_s(0, tile_of(0, 0));
@@ -247,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mma_f16_ts(tmem + 256 + x * D, tmem + x * BN + kk * 8, smem_desc_sw128(va + s * L::kTile + kk * 2048, BN * 128, 1024),
                      idO, i > 0 || kk > 0);
         mma_commit(&o_done[x]);
-        if (!ROWS2 || x == 1) mma_commit(&kv_empty[s]);
+        if (!ROWS2 || x == 1) mma_commit(&v_empty[s]);
         if (i + 1 < items(x)) ok = issue_s(x, tile_of(x, i + 1));
       }
       mma_commit(drain);
@@ -269,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int key = kb + e * 32 + lane;
         x[e] = key >= nkeys ? -INFINITY : bias ? bias[key] : 0.f;
       }
-      if (j >= S && !mbar_wait_warp(&kv_empty[s], ((j / S) - 1) & 1, abort_flag, err, 87)) break;
+      if (j >= S && !mbar_wait_warp(&v_empty[s], ((j / S) - 1) & 1, abort_flag, err, 87)) break;
 #pragma unroll
       for (int e = 0; e < BN / 32; ++e) sB[s * BN + e * 32 + lane] = x[e] <= kDeadBias ? -INFINITY : x[e];
       mbar_arrive(&k_full[s]);
