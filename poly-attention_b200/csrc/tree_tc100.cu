@@ -17,8 +17,11 @@
 // 256 + D. P V(i) precedes S(i + 1) of a warpgroup in issue order, so a full S says
 // that O is at rest and P's columns are free.
 //
-// Bound by HBM up to 256 rows (64 KB a tile of keys and values at d = 128 against about
-// 1.5 us of softmax).
+// Measured (4 sequences of up to 40001 tokens, d 128): 60 rows 67 us, 328 MB, 78 % of
+// the measured copy rate with its combine; 240 rows 121 us, bound by the chain score -
+// softmax - product of a tile, about 3 us, with two tiles in flight. Items of 64 keys
+// with S, P and O side by side in TMEM, so that S(i + 1) is formed during softmax(i),
+// were slower (84 and 159 us): the hand-offs per item cost more than they hid.
 #include <algorithm>
 #include <cstring>
 #include <mutex>
