@@ -58,7 +58,10 @@ struct PackedRow {
 };
 
 template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP, bool PACKED, int NMAX>
-__global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
+// packed, d = 64: bound by latency, so six (three) CTAs an SM. 256 sequences of 14001 tokens: 36 us for those of
+// up to 64 tokens and 33 for the longer ones (39 at two CTAs, which spills nothing); 37 and 38 with O in one piece
+__global__ void __launch_bounds__(2 * NMAX, PACKED && D == 64 ? (NMAX == 64 ? 6 : 3) : 1)
+pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
   constexpr int KS = D / 16, NB = D / 8, CH = D / 8;
   constexpr int KNB = NMAX / 8;   // key n-blocks
   const int bh = blockIdx.x;
@@ -221,75 +224,109 @@ __global__ void __launch_bounds__(2 * NMAX) pass_small_kernel(PolyPassArgs a, co
   l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
   l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
 
-  // O = P V, K steps of 16 keys (P from the score registers, V via ldmatrix.trans)
-  float o[NB][4];
+  if constexpr (PACKED) {
+    // P as operands first, then O 32 features at a time, written as it is done: scores and O
+    // never live together, which leaves registers for more CTAs per SM
+    uint32_t pa[NMAX / 16][4];
 #pragma unroll
-  for (int n = 0; n < NB; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-#pragma unroll
-  for (int kk = 0; kk < NMAX / 16; ++kk) {
-    if (kk * 16 < kp) {
-      const uint32_t pa0 = pk2<T>(s[2 * kk][0], s[2 * kk][1]), pa1 = pk2<T>(s[2 * kk][2], s[2 * kk][3]);
-      const uint32_t pa2 = pk2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
-      const uint32_t pa3 = pk2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
-      const int vkey = kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-#pragma unroll
-      for (int n2 = 0; n2 < NB / 2; ++n2) {
-        uint32_t v0, v1, v2, v3;
-        ldsm4t(sV + soff<D>(vkey, n2 * 2 + (lane >> 4)), v0, v1, v2, v3);
-        mma<T>(o[2 * n2], pa0, pa1, pa2, pa3, v0, v1);
-        mma<T>(o[2 * n2 + 1], pa0, pa1, pa2, pa3, v2, v3);
-      }
+    for (int kk = 0; kk < NMAX / 16; ++kk) {
+      pa[kk][0] = pk2<T>(s[2 * kk][0], s[2 * kk][1]);
+      pa[kk][1] = pk2<T>(s[2 * kk][2], s[2 * kk][3]);
+      pa[kk][2] = pk2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+      pa[kk][3] = pk2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
     }
-  }
-  bool fb0 = false, fb1 = false;   // row took the fully-excluded result
-  // A row whose every key is excluded (only dead keys can do that here) gets
-  // the reference's -finfo.max result: the uniform average over the keys that
-  // are not both causally masked and dead, lse = -FLT_MAX.
-  if (!PACKED && HAS_BIAS && (m0 == -INFINITY || m1 == -INFINITY)) {
+    const float j0 = l0 > 0.f ? 1.f / l0 : 0.f, j1 = l1 > 0.f ? 1.f / l1 : 0.f;
+    const PackedRow<T> row0(a, pk, h, first_row, r0), row1(a, pk, h, first_row, r1);   // used where r0, r1 < nq
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int row = hf ? r1 : r0;
-      if ((hf ? m1 : m0) != -INFINITY) continue;
-      int count = 0;
+    for (int n4 = 0; n4 < NB; n4 += 4) {
+      float o[4][4];
 #pragma unroll
-      for (int n = 0; n < NB; ++n) o[n][2 * hf] = o[n][2 * hf + 1] = 0.f;
-      for (int j = 0; j < nk; ++j) {
-        if (a.causal && j > row && sB[j] == -INFINITY) continue;
-        ++count;
+      for (int n = 0; n < 4; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(sm + kp * D * 2 + soff<D>(j, n) + 4 * tq);
-          const T* e = reinterpret_cast<const T*>(&w);
-          o[n][2 * hf] += to_f32(e[0]);
-          o[n][2 * hf + 1] += to_f32(e[1]);
+      for (int kk = 0; kk < NMAX / 16; ++kk) {
+        if (kk * 16 < kp) {
+          const int vkey = kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+          for (int n2 = 0; n2 < 2; ++n2) {
+            uint32_t v0, v1, v2, v3;
+            ldsm4t(sV + soff<D>(vkey, n4 + n2 * 2 + (lane >> 4)), v0, v1, v2, v3);
+            mma<T>(o[2 * n2], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], v0, v1);
+            mma<T>(o[2 * n2 + 1], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], v2, v3);
+          }
         }
       }
-      if (hf) { l1 = (float)count; fb1 = true; } else { l0 = (float)count; fb0 = true; }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int c = (n4 + n) * 8 + 2 * tq;
+        if (r0 < nq) row0.put(c, o[n][0] * j0, o[n][1] * j0);
+        if (r1 < nq) row1.put(c, o[n][2] * j1, o[n][3] * j1);
+      }
     }
-  }
-  const float j0 = l0 > 0.f ? 1.f / l0 : 0.f, j1 = l1 > 0.f ? 1.f / l1 : 0.f;
-  if constexpr (PACKED) {
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int row = hf ? r1 : r0;
-      if (row >= nq) continue;
-      const PackedRow<T> out(a, pk, h, first_row, row);
-      const float inv = hf ? j1 : j0;
-#pragma unroll
-      for (int n = 0; n < NB; ++n) out.put(n * 8 + 2 * tq, o[n][2 * hf] * inv, o[n][2 * hf + 1] * inv);
+    if (a.lse && tq == 0) {
+      float* lb = a.lse + h * a.lse_stride[1];
+      if (r0 < nq) lb[r0] = l0 == 0.f ? -FLT_MAX : (m0 + __log2f(l0)) * kLn2;
+      if (r1 < nq) lb[r1] = l1 == 0.f ? -FLT_MAX : (m1 + __log2f(l1)) * kLn2;
     }
-  }
-  T* ob = (T*)a.out + b * a.out_stride[0] + h * a.out_stride[1];
+  } else {
+    // O = P V, K steps of 16 keys (P from the score registers, V via ldmatrix.trans)
+    float o[NB][4];
 #pragma unroll
-  for (int n = 0; n < (PACKED ? 0 : NB); ++n) {
-    const int c = n * 8 + 2 * tq;
-    if (r0 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r0 * a.out_stride[2] + c) = pk2<T>(o[n][0] * j0, o[n][1] * j0);
-    if (r1 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r1 * a.out_stride[2] + c) = pk2<T>(o[n][2] * j1, o[n][3] * j1);
-  }
-  if (a.lse && tq == 0) {
-    float* lb = a.lse + b * a.lse_stride[0] + h * a.lse_stride[1];
-    if (r0 < nq) lb[r0] = fb0 || (PACKED && l0 == 0.f) ? -FLT_MAX : (m0 + __log2f(l0)) * kLn2;
-    if (r1 < nq) lb[r1] = fb1 || (PACKED && l1 == 0.f) ? -FLT_MAX : (m1 + __log2f(l1)) * kLn2;
+    for (int n = 0; n < NB; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < NMAX / 16; ++kk) {
+      if (kk * 16 < kp) {
+        const uint32_t pa0 = pk2<T>(s[2 * kk][0], s[2 * kk][1]), pa1 = pk2<T>(s[2 * kk][2], s[2 * kk][3]);
+        const uint32_t pa2 = pk2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+        const uint32_t pa3 = pk2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+        const int vkey = kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+        for (int n2 = 0; n2 < NB / 2; ++n2) {
+          uint32_t v0, v1, v2, v3;
+          ldsm4t(sV + soff<D>(vkey, n2 * 2 + (lane >> 4)), v0, v1, v2, v3);
+          mma<T>(o[2 * n2], pa0, pa1, pa2, pa3, v0, v1);
+          mma<T>(o[2 * n2 + 1], pa0, pa1, pa2, pa3, v2, v3);
+        }
+      }
+    }
+    bool fb0 = false, fb1 = false;   // row took the fully-excluded result
+    // A row whose every key is excluded (only dead keys can do that here) gets
+    // the reference's -finfo.max result: the uniform average over the keys that
+    // are not both causally masked and dead, lse = -FLT_MAX.
+    if (HAS_BIAS && (m0 == -INFINITY || m1 == -INFINITY)) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int row = hf ? r1 : r0;
+        if ((hf ? m1 : m0) != -INFINITY) continue;
+        int count = 0;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) o[n][2 * hf] = o[n][2 * hf + 1] = 0.f;
+        for (int j = 0; j < nk; ++j) {
+          if (a.causal && j > row && sB[j] == -INFINITY) continue;
+          ++count;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(sm + kp * D * 2 + soff<D>(j, n) + 4 * tq);
+            const T* e = reinterpret_cast<const T*>(&w);
+            o[n][2 * hf] += to_f32(e[0]);
+            o[n][2 * hf + 1] += to_f32(e[1]);
+          }
+        }
+        if (hf) { l1 = (float)count; fb1 = true; } else { l0 = (float)count; fb0 = true; }
+      }
+    }
+    const float j0 = l0 > 0.f ? 1.f / l0 : 0.f, j1 = l1 > 0.f ? 1.f / l1 : 0.f;
+    T* ob = (T*)a.out + b * a.out_stride[0] + h * a.out_stride[1];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int c = n * 8 + 2 * tq;
+      if (r0 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r0 * a.out_stride[2] + c) = pk2<T>(o[n][0] * j0, o[n][1] * j0);
+      if (r1 < nq) *reinterpret_cast<uint32_t*>(ob + (int64_t)r1 * a.out_stride[2] + c) = pk2<T>(o[n][2] * j1, o[n][3] * j1);
+    }
+    if (a.lse && tq == 0) {
+      float* lb = a.lse + b * a.lse_stride[0] + h * a.lse_stride[1];
+      if (r0 < nq) lb[r0] = fb0 ? -FLT_MAX : (m0 + __log2f(l0)) * kLn2;
+      if (r1 < nq) lb[r1] = fb1 ? -FLT_MAX : (m1 + __log2f(l1)) * kLn2;
+    }
   }
 }
 
