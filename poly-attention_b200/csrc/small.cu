@@ -57,9 +57,9 @@ struct PackedRow {
   }
 };
 
-template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP, bool PACKED, int NMAX>
 // packed, d = 64: bound by latency, so six (three) CTAs an SM. 256 sequences of 14001 tokens: 36 us for those of
 // up to 64 tokens and 33 for the longer ones (39 at two CTAs, which spills nothing); 37 and 38 with O in one piece
+template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP, bool PACKED, int NMAX>
 __global__ void __launch_bounds__(2 * NMAX, PACKED && D == 64 ? (NMAX == 64 ? 6 : 3) : 1)
 pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
   constexpr int KS = D / 16, NB = D / 8, CH = D / 8;

@@ -106,30 +106,48 @@ __global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_
     fill(sQ, (const T*)f.q + h * f.q_stride[1] + first * f.q_stride[2], f.q_stride[2]);
     fill(sG, gb, a.dout_stride[2]);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    // delta = dout . out - dlse and -log2 lse of every row (8 lanes a row); rows
-    // past the end, and rows that saw no live key, get p = 0
-    for (int r = threadIdx.x >> 3; r < np; r += blockDim.x >> 3) {
-      float s = 0.f, l = -FLT_MAX;
-      if (r < n) {
-        const int64_t at = h * f.out_stride[1] + (first + r) * f.out_stride[2];
-        for (int c = (threadIdx.x & 7) * 8; c < D; c += 64) {
-          const uint4 ov = *reinterpret_cast<const uint4*>((const T*)f.out + at + c);
-          const uint4 gv = *reinterpret_cast<const uint4*>(gb + (int64_t)r * a.dout_stride[2] + c);
-          uint4 lv = make_uint4(0u, 0u, 0u, 0u);
-          if (pk.out_lo) lv = *reinterpret_cast<const uint4*>((const T*)pk.out_lo + at + c);
-          const T *op = reinterpret_cast<const T*>(&ov), *gp = reinterpret_cast<const T*>(&gv), *lp = reinterpret_cast<const T*>(&lv);
+    // delta = dout . out - dlse and -log2 lse of every row, 8 lanes a row and at most four rows a
+    // lane, their loads issued together; rows past the end, and rows that saw no live key, get p = 0
+    {
+      const int row = threadIdx.x >> 3, step = blockDim.x >> 3, lane8 = threadIdx.x & 7;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f}, l[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s += (to_f32(op[e]) + to_f32(lp[e])) * to_f32(gp[e]);
-        }
-        l = f.lse[h * f.lse_stride[1] + first + r];
+      for (int u = 0; u < 4; ++u) {
+        const int r = row + u * step;
+        l[u] = r < n ? f.lse[h * f.lse_stride[1] + first + r] : -FLT_MAX;
       }
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      s += __shfl_xor_sync(0xffffffffu, s, 4);
-      if ((threadIdx.x & 7) == 0) {
-        const bool dead = l <= kDeadBias;
-        sLse[r] = dead ? -INFINITY : -l * kLog2e;
-        sDel[r] = dead ? 0.f : s - (a.dlse ? a.dlse[h * a.dlse_stride[1] + first + r] : 0.f);
+#pragma unroll
+      for (int c = 0; c < D; c += 64) {
+        uint4 ov[4], gv[4], lv[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int r = row + u * step;
+          const int64_t at = h * f.out_stride[1] + (first + r) * f.out_stride[2] + c + lane8 * 8;
+          ov[u] = gv[u] = lv[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < n) {
+            ov[u] = *reinterpret_cast<const uint4*>((const T*)f.out + at);
+            gv[u] = *reinterpret_cast<const uint4*>(gb + (int64_t)r * a.dout_stride[2] + c + lane8 * 8);
+            if (pk.out_lo) lv[u] = *reinterpret_cast<const uint4*>((const T*)pk.out_lo + at);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const T *op = reinterpret_cast<const T*>(&ov[u]), *gp = reinterpret_cast<const T*>(&gv[u]), *lp = reinterpret_cast<const T*>(&lv[u]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[u] += (to_f32(op[e]) + to_f32(lp[e])) * to_f32(gp[e]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int r = row + u * step;
+        sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 1);
+        sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 2);
+        sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 4);
+        if (lane8 == 0 && r < np) {
+          const bool dead = l[u] <= kDeadBias;
+          sLse[r] = dead ? -INFINITY : -l[u] * kLog2e;
+          sDel[r] = dead ? 0.f : sum[u] - (a.dlse ? a.dlse[h * a.dlse_stride[1] + first + r] : 0.f);
+        }
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -267,14 +285,23 @@ __global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_
     const T* vl = pk.v_left ? (const T*)pk.v_left + g * pk.v_left_stride[0] + r * pk.v_left_stride[1] : nullptr;
     const T* vr = pk.v_left ? (const T*)pk.v_right + g * pk.v_right_stride[0] + r * pk.v_right_stride[1] : nullptr;
     T* dr = pk.v_left ? (T*)pk.dv_right + g * pk.dv_right_stride[0] + r * pk.dv_right_stride[1] : nullptr;
+    uint32_t fl[NB], fr[NB];   // the value's factors: loaded before the first store
+    if (vl) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        fl[i] = *reinterpret_cast<const uint32_t*>(vl + i * 8 + 2 * tq);
+        fr[i] = *reinterpret_cast<const uint32_t*>(vr + i * 8 + 2 * tq);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int c = i * 8 + 2 * tq;
       *reinterpret_cast<uint32_t*>(dkp + c) = pk2<T>(dk[i][2 * hf] * f.scale, dk[i][2 * hf + 1] * f.scale);
       const float v0 = dv[i][2 * hf], v1 = dv[i][2 * hf + 1];
       if (vl) {
-        *reinterpret_cast<uint32_t*>(dvp + c) = pk2<T>(v0 * to_f32(vr[c]), v1 * to_f32(vr[c + 1]));
-        *reinterpret_cast<uint32_t*>(dr + c) = pk2<T>(v0 * to_f32(vl[c]), v1 * to_f32(vl[c + 1]));
+        const T *x = reinterpret_cast<const T*>(&fl[i]), *y = reinterpret_cast<const T*>(&fr[i]);
+        *reinterpret_cast<uint32_t*>(dvp + c) = pk2<T>(v0 * to_f32(y[0]), v1 * to_f32(y[1]));
+        *reinterpret_cast<uint32_t*>(dr + c) = pk2<T>(v0 * to_f32(x[0]), v1 * to_f32(x[1]));
       } else {
         *reinterpret_cast<uint32_t*>(dvp + c) = pk2<T>(v0, v1);
       }
