@@ -243,12 +243,15 @@ POLY_API int poly_head_rmsnorm(const PolyHeadNorm* norms, int n, void* stream);
  * rows [cu_seqlens[s], cu_seqlens[s + 1]) and its queries see its own keys only
  * (with causal, those at or before them). cu_seqlens is device memory: int32
  * [seqs + 1], not decreasing, within [0, seq_q]; lengths may be 0, and rows
- * outside every sequence are neither read into a result nor written. Offsets
+ * outside every sequence are neither read into a result nor (without zero_rest)
+ * written. Offsets
  * that break this give wrong rows, never an access outside the tensors.
  * max_len: an upper bound of the lengths if the caller has one, else 0. Up to
  * 128 it selects kernels that hold a whole sequence per CTA; all results of a
- * longer sequence are then NaN (it is not looked at otherwise). Bias, softclamp, grouped heads and the epilogue
- * product as in poly_pass_fwd; masks, v_mul and causal_offset are
+ * longer sequence are then NaN (it is not looked at otherwise). zero_rest: rows
+ * outside the sequences are set to 0 in every output, but for a dq that is
+ * accumulated into (seqs = 0 writes nothing). Bias, softclamp, grouped heads and
+ * the epilogue product as in poly_pass_fwd; masks, v_mul and causal_offset are
  * POLY_EUNSUPPORTED. A row whose every key is dead (bias <= -FLT_MAX / 2) gets
  * out = 0 and lse = -FLT_MAX, and no gradient. epi_out is epi_mul times the
  * unrounded out.

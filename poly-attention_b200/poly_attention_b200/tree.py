@@ -66,6 +66,7 @@ class TreeDecoder:
         self._bound = 0          # no sequence is longer than this ...
         self._replayed = False   # ... unless a captured commit is replayed
         self._stepped = False    # rows of a step wait for a commit
+        self._captured = 0       # nodes of the largest captured step: a replay is a step that the host does not see
         esz = self.keys[0].element_size()
 
         # one argument block per level, in launch order (element order - 1 - t is level t: queries q_{t+1}, keys q_{t+2})
@@ -148,7 +149,7 @@ class TreeDecoder:
             raise ValueError(f"cu_seqlens must hold {self.b} sequences")
         start = cu_seqlens[:-1].long()
         rows = start[:, None] + torch.arange(max_seqlen, device=start.device)
-        rows = rows.clamp_(max=max(keys[0].shape[0] - 1, 0))
+        rows = rows.clamp_(0, max(keys[0].shape[0] - 1, 0))
         pick = lambda t: t[rows].permute(0, 2, 1, 3)   # noqa: E731
         self.load([pick(t) for t in keys], [pick(t) for t in vals], [t.t()[rows].permute(0, 2, 1) for t in lses],
                   [pick(t) for t in msgs], (cu_seqlens[1:] - cu_seqlens[:-1]))
@@ -239,6 +240,8 @@ class TreeDecoder:
         with _on(self.device):
             check(lib.poly_tree_chain(ap, self._passes, order, _stream(self.device)), "poly_tree_chain")
         self._stepped = True
+        if torch.cuda.is_current_stream_capturing():
+            self._captured = max(self._captured, nodes)
         return (out, msgs, lses) if return_rows else out
 
     def commit(self, path, count):
@@ -249,11 +252,11 @@ class TreeDecoder:
             raise TypeError("path and count must be int32 tensors on the decoder's device")
         if path.dim() != 2 or path.shape[0] != self.b or path.shape[1] < 1 or count.shape != (self.b,):
             raise ValueError(f"path must be [{self.b}, n] and count [{self.b}]")
-        if not self._stepped:
+        if not (self._stepped or self._captured):
             raise ValueError("nothing to commit: no step since the last commit")
         path, count = path if path.stride(1) == 1 else path.contiguous(), count.contiguous()
         c = self._commit
-        c.nodes, c.path_len = self._append.nodes, path.shape[1]
+        c.nodes, c.path_len = max(self._append.nodes, self._captured), path.shape[1]
         c.path, c.path_stride, c.count = path.data_ptr(), path.stride(0), count.data_ptr()
         with _on(self.device):
             check(lib.poly_tree_commit(c, _stream(self.device)), "poly_tree_commit")

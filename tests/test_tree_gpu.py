@@ -309,6 +309,33 @@ def test_graph_replays_follow_the_lengths():
         assert torch.equal(x[0, :, :115], y[0, :, :115]) and torch.equal(x[1, :, :40], y[1, :, :40])
 
 
+def test_commits_between_replays_of_a_captured_step():
+    lens, parents = [40, 7], [[-1, 0, 1, 1]] * 2
+    c, other = (Case(order=2, h=4, g=2, d=64, dtype=torch.bfloat16, lens=lens, parents=parents, cap=100) for _ in range(2))
+    c.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.step()
+    path = torch.tensor([[0, 1, 3], [0, 1, 2]], dtype=torch.int32, device="cuda")
+    count = torch.tensor([3, 2], dtype=torch.int32, device="cuda")
+    for _ in range(4):     # the host sees no step between these commits
+        graph.replay()
+        assert torch.equal(out, other.step())
+        c.dec.commit(path, count)
+        other.dec.commit(path, count)
+    assert c.dec.lengths.tolist() == other.dec.lengths.tolist() == [52, 15]
+    for x, y in zip(c.dec.keys + c.dec.msgs, other.dec.keys + other.dec.msgs):
+        assert torch.equal(x[0, :, :52], y[0, :, :52]) and torch.equal(x[1, :, :15], y[1, :, :15])
+
+
+def test_packed_prompts_of_no_tokens():
+    import poly_attention_b200 as P
+    dec = P.TreeDecoder(batch=2, order=2, heads=2, kv_heads=2, dim_head=64, capacity=10, max_nodes=4)
+    none = torch.empty(0, 2, 64, device="cuda", dtype=torch.bfloat16)
+    dec.load_packed([none] * 2, [none], [torch.empty(2, 0, device="cuda")], [none], torch.zeros(3, dtype=torch.int32, device="cuda"), 0)
+    assert dec.lengths.tolist() == [0, 0]
+
+
 def test_two_decoders_on_two_streams():
     rng = random.Random(7)
     cases = [Case(order=3, h=8, g=2, d=128, dtype=torch.bfloat16, lens=[3000 + i, 500], parents=[tree("random", 10, rng)] * 2, seed=i)
