@@ -22,7 +22,6 @@
 // A preprocessing kernel forms delta_i = dout_i . out_i - dlse_i and the
 // log2-domain lse; a final kernel converts the fp32 dq accumulator.
 #include <cstdlib>
-#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -461,13 +460,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, bool SOFTCLAMP, bool HAS_BIAS, bool DB, bool PACKED>
 int launch_bwd_t(const PolyPassBwdArgs& a, const PackedSeqs* seqs, cudaStream_t s) {
   using L = BwdLayout;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(pass_bwd_tc_kernel<T, SOFTCLAMP, HAS_BIAS, DB, PACKED>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
-  });
-  if (attr_err != cudaSuccess) return cuda_status(attr_err, "cudaFuncSetAttribute(bwd tc)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)pass_bwd_tc_kernel<T, SOFTCLAMP, HAS_BIAS, DB, PACKED>, L::kAlloc, done,
+                                "cudaFuncSetAttribute(bwd tc)")) return rc;
   const PolyPassArgs& f = a.fwd;
   BwdWs w = bwd_ws<D, BQ>(a);
   PackedBwdWs pw{};

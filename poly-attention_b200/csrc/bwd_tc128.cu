@@ -20,7 +20,6 @@
 // TMEM (512 columns): S^T 0, dP^T 64, dV 128, dK 256, dQ^T 384, P^T 448.
 #include <algorithm>
 #include <cstdlib>
-#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -450,13 +449,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, bool SOFTCLAMP, bool HAS_BIAS, bool DB, bool PACKED>
 int launch_t(const PolyPassBwdArgs& a, const PackedSeqs* seqs, cudaStream_t s) {
   using L = Layout;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(pass_bwd_tc128_kernel<T, SOFTCLAMP, HAS_BIAS, DB, PACKED>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
-  });
-  if (attr_err != cudaSuccess) return cuda_status(attr_err, "cudaFuncSetAttribute(bwd tc128)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)pass_bwd_tc128_kernel<T, SOFTCLAMP, HAS_BIAS, DB, PACKED>, L::kAlloc, done,
+                                "cudaFuncSetAttribute(bwd tc128)")) return rc;
   const PolyPassArgs& f = a.fwd;
   BwdWs w = bwd_ws<D, BQ>(a);
   PackedBwdWs pw{};

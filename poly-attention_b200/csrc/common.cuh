@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cfloat>
 #include <string>
 
@@ -73,6 +74,19 @@ inline int cuda_status(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return POLY_OK;
   set_error(std::string(what) + ": " + cudaGetErrorString(e));
   return POLY_ECUDA;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device. The setting is the device's,
+// so it is made once for each; `done` is the kernel's mask of devices that have it.
+inline int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done, const char* what) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;   // a device past 64 is set every time
+  if (e == cudaSuccess && !(done.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  }
+  return cuda_status(e, what);
 }
 
 // Launchers implemented in the individual .cu files.

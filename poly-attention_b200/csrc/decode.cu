@@ -586,13 +586,9 @@ void map_strides(const int64_t* st, const PolyPassArgs& a, int64_t* out) {
 template <typename T, int D, int R, bool B, bool V, bool C>
 int launch_one(const PolyPassArgs& a, cudaStream_t s, bool dependent) {
   constexpr int smem = smem_bytes<D, R, V ? 3 : 2>();
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(decode_split_kernel<T, D, R, B, V, C>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  });
-  if (attr_err != cudaSuccess) return cuda_status(attr_err, "cudaFuncSetAttribute(decode)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)decode_split_kernel<T, D, R, B, V, C>, smem, done,
+                                "cudaFuncSetAttribute(decode)")) return rc;
   // resident CTAs per SM x SMs of the current device (cached per device)
   static std::mutex mu;
   static int slots_dev[64] = {0};

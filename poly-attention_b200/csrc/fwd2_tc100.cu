@@ -22,7 +22,6 @@
 // TMA cannot load (16-byte boundary), so warp 2 stages them and drops the dead
 // keys there. Softclamp is done here too (tanh from one ex2 and one reciprocal).
 #include <algorithm>
-#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -551,13 +550,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, bool HAS_BIAS, int D, bool PACKED, bool SOFTCLAMP>
 int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t st) {
   using L2 = L2T<D>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(pass_fwd_tc2_kernel<T, HAS_BIAS, D, PACKED, SOFTCLAMP>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, L2::kAlloc);
-  });
-  if (attr_err != cudaSuccess) return cuda_status(attr_err, "cudaFuncSetAttribute(fwd tc2)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)pass_fwd_tc2_kernel<T, HAS_BIAS, D, PACKED, SOFTCLAMP>, L2::kAlloc, done,
+                                "cudaFuncSetAttribute(fwd tc2)")) return rc;
   CUtensorMap tq, tk, tv, tb;
   int rc = make_map(&tq, a.q, a.dtype, D, a.seq_q, a.heads, a.batch, a.q_stride, BM);
   if (!rc) rc = make_map(&tk, a.k, a.dtype, D, a.seq_k, a.kv_heads, a.batch, a.k_stride, BN);

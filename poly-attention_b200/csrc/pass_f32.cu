@@ -21,7 +21,6 @@
 // the keys (some 5 us a tile) was what the launch waited for (270 -> 231 us an order-2
 // forward of 4099 tokens in 7 sequences, h8 d64).
 #include <cfloat>
-#include <mutex>
 
 #include "common.cuh"
 #include "packed.cuh"
@@ -351,13 +350,9 @@ bool pass_f32_eligible(const PolyPassArgs& a) {
 namespace {
 template <bool B, bool C, bool PACKED>
 int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
-  static std::once_flag once;
-  static cudaError_t err = cudaSuccess;
-  std::call_once(once, [] {
-    err = cudaFuncSetAttribute(pass_f32_kernel<B, C, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (PACKED ? 2 : 1) * kSmem);
-  });
-  if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(f32)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)pass_f32_kernel<B, C, PACKED>, (PACKED ? 2 : 1) * kSmem, done,
+                                "cudaFuncSetAttribute(f32)")) return rc;
   const dim3 grid = PACKED ? dim3(a.heads, a.seq_q / BM + pk->seqs + zero_ctas(*pk)) : dim3((a.seq_q + BM - 1) / BM, a.batch * a.heads);
   pass_f32_kernel<B, C, PACKED><<<grid, PACKED ? 256 : 128, (PACKED ? 2 : 1) * kSmem, s>>>(a, PACKED ? *pk : PackedSeqs{});
   note_launch(1);

@@ -18,7 +18,6 @@
 // Shared memory tiles are 128-byte swizzled (one 64-element atom per row
 // chunk); TMEM holds two S buffers (2 x 128 columns) and O (D columns).
 #include <cstdlib>
-#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -412,13 +411,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 template <int D, typename T, bool HAS_BIAS, bool SOFTCLAMP>
 int launch_fwd_tc_t(const PolyPassArgs& a, cudaStream_t s) {
   using L = FwdLayout<D>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(pass_fwd_tc_kernel<D, T, HAS_BIAS, SOFTCLAMP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    L::kAlloc);
-  });
-  if (attr_err != cudaSuccess) return cuda_status(attr_err, "cudaFuncSetAttribute(fwd tc)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)pass_fwd_tc_kernel<D, T, HAS_BIAS, SOFTCLAMP>, L::kAlloc, done,
+                                "cudaFuncSetAttribute(fwd tc)")) return rc;
   CUtensorMap tq, tk, tv;
   int rc = make_map(&tq, a.q, a.dtype, D, a.seq_q, a.heads, a.batch, a.q_stride, BM);
   if (!rc) rc = make_map(&tk, a.k, a.dtype, D, a.seq_k, a.kv_heads, a.batch, a.k_stride, BN);

@@ -16,7 +16,6 @@
 // of 128 rows, idle in a short sequence, left one CTA per SM.
 #include <algorithm>
 #include <cfloat>
-#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
@@ -333,12 +332,9 @@ pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
 template <typename T, int D, bool B, bool C, bool PACKED, int NMAX>
 int launch_n(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   constexpr int smem = 2 * NMAX * D * 2 + NMAX * 4;
-  static std::once_flag once;
-  static cudaError_t err = cudaSuccess;
-  std::call_once(once, [] {
-    err = cudaFuncSetAttribute(pass_small_kernel<T, D, B, C, PACKED, NMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  });
-  if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(small)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)pass_small_kernel<T, D, B, C, PACKED, NMAX>, smem, done,
+                                "cudaFuncSetAttribute(small)")) return rc;
   const int nq = PACKED ? std::min(pk->max_len, NMAX) : a.seq_q, nk = PACKED ? nq : a.seq_k;
   const int threads = 32 * ((nq + 15) / 16);
   const int kp = (nk + 15) & ~15;

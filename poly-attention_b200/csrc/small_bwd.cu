@@ -17,7 +17,6 @@
 // and 40 KB of shared memory at d = 64.
 #include <algorithm>
 #include <cfloat>
-#include <mutex>
 
 #include "common.cuh"
 #include "mma_sync.cuh"
@@ -312,12 +311,9 @@ __global__ void __launch_bounds__(2 * NMAX, D == 64 ? 256 / NMAX : 1) small_bwd_
 template <typename T, int D, bool B, bool C, int NMAX>
 int launch_n(SmallBwd p, cudaStream_t s) {
   constexpr int row = 4 * D * 2 + NMAX * 2 + 8;   // K, V, Q, dO, dS, lse and delta of one row
-  static std::once_flag once;
-  static cudaError_t err = cudaSuccess;
-  std::call_once(once, [] {
-    err = cudaFuncSetAttribute(small_bwd_kernel<T, D, B, C, NMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, NMAX * row);
-  });
-  if (err != cudaSuccess) return cuda_status(err, "cudaFuncSetAttribute(small bwd)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)small_bwd_kernel<T, D, B, C, NMAX>, NMAX * row, done,
+                                "cudaFuncSetAttribute(small bwd)")) return rc;
   p.rows = std::min(p.rows, NMAX);
   if (NMAX != 64) p.pk.zero.n = 0;   // done by the first launch
   cudaLaunchConfig_t cfg = {};

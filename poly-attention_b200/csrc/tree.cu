@@ -675,12 +675,9 @@ int launch_combine(const PolyTreePass& a, const TreeGeom& geo, cudaStream_t s) {
 template <typename T, int D, int WR, bool VMUL>
 int launch_tree(const PolyTreePass& a, cudaStream_t s, bool dep) {
   using R_ = Ring<D, VMUL ? 3 : 2>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(tree_kernel<T, D, WR, VMUL>, cudaFuncAttributeMaxDynamicSharedMemorySize, R_::kAlloc);
-  });
-  if (attr_err != cudaSuccess) return cuda_status(attr_err, "cudaFuncSetAttribute(tree)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)tree_kernel<T, D, WR, VMUL>, R_::kAlloc, done,
+                                "cudaFuncSetAttribute(tree)")) return rc;
   TreeGeom geo = geometry(a);
   geo.part = (float*)a.workspace;
   CUtensorMap tk, tv, tm;

@@ -24,7 +24,6 @@
 // were slower (84 and 159 us): the hand-offs per item cost more than they hid.
 #include <algorithm>
 #include <cstring>
-#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -463,12 +462,9 @@ int padded_nodes(const PolyTreePass& a) { return (a.nodes + 7) & ~7; }
 template <typename T, int D, bool ROWS2, bool SC>
 int launch_t(const PolyTreePass& a, const TreeGeom& geo, cudaStream_t s, bool dependent) {
   using L = Lay<D, ROWS2>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(tree_tc_kernel<T, D, ROWS2, SC>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
-  });
-  if (attr_err != cudaSuccess) return cuda_status(attr_err, "cudaFuncSetAttribute(tree tc)");
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_smem((const void*)tree_tc_kernel<T, D, ROWS2, SC>, L::kAlloc, done,
+                                "cudaFuncSetAttribute(tree tc)")) return rc;
   CUtensorMap tq, tk, tv;
   int rc = make_map(&tq, a.q, a.dtype, D, a.nodes, a.heads, a.batch, a.q_stride, a.nodes);
   if (!rc) rc = make_map(&tk, a.k, a.dtype, D, a.capacity, a.kv_heads, a.batch, a.k_stride, BN);
