@@ -44,6 +44,29 @@ __device__ __forceinline__ uint32_t pk2(float lo, float hi) {
   else return tc::pack_f16(lo, hi);
 }
 
+// Four 8-feature blocks of a row as a quad of lanes holds them in accumulators (lane t: features 2t, 2t + 1
+// of each) <-> whole blocks (lane t: block t), the form for 16-byte global accesses: 4-byte ones of
+// such fragments cost eight times the wavefronts. Its own inverse; every lane of the warp takes part.
+__device__ __forceinline__ void quad_transpose(uint32_t (&w)[4]) {
+  const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+  const uint32_t a = __shfl_xor_sync(0xffffffffu, odd ? w[0] : w[1], 1), b = __shfl_xor_sync(0xffffffffu, odd ? w[2] : w[3], 1);
+  const uint32_t w0 = odd ? a : w[0], w1 = odd ? w[1] : a, w2 = odd ? b : w[2], w3 = odd ? w[3] : b;
+  const uint32_t c = __shfl_xor_sync(0xffffffffu, high ? w0 : w2, 2), d = __shfl_xor_sync(0xffffffffu, high ? w1 : w3, 2);
+  w[0] = high ? c : w0;
+  w[1] = high ? d : w1;
+  w[2] = high ? w2 : c;
+  w[3] = high ? w3 : d;
+}
+__device__ __forceinline__ void quad_load(uint32_t (&w)[4], const void* block, bool live) {
+  uint4 x = make_uint4(0u, 0u, 0u, 0u);
+  if (live) x = *reinterpret_cast<const uint4*>(block);
+  w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+}
+__device__ __forceinline__ void quad_store(void* block, uint32_t (&w)[4], bool live) {   // w as in accumulators
+  quad_transpose(w);
+  if (live) *reinterpret_cast<uint4*>(block) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // byte offset of 16-byte chunk ch of row r in a [rows][D] 16-bit tile, chunks XOR-swizzled by row
 template <int D>
 __device__ __forceinline__ uint32_t soff(int r, int ch) {

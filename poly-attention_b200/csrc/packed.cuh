@@ -78,7 +78,7 @@ __device__ __forceinline__ void packed_zero_rest(const PackedSeqs& q, int part) 
 // longer than the caller's bound said.
 __device__ __forceinline__ void packed_nan_rows(void* p, int64_t head, int64_t row_stride, int64_t first, int rows, int dim) {
   if (!p) return;
-  for (int i = threadIdx.x; i < rows * dim; i += blockDim.x)
+  for (int64_t i = threadIdx.x; i < (int64_t)rows * dim; i += blockDim.x)
     ((uint16_t*)p)[head + (first + i / dim) * row_stride + i % dim] = 0x7fff;
 }
 

@@ -41,17 +41,31 @@ struct PackedRow {
     eo = a.epi_out ? (T*)a.epi_out + h * a.epi_out_stride[1] + row * a.epi_out_stride[2] : nullptr;
     em = a.epi_out ? (const T*)a.epi_mul + h * a.epi_mul_stride[1] + row * a.epi_mul_stride[2] : nullptr;
   }
-  __device__ __forceinline__ void put(int c, float x, float y) const {   // features c, c + 1
-    const uint32_t w = pk2<T>(x, y);
-    *reinterpret_cast<uint32_t*>(out + c) = w;
+  // Half hf of accumulator fragments o of features c0 .. c0 + 31, times `by`. Every lane of the warp
+  // calls; rows that are not live are not touched.
+  __device__ __forceinline__ void put(int c0, const float (&o)[4][4], int hf, float by, bool live) const {
+    const int c = c0 + 8 * (threadIdx.x & 3);
+    uint32_t w[4], m[4], r[4];
+    if (eo) quad_load(m, em + c, live);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pk2<T>(o[i][2 * hf] * by, o[i][2 * hf + 1] * by);
     if (lo) {
-      const T* e = reinterpret_cast<const T*>(&w);
-      *reinterpret_cast<uint32_t*>(lo + c) = pk2<T>(x - to_f32(e[0]), y - to_f32(e[1]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const T* e = reinterpret_cast<const T*>(&w[i]);
+        r[i] = pk2<T>(o[i][2 * hf] * by - to_f32(e[0]), o[i][2 * hf + 1] * by - to_f32(e[1]));
+      }
+      quad_store(lo + c, r, live);
     }
+    quad_store(out + c, w, live);
     if (eo) {
-      const uint32_t mw = *reinterpret_cast<const uint32_t*>(em + c);
-      const T* m = reinterpret_cast<const T*>(&mw);
-      *reinterpret_cast<uint32_t*>(eo + c) = pk2<T>(x * to_f32(m[0]), y * to_f32(m[1]));
+      quad_transpose(m);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const T* e = reinterpret_cast<const T*>(&m[i]);
+        r[i] = pk2<T>(o[i][2 * hf] * by * to_f32(e[0]), o[i][2 * hf + 1] * by * to_f32(e[1]));
+      }
+      quad_store(eo + c, r, live);
     }
   }
 };
@@ -235,7 +249,7 @@ pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
       pa[kk][3] = pk2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
     }
     const float j0 = l0 > 0.f ? 1.f / l0 : 0.f, j1 = l1 > 0.f ? 1.f / l1 : 0.f;
-    const PackedRow<T> row0(a, pk, h, first_row, r0), row1(a, pk, h, first_row, r1);   // used where r0, r1 < nq
+    const PackedRow<T> row0(a, pk, h, first_row, r0), row1(a, pk, h, first_row, r1);
 #pragma unroll
     for (int n4 = 0; n4 < NB; n4 += 4) {
       float o[4][4];
@@ -254,12 +268,8 @@ pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
           }
         }
       }
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int c = (n4 + n) * 8 + 2 * tq;
-        if (r0 < nq) row0.put(c, o[n][0] * j0, o[n][1] * j0);
-        if (r1 < nq) row1.put(c, o[n][2] * j1, o[n][3] * j1);
-      }
+      row0.put(n4 * 8, o, 0, j0, r0 < nq);
+      row1.put(n4 * 8, o, 1, j1, r1 < nq);
     }
     if (a.lse && tq == 0) {
       float* lb = a.lse + h * a.lse_stride[1];
