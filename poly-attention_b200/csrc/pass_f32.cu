@@ -15,11 +15,13 @@
 //
 // PACKED: sequences laid end to end, one CTA per 64-row slot (packed.cuh) and
 // head; slots are taken from the last to the first, so that of a causal sequence
-// the rows with the most keys start first. Two groups of 4 warps share the CTA's
-// rows, one taking the even key tiles, one the odd, and join at the end: sequences of
-// unequal lengths leave few CTAs for the longest one's last rows, and their walk over
-// the keys (some 5 us a tile) was what the launch waited for (270 -> 231 us an order-2
-// forward of 4099 tokens in 7 sequences, h8 d64).
+// the rows with the most keys start first. Three groups of 4 warps share the CTA's
+// rows, each with every third key tile, and join at the end: sequences of unequal
+// lengths leave few CTAs for the longest one's last rows. Bound by mma.sync's TF32 rate
+// (about 16 cycles an m16n8k8 per SM quarter: 9300 of them take 80 of the 105 us of
+// a pass of 4099 tokens in 7 sequences, h8 d64): a split in four instructions took an
+// order-2 forward from 231 us to 204, more warps (4 groups, 32-key tiles) or
+// an exact order by keys no more than 3% further.
 #include <cfloat>
 
 #include "common.cuh"
@@ -28,8 +30,13 @@
 namespace poly {
 namespace {
 
-constexpr int D = 64, BM = 64, BN = 64, LD = D + 4;   // padded row pitch (floats)
-constexpr int kSmem = (4 * BN * LD + 2 * BN) * 4;      // a two-stage ring: K, V, bias
+constexpr int D = 64, BM = 64, LD = D + 4;   // padded row pitch (floats)
+// groups of 4 warps over the key tiles, keys of a tile, bytes of a group's two-stage ring (K, V, bias)
+template <bool PACKED>
+struct Shape {
+  static constexpr int KG = PACKED ? 3 : 1, BN = 64, kRing = (4 * BN * LD + 2 * BN) * 4;
+  static constexpr int kSmem = KG * kRing;
+};
 
 __device__ __forceinline__ uint32_t tf32(float x) {
   uint32_t r;
@@ -39,6 +46,17 @@ __device__ __forceinline__ uint32_t tf32(float x) {
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
   hi = tf32(x);
   lo = tf32(x - __uint_as_float(hi));
+}
+// x_hi rounded to nearest (ties away) by integer arithmetic, x_lo cut off: 2^-21 of x is lost instead of
+// 2^-22, for 4 instructions instead of about 10. NaN and infinity leave a NaN in lo.
+__device__ __forceinline__ void split_fast(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+}
+template <bool PACKED>
+__device__ __forceinline__ void split_for(float x, uint32_t& hi, uint32_t& lo) {
+  if constexpr (PACKED) split_fast(x, hi, lo);
+  else split(x, hi, lo);
 }
 __device__ __forceinline__ void mma8(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                      uint32_t b1) {
@@ -53,11 +71,11 @@ __device__ __forceinline__ void cp16(uint32_t sa, const void* g, bool ok) {
 }
 
 template <bool HAS_BIAS, bool SOFTCLAMP, bool PACKED>
-__global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassArgs a, const PackedSeqs pk) {
-  constexpr int KG = PACKED ? 2 : 1;   // groups of 4 warps over the key tiles
+__global__ void __launch_bounds__(Shape<PACKED>::KG * 128) pass_f32_kernel(PolyPassArgs a, const PackedSeqs pk) {
+  constexpr int KG = Shape<PACKED>::KG, BN = Shape<PACKED>::BN;
   extern __shared__ __align__(16) float smf[];
   const int kg = PACKED ? threadIdx.x >> 7 : 0, tid = threadIdx.x & 127;
-  float* ring = smf + kg * (kSmem / 4);
+  float* ring = smf + kg * (Shape<PACKED>::kRing / 4);
   float(*sK)[BN * LD] = reinterpret_cast<float(*)[BN * LD]>(ring);
   float(*sV)[BN * LD] = reinterpret_cast<float(*)[BN * LD]>(ring + 2 * BN * LD);
   float(*sB)[BN] = reinterpret_cast<float(*)[BN]>(ring + 4 * BN * LD);
@@ -121,7 +139,7 @@ __global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassAr
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  // Q split into TF32 hi / lo A fragments (rows i0 / i1, K steps of 8)
+  // A fragments of Q split into TF32 hi / lo (rows i0 / i1, K steps of 8)
   uint32_t qh[D / 8][4], ql[D / 8][4];
   {
     const float* qb = (const float*)a.q + b * a.q_stride[0] + h * a.q_stride[1];
@@ -132,7 +150,7 @@ __global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassAr
       const float x[4] = {i0 < nq ? q0[ks * 8 + tq] : 0.f, i1 < nq ? q1[ks * 8 + tq] : 0.f,
                           i0 < nq ? q0[ks * 8 + tq + 4] : 0.f, i1 < nq ? q1[ks * 8 + tq + 4] : 0.f};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) split(x[e], qh[ks][e], ql[ks][e]);
+      for (int e = 0; e < 4; ++e) split_for<PACKED>(x[e], qh[ks][e], ql[ks][e]);
     }
   }
   const float qk = SOFTCLAMP ? a.scale / a.softclamp : a.scale * kLog2e;
@@ -166,8 +184,8 @@ __global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassAr
 #pragma unroll
       for (int nb = 0; nb < BN / 8; ++nb) {
         const float* kr = K + (nb * 8 + gq) * LD + ks * 8 + tq;
-        split(kr[0], bh[nb][0], bl[nb][0]);
-        split(kr[4], bh[nb][1], bl[nb][1]);
+        split_for<PACKED>(kr[0], bh[nb][0], bl[nb][0]);
+        split_for<PACKED>(kr[4], bh[nb][1], bl[nb][1]);
       }
 #pragma unroll
       for (int nb = 0; nb < BN / 8; ++nb) mma8(s[nb], ql[ks][0], ql[ks][1], ql[ks][2], ql[ks][3], bh[nb][0], bh[nb][1]);
@@ -177,6 +195,7 @@ __global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassAr
       for (int nb = 0; nb < BN / 8; ++nb) mma8(s[nb], qh[ks][0], qh[ks][1], qh[ks][2], qh[ks][3], bh[nb][0], bh[nb][1]);
     }
     float mx0 = m0, mx1 = m1;
+    const bool edge = !PACKED || j0 + BN > nk || (a.causal && j0 + BN - 1 > tile * BM);   // keys that some row does not see
 #pragma unroll
     for (int nb = 0; nb < BN / 8; ++nb)
 #pragma unroll
@@ -186,7 +205,7 @@ __global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassAr
         float x = s[nb][e] * qk;
         if (SOFTCLAMP) x = tanhf(x) * sc_out;
         if (HAS_BIAS) x += sB[st][jl];
-        if (j >= nk || (a.causal && j > row)) x = -INFINITY;
+        if (edge && (j >= nk || (a.causal && j > row))) x = -INFINITY;
         s[nb][e] = x;
         if (e < 2) mx0 = fmaxf(mx0, x); else mx1 = fmaxf(mx1, x);
       }
@@ -219,24 +238,28 @@ __global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassAr
 #pragma unroll
     for (int nb = 0; nb < BN / 8; ++nb) {
       uint32_t ph[4], pl[4];
-      split(s[nb][0], ph[0], pl[0]);
-      split(s[nb][2], ph[1], pl[1]);
-      split(s[nb][1], ph[2], pl[2]);
-      split(s[nb][3], ph[3], pl[3]);
+      split_for<PACKED>(s[nb][0], ph[0], pl[0]);
+      split_for<PACKED>(s[nb][2], ph[1], pl[1]);
+      split_for<PACKED>(s[nb][1], ph[2], pl[2]);
+      split_for<PACKED>(s[nb][3], ph[3], pl[3]);
       const float* v0 = V + (nb * 8 + 2 * tq) * LD;
       const float* v1 = v0 + LD;
-      uint32_t bh[D / 8][2], bl[D / 8][2];
+      constexpr int NH = D / 8;   // feature blocks at a time
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        split(v0[n * 8 + gq], bh[n][0], bl[n][0]);
-        split(v1[n * 8 + gq], bh[n][1], bl[n][1]);
+      for (int n0 = 0; n0 < D / 8; n0 += NH) {
+        uint32_t bh[NH][2], bl[NH][2];
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+          split_for<PACKED>(v0[(n0 + n) * 8 + gq], bh[n][0], bl[n][0]);
+          split_for<PACKED>(v1[(n0 + n) * 8 + gq], bh[n][1], bl[n][1]);
+        }
+#pragma unroll
+        for (int n = 0; n < NH; ++n) mma8(o[n0 + n], pl[0], pl[1], pl[2], pl[3], bh[n][0], bh[n][1]);
+#pragma unroll
+        for (int n = 0; n < NH; ++n) mma8(o[n0 + n], ph[0], ph[1], ph[2], ph[3], bl[n][0], bl[n][1]);
+#pragma unroll
+        for (int n = 0; n < NH; ++n) mma8(o[n0 + n], ph[0], ph[1], ph[2], ph[3], bh[n][0], bh[n][1]);
       }
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) mma8(o[n], pl[0], pl[1], pl[2], pl[3], bh[n][0], bh[n][1]);
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) mma8(o[n], ph[0], ph[1], ph[2], ph[3], bl[n][0], bl[n][1]);
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) mma8(o[n], ph[0], ph[1], ph[2], ph[3], bh[n][0], bh[n][1]);
     }
     sync();   // the stage is refilled next iteration
   }
@@ -245,10 +268,11 @@ __global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassAr
   l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
   l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
   if constexpr (PACKED) {
-    // the odd tiles' sums, thread by thread, through shared memory (the rings are idle)
-    float* side = smf + tid;   // [4 D / 8 + 4][128 threads]
+    // the other groups' sums, thread by thread, through shared memory (the rings are idle)
+    constexpr int kSide = (D / 2 + 4) * 128;   // [4 D / 8 + 4][128 threads]
     __syncthreads();
-    if (kg == 1) {
+    if (kg) {
+      float* side = smf + (kg - 1) * kSide + tid;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -259,19 +283,22 @@ __global__ void __launch_bounds__(PACKED ? 256 : 128) pass_f32_kernel(PolyPassAr
       side[(D / 2 + 3) * 128] = l1;
     }
     __syncthreads();
-    if (kg == 1) return;
-    const float y0 = side[D / 2 * 128], y1 = side[(D / 2 + 1) * 128];
-    const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
-    const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
-    const float g0 = y0 == -INFINITY ? 0.f : exp2f(y0 - n0), g1 = y1 == -INFINITY ? 0.f : exp2f(y1 - n1);
-    m0 = n0;
-    m1 = n1;
-    l0 = l0 * f0 + side[(D / 2 + 2) * 128] * g0;
-    l1 = l1 * f1 + side[(D / 2 + 3) * 128] * g1;
+    if (kg) return;
+    for (int k = 0; k < KG - 1; ++k) {
+      const float* side = smf + k * kSide + tid;
+      const float y0 = side[D / 2 * 128], y1 = side[(D / 2 + 1) * 128];
+      const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
+      const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
+      const float g0 = y0 == -INFINITY ? 0.f : exp2f(y0 - n0), g1 = y1 == -INFINITY ? 0.f : exp2f(y1 - n1);
+      m0 = n0;
+      m1 = n1;
+      l0 = l0 * f0 + side[(D / 2 + 2) * 128] * g0;
+      l1 = l1 * f1 + side[(D / 2 + 3) * 128] * g1;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
+      for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] = o[n][e] * (e < 2 ? f0 : f1) + side[(n * 4 + e) * 128] * (e < 2 ? g0 : g1);
+        for (int e = 0; e < 4; ++e) o[n][e] = o[n][e] * (e < 2 ? f0 : f1) + side[(n * 4 + e) * 128] * (e < 2 ? g0 : g1);
+    }
   }
 
   float* ob = (float*)a.out + b * a.out_stride[0] + h * a.out_stride[1];
@@ -350,11 +377,12 @@ bool pass_f32_eligible(const PolyPassArgs& a) {
 namespace {
 template <bool B, bool C, bool PACKED>
 int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
+  using S = Shape<PACKED>;
   static std::atomic<uint64_t> done{0};
-  if (const int rc = allow_smem((const void*)pass_f32_kernel<B, C, PACKED>, (PACKED ? 2 : 1) * kSmem, done,
+  if (const int rc = allow_smem((const void*)pass_f32_kernel<B, C, PACKED>, S::kSmem, done,
                                 "cudaFuncSetAttribute(f32)")) return rc;
   const dim3 grid = PACKED ? dim3(a.heads, a.seq_q / BM + pk->seqs + zero_ctas(*pk)) : dim3((a.seq_q + BM - 1) / BM, a.batch * a.heads);
-  pass_f32_kernel<B, C, PACKED><<<grid, PACKED ? 256 : 128, (PACKED ? 2 : 1) * kSmem, s>>>(a, PACKED ? *pk : PackedSeqs{});
+  pass_f32_kernel<B, C, PACKED><<<grid, S::KG * 128, S::kSmem, s>>>(a, PACKED ? *pk : PackedSeqs{});
   note_launch(1);
   return cuda_status(cudaGetLastError(), "pass_f32 launch");
 }
