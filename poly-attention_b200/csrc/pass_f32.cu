@@ -17,11 +17,11 @@
 // head; slots are taken from the last to the first, so that of a causal sequence
 // the rows with the most keys start first. Three groups of 4 warps share the CTA's
 // rows, each with every third key tile, and join at the end: sequences of unequal
-// lengths leave few CTAs for the longest one's last rows. Bound by mma.sync's TF32 rate
-// (about 16 cycles an m16n8k8 per SM quarter: 9300 of them take 80 of the 105 us of
-// a pass of 4099 tokens in 7 sequences, h8 d64): a split in four instructions took an
-// order-2 forward from 231 us to 204, more warps (4 groups, 32-key tiles) or
-// an exact order by keys no more than 3% further.
+// lengths leave few CTAs for the longest one's last rows. The MMAs alone (8 cycles an
+// m16n8k8 on a quarter of an SM, measured) would take 42 of the 105 us of a pass of
+// 4099 tokens in 7 sequences, h8 d64; the rest is the splits and the softmax that the
+// same warps do between them. A split in four instructions took an order-2 forward from 231 us
+// to 204; a fourth group with 32-key tiles or an exact order by keys gave no more than 3%.
 #include <cfloat>
 
 #include "common.cuh"
@@ -244,22 +244,18 @@ __global__ void __launch_bounds__(Shape<PACKED>::KG * 128) pass_f32_kernel(PolyP
       split_for<PACKED>(s[nb][3], ph[3], pl[3]);
       const float* v0 = V + (nb * 8 + 2 * tq) * LD;
       const float* v1 = v0 + LD;
-      constexpr int NH = D / 8;   // feature blocks at a time
+      uint32_t bh[D / 8][2], bl[D / 8][2];
 #pragma unroll
-      for (int n0 = 0; n0 < D / 8; n0 += NH) {
-        uint32_t bh[NH][2], bl[NH][2];
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
-          split_for<PACKED>(v0[(n0 + n) * 8 + gq], bh[n][0], bl[n][0]);
-          split_for<PACKED>(v1[(n0 + n) * 8 + gq], bh[n][1], bl[n][1]);
-        }
-#pragma unroll
-        for (int n = 0; n < NH; ++n) mma8(o[n0 + n], pl[0], pl[1], pl[2], pl[3], bh[n][0], bh[n][1]);
-#pragma unroll
-        for (int n = 0; n < NH; ++n) mma8(o[n0 + n], ph[0], ph[1], ph[2], ph[3], bl[n][0], bl[n][1]);
-#pragma unroll
-        for (int n = 0; n < NH; ++n) mma8(o[n0 + n], ph[0], ph[1], ph[2], ph[3], bh[n][0], bh[n][1]);
+      for (int n = 0; n < D / 8; ++n) {
+        split_for<PACKED>(v0[n * 8 + gq], bh[n][0], bl[n][0]);
+        split_for<PACKED>(v1[n * 8 + gq], bh[n][1], bl[n][1]);
       }
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) mma8(o[n], pl[0], pl[1], pl[2], pl[3], bh[n][0], bh[n][1]);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) mma8(o[n], ph[0], ph[1], ph[2], ph[3], bl[n][0], bl[n][1]);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) mma8(o[n], ph[0], ph[1], ph[2], ph[3], bh[n][0], bh[n][1]);
     }
     sync();   // the stage is refilled next iteration
   }
