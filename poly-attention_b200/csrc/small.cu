@@ -73,7 +73,7 @@ struct PackedRow {
 // packed, d = 64: bound by latency, so six (three) CTAs an SM. 256 sequences of 14001 tokens: 36 us for those of
 // up to 64 tokens and 33 for the longer ones (39 at two CTAs, which spills nothing); 37 and 38 with O in one piece
 template <typename T, int D, bool HAS_BIAS, bool SOFTCLAMP, bool PACKED, int NMAX>
-__global__ void __launch_bounds__(2 * NMAX, PACKED && D == 64 ? (NMAX == 64 ? 6 : 3) : 1)
+__global__ void __launch_bounds__(2 * NMAX, D != 64 ? 1 : !PACKED ? 2 : NMAX == 64 ? 6 : 3)
 pass_small_kernel(PolyPassArgs a, const PackedSeqs pk) {
   constexpr int KS = D / 16, NB = D / 8, CH = D / 8;
   constexpr int KNB = NMAX / 8;   // key n-blocks
@@ -371,6 +371,8 @@ int launch_t(const PolyPassArgs& a, const PackedSeqs* pk, cudaStream_t s) {
   if (PACKED) {
     const int rc = launch_n<T, D, B, C, true, 64>(a, pk, s);
     if (rc || pk->max_len <= 64) return rc;
+  } else if (a.seq_q <= 64 && a.seq_k <= 64) {
+    return launch_n<T, D, B, C, false, 64>(a, pk, s);
   }
   return launch_n<T, D, B, C, PACKED, kMaxN>(a, pk, s);
 }
