@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(Shape<PACKED>::KG * 128) pass_f32_kernel(PolyP
     if (row >= nq) continue;
     float lse;
     float r[D / 8][2];
-    if (m == -INFINITY) {
+    if (PACKED ? l == 0.f : m == -INFINITY) {   // (a row of NaN scores has no maximum, but a sum)
       // every key excluded: uniform average over keys not both masked and dead
       // (packed rows: zero)
       int count = 0;

@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(PolyPassArgs
     }
     s = keep ? s : -INFINITY;
     const float mn = fmaxf(m, warp_max(s));
-    if (mn == -INFINITY) continue;
+    // (packed: a row of NaN scores has no maximum either, but takes their sum)
+    if (mn == -INFINITY && !(PACKED && __any_sync(0xffffffffu, s != s))) continue;
     const float p = keep ? exp2f((s - mn) * kLog2e) : 0.f;
     const float alpha = exp2f((m - mn) * kLog2e);
     l = l * alpha + warp_sum(p);
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(kWarps * 32) pass_fwd_simt_kernel(PolyPassArgs
   if (!row_ok) return;
 
   float lse;
-  if (m == -INFINITY) {
+  if (PACKED ? l == 0.f : m == -INFINITY) {
     // Every entry excluded: the reference's -finfo.max fill makes the row a
     // uniform average over its keys, except keys that are both masked and
     // dead (-max + -max overflows to -inf there). Packed rows, which have no

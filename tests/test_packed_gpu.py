@@ -131,6 +131,31 @@ def test_a_sequence_of_nan_and_infinity_stays_alone(dtype, d, bound):
     assert torch.equal(out[:100], clean[:100]) and torch.equal(out[130:], clean[130:])
 
 
+# fp32 operands are split into two parts that together have to keep every kind of NaN
+NANS32 = [(torch.float32, 64, None, bits) for bits in (0x7fffffff, 0x7fc00000, -1, 0x7f800001, -0x400000)]
+
+
+@pytest.mark.parametrize("dtype,d,bound,bits", NANS32 + [
+    (torch.bfloat16, 64, None, 0x7fff), (torch.float16, 128, None, 0x7e00), (torch.bfloat16, 64, 80, 0x7fff), (torch.float16, 64, 128, -1),
+    (torch.float16, 128, 128, 0x7e00), (torch.bfloat16, 24, None, 0x7fff), (torch.float32, 24, None, 0x7fffffff)])
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+def test_every_nan_reaches_the_rows_that_see_it(which, dtype, d, bound, bits):
+    import poly_attention_b200 as P
+    t = {name: torch.randn(90, 2, d, device="cuda").to(dtype) for name in "qkv"}
+    t[which].view(torch.int32 if dtype == torch.float32 else torch.int16)[70, 1, 5] = bits
+    cu = torch.tensor([0, 20, 90], dtype=torch.int32, device="cuda")
+    out, lse = P.pass_fwd_packed(t["q"], t["k"], t["v"], cu, causal=True, max_seqlen=bound)
+    bad = out.isnan()
+    assert not bad[:, 0].any() and not bad[:20].any()
+    if which == "q":
+        assert bad[70, 1].all() and bad.sum() == d and lse[1, 70].isnan()
+    elif which == "k":
+        assert bad[70:, 1].all() and not bad[:70].any() and lse[1, 70:].isnan().all()
+    else:
+        # (0 * NaN may reach the rows before it, as in a matrix product)
+        assert bad[70:, 1, 5].all() and not bad[:, :, :5].any() and not bad[:, :, 6:].any() and not lse.isnan().any()
+
+
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64), (torch.float16, 24)])
 @pytest.mark.parametrize("bound", [None, 100])
 def test_dead_keys(dtype, d, bound):
