@@ -353,9 +353,9 @@ __global__ void __launch_bounds__(kThreads, 2) tree_kernel(const __grid_constant
     const int m = rb * 16 * WR + rr;
     if (m >= rows) return;
     const int h = g * R + m % R, node = m / R;
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = L == 0.f ? 0.f : 1.f / L;   // (NaN stays)
     write_row<T>(a, b, h, node, len, c, x * inv, y * inv);
-    if (c == 0) write_lse(a, b, h, node, len, L > 0.f ? (M + __log2f(L)) * kLn2 : -FLT_MAX);
+    if (c == 0) write_lse(a, b, h, node, len, L == 0.f ? -FLT_MAX : (M + __log2f(L)) * kLn2);
   };
   float* crec = rec + kWarps * 16 * RS;   // this CTA's
   const bool local = geo.splits == 1 || geo.cluster;
@@ -421,10 +421,10 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
     }
   }
   const int len = seq_length(a.lengths, b, a.capacity), h = g * R + m % R, node = m / R;
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = L == 0.f ? 0.f : 1.f / L;   // (NaN stays)
 #pragma unroll
   for (int t = 0; t < D / 64; ++t) write_row<T>(a, b, h, node, len, t * 64 + 2 * lane, acc[2 * t] * inv, acc[2 * t + 1] * inv);
-  if (lane == 0) write_lse(a, b, h, node, len, L > 0.f ? (M + __log2f(L)) * kLn2 : -FLT_MAX);
+  if (lane == 0) write_lse(a, b, h, node, len, L == 0.f ? -FLT_MAX : (M + __log2f(L)) * kLn2);
 }
 
 // ---------------------------------------------------------------- CUDA cores
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_simt_kernel(const __grid
     }
     s = keep ? s : -INFINITY;
     const float mn = fmaxf(mx, warp_max(s));
-    if (mn == -INFINITY) continue;
+    if (mn == -INFINITY && !__any_sync(0xffffffffu, s != s)) continue;   // (a row of NaN scores has a sum)
     const float p = keep ? exp2f((s - mn) * kLog2e) : 0.f, f = exp2f((mx - mn) * kLog2e);
     l = l * f + warp_sum(p);
 #pragma unroll
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_simt_kernel(const __grid
     mx = mn;
   }
   if (!ok) return;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int c = lane + 32 * t;
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_simt_kernel(const __grid
     if (a.cache_out && len + node < a.capacity)
       ((T*)a.cache_out)[b * a.cache_out_stride[0] + h * a.cache_out_stride[1] + (int64_t)(len + node) * a.cache_out_stride[2] + c] = x;
   }
-  if (lane == 0) write_lse(a, b, h, node, len, l > 0.f ? mx + logf(l) : -FLT_MAX);
+  if (lane == 0) write_lse(a, b, h, node, len, l == 0.f ? -FLT_MAX : mx + logf(l));
 }
 
 // ---------------------------------------------------------------- rows in and out

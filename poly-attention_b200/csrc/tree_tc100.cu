@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ROWS2 || x == 0) {
       const int rows = R * a.nodes, m = node * R + head;
       float* rec = P.geo.splits > 1 ? P.geo.part + (((int64_t)blockIdx.y * rows + m) * P.geo.splits + split) * kRecord<D> : nullptr;
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;   // (NaN stays)
       const bool keep0 = have && f0 != 0.f && l_run != 0.f, keep1 = !ROWS2 && f1 != 0.f && l_run != 0.f;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           rec[D] = m_run;
           rec[D + 1] = l_run;
         } else {
-          write_lse(a, b, g * R + head, node, len, l_run > 0.f ? (m_run + __log2f(l_run)) * kLn2 : -FLT_MAX);
+          write_lse(a, b, g * R + head, node, len, l_run == 0.f ? -FLT_MAX : (m_run + __log2f(l_run)) * kLn2);
         }
       }
     }

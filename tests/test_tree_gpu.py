@@ -309,6 +309,25 @@ def test_graph_replays_follow_the_lengths():
         assert torch.equal(x[0, :, :115], y[0, :, :115]) and torch.equal(x[1, :, :40], y[1, :, :40])
 
 
+@pytest.mark.parametrize("h,g,d,nodes,longest,dtype", [
+    (4, 4, 64, 5, 300, torch.bfloat16), (16, 4, 128, 16, 300, torch.bfloat16), (8, 2, 128, 60, 9000, torch.float16), (4, 2, 64, 6, 40000, torch.bfloat16),
+    (32, 2, 64, 20, 100, torch.float16), (4, 2, 24, 5, 100, torch.float32), (4, 2, 64, 5, 100, torch.float32)])
+@pytest.mark.parametrize("part", ["row", "feature"])
+def test_nan_of_a_query_stays_and_stays_its_own(h, g, d, nodes, longest, dtype, part):
+    rng = random.Random(3)
+    c = Case(order=2, h=h, g=g, d=d, dtype=dtype, lens=[longest, 3], parents=[tree("random", nodes, rng)] * 2, cap=longest + nodes)
+    want = c.step().clone()
+    c.q1[0, 1, nodes - 1, slice(None) if part == "row" else slice(3, 4)] = float("nan")
+    out, msgs, lses = c.step(return_rows=True)
+    assert out[0, 1, nodes - 1].isnan().all()
+    out[0, 1, nodes - 1] = want[0, 1, nodes - 1]
+    assert torch.equal(out, want)
+    c.nk[0][0, 0, nodes - 1] = float("nan")      # the last node's query of the top level
+    out, msgs, lses = c.step(return_rows=True)
+    assert lses[0][0, 0, nodes - 1].isnan() and msgs[0][0, 0, nodes - 1].isnan().all() and lses[0].isnan().sum() == 1
+    assert out[0, 0, nodes - 1].isnan().all()
+
+
 def test_commits_between_replays_of_a_captured_step():
     lens, parents = [40, 7], [[-1, 0, 1, 1]] * 2
     c, other = (Case(order=2, h=4, g=2, d=64, dtype=torch.bfloat16, lens=lens, parents=parents, cap=100) for _ in range(2))
