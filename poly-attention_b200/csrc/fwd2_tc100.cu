@@ -84,12 +84,6 @@ struct Fwd2Params {
   float sc_in, sc_out;                       // softclamp: x = sc_out tanh(s sc_in)
 };
 
-// tanh(z) = 1 - 2 / (e^2z + 1): off by about 2^-22 of 1, i.e. 2^-22 of the clamp
-// in a score, where tanhf's branches on 128 scores a thread would not fit.
-__device__ __forceinline__ float tanh_ex2(float z) {
-  return 1.f - __fdividef(2.f, ex2(fminf(z * (2.f * kLog2e), 126.f)) + 1.f);
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pk2(float a, float b);
 template <>

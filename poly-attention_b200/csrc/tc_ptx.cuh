@@ -284,6 +284,13 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// tanh(z) = 1 - 2 / (e^2z + 1): off by about 2^-22 of 1, i.e. 2^-22 of the clamp in a softclamped
+// score, where tanhf's branches on 128 scores a thread would not fit. The exponent's upper bound is
+// a comparison, false for a NaN, which stays one (a minimum would drop it: tanh(NaN) = 1).
+__device__ __forceinline__ float tanh_ex2(float z) {
+  const float t = z * (2.f * kLog2e);
+  return 1.f - __fdividef(2.f, ex2(t > 126.f ? 126.f : t) + 1.f);
+}
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   uint32_t r;

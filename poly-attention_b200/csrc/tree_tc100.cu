@@ -85,10 +85,6 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
   while (!mbar_try_wait(bar, parity))
     if (globaltimer() - t0 > kWaitNs) return;
 }
-// tanh(z) = 1 - 2 / (e^2z + 1), off by about 2^-22 of 1
-__device__ __forceinline__ float tanh_ex2(float z) {
-  return 1.f - __fdividef(2.f, ex2(fminf(z * (2.f * kLog2e), 126.f)) + 1.f);
-}
 // bits [0, 64) of: all ones below place -base, then `see` from there on
 __device__ __forceinline__ uint64_t window(uint64_t see, int base) {
   if (base <= -64) return ~0ull;

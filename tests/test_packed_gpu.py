@@ -156,6 +156,30 @@ def test_every_nan_reaches_the_rows_that_see_it(which, dtype, d, bound, bits):
         assert bad[70:, 1, 5].all() and not bad[:, :, :5].any() and not bad[:, :, 6:].any() and not lse.isnan().any()
 
 
+@pytest.mark.parametrize("dtype,d,bound", [
+    (torch.bfloat16, 64, None), (torch.float16, 64, 300), (torch.float16, 128, None), (torch.bfloat16, 128, None),
+    (torch.bfloat16, 64, 80), (torch.float16, 128, 128), (torch.float32, 64, None), (torch.bfloat16, 24, None)])
+@pytest.mark.parametrize("which", ["q", "k"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_every_nan_survives_the_softclamp(which, dtype, d, bound, bias):
+    import poly_attention_b200 as P
+    t = {name: torch.randn(90, 2, d, device="cuda").to(dtype) for name in "qkv"}
+    t[which][70, 1, 5] = float("nan")
+    b = torch.randn(2, 90, device="cuda") if bias else None
+    cu = torch.tensor([0, 20, 90], dtype=torch.int32, device="cuda")
+    out, lse = P.pass_fwd_packed(t["q"], t["k"], t["v"], cu, causal=True, max_seqlen=bound, softclamp=3.0, bias=b)
+    seen = slice(70, 71 if which == "q" else 90)
+    assert out[seen, 1].isnan().all() and lse[1, seen].isnan().all()
+    assert out.isnan().sum() == d * (seen.stop - 70) and lse.isnan().sum() == seen.stop - 70
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bias", [True, False])
+def test_softclamp_fp16(d, bias):
+    check_pass(LENGTHS["ragged"], 4, 2, d, torch.float16, True, bias=bias, clamp=3.0)
+    check_pass(LENGTHS["edges"], 4, 4, d, torch.float16, False, bias=bias, clamp=0.5)
+
+
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64), (torch.float16, 24)])
 @pytest.mark.parametrize("bound", [None, 100])
 def test_dead_keys(dtype, d, bound):

@@ -328,6 +328,39 @@ def test_nan_of_a_query_stays_and_stays_its_own(h, g, d, nodes, longest, dtype, 
     assert out[0, 0, nodes - 1].isnan().all()
 
 
+@pytest.mark.parametrize("h,g,d,nodes,longest", [
+    (16, 4, 128, 16, 300), (8, 2, 128, 60, 9000), (4, 4, 64, 40, 90), (32, 2, 64, 20, 100), (4, 2, 64, 33, 2000), (4, 4, 64, 5, 300)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_nan_of_a_query_survives_the_softclamp(h, g, d, nodes, longest, dtype):
+    rng = random.Random(3)
+    c = Case(order=2, h=h, g=g, d=d, dtype=dtype, lens=[longest, 3], parents=[tree("random", nodes, rng)] * 2, cap=longest + nodes,
+             clamp=4.0)
+    want, _, lses = c.step(return_rows=True)
+    want, lse = want.clone(), lses[0].clone()
+    c.q1[0, 1, nodes - 1, 3] = float("nan")
+    c.nk[0][1, 0, nodes - 1, 3] = float("nan")     # the last node's query of the top level, of the other sequence
+    out, _, lses = c.step(return_rows=True)
+    assert out[0, 1, nodes - 1].isnan().all() and lses[0][1, 0, nodes - 1].isnan()
+    out[0, 1, nodes - 1], lses[0][1, 0, nodes - 1] = want[0, 1, nodes - 1], lse[1, 0, nodes - 1]
+    assert torch.equal(out[0], want[0]) and torch.equal(lses[0], lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("h,g,nodes,lens", [
+    (4, 4, 40, [300, 17]), (4, 2, 33, [4000]), (16, 4, 16, [130, 0, 700]), (32, 2, 20, [100, 2500]), (6, 2, 64, [77]),
+    (2, 2, 36, [50 + i for i in range(80)])])
+def test_softclamp_with_many_rows_a_key(h, g, nodes, lens, d, dtype):
+    """The tcgen05 kernel's own tanh, with bias and dead keys: one and two row tiles, one and several key ranges."""
+    from poly_attention_b200 import _lib
+    rng = random.Random(nodes)
+    c = Case(order=2, h=h, g=g, d=d, dtype=dtype, lens=lens, parents=[tree("random", nodes, rng) for _ in lens], clamp=3.0)
+    for x in c.dec.lses:
+        x[0, :, :lens[0] // 3] = LOW
+    c.check()
+    assert _lib.lib.poly_tree_kernel_name(c.dec._passes[1]) == b"tc100"
+
+
 def test_commits_between_replays_of_a_captured_step():
     lens, parents = [40, 7], [[-1, 0, 1, 1]] * 2
     c, other = (Case(order=2, h=4, g=2, d=64, dtype=torch.bfloat16, lens=lens, parents=parents, cap=100) for _ in range(2))
