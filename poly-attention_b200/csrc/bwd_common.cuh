@@ -22,7 +22,7 @@ struct BwdParams {
   void* dk; int64_t dk_stride[3];
   void* dv; int64_t dv_stride[3];
   float* dbias; int64_t dbias_stride[2];
-  PackedSeqs pk;                 // packed sequences: rows of slots of 128 in dq_acc, lse2 and delta
+  PackedSeqs pk;                 // packed sequences: rows from packed_row0 on in dq_acc, of slots of 128 in lse2 and delta
   const int* order;              // and the slots, longest walk first (NULL: as they are)
 };
 
@@ -176,15 +176,18 @@ __global__ void bwd_dq_convert_kernel(const PolyPassBwdArgs a, const float* dq_a
   *reinterpret_cast<uint4*>(dst) = out;
 }
 
-// Packed sequences. The kernels' row statistics and the dQ accumulator are laid
-// out by slots of 128 rows (packed.cuh), so every sequence owns whole tiles: a
-// tile's rows past its sequence's end add to rows that nobody reads, not to the
-// next sequence's (0 * NaN), and the statistics are 16-byte aligned.
+// Packed sequences. The kernels' row statistics are laid out by slots of 128 rows
+// (packed.cuh), so every sequence owns whole tiles of them, 16-byte aligned. The dQ
+// accumulator, 64 or 128 times as wide, has whole blocks of 8 rows for a sequence: a
+// query tile cut by its sequence's end is added in such blocks, and what its rows past
+// the end hold (0 * NaN) lands in rows that nobody reads. So the workspace follows the
+// tokens: 160000 of them in 20000 sequences, h16 d64, take 1.7 GB (11.5 GB with dQ in slots).
 // One block per 32 rows of a slot and head: delta and -log2 lse as above, and
 // the accumulator's rows as zeros. A row that saw no live key gets p = 0.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) packed_bwd_prep_kernel(const PolyPassBwdArgs a, const PackedSeqs q, float* dq_acc,
-                                                              float* lse2, float* delta, int64_t nq_pad, int* order) {
+                                                              float* lse2, float* delta, int64_t nq_pad, int64_t dq_rows,
+                                                              int* order) {
   if (order) {   // CTA 0 of every head is extra: the first sorts the slots
     if (blockIdx.x == 0) {
       if (blockIdx.y == 0) packed_order<128>(q, q.total / 128 + q.seqs, a.fwd.causal != 0, order);
@@ -207,10 +210,10 @@ __global__ void __launch_bounds__(256) packed_bwd_prep_kernel(const PolyPassBwdA
   const bool live = i < t.len;
   const int64_t row = (int64_t)t.start + i;
   float s = 0.f;
-  float* acc = dq_acc + w * D + sub * (D / 8);
-#pragma unroll
-  for (int v4 = 0; v4 < D / 32; ++v4) *reinterpret_cast<float4*>(acc + v4 * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
   if (live) {
+    float* acc = dq_acc + (h * dq_rows + packed_row0(t) + i) * D + sub * (D / 8);
+#pragma unroll
+    for (int v4 = 0; v4 < D / 32; ++v4) *reinterpret_cast<float4*>(acc + v4 * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
     const T* o = (const T*)a.fwd.out + h * a.fwd.out_stride[1] + row * a.fwd.out_stride[2] + sub * (D / 8);
     const T* g = (const T*)a.dout + h * a.dout_stride[1] + row * a.dout_stride[2] + sub * (D / 8);
     const T* ol = q.out_lo ? (const T*)q.out_lo + h * a.fwd.out_stride[1] + row * a.fwd.out_stride[2] + sub * (D / 8) : nullptr;
@@ -243,10 +246,10 @@ __global__ void __launch_bounds__(256) packed_bwd_prep_kernel(const PolyPassBwdA
   }
 }
 
-// dq = scale * dq_acc (+ dq), from slot rows to the sequences' rows.
+// dq = scale * dq_acc (+ dq), from the accumulator's rows to the sequences'.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) packed_bwd_dq_kernel(const PolyPassBwdArgs a, const PackedSeqs q,
-                                                            const float* dq_acc, int64_t nq_pad) {
+                                                            const float* dq_acc, int64_t dq_rows) {
   PackedTile t;
   const int slot = blockIdx.x >> 2;
   if (!packed_tile<128>(q.cu, q.seqs, q.total, slot, t)) return;
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(256) packed_bwd_dq_kernel(const PolyPassBwdArg
     const int r = r0 + idx / (D / 8), c = (idx % (D / 8)) * 8;
     const int i = t.tile * 128 + r;
     if (i >= t.len) return;
-    const float* src = dq_acc + (h * nq_pad + (int64_t)slot * 128 + r) * D + c;
+    const float* src = dq_acc + (h * dq_rows + packed_row0(t) + i) * D + c;
     T* dst = (T*)a.dq + h * a.dq_stride[1] + ((int64_t)t.start + i) * a.dq_stride[2] + c;
     const float4 x0 = *reinterpret_cast<const float4*>(src);
     const float4 x1 = *reinterpret_cast<const float4*>(src + 4);
@@ -329,14 +332,14 @@ BwdWs bwd_ws(const PolyPassBwdArgs& a) {
   return w;
 }
 
-// The same for packed sequences: nq_pad rows of slots per head.
+// The same for packed sequences: per head, dq_rows rows of dq_acc and nq_pad rows of slots of the statistics.
 struct PackedBwdWs {
   float* dq_acc;
   float* lse2;
   float* delta;
   int* order;
   int slots;
-  int64_t nq_pad;
+  int64_t nq_pad, dq_rows;
   size_t bytes;
 };
 
@@ -344,11 +347,12 @@ inline PackedBwdWs packed_bwd_ws(const PolyPassBwdArgs& a, int seqs) {
   PackedBwdWs w{};
   w.slots = a.fwd.seq_q / 128 + seqs;
   w.nq_pad = (int64_t)w.slots * 128;
-  const size_t rows = (size_t)a.fwd.heads * w.nq_pad;
+  w.dq_rows = packed_rows(a.fwd.seq_q, seqs);
+  const size_t rows = (size_t)a.fwd.heads * w.nq_pad, acc = (size_t)a.fwd.heads * w.dq_rows * a.fwd.head_dim;
   const bool sorted = w.slots <= kOrderSlots;
-  w.bytes = rows * (a.fwd.head_dim + 2) * 4 + (sorted ? (size_t)w.slots * 4 : 0);
+  w.bytes = (acc + rows * 2) * 4 + (sorted ? (size_t)w.slots * 4 : 0);
   w.dq_acc = (float*)a.workspace;
-  w.lse2 = w.dq_acc + rows * a.fwd.head_dim;
+  w.lse2 = w.dq_acc + acc;
   w.delta = w.lse2 + rows;
   w.order = sorted ? (int*)(w.delta + rows) : nullptr;
   return w;

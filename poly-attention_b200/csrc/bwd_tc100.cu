@@ -81,7 +81,7 @@ template <typename T, bool SOFTCLAMP, bool HAS_BIAS, bool DB, bool PACKED>
 __global__ void __launch_bounds__(kThreads, 1)
     pass_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                        const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                       const __grid_constant__ CUtensorMap tm_dq, const BwdParams p) {
+                       const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ CUtensorMap tm_dq_block, const BwdParams p) {
   using L = BwdLayout;
   constexpr int kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   extern __shared__ uint8_t smem_raw[];
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int b = bh / p.kv_heads, kvh = bh - b * p.kv_heads;
   const int rep = p.heads / p.kv_heads;
-  int first = 0, slot_row = 0;   // PACKED: the sequence's first row, and its first row of slots
+  int first = 0, slot_row = 0, dq_row = 0;   // PACKED: the sequence's first row, of slots and of the dQ accumulator
   int seq_k = p.seq_k, q_tiles = p.q_tiles;
   if constexpr (PACKED) {
     PackedTile t;
@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     kt = t.tile;
     first = t.start;
     slot_row = t.slot0 * BK;
+    dq_row = packed_row0(t);
     seq_k = t.len;
     q_tiles = (t.len + BQ - 1) / BQ;
   }
@@ -218,8 +219,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     named_bar_sync(2, 128);
     if (lane == 0 && warp == 4) {
       const int plane = b * p.heads + h;
-      tma_reduce_add_3d(&tm_dq, sDQ, 0, slot_row + qt * BQ, plane);
-      tma_reduce_add_3d(&tm_dq, sDQ + 128 * 128, 32, slot_row + qt * BQ, plane);
+      if (PACKED && q_cut && qt == q_tiles - 1) {
+        for (int i = 0; i < q_cut; i += kRowBlock)
+          for (int hb = 0; hb < 2; ++hb)
+            tma_reduce_add_3d(&tm_dq_block, sDQ + hb * (128 * 128) + i * 128, hb * 32, dq_row + qt * BQ + i, plane);
+      } else {
+        tma_reduce_add_3d(&tm_dq, sDQ, 0, dq_row + qt * BQ, plane);
+        tma_reduce_add_3d(&tm_dq, sDQ + 128 * 128, 32, dq_row + qt * BQ, plane);
+      }
       bulk_commit_group();
     }
     return true;
@@ -473,17 +480,19 @@ int launch_bwd_t(const PolyPassBwdArgs& a, const PackedSeqs* seqs, cudaStream_t 
     w.delta = pw.delta;
     w.nq_pad = (int)pw.nq_pad;
   }
-  CUtensorMap tq, tdo, tk, tv, tdq;
+  CUtensorMap tq, tdo, tk, tv, tdq, tdq_block;
   int rc = make_map(&tq, f.q, f.dtype, D, f.seq_q, f.heads, f.batch, f.q_stride, BQ);
   if (!rc) rc = make_map(&tdo, a.dout, f.dtype, D, f.seq_q, f.heads, f.batch, a.dout_stride, BQ);
   if (!rc) rc = make_map(&tk, f.k, f.dtype, D, f.seq_k, f.kv_heads, f.batch, f.k_stride, BK);
   if (!rc) rc = make_map(&tv, f.v, f.dtype, D, f.seq_k, f.kv_heads, f.batch, f.v_stride, BK);
-  if (!rc) rc = make_map_f32_acc(&tdq, w.dq_acc, PACKED ? w.nq_pad : f.seq_q, f.batch * f.heads);
+  if (!rc) rc = make_map_f32_acc(&tdq, w.dq_acc, PACKED ? (int)pw.dq_rows : f.seq_q, f.batch * f.heads);
+  tdq_block = tdq;
+  if (PACKED && !rc) rc = make_map_f32_acc(&tdq_block, w.dq_acc, (int)pw.dq_rows, f.heads, D, kRowBlock);
   if (rc) return rc;
   const dim3 pgrid((unsigned)(pw.slots * 4), (unsigned)f.heads);
   if (PACKED) {
     packed_bwd_prep_kernel<T, D><<<dim3(pgrid.x + (pw.order ? 1 : 0) + zero_ctas(*seqs), pgrid.y), 256, 0, s>>>(
-        a, *seqs, w.dq_acc, w.lse2, w.delta, pw.nq_pad, pw.order);
+        a, *seqs, w.dq_acc, w.lse2, w.delta, pw.nq_pad, pw.dq_rows, pw.order);
   } else {
     rc = cuda_status(cudaMemsetAsync(w.dq_acc, 0, (size_t)f.batch * f.heads * f.seq_q * D * 4, s), "memset dq acc");
     if (rc) return rc;
@@ -521,9 +530,9 @@ int launch_bwd_t(const PolyPassBwdArgs& a, const PackedSeqs* seqs, cudaStream_t 
   if (PACKED) p.pk = *seqs;
   p.order = pw.order;
   dim3 grid(p.k_tiles * f.batch * f.kv_heads);
-  pass_bwd_tc_kernel<T, SOFTCLAMP, HAS_BIAS, DB, PACKED><<<grid, kThreads, L::kAlloc, s>>>(tq, tdo, tk, tv, tdq, p);
+  pass_bwd_tc_kernel<T, SOFTCLAMP, HAS_BIAS, DB, PACKED><<<grid, kThreads, L::kAlloc, s>>>(tq, tdo, tk, tv, tdq, tdq_block, p);
   if (PACKED) {
-    packed_bwd_dq_kernel<T, D><<<pgrid, 256, 0, s>>>(a, *seqs, w.dq_acc, pw.nq_pad);
+    packed_bwd_dq_kernel<T, D><<<pgrid, 256, 0, s>>>(a, *seqs, w.dq_acc, pw.dq_rows);
   } else {
     const int64_t cthreads = (int64_t)f.batch * f.heads * f.seq_q * (D / 8);
     bwd_dq_convert_kernel<T, D><<<(unsigned)((cthreads + 255) / 256), 256, 0, s>>>(a, w.dq_acc);

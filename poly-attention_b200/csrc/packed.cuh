@@ -50,6 +50,12 @@ __device__ __forceinline__ bool packed_tile(const int* cu, int seqs, int total, 
   return t.tile >= 0 && t.tile * B < t.len;
 }
 
+// The same numbering in blocks of 8 rows, for a workspace in which every sequence has rows of its own: the
+// first row of a tile's sequence, and the rows in all.
+constexpr int kRowBlock = 8;
+__device__ __forceinline__ int packed_row0(const PackedTile& t) { return (t.start / kRowBlock + t.seq) * kRowBlock; }
+inline int64_t packed_rows(int total, int seqs) { return ((int64_t)(total / kRowBlock) + seqs) * kRowBlock; }
+
 // Rows before the first and behind the last sequence of a pass's outputs, as zeros:
 // CTA `part` of kZeroCtas that the pass's first kernel has for it beside its own.
 // Usually there are none, and the CTA reads two offsets and leaves.

@@ -100,6 +100,52 @@ def test_slot_numbering_covers_every_tile_once(block):
                 assert 0 <= t[1] and t[1] + t[2] <= total and t[1] + t[3] * block < total
 
 
+def test_workspace_rows_of_sequences_are_apart():
+    """csrc/packed.cuh's workspace rows restated: a sequence owns 8 (start / 8 + its number) and on, whole blocks of 8."""
+    rng = random.Random(1)
+    for _ in range(2000):
+        lens = [rng.choice([0, 0, 1, 2, 3, 4, 5, rng.randrange(300)]) for _ in range(rng.randrange(1, 40))]
+        cu = [rng.choice([0, 0, 1, 7])]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        total = cu[-1] + rng.choice([0, 0, 1, 50])
+        end = 0
+        for s, n in enumerate(lens):
+            row = 8 * (cu[s] // 8 + s)
+            assert row >= end
+            end = row + (n + 7) // 8 * 8
+        assert end <= 8 * (total // 8 + len(lens))
+        # offsets that break the contract: a sequence's rows lie within [0, total], so its workspace rows stay inside too
+        for s in range(len(lens)):
+            start = rng.randrange(total + 1)
+            n = rng.randrange(total - start + 1)
+            assert 8 * (start // 8 + s) + (n + 7) // 8 * 8 <= 8 * (total // 8 + len(lens))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_backward_workspace_follows_the_tokens(d):
+    """Many short sequences without a length bound: scratch for the tokens, not for a tile of rows a sequence."""
+    from poly_attention_b200 import _lib
+
+    def need(total, seqs):
+        a = _lib.PolyPackedBwdArgs()
+        f = a.bwd.fwd
+        f.batch, f.heads, f.kv_heads, f.seq_q, f.seq_k, f.head_dim, f.scale, f.dtype = 1, 16, 16, total, total, d, 0.1, _lib.POLY_BF16
+        for x, names in ((f, ("q", "k", "v", "out")), (a.bwd, ("dout", "dq", "dk", "dv"))):
+            for name in names:
+                setattr(x, name, 256)
+                st = getattr(x, name + "_stride")
+                st[1], st[2] = d, 16 * d
+        a.cu_seqlens, a.seqs = 256, seqs
+        assert _lib.lib.poly_packed_pass_bwd_kernel_name(a) == b"tc100"
+        return _lib.lib.poly_packed_pass_bwd_workspace_size(a)
+
+    for total, seqs in ((32768, 4096), (160000, 20000), (100, 1), (1, 1), (16411, 12)):
+        # dq of the rows and 8 more a sequence; lse and delta in slots of 128; an order of 8192 slots at most
+        slots = total // 128 + seqs
+        assert need(total, seqs) <= 16 * ((total + 8 * seqs) * d + slots * 128 * 2) * 4 + 4 * 8192
+
+
 @pytest.mark.parametrize("dtype,d,bound,want", [
     (torch.bfloat16, 64, None, ("tc100", "tc100")), (torch.float16, 128, 129, ("tc100", "tc100")),
     (torch.bfloat16, 64, 128, ("small", "small")), (torch.float16, 128, 1, ("small", "small")),

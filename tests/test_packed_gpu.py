@@ -108,6 +108,13 @@ def test_rows_outside_the_sequences(dtype, d, bound):
     check_pass(lens, 4, 2, d, dtype, True, rest=70, data=data, max_seqlen=bound)
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_short_sequences_without_their_bound(dtype, d, causal):
+    """Sequences of no whole 8 rows, beside one another in the backward's dQ accumulator."""
+    check_pass([(i * 7) % 17 for i in range(60)] + [129, 3, 64], 4, 2, d, dtype, causal, bias=True)
+
+
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 64), (torch.float32, 40)])
 @pytest.mark.parametrize("bound", [None, 130])
 def test_a_sequence_of_nan_and_infinity_stays_alone(dtype, d, bound):
