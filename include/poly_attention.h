@@ -421,6 +421,13 @@ typedef struct PolyTreeCommit {
 POLY_API int poly_tree_chain(const PolyTreeAppend* append, const PolyTreePass* passes, int n, void* stream);
 POLY_API size_t poly_tree_workspace_size(const PolyTreePass* pass);
 POLY_API int poly_tree_commit(const PolyTreeCommit* args, void* stream);
+/* The same with the nodes of the last step kept on the device, where a replayed
+ * step counts too: the append writes its nodes to *step_nodes (device int32), and
+ * the commit takes min(*step_nodes, nodes) for nodes, then sets *step_nodes to 0,
+ * so that a second commit keeps nothing. NULL: as above. */
+POLY_API int poly_tree_chain_counted(const PolyTreeAppend* append, const PolyTreePass* passes, int n, int32_t* step_nodes,
+                                     void* stream);
+POLY_API int poly_tree_commit_counted(const PolyTreeCommit* args, int32_t* step_nodes, void* stream);
 /* positions[b][node] = lengths[b] + the node's ancestors in the tree (rotary
  * positions of the drafted tokens); lengths[b] for padding. */
 POLY_API int poly_tree_positions(const int32_t* lengths, const int32_t* parents, int64_t parents_stride, int batch,

@@ -510,12 +510,13 @@ __global__ void __launch_bounds__(kSimtWarps * 32) tree_simt_kernel(const __grid
 // ---------------------------------------------------------------- rows in and out
 // One CTA per (cache, sequence, head): nodes rows of row_bytes.
 template <typename W>
-__global__ void __launch_bounds__(128) tree_append_kernel(const __grid_constant__ PolyTreeAppend a) {
+__global__ void __launch_bounds__(128) tree_append_kernel(const __grid_constant__ PolyTreeAppend a, int32_t* step_nodes) {
   __shared__ uint64_t anc[kNodes];
   __shared__ int up[kNodes];
   const int k = blockIdx.y, b = blockIdx.x / a.kv_heads, g = blockIdx.x - b * a.kv_heads;
   const int len = seq_length(a.lengths, b, a.capacity);
   pdl_launch();
+  if (step_nodes && blockIdx.x == 0 && k == 0 && threadIdx.x == 0) *step_nodes = a.nodes;
   ancestors(a.parents + b * a.parents_stride, a.nodes, a.capacity - len, anc, up);
   const auto& t = a.t[k];
   const char* src = (const char*)t.src + b * t.src_stride[0] + g * t.src_stride[1];
@@ -529,14 +530,19 @@ __global__ void __launch_bounds__(128) tree_append_kernel(const __grid_constant_
   }
 }
 
+// Nodes that a commit may keep: those of the last step, where the step left their number.
+__device__ __forceinline__ int kept_nodes(const PolyTreeCommit& a, const int32_t* step_nodes) {
+  return step_nodes ? min(max(*step_nodes, 0), a.nodes) : a.nodes;
+}
+
 // One CTA per (cache, sequence, head). A thread owns its words of every row and
 // moves them in path order; an entry's row is at or behind its place, so nothing
 // is overwritten before it is read.
 template <typename W>
-__global__ void __launch_bounds__(64) tree_commit_kernel(const __grid_constant__ PolyTreeCommit a) {
+__global__ void __launch_bounds__(64) tree_commit_kernel(const __grid_constant__ PolyTreeCommit a, const int32_t* step_nodes) {
   const int k = blockIdx.y, b = blockIdx.x / a.kv_heads, g = blockIdx.x - b * a.kv_heads;
   const int len = seq_length(a.lengths, b, a.capacity);
-  const int room = min(a.nodes, a.capacity - len), n = min(max(a.count[b], 0), min(room, a.path_len));
+  const int room = min(kept_nodes(a, step_nodes), a.capacity - len), n = min(max(a.count[b], 0), min(room, a.path_len));
   const auto& t = a.t[k];
   char* base = (char*)t.cache + b * t.cache_stride[0] + g * t.cache_stride[1] + (int64_t)len * t.cache_stride[2];
   const int32_t* path = a.path + b * a.path_stride;
@@ -558,11 +564,16 @@ __global__ void __launch_bounds__(kNodes) tree_positions_kernel(const int32_t* l
   if (i < nodes) positions[b * pstride + i] = lengths[b] + (anc[i] ? __popcll(anc[i]) - 1 : 0);
 }
 
-__global__ void tree_lengths_kernel(const __grid_constant__ PolyTreeCommit a) {
-  const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  if (b >= a.batch) return;
-  const int len = seq_length(a.lengths, b, a.capacity);
-  a.lengths[b] = len + min(max(a.count[b], 0), min(min(a.nodes, a.path_len), a.capacity - len));
+// One CTA: every thread has the step's number of nodes before it is taken back.
+__global__ void __launch_bounds__(128) tree_lengths_kernel(const __grid_constant__ PolyTreeCommit a, int32_t* step_nodes) {
+  const int nodes = min(kept_nodes(a, step_nodes), a.path_len);
+  for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+    const int len = seq_length(a.lengths, b, a.capacity);
+    a.lengths[b] = len + min(max(a.count[b], 0), min(nodes, a.capacity - len));
+  }
+  if (!step_nodes) return;
+  __syncthreads();
+  if (threadIdx.x == 0) *step_nodes = 0;
 }
 
 // ---------------------------------------------------------------- host
@@ -741,15 +752,15 @@ int check_append(const PolyTreeAppend& a) {
   return POLY_OK;
 }
 
-int launch_append(const PolyTreeAppend& a, cudaStream_t s) {
+int launch_append(const PolyTreeAppend& a, int32_t* step_nodes, cudaStream_t s) {
   uint64_t bits = (uint64_t)a.row_bytes;
   for (int i = 0; i < a.n; ++i) {
     bits |= (uint64_t)(uintptr_t)a.t[i].src | (uint64_t)(uintptr_t)a.t[i].cache;
     for (int x = 0; x < 3; ++x) bits |= (uint64_t)a.t[i].src_stride[x] | (uint64_t)a.t[i].cache_stride[x];
   }
   const dim3 grid(a.batch * a.kv_heads, a.n);
-  const cudaError_t e = bits & 15 ? launch(tree_append_kernel<uint16_t>, grid, 128, 0, s, false, 0, a)
-                                  : launch(tree_append_kernel<uint4>, grid, 128, 0, s, false, 0, a);
+  const cudaError_t e = bits & 15 ? launch(tree_append_kernel<uint16_t>, grid, 128, 0, s, false, 0, a, step_nodes)
+                                  : launch(tree_append_kernel<uint4>, grid, 128, 0, s, false, 0, a, step_nodes);
   return cuda_status(e, "tree append launch");
 }
 
@@ -787,7 +798,12 @@ size_t poly_tree_workspace_size(const PolyTreePass* a) {
 }
 
 int poly_tree_chain(const PolyTreeAppend* append, const PolyTreePass* passes, int n, void* stream) {
+  return poly_tree_chain_counted(append, passes, n, nullptr, stream);
+}
+
+int poly_tree_chain_counted(const PolyTreeAppend* append, const PolyTreePass* passes, int n, int32_t* step_nodes, void* stream) {
   if (n < 0 || (n > 0 && !passes)) return fail(POLY_EINVAL, "poly_tree_chain: null passes or negative count");
+  if (step_nodes && !append) return fail(POLY_EINVAL, "poly_tree_chain_counted: step_nodes is written by the append");
   int rc;
   if (append && (rc = check_append(*append))) return rc;
   for (int i = 0; i < n; ++i) {
@@ -800,7 +816,7 @@ int poly_tree_chain(const PolyTreeAppend* append, const PolyTreePass* passes, in
   cudaStream_t s = (cudaStream_t)stream;
   bool dep = false;
   if (append && append->n > 0 && append->batch > 0 && append->nodes > 0 && append->capacity > 0) {
-    if ((rc = launch_append(*append, s))) return rc;
+    if ((rc = launch_append(*append, step_nodes, s))) return rc;
     dep = true;
   }
   for (int i = 0; i < n; ++i) {
@@ -822,7 +838,9 @@ int poly_tree_positions(const int32_t* lengths, const int32_t* parents, int64_t 
   return cuda_status(cudaGetLastError(), "tree positions launch");
 }
 
-int poly_tree_commit(const PolyTreeCommit* args, void* stream) {
+int poly_tree_commit(const PolyTreeCommit* args, void* stream) { return poly_tree_commit_counted(args, nullptr, stream); }
+
+int poly_tree_commit_counted(const PolyTreeCommit* args, int32_t* step_nodes, void* stream) {
   if (!args) return fail(POLY_EINVAL, "null tree commit");
   const PolyTreeCommit& a = *args;
   if (a.batch < 0 || a.kv_heads <= 0 || a.nodes < 0 || a.nodes > kNodes || a.path_len < 0 || a.capacity < 0 || a.n < 0 ||
@@ -839,13 +857,13 @@ int poly_tree_commit(const PolyTreeCommit* args, void* stream) {
   cudaStream_t s = (cudaStream_t)stream;
   if (a.n > 0) {
     const dim3 grid(a.batch * a.kv_heads, a.n);
-    if (bits & 3) tree_commit_kernel<uint16_t><<<grid, 64, 0, s>>>(a);
-    else tree_commit_kernel<uint32_t><<<grid, 64, 0, s>>>(a);
+    if (bits & 3) tree_commit_kernel<uint16_t><<<grid, 64, 0, s>>>(a, step_nodes);
+    else tree_commit_kernel<uint32_t><<<grid, 64, 0, s>>>(a, step_nodes);
     note_launch(1);
     const int rc = cuda_status(cudaGetLastError(), "tree commit launch");
     if (rc) return rc;
   }
-  tree_lengths_kernel<<<(a.batch + 127) / 128, 128, 0, s>>>(a);
+  tree_lengths_kernel<<<1, 128, 0, s>>>(a, step_nodes);
   note_launch(1);
   return cuda_status(cudaGetLastError(), "tree lengths launch");
 }

@@ -181,8 +181,11 @@ EXPORTS = {
     "poly_packed_pass_fwd_kernel_name": (ctypes.c_char_p, [ctypes.POINTER(PolyPackedArgs)]),
     "poly_packed_pass_bwd_kernel_name": (ctypes.c_char_p, [ctypes.POINTER(PolyPackedBwdArgs)]),
     "poly_tree_chain": (ctypes.c_int, [ctypes.POINTER(PolyTreeAppend), ctypes.POINTER(PolyTreePass), ctypes.c_int, c_vp]),
+    "poly_tree_chain_counted": (ctypes.c_int, [ctypes.POINTER(PolyTreeAppend), ctypes.POINTER(PolyTreePass), ctypes.c_int, c_vp,
+                                               c_vp]),
     "poly_tree_workspace_size": (c_sz, [ctypes.POINTER(PolyTreePass)]),
     "poly_tree_commit": (ctypes.c_int, [ctypes.POINTER(PolyTreeCommit), c_vp]),
+    "poly_tree_commit_counted": (ctypes.c_int, [ctypes.POINTER(PolyTreeCommit), c_vp, c_vp]),
     "poly_tree_positions": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp]),
     "poly_tree_kernel_name": (ctypes.c_char_p, [ctypes.POINTER(PolyTreePass)]),
     "poly_rotary": (ctypes.c_int, [ctypes.POINTER(PolyRotaryArgs), c_vp]),

@@ -63,10 +63,12 @@ class TreeDecoder:
         self.lses = [torch.zeros(batch, kv_heads, capacity, device=device, dtype=torch.float32) for _ in range(order - 1)]
         self.lengths = torch.zeros(batch, device=device, dtype=torch.int32)
         self.device = self.lengths.device
+        # nodes of the last step that no commit has followed; on the device, as the host does not see a replayed step
+        self._step_nodes = torch.zeros(1, device=self.device, dtype=torch.int32)
         self._bound = 0          # no sequence is longer than this ...
         self._replayed = False   # ... unless a captured commit is replayed
-        self._stepped = False    # rows of a step wait for a commit
-        self._captured = 0       # nodes of the largest captured step: a replay is a step that the host does not see
+        self._stepped = False    # a step of the host waits for a commit
+        self._captured = 0       # nodes of the largest captured step, which may have been replayed
         esz = self.keys[0].element_size()
 
         # one argument block per level, in launch order (element order - 1 - t is level t: queries q_{t+1}, keys q_{t+2})
@@ -140,6 +142,7 @@ class TreeDecoder:
                 raise ValueError(f"cache rows {tuple(t.shape)} do not fit {tuple(c.shape)} and lengths up to {longest}")
             c[:, :, :n].copy_(t)
         self.lengths.copy_(lengths)
+        self._step_nodes.zero_()
         self._bound, self._stepped = longest, False
 
     def load_packed(self, keys, vals, lses, msgs, cu_seqlens, max_seqlen):
@@ -238,7 +241,8 @@ class TreeDecoder:
             else:
                 a.out = a.lse = None
         with _on(self.device):
-            check(lib.poly_tree_chain(ap, self._passes, order, _stream(self.device)), "poly_tree_chain")
+            check(lib.poly_tree_chain_counted(ap, self._passes, order, self._step_nodes.data_ptr(), _stream(self.device)),
+                  "poly_tree_chain")
         self._stepped = True
         if torch.cuda.is_current_stream_capturing():
             self._captured = max(self._captured, nodes)
@@ -246,7 +250,8 @@ class TreeDecoder:
 
     def commit(self, path, count):
         """Keep, of the last step's nodes, path[i, :count[i]] (int32 [b, n], ascending node indices) of each sequence;
-        count int32 [b]. Both stay on the device."""
+        count int32 [b]. Both stay on the device. An entry past those nodes is their last one, a count is at most their
+        number, and a second commit keeps nothing (it raises, unless a captured step may have been replayed since)."""
         _require_cuda(path, count)
         if path.dtype != torch.int32 or count.dtype != torch.int32 or path.device != self.device or count.device != self.device:
             raise TypeError("path and count must be int32 tensors on the decoder's device")
@@ -256,10 +261,10 @@ class TreeDecoder:
             raise ValueError("nothing to commit: no step since the last commit")
         path, count = path if path.stride(1) == 1 else path.contiguous(), count.contiguous()
         c = self._commit
-        c.nodes, c.path_len = max(self._append.nodes, self._captured), path.shape[1]
+        c.nodes, c.path_len = max(self._append.nodes, self._captured), path.shape[1]   # at most; _step_nodes says which
         c.path, c.path_stride, c.count = path.data_ptr(), path.stride(0), count.data_ptr()
         with _on(self.device):
-            check(lib.poly_tree_commit(c, _stream(self.device)), "poly_tree_commit")
+            check(lib.poly_tree_commit_counted(c, self._step_nodes.data_ptr(), _stream(self.device)), "poly_tree_commit")
         self._stepped = False
         self._replayed = self._replayed or torch.cuda.is_current_stream_capturing()
         self._bound = min(self.cap, self._bound + min(c.nodes, c.path_len))

@@ -69,6 +69,16 @@ def test_struct_sizes_and_checks():
     assert lib.poly_tree_positions(None, None, 0, 0, 4, None, 0, None) == _lib.POLY_OK
 
 
+def test_counted_entries_check_like_the_plain_ones():
+    from poly_attention_b200 import _lib
+    lib = _lib.lib
+    assert lib.poly_tree_chain_counted(None, None, 0, 256, None) == _lib.POLY_EINVAL     # nothing would write the count
+    assert lib.poly_tree_chain_counted(None, None, 0, None, None) == _lib.POLY_OK
+    assert lib.poly_tree_chain_counted(_lib.PolyTreeAppend(), None, 0, 256, None) == _lib.POLY_EINVAL
+    assert lib.poly_tree_commit_counted(None, 256, None) == _lib.POLY_EINVAL
+    assert lib.poly_tree_commit_counted(_lib.PolyTreeCommit(), 256, None) == _lib.POLY_EINVAL
+
+
 @pytest.mark.parametrize("kw,err", [(dict(order=1), ValueError), (dict(heads=3), ValueError), (dict(max_nodes=0), ValueError),
                                     (dict(max_nodes=65), ValueError), (dict(order=5), ValueError), (dict(dtype=torch.float64), TypeError),
                                     (dict(dim_head=160), NotImplementedError)])

@@ -380,6 +380,39 @@ def test_commits_between_replays_of_a_captured_step():
         assert torch.equal(x[0, :, :52], y[0, :, :52]) and torch.equal(x[1, :, :15], y[1, :, :15])
 
 
+def test_a_commit_keeps_nodes_of_the_last_step_only():
+    """Captured, replayed and eager steps of different sizes: what follows each is held to its nodes."""
+    c = Case(order=2, h=4, g=2, d=64, dtype=torch.bfloat16, lens=[40, 7], parents=[[-1, 0, 1, 1, 2, 4]] * 2, cap=200)
+    dec = c.dec
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+    two = lambda t: t[:, :, :2].contiguous()   # noqa: E731
+    path = i32([[0, 1, 2, 3, 4, 5], [1, 5, 5, 5, 5, 5]])
+    c.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.step()
+    small = [two(c.q1), [two(t) for t in c.nk], [two(t) for t in c.nv], i32([-1, 0])]
+    graph.replay()
+    dec.step(*small)                      # fewer nodes than the captured step
+    rows = [x[1, :, 8].clone() for x in dec.keys]
+    dec.commit(path, i32([6, 6]))
+    assert dec.lengths.tolist() == [42, 9]
+    for x, row in zip(dec.keys, rows):    # entries 1 and (past the nodes) 5 are both the last node
+        assert torch.equal(x[1, :, 7], row) and torch.equal(x[1, :, 8], row)
+    dec.commit(path, i32([6, 6]))         # no step since
+    assert dec.lengths.tolist() == [42, 9]
+    dec.step(*small)
+    graph.replay()                        # the last step, not seen by the host
+    dec.commit(path, i32([5, 3]))
+    assert dec.lengths.tolist() == [47, 12]
+    graph.replay()
+    n = 3
+    dec.load([x[:, :, :n] for x in dec.keys], [x[:, :, :n] for x in dec.vals], [x[:, :, :n] for x in dec.lses],
+             [x[:, :, :n] for x in dec.msgs], [3, 1])
+    dec.commit(path, i32([2, 2]))         # a load drops the step's rows
+    assert dec.lengths.tolist() == [3, 1]
+
+
 def test_packed_prompts_of_no_tokens():
     import poly_attention_b200 as P
     dec = P.TreeDecoder(batch=2, order=2, heads=2, kv_heads=2, dim_head=64, capacity=10, max_nodes=4)
