@@ -124,7 +124,7 @@ class NPolyAttention(TreeDecoding, Module):
             root_value = kv1[1] if self.has_root_v else None
         qs = tuple(head_rmsnorm(self.q_norms, (q1, *qs_rest)))
         if exists(rotary_pos_emb):
-            qs = tuple(rotate_by_angles(rotary_pos_emb, [q])[0] for q in qs)
+            qs = tuple(rotate_by_angles(rotary_pos_emb, qs))
         q1, qs_rest = qs[0], qs[1:]
 
         inplace = (_inplace_usable(q1.dtype, q1.device, self.dim_head, exists(mask) or any(exists(m) for m in context_mask),

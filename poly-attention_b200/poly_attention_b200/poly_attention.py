@@ -41,10 +41,27 @@ def merge_heads(t):
 
 
 def rotate_by_angles(rotary_pos_emb, qs):
-    """The modules' ``rotary_pos_emb``: angles [n, rot] or [b, n, rot] of the features,
-    both features (2i, 2i + 1) of a pair holding the pair's angle
-    (poly_attention/poly_attention.py:276-277)."""
-    return apply_rotary(qs, angles=rotary_pos_emb[..., ::2])
+    """The modules' ``rotary_pos_emb``: angles [n, rot], [b, n, rot] or [b, 1, n, rot] of the
+    features, both features (2i, 2i + 1) of a pair holding the pair's angle
+    (poly_attention/poly_attention.py:276-277). A tensor of fewer rows takes the last
+    ones, one row of angles serves every row. A pair of two different angles comes out
+    as NaN (the comparison stays on the device); tensors of one length are rotated in one launch."""
+    if rotary_pos_emb.dim() not in (2, 3, 4) or rotary_pos_emb.shape[-1] % 2:
+        raise ValueError(f"rotary_pos_emb must be [n, rot] or [b, n, rot] with an even rot, got {tuple(rotary_pos_emb.shape)}")
+    if rotary_pos_emb.dim() == 4:
+        if rotary_pos_emb.shape[1] != 1:
+            raise ValueError("rotary_pos_emb [b, 1, n, rot] holds the same angles for every head")
+        rotary_pos_emb = rotary_pos_emb.squeeze(1)
+    even, odd = rotary_pos_emb[..., ::2], rotary_pos_emb[..., 1::2]
+    angles = torch.where(even == odd, even, float('nan'))
+    rows = angles.shape[-2]
+    out = list(qs)
+    for n in dict.fromkeys(q.shape[-2] for q in qs):
+        at = [i for i, q in enumerate(qs) if q.shape[-2] == n]
+        mine = angles.expand(*angles.shape[:-2], n, -1) if rows == 1 else angles[..., max(rows - n, 0):, :]
+        for i, y in zip(at, apply_rotary([qs[i] for i in at], angles=mine)):
+            out[i] = y
+    return out
 
 
 class Order2PolyAttention(TreeDecoding, Module):
@@ -151,7 +168,7 @@ class Order2PolyAttention(TreeDecoding, Module):
             q3, v3 = kv2[0], kv2[1]
         q1, q2, q3 = head_rmsnorm(self.q_norms, (q1, q2, q3))
         if exists(rotary_pos_emb):
-            q1, q2, q3 = (rotate_by_angles(rotary_pos_emb, [q])[0] for q in (q1, q2, q3))
+            q1, q2, q3 = rotate_by_angles(rotary_pos_emb, (q1, q2, q3))
 
         cq2, cq3, cv3, clse23, cmsg = cache if has_cache else (None,) * 5
         inplace = (_inplace_usable(q1.dtype, q1.device, self.dim_head,

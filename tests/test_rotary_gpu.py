@@ -254,6 +254,62 @@ def test_module_given_angles_and_gradients():
     assert (gw - gg).abs().max() < 1e-3 * gw.abs().max()
 
 
+def test_a_table_of_angles_serves_tensors_of_every_length():
+    """Its last rows, as the last tokens of a sequence want them; one launch for the tensors of a length."""
+    import poly_attention_b200 as P
+    from poly_attention_b200 import _lib
+    from poly_attention_b200.poly_attention import rotate_by_angles
+    g = torch.Generator(device="cuda").manual_seed(4)
+    table = torch.randn(13, 16, generator=g, device="cuda").repeat_interleave(2, -1)
+    qs = [torch.randn(2, 3, n, 64, generator=g, device="cuda") for n in (5, 13, 1, 5, 13)]
+    for t in (table, table.expand(2, 13, 32), table.expand(2, 1, 13, 32)):
+        before = _lib.lib.poly_launch_count()
+        ys = rotate_by_angles(t, qs)
+        assert _lib.lib.poly_launch_count() == before + 3
+        for q, y in zip(qs, ys):
+            assert torch.equal(y, P.apply_rotary(q, angles=table[13 - q.shape[2]:, ::2].contiguous()))
+    one, = rotate_by_angles(table[:1], qs[:1])
+    assert torch.equal(one, P.apply_rotary(qs[0], angles=table[:1, ::2].expand(5, 16)))
+    for bad in (table[:4], table[..., :31], table.expand(2, 3, 13, 32), table[0]):
+        with pytest.raises(ValueError):
+            rotate_by_angles(bad, qs[:1])
+
+
+def test_pairs_of_two_angles_are_nan():
+    from poly_attention_b200.poly_attention import rotate_by_angles
+    half = torch.arange(1.0, 17.0, device="cuda").expand(5, 16).contiguous()
+    q = torch.randn(2, 3, 5, 64, device="cuda")
+    y, = rotate_by_angles(torch.cat((half, half), -1), [q])         # the half-and-half layout: no pair is equal
+    assert y[..., :32].isnan().all() and torch.equal(y[..., 32:], q[..., 32:])
+
+
+@pytest.mark.parametrize("order", [2, 3])
+def test_given_angles_step_by_step(order):
+    """Cached steps with the angles so far equal the parallel call (fp32: 1e-4, as test_modules_step_by_step_equals_parallel)."""
+    import poly_attention_b200 as P
+    torch.manual_seed(0)
+    kw = dict(dim=64, heads=2, dim_head=64, causal=True)
+    attn = (P.PolyAttention(**kw) if order == 2 else P.NPolyAttention(order=3, **kw)).cuda()
+    x = torch.randn(1, 20, 64, device="cuda")
+    ang = (torch.arange(20, device="cuda")[:, None] * P.rotary_frequencies(64)[0].cuda()).repeat_interleave(2, -1)
+    with torch.no_grad():
+        full = attn(x, rotary_pos_emb=ang)
+        _, cache = attn(x[:, :7], rotary_pos_emb=ang[:7], return_cache=True)
+        for i in range(7, 20):
+            y, cache = attn(x[:, i:i + 1], rotary_pos_emb=ang[:i + 1], cache=cache, return_cache=True)
+            assert (y[:, 0] - full[:, i]).abs().max() < 1e-4
+
+
+def test_given_angles_with_contexts_of_other_lengths():
+    import poly_attention_b200 as P
+    torch.manual_seed(0)
+    attn = P.PolyAttention(dim=64, heads=2, dim_head=64).cuda()
+    x, c1, c2 = (torch.randn(1, n, 64, device="cuda") for n in (4, 9, 13))
+    ang = torch.randn(13, 32, device="cuda").repeat_interleave(2, -1)
+    y = attn(x, context=(c1, c2), rotary_pos_emb=ang)
+    assert y.shape == x.shape and torch.isfinite(y).all()
+
+
 def test_compile_and_opcheck():
     import poly_attention_b200 as P
     attn = P.PolyAttention(dim=64, heads=2, dim_head=64, causal=True, use_rotary_embed=True).cuda().bfloat16()
