@@ -9,6 +9,7 @@ import contextlib
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import PolyMergeArgs, PolyPassArgs, PolyPassBwdArgs, check, lib
@@ -20,6 +21,12 @@ def _require_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError("poly_attention_b200 runs on CUDA tensors only (no CPU implementation)")
+
+
+def _no_tangents(*ts):
+    """Forward-mode derivatives do not exist here: a dual tensor is refused, since its tangent would be lost."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("poly_attention_b200 has no forward-mode derivatives")
 
 
 def _rows(t):

@@ -22,7 +22,7 @@ from torch import nn
 
 from . import _lib
 from ._lib import PolyRotaryArgs, check, lib
-from .ops import _DTYPES, _on, _require_cuda, _stream
+from .ops import _DTYPES, _no_tangents, _on, _require_cuda, _stream
 
 
 def rotary_frequencies(dim, *, theta=10000.0, scaling=None, factor=1.0, original_length=None, fast_turns=32.0,
@@ -202,6 +202,7 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
     _require_cuda(inv_freq, angles, cu_seqlens)
     if (inv_freq is None) == (angles is None):
         raise ValueError("give either inv_freq or angles")
+    _no_tangents(*xs, inv_freq, angles)
     table = inv_freq if angles is None else angles
     if table.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("rotary frequencies and angles have no gradient")

@@ -32,7 +32,7 @@ import torch
 from . import _lib
 from ._lib import PolyTreeAppend, PolyTreeCommit, PolyTreePass, check, lib
 from .head_norm import head_rmsnorm
-from .ops import _DTYPES, _on, _require_cuda, _stream
+from .ops import _DTYPES, _no_tangents, _on, _require_cuda, _stream
 from .packed import check_packed, poly_attention_chain_packed, split_heads, token_rows
 
 
@@ -193,7 +193,8 @@ class TreeDecoder:
 
         q1 [b, h, T, d]; new_keys (order) and new_vals (order - 1) [b, g, T, d]; parents int32 [b, T] (or [T] for
         all). Returns out [b, h, T, d], or with ``return_rows`` (out, msgs, lses): the nodes' messages [b, g, T, d] and
-        log-sum-exps [b, g, T] of every level, in the caches' order. Padding nodes come out as zeros.
+        log-sum-exps [b, g, T] of every level, in the caches' order. Padding nodes come out as zeros. Results carry no
+        gradients, whether or not the inputs require them.
         """
         b, order, g = self.b, self.order, self.g
         news = [*new_keys, *new_vals]
@@ -207,6 +208,7 @@ class TreeDecoder:
                 _require_cuda(t)
             if t.dtype != self.dtype or t.device != self.device:
                 raise TypeError(f"tree tensors must be {self.dtype} on {self.device}")
+        _no_tangents(q1, *news)
         parents = self._parents(parents, nodes)
         self._room(nodes)
         rows = lambda t: t if t.stride(-1) == 1 else t.contiguous()   # noqa: E731

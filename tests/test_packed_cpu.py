@@ -27,6 +27,25 @@ def test_cpu_tensors_are_refused():
         attn(torch.randn(2, 4, 16), cu_seqlens=torch.tensor([0, 4]))
 
 
+def test_dual_tensors_are_refused():
+    """A forward-mode tangent would be lost: the refusal comes before the one of CPU tensors."""
+    import torch.autograd.forward_ad as fw
+
+    import poly_attention_b200 as P
+    cu = torch.tensor([0, 8], dtype=torch.int32)
+    t, inv = torch.randn(8, 2, 64), P.rotary_frequencies(64)[0]
+    with fw.dual_level():
+        d = fw.make_dual(t, torch.ones_like(t))
+        for call in (lambda: P.poly_attention_order2_packed(d, t, t, t, cu),
+                     lambda: P.poly_attention_chain_packed([t, t, t], [t, t, t], [t, d], cu),
+                     lambda: P.pass_fwd_packed(t, t, d, cu),
+                     lambda: P.pass_bwd_packed(t, t, t, cu, t, torch.zeros(2, 8), d)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="CUDA"):       # a plain tensor inside the level is not refused
+            P.pass_fwd_packed(t, t, t, cu)
+
+
 def test_c_entries_check_before_launching():
     from poly_attention_b200 import _lib
     lib = _lib.lib

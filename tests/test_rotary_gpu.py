@@ -194,6 +194,21 @@ def test_refusals():
             P.apply_rotary(args.pop("xs"), args.pop("inv_freq"), **args)
 
 
+def test_dual_tensors_are_refused():
+    import torch.autograd.forward_ad as fw
+
+    import poly_attention_b200 as P
+    inv = P.rotary_frequencies(16)[0].cuda()
+    x = torch.randn(2, 3, 4, 16, device="cuda")
+    with fw.dual_level():
+        for xs in (fw.make_dual(x, x), [x, fw.make_dual(x, x)]):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                P.apply_rotary(xs, inv)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            P.apply_rotary(x, fw.make_dual(inv, inv))
+        P.apply_rotary(x, inv)
+
+
 def test_stream_and_graph():
     import poly_attention_b200 as P
     inv = P.rotary_frequencies(64)[0].cuda()

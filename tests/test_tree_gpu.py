@@ -380,6 +380,15 @@ def test_commits_between_replays_of_a_captured_step():
         assert torch.equal(x[0, :, :52], y[0, :, :52]) and torch.equal(x[1, :, :15], y[1, :, :15])
 
 
+def test_dual_tensors_are_refused():
+    import torch.autograd.forward_ad as fw
+    c = Case(order=2, h=2, g=2, d=64, dtype=torch.bfloat16, lens=[3], parents=[[-1]])
+    with fw.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            c.dec.step(fw.make_dual(c.q1, c.q1), c.nk, c.nv, c.par)
+    c.check()
+
+
 def test_a_commit_keeps_nodes_of_the_last_step_only():
     """Captured, replayed and eager steps of different sizes: what follows each is held to its nodes."""
     c = Case(order=2, h=4, g=2, d=64, dtype=torch.bfloat16, lens=[40, 7], parents=[[-1, 0, 1, 1, 2, 4]] * 2, cap=200)
