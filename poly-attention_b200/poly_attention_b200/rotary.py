@@ -262,22 +262,23 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
 
 
 class RotaryEmbedding(nn.Module):
-    """Rotary positions of one head size; ``freqs`` [dim / 2] is kept in fp32
-    whatever dtype the surrounding module is cast to (a frequency rounded to 16
+    """Rotary positions of one head size; ``freqs`` [dim / 2] is a constant (a buffer:
+    ``requires_grad_`` of a surrounding module does not reach it), kept in fp32
+    whatever dtype that module is cast to (a frequency rounded to 16
     bits is off by whole turns after a few hundred positions)."""
 
     def __init__(self, dim, *, theta=10000.0, interleaved=True, scaling=None, factor=1.0, original_length=None):
         super().__init__()
         freqs, self.attention_factor = rotary_frequencies(dim, theta=theta, scaling=scaling, factor=factor,
                                                           original_length=original_length)
-        self.freqs = nn.Parameter(freqs, requires_grad=False)
+        self.register_buffer("freqs", freqs)
         self.interleaved = interleaved
 
     def _apply(self, fn, recurse=True):
-        keep = self.freqs.detach()
+        keep = self.freqs
         super()._apply(fn, recurse)
         if self.freqs.dtype != torch.float32:
-            self.freqs = nn.Parameter(keep.float().to(self.freqs.device), requires_grad=False)
+            self.freqs = keep.float().to(self.freqs.device)
         return self
 
     def forward(self, xs, positions=0, cu_seqlens=None):

@@ -83,3 +83,15 @@ def test_embedding_keeps_fp32_frequencies():
     assert "rotary_emb.freqs" in attn.state_dict() and not attn.rotary_emb.freqs.requires_grad
     attn = attn.bfloat16().half().double().float()
     assert attn.rotary_emb.freqs.dtype == torch.float32 and torch.equal(attn.rotary_emb.freqs, want)
+
+
+def test_frequencies_of_an_unfrozen_module_stay_constants():
+    import poly_attention_b200 as P
+    attn = P.PolyAttention(dim=32, heads=2, dim_head=16, use_rotary_embed=True)
+    attn.requires_grad_(False).requires_grad_(True)
+    assert not attn.rotary_emb.freqs.requires_grad and all(p.requires_grad for p in attn.parameters())
+    other = P.PolyAttention(dim=32, heads=2, dim_head=16, use_rotary_embed=True)
+    with torch.no_grad():
+        other.rotary_emb.freqs.zero_()
+    other.load_state_dict(attn.state_dict())
+    assert torch.equal(other.rotary_emb.freqs, attn.rotary_emb.freqs)

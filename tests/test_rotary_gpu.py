@@ -325,6 +325,13 @@ def test_given_angles_with_contexts_of_other_lengths():
     assert y.shape == x.shape and torch.isfinite(y).all()
 
 
+def test_an_unfrozen_module_runs():
+    import poly_attention_b200 as P
+    attn = P.PolyAttention(dim=64, heads=2, dim_head=64, causal=True, use_rotary_embed=True).cuda().requires_grad_(True)
+    attn(torch.randn(1, 5, 64, device="cuda")).square().sum().backward()
+    assert all(p.grad is not None for p in attn.parameters())
+
+
 def test_compile_and_opcheck():
     import poly_attention_b200 as P
     attn = P.PolyAttention(dim=64, heads=2, dim_head=64, causal=True, use_rotary_embed=True).cuda().bfloat16()
