@@ -29,6 +29,17 @@ def _no_tangents(*ts):
         raise NotImplementedError("poly_attention_b200 has no forward-mode derivatives")
 
 
+def packed_cu(cu_seqlens, like):
+    """Offsets of packed sequences, checked, as contiguous int32."""
+    _require_cuda(cu_seqlens)
+    if (cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64)
+            or cu_seqlens.device != like.device):
+        raise ValueError("cu_seqlens must be an int32 / int64 tensor [s + 1] on the tensors' device")
+    if cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous():
+        return cu_seqlens
+    return cu_seqlens.to(torch.int32).contiguous()
+
+
 def _rows(t):
     """Make the last dim contiguous; return (tensor, stride3)."""
     if t.stride(-1) != 1:

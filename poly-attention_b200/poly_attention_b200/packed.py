@@ -28,7 +28,7 @@ import torch
 from . import _lib
 from ._lib import PolyPackedArgs, PolyPackedBwdArgs, check, lib
 from .core import _autocast, _sc
-from .ops import _DTYPES, _no_tangents, _on, _require_cuda, _stream
+from .ops import _DTYPES, _no_tangents, _on, _require_cuda, _stream, packed_cu
 
 
 def split_heads(t, split, heads):
@@ -60,16 +60,6 @@ def packed_offsets(lengths, device="cuda"):
     for n in lengths:
         cu.append(cu[-1] + n)
     return torch.tensor(cu, dtype=torch.int32).to(device), max(lengths, default=0)
-
-
-def _offsets(cu_seqlens, like):
-    _require_cuda(cu_seqlens)
-    if (cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64)
-            or cu_seqlens.device != like.device):
-        raise ValueError("cu_seqlens must be an int32 / int64 tensor [s + 1] on the tensors' device")
-    if cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous():
-        return cu_seqlens
-    return cu_seqlens.to(torch.int32).contiguous()
 
 
 def _tensors(q, k, v, *same):
@@ -153,7 +143,7 @@ def pass_fwd_packed(q, k, v, cu_seqlens, *, causal=False, softclamp=None, scale=
     """
     _no_tangents(q, k, v, bias, epi_mul)
     _tensors(q, k, v, bias, epi_mul)
-    cu = _offsets(cu_seqlens, q)
+    cu = packed_cu(cu_seqlens, q)
     if bias is not None:
         bias = _vec(bias, k.shape[1], q.shape[0], "bias")
     if q.shape[1] % max(k.shape[1], 1):
@@ -219,7 +209,7 @@ def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softcl
     values were, dv is the pair of their gradients."""
     _no_tangents(q, k, v, out, lse, dout, bias, dlse, dq, out_lo, *(factors or ()))
     _tensors(q, k, v, out, lse, dout, bias, dlse, dq, out_lo, *(factors or ()))
-    cu = _offsets(cu_seqlens, q)
+    cu = packed_cu(cu_seqlens, q)
     total, h = q.shape[:2]
     g = k.shape[1]
     if h % max(g, 1):
@@ -333,7 +323,7 @@ def _chain(q_left, q_right, vs, cu_seqlens, softclamp_value, causal, max_seqlen)
             raise ValueError("key, value and lower query tensors must share one shape and dtype")
     if ql[0].shape[1] % max(qr[0].shape[1], 1):
         raise ValueError("heads must be divisible by kv_heads")
-    cu = _offsets(cu_seqlens, ql[0])
+    cu = packed_cu(cu_seqlens, ql[0])
     opts = (bool(causal), softclamp_value, None, _bound(max_seqlen))
     if torch.is_grad_enabled() and any(t.requires_grad for t in (*ql, *qr, *vv)):
         res = _PackedChain.apply(order, shared, cu, opts, *ql, *qr, *vv)

@@ -22,7 +22,7 @@ from torch import nn
 
 from . import _lib
 from ._lib import PolyRotaryArgs, check, lib
-from .ops import _DTYPES, _no_tangents, _on, _require_cuda, _stream
+from .ops import _DTYPES, _no_tangents, _on, _require_cuda, _stream, packed_cu
 
 
 def rotary_frequencies(dim, *, theta=10000.0, scaling=None, factor=1.0, original_length=None, fast_turns=32.0,
@@ -169,7 +169,8 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
     in 64 bits, so far positions keep their angle) or ``angles`` (fp32 [n, rot / 2] or
     [b, n, rot / 2]). ``positions`` is the first row's position (rows count up from
     it), or an int32 / int64 tensor [n] or [b, n]; with ``cu_seqlens`` (int32 [s + 1],
-    packed sequences, batch 1) every sequence counts from 0. ``interleaved`` pairs
+    packed sequences, batch 1) every sequence counts from 0, and rows behind the last
+    count on. ``interleaved`` pairs
     features (2i, 2i + 1), otherwise (i, i + rot / 2). ``attention_factor``
     multiplies cos and sin. Gradients reach xs; frequencies and angles get none.
     """
@@ -232,9 +233,11 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
         if cu_seqlens is not None:
             if torch.is_tensor(positions) or positions != 0:
                 raise ValueError("positions and cu_seqlens exclude one another")
-            if b != 1 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2 or cu_seqlens.device != x0.device:
-                raise ValueError("cu_seqlens must be int32 [s + 1] on the tensors' device, with batch 1")
-            cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+            if b != 1:
+                raise ValueError("packed sequences (cu_seqlens) are rotated with batch 1")
+            cu_seqlens = packed_cu(cu_seqlens, x0)
+            if cu_seqlens.shape[0] == 1:
+                cu_seqlens = None          # no sequence: rows behind the last one count on, here from 0
             positions = None
         elif torch.is_tensor(positions):
             _require_cuda(positions)

@@ -158,6 +158,27 @@ def test_positions_changed_before_the_backward_are_refused():
         P.apply_rotary(x, inv, positions=1.5)
 
 
+def test_offsets_as_the_packed_passes_take_them():
+    """No sequence at all is a batch, offsets that are no integers are not."""
+    import poly_attention_b200 as P
+    inv = P.rotary_frequencies(16)[0].cuda()
+    x = torch.randn(5, 2, 16, device="cuda")
+    none, longest = P.packed_offsets([])
+    assert P.apply_rotary(x[:0], inv, cu_seqlens=none).shape == (0, 2, 16)
+    assert torch.equal(P.apply_rotary(x, inv, cu_seqlens=none), P.apply_rotary(x, inv))
+    assert torch.equal(P.apply_rotary(x, inv, cu_seqlens=torch.tensor([0, 2, 5], device="cuda")),
+                       P.apply_rotary(x, inv, cu_seqlens=torch.tensor([0, 2, 5], device="cuda", dtype=torch.int32)))
+    for bad in (torch.tensor([0.0, 5.0], device="cuda"), torch.zeros(2, 2, dtype=torch.int32, device="cuda"),
+                torch.empty(0, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError):
+            P.apply_rotary(x, inv, cu_seqlens=bad)
+    for kw in (dict(use_rotary_embed=True), {}):
+        attn = P.PolyAttention(dim=64, heads=2, dim_head=64, causal=True, **kw).cuda()
+        for n in (0, 3):
+            y = attn(torch.randn(1, n, 64, device="cuda"), cu_seqlens=none, max_seqlen=longest)
+            assert y.shape == (1, n, 64)
+
+
 def test_strides_alignment_and_empty():
     import poly_attention_b200 as P
     inv = P.rotary_frequencies(16)[0].cuda()
