@@ -223,6 +223,12 @@ class TreeDecoder:
             r.src = t.data_ptr()
             _st3(r.src_stride, t, esz)
         msgs, lses = [], []
+        if b == 0:      # no sequence: nothing to append (empty tensors have no address for the library)
+            if return_rows:
+                msgs = [torch.empty(0, g, nodes, self.d, device=self.device, dtype=self.dtype) for _ in range(order - 1)]
+                lses = [torch.empty(0, g, nodes, device=self.device, dtype=torch.float32) for _ in range(order - 1)]
+            self._stepped = True
+            return (out, msgs, lses) if return_rows else out
         for t in range(order - 1, -1, -1):
             a = self._passes[order - 1 - t]
             q = q1 if t == 0 else news[t - 1]
@@ -265,6 +271,9 @@ class TreeDecoder:
         c = self._commit
         c.nodes, c.path_len = max(self._append.nodes, self._captured), path.shape[1]   # at most; _step_nodes says which
         c.path, c.path_stride, c.count = path.data_ptr(), path.stride(0), count.data_ptr()
+        if self.b == 0:
+            self._stepped = False
+            return
         with _on(self.device):
             check(lib.poly_tree_commit_counted(c, self._step_nodes.data_ptr(), _stream(self.device)), "poly_tree_commit")
         self._stepped = False

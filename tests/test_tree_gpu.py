@@ -430,6 +430,22 @@ def test_packed_prompts_of_no_tokens():
     assert dec.lengths.tolist() == [0, 0]
 
 
+def test_a_decoder_of_no_sequences():
+    import poly_attention_b200 as P
+    none, longest = P.packed_offsets([])
+    attn = P.PolyAttention(dim=64, heads=2, dim_head=64, causal=True, use_rotary_embed=True).cuda()
+    y, dec = attn.tree_prefill(torch.randn(1, 0, 64, device="cuda"), none, max_seqlen=longest, capacity=8, max_nodes=2)
+    parents = torch.empty(0, 2, dtype=torch.int32, device="cuda")
+    assert y.shape == (1, 0, 64)
+    assert attn.tree_step(torch.randn(0, 2, 64, device="cuda"), dec, parents).shape == (0, 2, 64)
+    dec.commit(parents, torch.empty(0, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="since the last commit"):
+        dec.commit(parents, torch.empty(0, dtype=torch.int32, device="cuda"))
+    row = torch.randn(0, 2, 2, 64, device="cuda")
+    out, msgs, lses = dec.step(row, [row] * 2, [row], parents, return_rows=True)
+    assert out.shape == msgs[0].shape == (0, 2, 2, 64) and lses[0].shape == (0, 2, 2)
+
+
 def test_two_decoders_on_two_streams():
     rng = random.Random(7)
     cases = [Case(order=3, h=8, g=2, d=128, dtype=torch.bfloat16, lens=[3000 + i, 500], parents=[tree("random", 10, rng)] * 2, seed=i)
