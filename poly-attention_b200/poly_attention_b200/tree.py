@@ -135,12 +135,13 @@ class TreeDecoder:
             raise ValueError(f"lengths must be [{self.b}] and non-negative")
         if any(len(x) != n for x, n in ((keys, self.order), (vals, self.order - 1), (lses, self.order - 1), (msgs, self.order - 1))):
             raise ValueError("an order-n decoder holds n key caches and n - 1 of values, lses and messages")
-        for c, t in zip(self.keys + self.vals + self.msgs + self.lses, (*keys, *vals, *msgs, *lses)):
-            t = t.detach()
-            n = t.shape[2]
-            if longest > n or n > self.cap or t.shape[:2] != c.shape[:2] or t.shape[3:] != c.shape[3:]:
+        pairs = list(zip(self.keys + self.vals + self.msgs + self.lses, (*keys, *vals, *msgs, *lses)))
+        for c, t in pairs:      # all of them before the first is written
+            if (t.dim() != c.dim() or longest > t.shape[2] or t.shape[2] > self.cap or t.shape[:2] != c.shape[:2]
+                    or t.shape[3:] != c.shape[3:]):
                 raise ValueError(f"cache rows {tuple(t.shape)} do not fit {tuple(c.shape)} and lengths up to {longest}")
-            c[:, :, :n].copy_(t)
+        for c, t in pairs:
+            c[:, :, :t.shape[2]].copy_(t.detach())
         self.lengths.copy_(lengths)
         self._step_nodes.zero_()
         self._bound, self._stepped = longest, False

@@ -430,6 +430,19 @@ def test_packed_prompts_of_no_tokens():
     assert dec.lengths.tolist() == [0, 0]
 
 
+def test_a_refused_load_changes_nothing():
+    c = Case(order=2, h=2, g=2, d=64, dtype=torch.bfloat16, lens=[5], parents=[[-1]], cap=20)
+    caches = c.dec.keys + c.dec.vals + c.dec.lses + c.dec.msgs
+    before = [x.clone() for x in caches]
+    rows, lse = torch.zeros(1, 2, 10, 64, device="cuda"), torch.zeros(1, 2, 10, device="cuda")
+    for bad in (([rows] * 2, [rows], [lse], [rows[..., :32]], [7]), ([rows] * 2, [rows], [lse], [lse], [7]),
+                ([rows, rows[:, :, :6]], [rows], [lse], [rows], [7])):
+        with pytest.raises(ValueError):
+            c.dec.load(*bad)
+        assert all(torch.equal(x, y) for x, y in zip(caches, before)) and c.dec.lengths.tolist() == [5]
+    c.check()
+
+
 def test_a_decoder_of_no_sequences():
     import poly_attention_b200 as P
     none, longest = P.packed_offsets([])
