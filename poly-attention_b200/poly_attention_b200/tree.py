@@ -148,11 +148,12 @@ class TreeDecoder:
 
     def load_packed(self, keys, vals, lses, msgs, cu_seqlens, max_seqlen):
         """The same from a packed prompt batch: keys / vals / msgs [total, g, d], lses [g, total] (what
-        ``poly_attention_chain_packed`` takes and returns), sequence i being rows cu_seqlens[i] .. cu_seqlens[i + 1]."""
+        ``poly_attention_chain_packed`` takes and returns), sequence i being rows cu_seqlens[i] .. cu_seqlens[i + 1].
+        ``max_seqlen`` bounds the lengths; the sequences themselves have to fit the capacity."""
         if cu_seqlens.shape[0] != self.b + 1:
             raise ValueError(f"cu_seqlens must hold {self.b} sequences")
         start = cu_seqlens[:-1].long()
-        rows = start[:, None] + torch.arange(max_seqlen, device=start.device)
+        rows = start[:, None] + torch.arange(min(max_seqlen, self.cap), device=start.device)
         rows = rows.clamp_(0, max(keys[0].shape[0] - 1, 0))
         pick = lambda t: t[rows].permute(0, 2, 1, 3)   # noqa: E731
         self.load([pick(t) for t in keys], [pick(t) for t in vals], [t.t()[rows].permute(0, 2, 1) for t in lses],

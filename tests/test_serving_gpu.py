@@ -63,6 +63,23 @@ def test_prompt_drafts_commit(kind, rotary, dtype, tol, kw):
             assert dec.lengths.tolist() == [len(t) for t in tokens]
 
 
+def test_a_bound_above_the_capacity():
+    """max_seqlen is a bound: the prompts have to fit the cache, it does not."""
+    import poly_attention_b200 as P
+    attn = build(2, False, torch.float32)
+    cu, _ = P.packed_offsets([5, 16])
+    x = torch.randn(1, 21, 64, device="cuda")
+    y, dec = attn.tree_prefill(x, cu, max_seqlen=4096, capacity=16, max_nodes=2)
+    want, other = attn.tree_prefill(x, cu, max_seqlen=16, capacity=16, max_nodes=2)
+    assert dec.lengths.tolist() == [5, 16]
+    assert (y - want).abs().max() < 1e-4      # (another kernel: fp32, 3xTF32 products)
+    for a, b in zip(dec.keys + dec.vals, other.keys + other.vals):
+        assert torch.equal(a[0, :, :5], b[0, :, :5]) and torch.equal(a[1], b[1])
+    for bound, cap in ((4096, 15), (15, 20)):     # a sequence that does not fit, a bound that is none
+        with pytest.raises(ValueError, match="do not fit"):
+            attn.tree_prefill(x, cu, max_seqlen=bound, capacity=cap, max_nodes=2)
+
+
 def test_training_step_of_packed_rotary_module():
     """Gradients of a packed layer with positions are those of its sequences one by one (fp32, 1e-4 of the largest)."""
     import poly_attention_b200 as P
