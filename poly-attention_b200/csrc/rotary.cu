@@ -226,13 +226,13 @@ int launch_t(RotaryPlan& p, cudaStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
   PolyRotaryArgs& a = p.a;
   const int half = a.rot / 2;
-  static int sms[64] = {};
+  static std::atomic<int> sms[64] = {};   // per device; host threads may call at once
   int dev = 0;
-  cudaGetDevice(&dev);
-  int n_sm = dev < 64 ? sms[dev] : 0;
+  if (const int rc = cuda_status(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
+  int n_sm = dev < 64 ? sms[dev].load(std::memory_order_relaxed) : 0;
   if (!n_sm) {
     if (cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n_sm <= 0) n_sm = 148;
-    if (dev < 64) sms[dev] = n_sm;
+    if (dev < 64) sms[dev].store(n_sm, std::memory_order_relaxed);
   }
   const bool vec = vector_ok(a, V, sizeof(T));
   const int v = vec ? V : 1, run = a.interleaved && vec ? a.rot : half, rest = a.dim - a.rot;

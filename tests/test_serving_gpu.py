@@ -80,6 +80,35 @@ def test_a_bound_above_the_capacity():
             attn.tree_prefill(x, cu, max_seqlen=bound, capacity=cap, max_nodes=2)
 
 
+def test_host_threads_at_once():
+    """Several host threads, a stream each, through all three operators: every one gets the single thread's results."""
+    import threading
+
+    import poly_attention_b200 as P
+    attn = build(2, True, torch.bfloat16)
+    cu, longest = P.packed_offsets([30, 200])
+    x, drafts = (torch.randn(*s, 64, device="cuda").bfloat16() for s in ((1, 230), (2, 3)))
+    parents = torch.tensor([-1, 0, 0], dtype=torch.int32, device="cuda")
+
+    def work(out):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                y, dec = attn.tree_prefill(x, cu, max_seqlen=longest, capacity=210, max_nodes=3)
+                out.append((y, attn.tree_step(drafts, dec, parents)))
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    results = [[] for _ in range(5)]
+    work(results[0])
+    threads = [threading.Thread(target=work, args=(r,)) for r in results[1:]]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for r in results:
+        assert len(r) == 5 and all(torch.equal(a, b) for pair in r for a, b in zip(pair, results[0][0]))
+
+
 def test_training_step_of_packed_rotary_module():
     """Gradients of a packed layer with positions are those of its sequences one by one (fp32, 1e-4 of the largest)."""
     import poly_attention_b200 as P
