@@ -149,9 +149,10 @@ class PolyRotaryArgs(ctypes.Structure):
     ]
 
 
-def packer(cls):
-    """struct.Struct of a ctypes Structure without nested arrays of structures: argument blocks of calls whose
-    latency counts are packed in one go (some 60 attribute writes cost more than the launch)."""
+def packer(cls, before=None):
+    """struct.Struct of a ctypes Structure (of its fields before ``before``, if given) without nested arrays of
+    structures: argument blocks of calls whose latency counts are packed in one go (some 60 attribute writes
+    cost more than the launch)."""
     codes = {c_i32: "i", c_i64: "q", c_f32: "f", c_vp: "Q", c_sz: "Q"}
 
     def flat(t):
@@ -160,8 +161,10 @@ def packer(cls):
         if issubclass(t, ctypes.Array):
             return flat(t._type_) * t._length_
         return codes[t]
-    st = struct.Struct("@" + flat(cls))
-    if st.size > ctypes.sizeof(cls):
+    names = [f[0] for f in cls._fields_]
+    fields = cls._fields_[:names.index(before)] if before else cls._fields_
+    st = struct.Struct("@" + "".join(flat(f[1]) for f in fields))
+    if st.size > (getattr(cls, before).offset if before else ctypes.sizeof(cls)):
         raise ImportError(f"cannot pack {cls.__name__}")
     return st
 

@@ -14,14 +14,13 @@ from __future__ import annotations
 import ctypes
 import math
 import operator
-import struct
 from typing import List, Optional
 
 import torch
 from torch import nn
 
 from . import _lib
-from ._lib import PolyRotaryArgs, check, lib
+from ._lib import PolyRotaryArgs, PolyRotaryTensor, check, lib
 from .ops import _DTYPES, _no_tangents, _on, _require_cuda, _stream, packed_cu
 
 
@@ -66,9 +65,8 @@ def _empty_like(x):
                                dtype=x.dtype, device=x.device)
 
 
-_HEAD = struct.Struct("@8if i Qqqq QQqq Qii")    # PolyRotaryArgs before its tensors
-_TENSOR = struct.Struct("@QQii6q")
-assert _HEAD.size + _lib.MAX_ROTARY * _TENSOR.size == ctypes.sizeof(PolyRotaryArgs)
+_HEAD = _lib.packer(PolyRotaryArgs, before="t")
+_TENSOR = _lib.packer(PolyRotaryTensor)
 
 
 def _rotate(xs, inv_freq, positions, start, cu_seqlens, angles, interleaved, factor, inverse):
@@ -90,11 +88,11 @@ def _rotate(xs, inv_freq, positions, start, cu_seqlens, angles, interleaved, fac
                             inv_freq.data_ptr() if angles is None else 0, 0 if angles is None else angles.data_ptr(), an[0], an[1],
                             cu_seqlens.data_ptr() if cu_seqlens is not None else 0,
                             cu_seqlens.shape[0] - 1 if cu_seqlens is not None else 0, 0)
-            at = _HEAD.size
+            at = PolyRotaryArgs.t.offset
             for x, y in zip(part, outs[i0:]):
                 s, t = x.stride(), y.stride()
                 _TENSOR.pack_into(buf, at, x.data_ptr(), y.data_ptr(), x.shape[1], 0, s[0], s[1], s[2], t[0], t[1], t[2])
-                at += _TENSOR.size
+                at += ctypes.sizeof(PolyRotaryTensor)
             check(lib.poly_rotary(PolyRotaryArgs.from_buffer(buf), stream), "poly_rotary")
     return outs
 
