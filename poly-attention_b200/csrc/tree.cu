@@ -614,9 +614,12 @@ int warp_rows(const PolyTreePass& a) {
   return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
 }
 
-// Key ranges per (sequence, kv head): as many as fill the CTAs that fit at once (two
-// of tree_kernel per SM, one of the tcgen05 kernel), at least one key tile of the
-// capacity each.
+// Key ranges per (sequence, kv head), at least one key tile of the capacity each. tcgen05
+// kernel: as many as fill the CTAs that fit at once, one per SM. tree_kernel, of which two fit:
+// up to 8 that join in a cluster, filling both places (16 sequences of up to 9000 tokens,
+// 8 nodes, h16 g4 d128: 133 us a step, 155 with 3 CTAs per 2 SMs; 8 sequences: 80 and 91; 32 of
+// up to 2304: 82 and 80). More than 8, which go through the workspace, fill 3 places of 4:
+// 2 sequences of up to 40001 tokens take 96 us a step so, 121 with every place filled.
 TreeGeom geometry(const PolyTreePass& a, bool may_tc = true) {
   TreeGeom geo{};
   const int rows = a.nodes * (a.heads / a.kv_heads), wr = warp_rows(a);
@@ -625,15 +628,14 @@ TreeGeom geometry(const PolyTreePass& a, bool may_tc = true) {
   if (!geo.tcgen05) geo.row_blocks = (rows + 16 * wr - 1) / (16 * wr);
   const int64_t ctas = (int64_t)a.batch * a.kv_heads * geo.row_blocks;
   const int keys = geo.tcgen05 ? 128 : kKeys, tiles = (a.capacity + keys - 1) / keys;
-  const int slots = geo.tcgen05 ? sm_count() : sm_count() * 3 / 2;
-  const int want = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxSplits, tiles), slots / ctas));
+  auto fill = [&](int slots) { return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxSplits, tiles), slots / ctas)); };
   if (geo.tcgen05) {
-    geo.splits = want;
+    geo.splits = fill(sm_count());
   } else {
     // a cluster's 8 splits, or more of at least 16 tiles each (a second launch and the records' way through
     // L2 cost about 5 us)
-    const int long_splits = std::min(want, tiles / 16);
-    geo.splits = long_splits > 8 ? long_splits : std::min(want, 8);
+    const int long_splits = std::min(fill(sm_count() * 3 / 2), tiles / 16);
+    geo.splits = long_splits > 8 ? long_splits : std::min(fill(sm_count() * 2), 8);
     geo.cluster = geo.splits > 1 && geo.splits <= 8;
   }
   return geo;
