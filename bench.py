@@ -763,7 +763,7 @@ def run_reference(args, rank):
     except Exception as exc:  # noqa: BLE001
         port = cpu_baseline_port(str(exc))
         v = port["value"]
-        return {**common, "value": v, "cpu_baseline": port,
+        return {**common, "value": v, "ms_per_step": N / (v * H) * 1e3, "cpu_baseline": port,   # a step: one (batch, head) unit
                 "e2e": {"value": v, "unit": "tokens/s", "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0}}
     g = torch.Generator().manual_seed(1234)
 
