@@ -67,7 +67,8 @@ def _setup(ctx, inputs, output):
 
 def _backward(ctx, grads):
     n = ctx.n
-    xs, ws = ctx.saved_tensors[:n], ctx.saved_tensors[n:]
+    saved = ctx.saved_tensors      # read once: checkpointed activations are unpacked by the read
+    xs, ws = saved[:n], saved[n:]
     dxs, dws = [], []
     for x, w, g, e in zip(xs, ws, grads, ctx.eps):
         if g is None:

@@ -434,6 +434,25 @@ def test_modules_on_packed_sequences(kind, rotary, dtype):
         assert (a.float() - b.float()).norm() <= (1e-4 if dtype == torch.float32 else 3e-2) * b.float().norm() + 1e-6
 
 
+@pytest.mark.parametrize("order", [2, 3])
+def test_a_checkpointed_packed_module(order):
+    """Activations formed again in the backward: the same kernels on the same inputs."""
+    from torch.utils.checkpoint import checkpoint
+
+    import poly_attention_b200 as P
+    torch.manual_seed(0)
+    kw = dict(dim=64, heads=2, dim_head=64, causal=True, use_rotary_embed=True, prenorm=True)
+    attn = (P.PolyAttention(**kw) if order == 2 else P.NPolyAttention(order=3, **kw)).cuda()
+    cu, longest = P.packed_offsets([7, 0, 30])
+    x = torch.randn(1, 37, 64, device="cuda")
+    grads = []
+    for call in (attn, lambda *a, **k: checkpoint(attn, *a, use_reentrant=False, **k)):
+        y = x.clone().requires_grad_(True)
+        call(y, cu_seqlens=cu, max_seqlen=longest).square().sum().backward()
+        grads.append(y.grad)
+    assert torch.equal(*grads)
+
+
 def test_module_refusals():
     import poly_attention_b200 as P
     attn = P.PolyAttention(dim=64, heads=2, dim_head=64).cuda()
