@@ -23,9 +23,9 @@ def _require_cuda(*ts):
             raise RuntimeError("poly_attention_b200 runs on CUDA tensors only (no CPU implementation)")
 
 
-def _no_tangents(*ts):
+def _no_tangents(ts, *more):
     """Forward-mode derivatives do not exist here: a dual tensor is refused, since its tangent would be lost."""
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (*ts, *more)):
         raise NotImplementedError("poly_attention_b200 has no forward-mode derivatives")
 
 

@@ -141,7 +141,7 @@ def pass_fwd_packed(q, k, v, cu_seqlens, *, causal=False, softclamp=None, scale=
     fp32 [h, total]; out_lo is what rounding took off out, which ``pass_bwd_packed`` takes
     (None for float32).
     """
-    _no_tangents(q, k, v, bias, epi_mul)
+    _no_tangents((q, k, v, bias, epi_mul))
     _tensors(q, k, v, bias, epi_mul)
     cu = packed_cu(cu_seqlens, q)
     if bias is not None:
@@ -207,7 +207,7 @@ def pass_bwd_packed(q, k, v, cu_seqlens, out, lse, dout, *, causal=False, softcl
     """Backward of ``pass_fwd_packed``. Returns (dq, dk, dv, dbias-or-None). With ``dq`` given the
     query gradient is added to it in place. With ``factors`` = (left, right), whose product the
     values were, dv is the pair of their gradients."""
-    _no_tangents(q, k, v, out, lse, dout, bias, dlse, dq, out_lo, *(factors or ()))
+    _no_tangents((q, k, v, out, lse, dout, bias, dlse, dq, out_lo), *(factors or ()))
     _tensors(q, k, v, out, lse, dout, bias, dlse, dq, out_lo, *(factors or ()))
     cu = packed_cu(cu_seqlens, q)
     total, h = q.shape[:2]
@@ -315,7 +315,7 @@ def _chain(q_left, q_right, vs, cu_seqlens, softclamp_value, causal, max_seqlen)
     shared = tuple(t >= 1 and q_left[t] is q_right[t - 1] for t in range(order))
     ql, qr, vv = _autocast(*q_left), _autocast(*q_right), _autocast(*vs)
     ql = [qr[t - 1] if shared[t] else ql[t] for t in range(order)]
-    _no_tangents(*ql, *qr, *vv)
+    _no_tangents((*ql, *qr, *vv))
     _tensors(ql[0], qr[0], vv[0], *ql[1:], *qr[1:], *vv[1:])
     shape, dtype = qr[0].shape, qr[0].dtype
     for t in (*ql[1:], *qr[1:], *vv):

@@ -201,7 +201,7 @@ def apply_rotary(xs, inv_freq=None, *, positions=0, cu_seqlens=None, angles=None
     _require_cuda(inv_freq, angles, cu_seqlens)
     if (inv_freq is None) == (angles is None):
         raise ValueError("give either inv_freq or angles")
-    _no_tangents(*xs, inv_freq, angles)
+    _no_tangents(xs, inv_freq, angles)
     table = inv_freq if angles is None else angles
     if table.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("rotary frequencies and angles have no gradient")

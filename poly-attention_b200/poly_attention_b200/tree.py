@@ -27,6 +27,8 @@ Cache layout as ``ChainDecoder``'s (kv-head width):
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -65,6 +67,7 @@ class TreeDecoder:
         self.device = self.lengths.device
         # nodes of the last step that no commit has followed; on the device, as the host does not see a replayed step
         self._step_nodes = torch.zeros(1, device=self.device, dtype=torch.int32)
+        self._step_nodes_at = ctypes.c_void_p(self._step_nodes.data_ptr())
         self._bound = 0          # no sequence is longer than this ...
         self._replayed = False   # ... unless a captured commit is replayed
         self._stepped = False    # a step of the host waits for a commit
@@ -210,7 +213,7 @@ class TreeDecoder:
                 _require_cuda(t)
             if t.dtype != self.dtype or t.device != self.device:
                 raise TypeError(f"tree tensors must be {self.dtype} on {self.device}")
-        _no_tangents(q1, *news)
+        _no_tangents(news, q1)
         parents = self._parents(parents, nodes)
         self._room(nodes)
         rows = lambda t: t if t.stride(-1) == 1 else t.contiguous()   # noqa: E731
@@ -251,8 +254,7 @@ class TreeDecoder:
             else:
                 a.out = a.lse = None
         with _on(self.device):
-            check(lib.poly_tree_chain_counted(ap, self._passes, order, self._step_nodes.data_ptr(), _stream(self.device)),
-                  "poly_tree_chain")
+            check(lib.poly_tree_chain_counted(ap, self._passes, order, self._step_nodes_at, _stream(self.device)), "poly_tree_chain")
         self._stepped = True
         if torch.cuda.is_current_stream_capturing():
             self._captured = max(self._captured, nodes)
@@ -277,7 +279,7 @@ class TreeDecoder:
             self._stepped = False
             return
         with _on(self.device):
-            check(lib.poly_tree_commit_counted(c, self._step_nodes.data_ptr(), _stream(self.device)), "poly_tree_commit")
+            check(lib.poly_tree_commit_counted(c, self._step_nodes_at, _stream(self.device)), "poly_tree_commit")
         self._stepped = False
         self._replayed = self._replayed or torch.cuda.is_current_stream_capturing()
         self._bound = min(self.cap, self._bound + min(c.nodes, c.path_len))
