@@ -17,9 +17,9 @@
 // 256 + D. P V(i) precedes S(i + 1) of a warpgroup in issue order, so a full S says
 // that O is at rest and P's columns are free.
 //
-// Measured (4 sequences of up to 40001 tokens, d 128): 60 rows 67 us, 328 MB, 78 % of
-// the measured copy rate with its combine; 240 rows 121 us, bound by the chain score -
-// softmax - product of a tile, about 3 us, with two tiles in flight. Items of 64 keys
+// Measured (4 sequences of up to 40001 tokens, 128492 in all, d 128): 60 rows 67 us for 263 MB,
+// 60 % of the measured copy rate (the longest sequence's ranges set the time); 240 rows 121 us,
+// bound by the chain score - softmax - product of a tile, about 3 us, with two tiles in flight. Items of 64 keys
 // with S, P and O side by side in TMEM, so that S(i + 1) is formed during softmax(i),
 // were slower (84 and 159 us): the hand-offs per item cost more than they hid.
 #include <algorithm>
