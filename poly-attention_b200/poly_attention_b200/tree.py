@@ -133,6 +133,8 @@ class TreeDecoder:
         """Cached rows of every sequence: keys / vals / msgs [b, g, n, d] and lses [b, g, n] of n <= capacity rows,
         of which sequence i uses the first lengths[i] (a list or an integer tensor [b])."""
         lengths = torch.as_tensor(lengths)
+        if lengths.numel() and (lengths.is_floating_point() or lengths.is_complex() or lengths.dtype == torch.bool):
+            raise TypeError(f"lengths must be integers, got {lengths.dtype}")
         longest = int(lengths.max()) if lengths.numel() else 0
         if lengths.shape != (self.b,) or (lengths.numel() and int(lengths.min()) < 0):
             raise ValueError(f"lengths must be [{self.b}] and non-negative")

@@ -440,6 +440,10 @@ def test_a_refused_load_changes_nothing():
         with pytest.raises(ValueError):
             c.dec.load(*bad)
         assert all(torch.equal(x, y) for x, y in zip(caches, before)) and c.dec.lengths.tolist() == [5]
+    for lens in ([6.5], torch.tensor([True])):
+        with pytest.raises(TypeError, match="integers"):
+            c.dec.load([rows] * 2, [rows], [lse], [rows], lens)
+        assert c.dec.lengths.tolist() == [5]
     c.check()
 
 
